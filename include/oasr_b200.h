@@ -710,6 +710,71 @@ OASR_API int oasr_b200_fmha_window_paged(void* out, const void* qkv4, void* k_po
                                          int64_t num_blocks, int64_t chunk, int64_t left_chunks, double scale,
                                          int dtype, void* stream);
 
+/* ---- decoding step: rotation, 4-bit pages, scores (no reference counterparts) ----------------
+ * Position tables are fp32 (table_rows, rotary_dim): the cosines of a position's rotary_dim / 2 angles, then the sines.
+ * rotary_dim is a multiple of 16 up to head_dim; the first rotary_dim dims of a head turn in pairs (i, i + rotary_dim / 2),
+ * with `interleaved` (2 i, 2 i + 1), the others pass.  A norm weight (head_dim) of NULL skips that norm; with one a head row
+ * becomes x * rsqrt(mean(x^2) + eps) * weight before it turns.  fp32 arithmetic, rounded once on the store.
+ *
+ * 4-bit pages: codes (num_blocks, Hkv, block_size, D / 2) bytes and scales (num_blocks, Hkv, block_size, D / 32) in the
+ * element type.  A group of 32 dims has scale s = max|x| / 7 rounded up to five significant bits (at least 2^-20 in fp16 and
+ * 2^-120 in bf16, at most 9216 and 1.125 * 2^125; NaN where the group holds one; infinities saturate) and codes
+ * c = rint(x / s) in [-7, 7]; c * s is exact in the element type.  Word j (32 bits) of a row holds dims 32 (j mod G) +
+ * 8 (j div G) + i, G = D / 32, as c + 8 in bits 4 i .. 4 i + 3. */
+
+/* q (N, H, D) and k (N, Hkv, D): norm of each head row, then the rotation at positions[n] (int64 with pos_i64, else int32).
+ * A position outside the table gives a zero row.  Strides (token, head) in elements, multiples of 16 bytes; D a multiple of
+ * 16 up to 512; q_out / k_out may be q / k themselves, and overlap nothing else.  Hkv 0: queries only. */
+OASR_API int oasr_b200_qk_norm_rope(void* q_out, void* k_out, const void* q, const void* k, const void* q_weight,
+                                    const void* k_weight, const float* table, int64_t table_rows, int64_t rotary_dim,
+                                    const void* positions, int pos_i64, int64_t N, int64_t H, int64_t Hkv, int64_t D,
+                                    int64_t q_stride_n, int64_t q_stride_h, int64_t k_stride_n, int64_t k_stride_h,
+                                    int64_t q_out_stride_n, int64_t q_out_stride_h, int64_t k_out_stride_n,
+                                    int64_t k_out_stride_h, double eps, int interleaved, int dtype, void* stream);
+/* oasr_b200_paged_kv_write with norm and rotation of the keys on the way: frame t of stream b goes to logical position
+ * offsets[b] + t and turns by rope_offsets[b] + t (NULL: the same position); frames t >= new_lens[b] (NULL: none) write no
+ * page.  With H > 0 the queries are normed and turned into q_out in the same launch (padding frames: zeros).  Strides are
+ * host int64[3] (batch, head, frame) in elements, multiples of 8.  A position outside the position table gives a zero key
+ * and query; a frame whose page lies outside the block table or the pool is dropped.  fp16 and bf16. */
+OASR_API int oasr_b200_write_kv_rope(void* q_out, const int64_t* q_out_strides, void* k_pool, void* v_pool, const void* q,
+                                     const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                                     const int64_t* v_strides, const void* q_weight, const void* k_weight, const float* table,
+                                     int64_t table_rows, int64_t rotary_dim, const int32_t* block_table,
+                                     const int32_t* offsets, const int32_t* rope_offsets, const int32_t* new_lens, int64_t B,
+                                     int64_t H, int64_t Hkv, int64_t T, int64_t D, int64_t blocks_per_seq, int64_t block_size,
+                                     int64_t num_blocks, double eps, int interleaved, int dtype, void* stream);
+/* The same into 4-bit pages (D a multiple of 32). */
+OASR_API int oasr_b200_write_kv_rope_q4(void* q_out, const int64_t* q_out_strides, void* k_codes, void* k_scales,
+                                        void* v_codes, void* v_scales, const void* q, const int64_t* q_strides, const void* k,
+                                        const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                                        const void* q_weight, const void* k_weight, const float* table, int64_t table_rows,
+                                        int64_t rotary_dim, const int32_t* block_table, const int32_t* offsets,
+                                        const int32_t* rope_offsets, const int32_t* new_lens, int64_t B, int64_t H,
+                                        int64_t Hkv, int64_t T, int64_t D, int64_t blocks_per_seq, int64_t block_size,
+                                        int64_t num_blocks, double eps, int interleaved, int dtype, void* stream);
+/* Values of T positions from starts[b] on (NULL: from 0) as dense (B, Hkv, T, D); positions without a page give zeros. */
+OASR_API int oasr_b200_paged_kv_gather_q4(void* k_out, void* v_out, const void* k_codes, const void* k_scales,
+                                          const void* v_codes, const void* v_scales, const int32_t* block_table,
+                                          const int32_t* starts, int64_t B, int64_t Hkv, int64_t T, int64_t D,
+                                          int64_t blocks_per_seq, int64_t block_size, int64_t num_blocks, int dtype,
+                                          void* stream);
+/* Attention of q (B, H, Tq, D) over 4-bit pages: out[t] = softmax(scale q_t . k_j) v over the keys j with
+ * seqstarts[b] <= j < seqlens[b] (seqstarts NULL: 0) whose page lies in the pool, and with `causal`
+ * j <= seqlens[b] - q_lens[b] + t (q_lens NULL: Tq).  Rows t >= q_lens[b] and rows that see nothing are zeros.  Strides are host
+ * int64[3] (batch, head, row) in elements, multiples of 8.  D 64 or 128, H a multiple of Hkv, block_size of 16. */
+OASR_API int oasr_b200_fmha_q4(void* out, const int64_t* out_strides, const void* q, const int64_t* q_strides,
+                               const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+                               const int32_t* block_table, const int32_t* seqlens, const int32_t* seqstarts,
+                               const int32_t* q_lens, int64_t blocks_per_seq, int64_t block_size, int64_t num_blocks, int64_t B,
+                               int64_t H, int64_t Hkv, int64_t Tq, int64_t D, double scale, int causal, int dtype, void* stream);
+/* Scores of logits (rows, vocab), rows `stride` elements apart, vocab up to 262144, fp32 / fp16 / bf16; all outputs fp32.
+ * log_probs (rows, num_tokens): of tokens (rows, num_tokens) (int64 with tokens_i64, else int32), 0 for a token outside the
+ * vocabulary.  entropy (rows), NULL: not wanted.  top_log_probs / top_ids (rows, top_k), top_k up to 32: by value, equal values
+ * by lowest id, NaN above everything.  A row of nothing but -inf has log-probs of -inf and entropy 0. */
+OASR_API int oasr_b200_token_log_probs(float* log_probs, float* entropy, float* top_log_probs, int32_t* top_ids,
+                                       const void* logits, const void* tokens, int tokens_i64, int64_t rows, int64_t vocab,
+                                       int64_t stride, int64_t num_tokens, int64_t top_k, int dtype, void* stream);
+
 /* ---- packed-layout glue ------------------------------------------------ */
 /* out[i, :] = in[index[i], :] for i < n_out (rows of `row_bytes` bytes,
  * multiple of 16; index int64; `in` has `in_rows` rows and an index outside

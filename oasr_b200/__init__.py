@@ -9,8 +9,16 @@ reference package so its layers, models and engine run on these kernels.
 from __future__ import annotations
 
 from . import _lib
-from .attention import fmha, fmha_varlen, gather_paged_kv  # noqa: F401
-from .cache import PagedKVCache, gather_rows, scatter_rows, write_kv_chunk  # noqa: F401
+from .attention import fmha, fmha_q4, fmha_varlen, gather_paged_kv, gather_paged_kv_q4  # noqa: F401
+from .cache import (  # noqa: F401
+    PagedKVCache,
+    PagedKVCacheQ4,
+    gather_rows,
+    scatter_rows,
+    write_kv_chunk,
+    write_kv_rope,
+    write_kv_rope_q4,
+)
 from .functional import (  # noqa: F401
     add_layer_norm,
     add_layer_norm_residual,
@@ -34,9 +42,13 @@ from .functional import (  # noqa: F401
     group_gemm,
     layer_norm,
     layer_norm_activation,
+    qk_norm_rope,
     rms_norm,
     rms_norm_activation,
+    rope_table,
     swish,
+    token_log_probs,
+    TokenLogProbs,
 )
 
 __version__ = "0.1.0"

@@ -99,6 +99,12 @@ _SIGNATURES = {
     "oasr_b200_fmha_varlen": [P, P, P, P, P, P, c_int, P, P, I, I, I, I, I, I, I, c_double, c_int, P],
     "oasr_b200_paged_kv_write": [P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, c_int, P],
     "oasr_b200_paged_kv_gather": [P, P, P, P, P, I, I, I, I, I, I, c_int, P],
+    "oasr_b200_qk_norm_rope": [P] * 7 + [I, I, P, c_int] + [I] * 12 + [c_double, c_int, c_int, P],
+    "oasr_b200_write_kv_rope": [P] * 13 + [I, I] + [P] * 4 + [I] * 8 + [c_double, c_int, c_int, P],
+    "oasr_b200_write_kv_rope_q4": [P] * 15 + [I, I] + [P] * 4 + [I] * 8 + [c_double, c_int, c_int, P],
+    "oasr_b200_paged_kv_gather_q4": [P] * 8 + [I] * 7 + [c_int, P],
+    "oasr_b200_fmha_q4": [P] * 12 + [I] * 8 + [c_double, c_int, c_int, P],
+    "oasr_b200_token_log_probs": [P] * 6 + [c_int] + [I] * 5 + [c_int, P],
     "oasr_b200_gather_rows": [P, P, P, I, I, I, P],
     "oasr_b200_scatter_rows": [P, P, P, I, I, I, P],
 }

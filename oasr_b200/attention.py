@@ -7,7 +7,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .functional import _DTYPE_ID, _need_cuda, _p, _stream
+from .functional import _DTYPE_ID, _check_distinct_rows, _need_cuda, _p, _same_device, _stream
 
 _HALF = (torch.float16, torch.bfloat16)
 _Strides = ctypes.c_int64 * 3
@@ -205,4 +205,94 @@ def fmha_varlen(q, k, v, *, softmax_scale: float, cu_seqlens_q: torch.Tensor, cu
               _p(cu_seqlens_q), _p(cu_seqlens_k), S, q.size(0), k.size(0),
               int(max_seqlen_q), q.size(1), k.size(1), q.size(2), float(softmax_scale), _DTYPE_ID[q.dtype],
               _stream(q))
+    return out
+
+
+def _check_q4_pools(k_codes, k_scales, v_codes, v_scales, dtype):
+    """``(num_blocks, H_kv, block_size, D)`` of 4-bit pools, or an error."""
+    _need_cuda(k_codes, k_scales, v_codes, v_scales)
+    if k_codes.dim() != 4 or k_codes.dtype != torch.uint8 or v_codes.dtype != torch.uint8 or v_codes.shape != k_codes.shape:
+        raise ValueError("codes must be uint8 (num_blocks, H_kv, block_size, D / 2) and match")
+    num_blocks, Hkv, block_size, half = k_codes.shape
+    if half % 16 or half == 0:
+        raise ValueError(f"head_dim must be a multiple of 32, got {2 * half}")
+    want = (num_blocks, Hkv, block_size, half // 16)
+    if k_scales.shape != want or v_scales.shape != want:
+        raise ValueError(f"scales must be (num_blocks, H_kv, block_size, D / 32) = {want}, got {tuple(k_scales.shape)}")
+    if dtype not in _HALF:
+        raise ValueError(f"4-bit pages go with fp16 or bf16, got {dtype}")
+    if k_scales.dtype != dtype or v_scales.dtype != dtype:
+        raise ValueError(f"scales must have dtype {dtype}, got {k_scales.dtype} / {v_scales.dtype}")
+    if not (k_codes.is_contiguous() and k_scales.is_contiguous() and v_codes.is_contiguous() and v_scales.is_contiguous()):
+        raise ValueError("pools must be contiguous")
+    return num_blocks, Hkv, block_size, 2 * half
+
+
+def gather_paged_kv_q4(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor,
+                       block_table: torch.Tensor, start: Optional[torch.Tensor], length: int):
+    """The values of ``length`` positions from ``start[b]`` on (None: from 0) out of 4-bit pages, as dense
+    ``(B, H_kv, length, D)`` tensors in the scales' type (exact).  A position without a page gives zeros."""
+    num_blocks, Hkv, block_size, D = _check_q4_pools(k_codes, k_scales, v_codes, v_scales, k_scales.dtype)
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be (B, max_blocks_per_seq)")
+    B, length = block_table.size(0), int(length)
+    if length < 0:
+        raise ValueError(f"length must not be negative, got {length}")
+    if start is not None:
+        if start.shape != (B,):
+            raise ValueError(f"start must be ({B},), got {tuple(start.shape)}")
+        start = (start if start.dtype == torch.int32 else start.to(torch.int32)).contiguous()
+    _need_cuda(block_table, start)
+    _same_device(k_codes, k_scales, v_codes, v_scales, block_table, start)
+    block_table = (block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)).contiguous()
+    k = torch.empty(B, Hkv, length, D, device=k_codes.device, dtype=k_scales.dtype)
+    v = torch.empty_like(k)
+    _lib.call("oasr_b200_paged_kv_gather_q4", _p(k), _p(v), _p(k_codes), _p(k_scales), _p(v_codes), _p(v_scales), _p(block_table),
+              _p(start), B, Hkv, length, D, block_table.size(1), block_size, num_blocks, _DTYPE_ID[k.dtype], _stream(k))
+    return k, v
+
+
+def fmha_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor, *,
+            softmax_scale: float, block_table: torch.Tensor, cache_seqlens: torch.Tensor,
+            cache_seqstarts: Optional[torch.Tensor] = None, q_lens: Optional[torch.Tensor] = None, causal: bool = False,
+            out: Optional[torch.Tensor] = None, token_major: bool = False) -> torch.Tensor:
+    """Attention of ``q (B, H, T_q, D)`` over 4-bit pages (``PagedKVCacheQ4``), D 64 or 128, pages of a multiple of 16 rows.
+
+    Row ``t`` of sequence ``b`` sees the keys ``cache_seqstarts[b] <= j < cache_seqlens[b]`` (no start: from 0); with ``causal``
+    it stands at position ``cache_seqlens[b] - q_lens[b] + t`` and sees none behind that (``q_lens`` None: T_q), so the same
+    call serves a prompt, a chunk and a single token whose keys have been written.  (``fmha``'s ``causal`` counts rows from key
+    0.)  Rows ``t >= q_lens[b]`` are padding; those and rows that see nothing are zeros, and so is a sequence of length 0.  Keys
+    whose page lies outside the pool are not seen.  ``token_major=True`` returns ``(B, T_q, H, D)``."""
+    if q.dim() != 4:
+        raise ValueError(f"q must be (B, H, T_q, D); got {tuple(q.shape)}")
+    B, H, T, D = q.shape
+    num_blocks, Hkv, block_size, pool_dim = _check_q4_pools(k_codes, k_scales, v_codes, v_scales, q.dtype)
+    if pool_dim != D:
+        raise ValueError("q and k head_dim must match")
+    if Hkv == 0 or H % Hkv:
+        raise ValueError(f"H ({H}) must be divisible by H_kv ({Hkv})")
+    if block_table.dim() != 2 or block_table.size(0) != B:
+        raise ValueError("block_table must be (B, max_blocks_per_seq)")
+    lens = []
+    for name, t in (("cache_seqlens", cache_seqlens), ("cache_seqstarts", cache_seqstarts), ("q_lens", q_lens)):
+        if t is not None:
+            if t.shape != (B,):
+                raise ValueError(f"{name} must be (B,) = ({B},); got {tuple(t.shape)}")
+            t = (t if t.dtype == torch.int32 else t.to(torch.int32)).contiguous()
+        lens.append(t)
+    _need_cuda(q, block_table, *lens, out)
+    _same_device(q, k_codes, k_scales, v_codes, v_scales, block_table, *lens, out)
+    block_table = (block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)).contiguous()
+    want = (B, T, H, D) if token_major else (B, H, T, D)
+    if out is None:
+        out = torch.empty(want, dtype=q.dtype, device=q.device)
+    elif tuple(out.shape) != want or out.dtype != q.dtype or out.stride(3) != 1:
+        raise ValueError(f"out must be {want} in q's dtype, with unit stride along D")
+    _check_distinct_rows(out=out)
+    q, qs = _canon(q)
+    os = out.stride()
+    os = _Strides(os[0], os[2], os[1]) if token_major else _Strides(*os[:3])
+    _lib.call("oasr_b200_fmha_q4", _p(out), os, _p(q), qs, _p(k_codes), _p(k_scales), _p(v_codes), _p(v_scales), _p(block_table),
+              _p(lens[0]), _p(lens[1]), _p(lens[2]), block_table.size(1), block_size, num_blocks, B, H, Hkv, T, D, float(softmax_scale),
+              int(bool(causal)), _DTYPE_ID[q.dtype], _stream(q))
     return out

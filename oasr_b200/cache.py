@@ -4,13 +4,13 @@ oasr/cache/block_pool.py:33-41): per-layer pools ``(num_blocks, block_size, H_kv
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Union
+from typing import Optional, Union
 
 import torch
 
 from . import _lib
-from .attention import gather_paged_kv  # noqa: F401  (re-exported)
-from .functional import _need_cuda, _p, _stream
+from .attention import _HALF, _Strides, _check_q4_pools, fmha_q4, gather_paged_kv, gather_paged_kv_q4  # noqa: F401  (re-exported)
+from .functional import _DTYPE_ID, _check_distinct_rows, _check_head_weight, _check_rope_table, _need_cuda, _p, _same_device, _stream
 
 
 def write_kv_chunk(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, new_k: torch.Tensor,
@@ -72,6 +72,145 @@ class PagedKVCache:
         nblk = (max_total_kv + self.block_size - 1) // self.block_size
         k, v = gather_paged_kv(self.k_cache, self.v_cache, self.block_table[:, :nblk])
         return k[:, :, :max_total_kv], v[:, :, :max_total_kv]
+
+
+def _index32(name: str, t: Optional[torch.Tensor], B: int) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if t.shape != (B,):
+        raise ValueError(f"{name} must be ({B},), got {tuple(t.shape)}")
+    return (t if t.dtype == torch.int32 else t.to(torch.int32)).contiguous()
+
+
+def _write_rope(q4, pools, page_shape, block_table, new_k, new_v, offset, cos_sin, q, q_weight, k_weight, eps, interleaved,
+                rope_offset, new_lens, q_out):
+    _need_cuda(*pools, block_table, new_k, new_v, cos_sin, q, q_weight, k_weight, q_out)
+    if new_k.dim() != 4 or new_k.shape != new_v.shape:
+        raise ValueError("new_k / new_v must be (B, H_kv, T, D) and match")
+    B, Hkv, T, D = new_k.shape
+    num_blocks, block_size, pool_heads, pool_dim = page_shape
+    if new_k.dtype not in _HALF or new_v.dtype != new_k.dtype:
+        raise ValueError(f"new_k / new_v must share fp16 or bf16, got {new_k.dtype} / {new_v.dtype}")
+    if pool_heads != Hkv or pool_dim != D:
+        raise ValueError(f"pools hold {pool_heads} heads of {pool_dim}, the chunk has {Hkv} of {D}")
+    if block_table.dim() != 2 or block_table.size(0) != B:
+        raise ValueError("block_table must be (B, max_blocks_per_seq)")
+    if isinstance(offset, int):
+        offset = torch.full((B,), offset, dtype=torch.int32, device=new_k.device)
+    offset, rope_offset, new_lens = _index32("offset", offset, B), _index32("rope_offset", rope_offset, B), _index32("new_lens", new_lens, B)
+    if block_table.dtype != torch.int32:
+        block_table = block_table.to(torch.int32)
+    block_table = block_table.contiguous()
+    _same_device(new_k, *pools, block_table, new_v, offset, rope_offset, new_lens, cos_sin, q, q_weight, k_weight, q_out)
+    _check_rope_table(cos_sin, D)
+    _check_head_weight(new_k, D, q_weight=q_weight, k_weight=k_weight)
+    H = 0
+    if q is not None:
+        if q.dim() != 4 or q.size(0) != B or q.size(2) != T or q.size(3) != D or q.dtype != new_k.dtype:
+            raise ValueError(f"q must be ({B}, H, {T}, {D}) {new_k.dtype}, got {tuple(q.shape)} {q.dtype}")
+        H = q.size(1)
+        if q_out is None:
+            q_out = torch.empty_like(q)
+        elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(3) != 1:
+            raise ValueError("q_out must have q's shape and dtype, with unit stride along D")
+        _check_distinct_rows(q_out=q_out)
+    elif q_out is not None or q_weight is not None:
+        raise ValueError("q_out and q_weight need q")
+    if new_k.stride(3) != 1:
+        new_k = new_k.contiguous()
+    if new_v.stride(3) != 1:
+        new_v = new_v.contiguous()
+    qs = qo = None
+    if q is not None:
+        if q.stride(3) != 1:
+            q = q.contiguous()
+        qs, qo = _Strides(*q.stride()[:3]), _Strides(*q_out.stride()[:3])
+    _lib.call("oasr_b200_write_kv_rope_q4" if q4 else "oasr_b200_write_kv_rope", _p(q_out), qo, *map(_p, pools), _p(q), qs,
+              _p(new_k), _Strides(*new_k.stride()[:3]), _p(new_v), _Strides(*new_v.stride()[:3]), _p(q_weight), _p(k_weight),
+              _p(cos_sin), cos_sin.size(0), cos_sin.size(1), _p(block_table), _p(offset), _p(rope_offset), _p(new_lens), B, H, Hkv, T, D,
+              block_table.size(1), block_size, num_blocks, float(eps), int(bool(interleaved)), _DTYPE_ID[new_k.dtype], _stream(new_k))
+    return q_out
+
+
+def write_kv_rope(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, new_k: torch.Tensor,
+                  new_v: torch.Tensor, offset: Union[int, torch.Tensor], cos_sin: torch.Tensor, *,
+                  q: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
+                  k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+                  rope_offset: Optional[torch.Tensor] = None, new_lens: Optional[torch.Tensor] = None,
+                  q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """``write_kv_chunk`` with the keys' norm (``k_weight``) and rotation on the way, and with ``q (B, H, T, D)`` the queries'
+    (``q_weight``) in the same launch; returns the turned queries (None without ``q``).
+
+    Frame ``t`` of stream ``b`` lands at logical position ``offset[b] + t`` and turns by the ``rope_table`` row of
+    ``rope_offset[b] + t`` (None: the logical position; streams that have evicted pages pass their own).  Frames ``t >=
+    new_lens[b]`` are padding: no page is written and their query rows are zeros.  A position outside the table gives a zero key
+    and query.  ``q_out`` may be ``q`` itself.  ``interleaved``, weights and table as in ``qk_norm_rope``."""
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+        raise ValueError("pools must be (num_blocks, block_size, H_kv, D) and match")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("pools must be contiguous")
+    if k_cache.dtype != new_k.dtype or v_cache.dtype != new_k.dtype:
+        raise ValueError("chunk and pool dtypes must match")
+    return _write_rope(False, (k_cache, v_cache), tuple(k_cache.shape), block_table, new_k, new_v, offset, cos_sin, q, q_weight,
+                       k_weight, eps, interleaved, rope_offset, new_lens, q_out)
+
+
+def write_kv_rope_q4(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor,
+                     block_table: torch.Tensor, new_k: torch.Tensor, new_v: torch.Tensor, offset: Union[int, torch.Tensor],
+                     cos_sin: torch.Tensor, *, q: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
+                     k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+                     rope_offset: Optional[torch.Tensor] = None, new_lens: Optional[torch.Tensor] = None,
+                     q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """``write_kv_rope`` into 4-bit pages (``PagedKVCacheQ4`` describes them): the turned keys and the values are rounded to
+    codes and scales from fp32."""
+    num_blocks, Hkv, block_size, D = _check_q4_pools(k_codes, k_scales, v_codes, v_scales, new_k.dtype)
+    return _write_rope(True, (k_codes, k_scales, v_codes, v_scales), (num_blocks, block_size, Hkv, D), block_table, new_k, new_v, offset,
+                       cos_sin, q, q_weight, k_weight, eps, interleaved, rope_offset, new_lens, q_out)
+
+
+@dataclass
+class PagedKVCacheQ4:
+    """Paged keys and values in 4 bits: 0.28 of the bytes of 16-bit pages.
+
+    Codes are ``(num_blocks, H_kv, block_size, D / 2)`` uint8 and scales ``(num_blocks, H_kv, block_size, D / 32)`` in the
+    model's 16-bit type (heads outside the rows, so that a head's rows of a page lie together).  Each 32 dims of a row share the
+    scale ``max|x| / 7`` rounded up to five significant bits; a value is ``code * scale`` with a code in [-7, 7], which fp16 and
+    bf16 hold exactly.  The row's 32-bit word ``j`` holds dims ``32 (j % G) + 8 (j // G) + i`` (``G = D / 32``) as ``code + 8`` in
+    bits ``4 i .. 4 i + 3``.  Logical positions, ``block_table`` and ``cache_seqlens`` are those of ``PagedKVCache``."""
+
+    k_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_codes: torch.Tensor
+    v_scales: torch.Tensor
+    block_table: torch.Tensor
+    cache_seqlens: torch.Tensor
+
+    @staticmethod
+    def empty_pools(num_blocks: int, kv_heads: int, block_size: int, head_dim: int, dtype=torch.bfloat16, device="cuda"):
+        """``(k_codes, k_scales, v_codes, v_scales)`` of value 0."""
+        if head_dim % 32:
+            raise ValueError(f"head_dim must be a multiple of 32, got {head_dim}")
+        if dtype not in _HALF:
+            raise ValueError(f"4-bit pages have fp16 or bf16 scales, got {dtype}")
+        def codes():
+            return torch.zeros(num_blocks, kv_heads, block_size, head_dim // 2, dtype=torch.uint8, device=device)
+        def scales():
+            return torch.zeros(num_blocks, kv_heads, block_size, head_dim // 32, dtype=dtype, device=device)
+        return codes(), scales(), codes(), scales()
+
+    @property
+    def pools(self):
+        return self.k_codes, self.k_scales, self.v_codes, self.v_scales
+
+    def write_kv_rope(self, new_k: torch.Tensor, new_v: torch.Tensor, cos_sin: torch.Tensor, *, offset: Union[int, torch.Tensor],
+                      **how) -> Optional[torch.Tensor]:
+        return write_kv_rope_q4(*self.pools, self.block_table, new_k, new_v, offset, cos_sin, **how)
+
+    def fmha(self, q: torch.Tensor, *, softmax_scale: float, **how) -> torch.Tensor:
+        return fmha_q4(q, *self.pools, softmax_scale=softmax_scale, block_table=self.block_table, cache_seqlens=self.cache_seqlens, **how)
+
+    def gather_full_kv(self, max_total_kv: int):
+        return gather_paged_kv_q4(*self.pools, self.block_table, None, max_total_kv)
 
 
 def gather_rows(src: torch.Tensor, index: torch.Tensor, out: torch.Tensor = None) -> torch.Tensor:

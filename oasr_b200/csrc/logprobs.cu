@@ -1,0 +1,397 @@
+// Log-probs of given tokens, entropy and top alternatives of every row of logits, in one pass over the logits.
+//
+//   lse = M + log S,  S = sum_j exp(x_j - M);   log p(t) = x_t - lse;   H = log S - (1 / S) sum_j (x_j - M) exp(x_j - M)
+//   top k by (value, then lowest index)
+//
+// Sums run in fp32 and in the log2 domain, d_j = x_j log2(e) - m2 with m2 = M log2(e) rounded: one fused multiply-add a value.
+// What the rounding of m2 shifts all of them by is taken out of the two sums afterwards.
+//
+// A warp owns up to 32 * NV granules of 16 bytes of one row and holds them in registers: they are read from memory once, and the
+// maximum, the sums and the selection all run on that copy.  Selection: the k-th largest of the 32 lane maxima is a lower bound
+// of the k-th largest value, so only what reaches it (a little over k values) goes to a list in shared memory, from which k
+// rounds of a warp-wide maximum take the alternatives in order.  A row whose list overflows (many equal values: a mask that
+// leaves fewer than k tokens) or that holds a NaN takes its rounds over the registers instead; the result is the same.
+// Larger rows are split over the warps of a block, and over a cluster of blocks where the rows are few: the parts' statistics
+// and sorted lists meet in shared memory (the first block's, written through the cluster).
+#include <type_traits>
+
+#include "common.cuh"
+#include "sm100_ptx.cuh"
+
+namespace ob {
+namespace {
+
+constexpr int kMaxTop = 32;
+constexpr int kList = 128;          // candidates a warp can hold
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+constexpr float kFar = -200.f;      // 2^-200 is zero in fp32: the exponent of a masked (-inf) logit, which keeps d * exp2(d) at zero
+
+struct Args {
+  float *log_probs, *entropy, *top_log_probs;
+  int32_t* top_ids;
+  const void *logits, *tokens;
+  int64_t rows, stride;
+  int vocab, num_tokens, top_k, tokens_i64;
+};
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Order of the values as unsigned numbers; a NaN ranks above everything.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(x + 0.f);   // -0 ranks with +0
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float from_ordered(uint32_t o) {
+  if (o == 0xffffffffu) return __uint_as_float(0x7fffffffu);
+  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+// (value, lowest index first) as one unsigned number; 0 is below every element
+__device__ __forceinline__ uint64_t key_of(float x, int index) {
+  return (static_cast<uint64_t>(ordered(x)) << 32) | static_cast<uint32_t>(~index);
+}
+__device__ __forceinline__ int index_of(uint64_t key) { return ~static_cast<int>(static_cast<uint32_t>(key)); }
+
+__device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(k >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(k >> 32) == hi ? static_cast<uint32_t>(k) : 0u);
+  return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& g, float (&x)[Elem<T>::kVec]) {
+  const Pack<T> p = *reinterpret_cast<const Pack<T>*>(&g);
+#pragma unroll
+  for (int i = 0; i < Elem<T>::kVec; ++i) x[i] = Elem<T>::to_f(p.v[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ float granule_max(const uint4& g) {
+  if constexpr (sizeof(T) == 4) {
+    return max_nan(max_nan(__uint_as_float(g.x), __uint_as_float(g.y)), max_nan(__uint_as_float(g.z), __uint_as_float(g.w)));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2* h = reinterpret_cast<const __half2*>(&g);
+    const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return max_nan(__low2float(m), __high2float(m));
+  } else {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&g);
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return max_nan(__low2float(m), __high2float(m));
+  }
+}
+
+struct Stats {
+  float m, s, w;   // maximum (-inf: nothing there), sum of exp2(d), sum of d exp2(d) with d = (x - m) log2(e)
+};
+
+__device__ __forceinline__ Stats merge(Stats a, Stats b) {
+  Stats r;
+  r.m = max_nan(a.m, b.m);
+  if (r.m == -INFINITY) return Stats{-INFINITY, 0.f, 0.f};
+  // a part whose weight is zero (empty, or that far below) has no say, whatever its distance
+  const float da = (a.m - r.m) * kLog2e, db = (b.m - r.m) * kLog2e;
+  const float fa = ex2(da), fb = ex2(db);
+  r.s = r.w = 0.f;
+  if (fa != 0.f) r.s = a.s * fa, r.w = fa * fmaf(da, a.s, a.w);
+  if (fb != 0.f) r.s = fmaf(b.s, fb, r.s), r.w = fmaf(fb, fmaf(db, b.s, b.w), r.w);
+  return r;
+}
+
+__device__ __forceinline__ Stats warp_merge(Stats v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Stats b;
+    b.m = __shfl_xor_sync(0xffffffffu, v.m, o);
+    b.s = __shfl_xor_sync(0xffffffffu, v.s, o);
+    b.w = __shfl_xor_sync(0xffffffffu, v.w, o);
+    v = merge(v, b);
+  }
+  return v;
+}
+
+template <int W>
+struct Shared {
+  uint64_t list[W][kList];
+  uint64_t sorted[W][kMaxTop];
+  int count[W];
+  Stats stats[W];
+  // written by the other blocks of the cluster, read by the first
+  uint64_t part_sorted[8][kMaxTop];
+  Stats part_stats[8];
+};
+
+// k rounds over `lists` sorted lists of k keys each (lane l walks list l); the result is sorted into `out`.
+__device__ __forceinline__ void merge_lists(const uint64_t (*lists)[kMaxTop], int n, int k, uint64_t* out, int lane) {
+  int at = 0;
+  uint64_t head = lane < n ? lists[lane][0] : 0;
+  for (int r = 0; r < k; ++r) {
+    const uint64_t best = warp_max_key(head);
+    if (lane == 0) out[r] = best;
+    if (head == best && best != 0) head = ++at < k ? lists[lane][at] : 0;
+  }
+}
+
+// W warps of a block share a row's slice; `parts` blocks of a cluster share a row.
+template <typename T, int W, int NV>
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_log_probs_kernel(const Args a, const int parts) {
+  constexpr int VE = Elem<T>::kVec;
+  constexpr int kRows = W == 1 ? 4 : 1;                 // rows of a block
+  __shared__ Shared<W * kRows> sh;
+  ptx::grid_dep_launch();
+  ptx::grid_dep_wait();
+  if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // waited for before the first remote write
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int part = W == 1 ? 0 : static_cast<int>(blockIdx.x % parts);
+  const int64_t row = W == 1 ? static_cast<int64_t>(blockIdx.x) * kRows + warp : blockIdx.x / parts;
+  if (W == 1 && row >= a.rows) return;
+  const T* x0 = static_cast<const T*>(a.logits) + row * a.stride;
+  // granules start at the 16-byte boundary at or before the row; what lies outside the row is never read
+  const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));
+  const int granules = (a.vocab + lead + VE - 1) / VE;
+  const int first = W == 1 ? lane : part * W * 32 + threadIdx.x;
+  const int step = W == 1 ? 32 : parts * W * 32;
+
+  uint4 g[NV];
+  const uint32_t low = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;   // -inf
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int gi = first + i * step, e0 = gi * VE - lead;
+    g[i] = make_uint4(low, low, low, low);
+    if (gi < granules) {
+      if (e0 >= 0 && e0 + VE <= a.vocab) {
+        g[i] = *reinterpret_cast<const uint4*>(ld128_stream(x0 + e0).v);
+      } else {
+        T* p = reinterpret_cast<T*>(&g[i]);
+#pragma unroll
+        for (int j = 0; j < VE; ++j)
+          if (e0 + j >= 0 && e0 + j < a.vocab) p[j] = x0[e0 + j];
+      }
+    }
+  }
+
+  // ---- maximum and sums of the warp's part
+  float lane_max = granule_max<T>(g[0]);
+#pragma unroll
+  for (int i = 1; i < NV; ++i) lane_max = max_nan(lane_max, granule_max<T>(g[i]));
+  float m = lane_max;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  // Logits near the type's limit (a mask of its lowest value that leaves nothing) would overflow when multiplied.  Two of that
+  // size that differ at all differ by 2^102 or more, so any factor gives exponents of 0 or below kFar.
+  const float unit = fabsf(m) > 1e38f ? 0x1p-90f : kLog2e;
+  const float m2 = m == -INFINITY ? 0.f : m * unit;
+  float s = 0.f, w = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float x[VE];
+    unpack<T>(g[i], x);
+#pragma unroll
+    for (int j = 0; j < VE; ++j) {
+      const float d = max_nan(fmaf(x[j], unit, -m2), kFar);
+      const float e = ex2(d);
+      s += e;
+      w = fmaf(d, e, w);
+    }
+  }
+  s = warp_sum(s);
+  w = warp_sum(w);
+  if (m != -INFINITY) {
+    const float shift = fmaf(m, unit, -m2), f = ex2(-shift);   // m2 + shift is m * unit
+    w = fmaf(-shift, s, w) * f;
+    s *= f;
+  }
+  Stats st{m, s, w};
+
+  // ---- the warp's top k
+  const int k = a.top_k;
+  uint64_t* sorted = sh.sorted[warp];
+  if (k > 0) {
+    bool fast = m == m && m != -INFINITY;
+    float threshold = 0.f;
+    int found = 0;
+    if (fast) {
+      uint32_t cur = ordered(lane_max), top = 0;
+      for (int n = 0; n < k;) {
+        top = __reduce_max_sync(0xffffffffu, cur);
+        n += __popc(__ballot_sync(0xffffffffu, cur == top));
+        if (cur == top) cur = 0;
+      }
+      threshold = from_ordered(top);
+      if (lane == 0) sh.count[warp] = 0;
+      __syncwarp();
+      if (threshold != -INFINITY && lane_max >= threshold) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (granule_max<T>(g[i]) >= threshold) {
+            float x[VE];
+            unpack<T>(g[i], x);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {
+              if (x[j] >= threshold) {
+                const int at = atomicAdd(&sh.count[warp], 1);
+                if (at < kList) sh.list[warp][at] = key_of(x[j], (first + i * step) * VE - lead + j);
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();
+      found = sh.count[warp];
+      fast = threshold != -INFINITY && found <= kList;
+    }
+    if (fast) {
+      uint64_t best = 0;
+      for (int i = lane; i < found; i += 32) best = max(best, sh.list[warp][i]);
+      for (int r = 0; r < k; ++r) {
+        const uint64_t won = warp_max_key(best);
+        if (lane == 0) sorted[r] = won;
+        if (best == won) {
+          best = 0;
+          for (int i = lane; i < found; i += 32) {
+            const uint64_t c = sh.list[warp][i];
+            if (c < won) best = max(best, c);
+          }
+        }
+      }
+    } else {
+      // rounds over the warp's part of the row, from memory again (a copy in the caches): rare, and without a limit on equal values
+      uint64_t last = ~0ull;
+      for (int r = 0; r < k; ++r) {
+        uint64_t best = 0;
+        for (int gi = first; gi < granules; gi += step) {
+          for (int e = max(gi * VE - lead, 0); e < min(gi * VE - lead + VE, a.vocab); ++e) {
+            const uint64_t c = key_of(Elem<T>::to_f(x0[e]), e);
+            if (c < last) best = max(best, c);
+          }
+        }
+        last = warp_max_key(best);
+        if (lane == 0) sorted[r] = last;
+      }
+    }
+    __syncwarp();
+  }
+
+  // ---- the row's: parts meet
+  if constexpr (W > 1) {
+    if (lane == 0) sh.stats[warp] = st;
+    __syncthreads();
+    if (parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (warp == 0) {
+      st = warp_merge(lane < W ? sh.stats[lane] : Stats{-INFINITY, 0.f, 0.f});
+      uint64_t* dst = parts > 1 ? sh.list[0] : sh.list[1];   // lists of the warps are done with
+      if (k > 0) merge_lists(sh.sorted, W, k, dst, lane);
+      __syncwarp();
+      if (parts > 1) {   // into the first block's shared memory
+        if (k > 0 && lane < k) {
+          const uint32_t to = ptx::map_to_cta(&sh.part_sorted[part][lane], 0);
+          asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(dst[lane]) : "memory");
+        }
+        if (lane < 3) {
+          const float v = lane == 0 ? st.m : lane == 1 ? st.s : st.w;
+          const uint32_t to = ptx::map_to_cta(reinterpret_cast<float*>(&sh.part_stats[part]) + lane, 0);
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
+        }
+      }
+    }
+    if (parts > 1) {
+      ptx::cluster_sync();
+      if (part != 0) return;
+      if (warp == 0) {
+        st = warp_merge(lane < parts ? sh.part_stats[lane] : Stats{-INFINITY, 0.f, 0.f});
+        if (k > 0) merge_lists(sh.part_sorted, parts, k, sh.list[1], lane);
+        __syncwarp();
+      }
+    }
+    if (warp != 0) return;
+    sorted = sh.list[1];
+  }
+  const bool none = st.m == -INFINITY;             // a row of -inf: every log-prob is -inf, the entropy 0
+  const float log_s = logf(st.s);
+  auto log_prob = [&](float x) { return none ? -INFINITY : (x - st.m) - log_s; };
+  if (a.entropy && lane == 0) a.entropy[row] = none ? 0.f : fmaf(-kLn2, st.w / st.s, log_s);
+  for (int j = lane; j < a.num_tokens; j += 32) {
+    const int64_t at = row * a.num_tokens + j;
+    const int64_t t = a.tokens_i64 ? static_cast<const int64_t*>(a.tokens)[at] : static_cast<const int32_t*>(a.tokens)[at];
+    a.log_probs[at] = t >= 0 && t < a.vocab ? log_prob(Elem<T>::to_f(x0[t])) : 0.f;   // padding scores nothing
+  }
+  if (lane < k) {
+    const uint64_t key = sorted[lane];
+    a.top_ids[row * k + lane] = index_of(key);
+    a.top_log_probs[row * k + lane] = log_prob(from_ordered(static_cast<uint32_t>(key >> 32)));
+  }
+}
+
+template <typename T, int W, int NV>
+int launch(const Args& a, int parts, cudaStream_t s) {
+  cudaLaunchConfig_t cfg{};
+  const int64_t blocks = W == 1 ? (a.rows + 3) / 4 : a.rows * parts;
+  OB_REQUIRE(blocks <= 0x7fffffff, OASR_ERR_INVALID, "token_log_probs: too many rows for one call");
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(W == 1 ? 128 : W * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = g_pdl ? 1 : 0;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim = {static_cast<unsigned>(parts), 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = parts > 1 ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, token_log_probs_kernel<T, W, NV>, a, parts);
+  return check_launch("token_log_probs launch");
+}
+
+template <typename T>
+int run(const Args& a, cudaStream_t s) {
+  constexpr int VE = Elem<T>::kVec;
+  const int64_t granules = (a.vocab + 2 * VE - 2) / VE;   // at the worst alignment
+  const int64_t sms = sm_count();
+  // many rows: a warp each, without a block's barriers
+  if (a.rows >= sms * 4 && granules <= 32 * 20) {
+    if (granules <= 32 * 5) return launch<T, 1, 5>(a, 1, s);
+    if (granules <= 32 * 10) return launch<T, 1, 10>(a, 1, s);
+    return launch<T, 1, 20>(a, 1, s);
+  }
+  if (granules <= 128 * 5) return launch<T, 4, 5>(a, 1, s);
+  if (a.rows >= sms * 2 && granules <= 128 * 10) return launch<T, 4, 10>(a, 1, s);
+  int parts = 1;   // few rows: a cluster each
+  while (parts < 8 && (a.rows * parts < sms || granules > 512 * 16 * parts) && granules > 512 * parts) parts *= 2;
+  const int64_t per = (granules + 512 * parts - 1) / (512 * parts);
+  if (per <= 2) return launch<T, 16, 2>(a, parts, s);
+  if (per <= 4) return launch<T, 16, 4>(a, parts, s);
+  if (per <= 8) return launch<T, 16, 8>(a, parts, s);
+  return launch<T, 16, 16>(a, parts, s);
+}
+
+}  // namespace
+}  // namespace ob
+
+extern "C" int oasr_b200_token_log_probs(float* log_probs, float* entropy, float* top_log_probs, int32_t* top_ids, const void* logits,
+                                         const void* tokens, int tokens_i64, int64_t rows, int64_t vocab, int64_t stride,
+                                         int64_t num_tokens, int64_t top_k, int dtype, void* stream) {
+  using namespace ob;
+  OB_REQUIRE(rows >= 0 && vocab > 0 && num_tokens >= 0 && top_k >= 0, OASR_ERR_INVALID, "token_log_probs: bad shape");
+  OB_REQUIRE(vocab <= 262144, OASR_ERR_UNSUPPORTED, "token_log_probs: at most 262144 tokens in the vocabulary (got %lld)", (long long)vocab);
+  OB_REQUIRE(stride >= vocab || rows <= 1, OASR_ERR_INVALID, "token_log_probs: rows of %lld logits %lld apart", (long long)vocab, (long long)stride);
+  OB_REQUIRE(top_k <= kMaxTop && top_k <= vocab, OASR_ERR_INVALID, "token_log_probs: top_k must be at most %d and the vocabulary (got %lld)",
+             kMaxTop, (long long)top_k);
+  if (rows == 0) return OASR_OK;
+  OB_REQUIRE(logits && (num_tokens == 0 || (tokens && log_probs)) && (top_k == 0 || (top_log_probs && top_ids)), OASR_ERR_INVALID,
+             "token_log_probs: null pointer argument");
+  OB_REQUIRE(num_tokens <= 0x7fffffff, OASR_ERR_INVALID, "token_log_probs: too many tokens a row");
+  const Args a{log_probs, entropy, top_log_probs, top_ids, logits, tokens, rows, stride, static_cast<int>(vocab), static_cast<int>(num_tokens),
+               static_cast<int>(top_k), tokens_i64};
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return OB_DISPATCH_FLOAT(dtype, T_, [&]() -> int {
+    OB_REQUIRE(is_aligned(logits, sizeof(T_)), OASR_ERR_ALIGN, "token_log_probs: logits must be aligned to their type");
+    return run<T_>(a, s);
+  });
+}

@@ -1,0 +1,511 @@
+// Norms of queries and keys for each head with the position rotation, and the same on the way into the paged cache.
+//
+//   n(x) = x * rsqrt(mean(x^2) + eps) * w                         per head row, skipped without a weight
+//   y_a  = x_a cos - x_b sin,  y_b = x_b cos + x_a sin            pairs (a, b) of the first R dims: (i, i + R / 2), or (2 i, 2 i + 1)
+//
+// cos | sin come from an fp32 table row per position.  All arithmetic is fp32; the products and sums of the rotation are
+// rounded one by one (no contraction), so that a 4-bit code or a 16-bit rounding does not depend on how the compiler fuses
+// them.  Everything is read once and written once: HBM-bound from some thousand rows on, launch-bound below.
+//
+// A lane owns a unit of 16 dims: the two octets whose dims pair up (u and u + R / 16), or two neighbouring octets where pairs
+// are neighbours or nothing is rotated.  So a lane reads what it writes and nothing else (rows may be turned in place), the
+// row sum is a shuffle over D / 16 lanes, and cos / sin are loaded once for the heads that a lane walks over.
+#include "common.cuh"
+#include "q4.cuh"
+#include "sm100_ptx.cuh"
+
+namespace ob {
+namespace {
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    const Pack<T> v = ld128(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = Elem<T>::to_f(v.v[i]);
+  } else {
+    const Pack<T> v = ld128(p), w = ld128(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = v.v[i], x[4 + i] = w.v[i];
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    Pack<T> v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v.v[i] = Elem<T>::from_f(x[i]);
+    st128(p, v);
+  } else {
+    Pack<T> v, w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v.v[i] = x[i], w.v[i] = x[4 + i];
+    st128(p, v);
+    st128(p + 4, w);
+  }
+}
+
+// The two octets of unit u; `units` of them are rotated.
+template <bool kInter>
+__device__ __forceinline__ int2 unit_octets(int u, int rotated) {
+  return (!kInter && u < rotated) ? make_int2(u, u + rotated) : make_int2(2 * u, 2 * u + 1);
+}
+
+struct Turn {
+  float c[8], s[8];
+};
+
+__device__ __forceinline__ Turn load_turn(const float* row, int half, int u) {
+  Turn t;
+  load8(row + u * 8, t.c);
+  load8(row + half + u * 8, t.s);
+  return t;
+}
+
+template <bool kInter>
+__device__ __forceinline__ void rotate(float (&a)[8], float (&b)[8], const Turn& t) {
+  auto turn = [](float& x, float& y, float c, float s) {
+    const float nx = __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s));
+    y = __fadd_rn(__fmul_rn(y, c), __fmul_rn(x, s));
+    x = nx;
+  };
+  if constexpr (kInter) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      turn(a[2 * i], a[2 * i + 1], t.c[i], t.s[i]);
+      turn(b[2 * i], b[2 * i + 1], t.c[4 + i], t.s[4 + i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) turn(a[i], b[i], t.c[i], t.s[i]);
+  }
+}
+
+// x * rsqrt(mean(x^2) + eps) * w over the `lanes` lanes of a row; every lane of the warp calls it (idle ones with zeros).
+template <typename T>
+__device__ __forceinline__ void norm_row(float (&a)[8], float (&b)[8], const Pack<T>* w, int lanes, float inv_d, float eps) {
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum = fmaf(a[i], a[i], fmaf(b[i], b[i], sum));
+  for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float r = rsqrtf(fmaf(sum, inv_d, eps));
+  const T* wa = reinterpret_cast<const T*>(w);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    a[i] = a[i] * r * Elem<T>::to_f(wa[i]);
+    b[i] = b[i] * r * Elem<T>::to_f(wa[8 + i]);
+  }
+}
+
+// 16 values of a weight row as a lane holds them
+template <typename T>
+struct UnitWeight {
+  static constexpr int kPacks = 16 / Elem<T>::kVec;
+  Pack<T> w[kPacks];
+  __device__ void load(const T* row, int2 oct) {
+#pragma unroll
+    for (int i = 0; i < kPacks / 2; ++i) {
+      w[i] = ld128_nc(row + oct.x * 8 + i * Elem<T>::kVec);
+      w[kPacks / 2 + i] = ld128_nc(row + oct.y * 8 + i * Elem<T>::kVec);
+    }
+  }
+};
+
+struct QkArgs {
+  void *q_out, *k_out;
+  const void *q, *k, *q_weight, *k_weight;
+  const float* table;
+  const void* positions;
+  int64_t table_rows, tokens, qs_n, qs_h, ks_n, ks_h, qo_n, qo_h, ko_n, ko_h;
+  int half, heads, kv_heads, units, lanes, lane_shift, per_lane, chunks, pos_i64;
+  float inv_d, eps;
+};
+
+template <typename T, bool kInter>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkArgs a) {
+  ptx::grid_dep_launch();
+  ptx::grid_dep_wait();
+  const int64_t group = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> a.lane_shift;
+  const int u = threadIdx.x & (a.lanes - 1);
+  const int64_t n = group / a.chunks;
+  const int head0 = static_cast<int>(group - n * a.chunks) * a.per_lane;
+  const bool mine = n < a.tokens && u < a.units;
+  const int rotated = a.half / 8;
+  const int2 oct = unit_octets<kInter>(u, rotated);
+  int64_t pos = -1;
+  if (mine) pos = a.pos_i64 ? static_cast<const int64_t*>(a.positions)[n] : static_cast<const int32_t*>(a.positions)[n];
+  const bool known = pos >= 0 && pos < a.table_rows;   // other positions: a zero row
+  const bool turned = known && u < rotated;
+  Turn t;
+  if (turned) t = load_turn(a.table + pos * 2 * a.half, a.half, u);
+  for (int i = 0; i < a.per_lane; ++i) {
+    const int head = head0 + i;
+    const bool is_q = head < a.heads;
+    const int h = is_q ? head : head - a.heads;
+    const bool live = mine && head < a.heads + a.kv_heads;
+    float xa[8] = {}, xb[8] = {};
+    if (live && known) {
+      const T* src = is_q ? static_cast<const T*>(a.q) + n * a.qs_n + h * a.qs_h : static_cast<const T*>(a.k) + n * a.ks_n + h * a.ks_h;
+      load8(src + oct.x * 8, xa);
+      load8(src + oct.y * 8, xb);
+    }
+    const T* weight = static_cast<const T*>(is_q ? a.q_weight : a.k_weight);
+    if (a.q_weight || a.k_weight) {   // uniform: the shuffles inside take every lane
+      UnitWeight<T> w;
+      if (weight && live) {
+        w.load(weight, oct);
+      }
+      float na[8], nb[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) na[j] = xa[j], nb[j] = xb[j];
+      norm_row<T>(na, nb, w.w, a.lanes, a.inv_d, a.eps);
+      if (weight) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) xa[j] = na[j], xb[j] = nb[j];
+      }
+    }
+    if (turned) rotate<kInter>(xa, xb, t);
+    if (live) {
+      if (!known) {   // a NaN weight must not reach a row that has no position
+#pragma unroll
+        for (int j = 0; j < 8; ++j) xa[j] = xb[j] = 0.f;
+      }
+      T* dst = is_q ? static_cast<T*>(a.q_out) + n * a.qo_n + h * a.qo_h : static_cast<T*>(a.k_out) + n * a.ko_n + h * a.ko_h;
+      store8(dst + oct.x * 8, xa);
+      store8(dst + oct.y * 8, xb);
+    }
+  }
+}
+
+struct WriteArgs {
+  void *q_out, *k_pool, *v_pool;       // pools: 16-bit rows, or codes
+  void *k_scales, *v_scales;           // 4-bit pools only
+  const void *q, *k, *v, *q_weight, *k_weight;
+  const float* table;
+  const int32_t *block_table, *offsets, *rope_offsets, *new_lens;
+  int64_t table_rows, B, T, qs_b, qs_h, qs_t, ks_b, ks_h, ks_t, vs_b, vs_h, vs_t, qo_b, qo_h, qo_t;
+  int64_t blocks_per_seq, block_size, num_blocks;
+  int half, heads, kv_heads, units, lanes, lane_shift, per_lane, chunks, groups;
+  float inv_d, eps;
+};
+
+// Largest magnitude of each of the lane's two octets' groups.  `owner` of an octet: the lane and slot that hold it.
+template <bool kPairs>
+__device__ __forceinline__ float2 group_max(float ma, float mb, int2 oct, int rotated, int lanes) {
+  if constexpr (kPairs) {
+    float m = q4::max_nan(ma, mb);
+    m = q4::max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    return make_float2(m, m);
+  } else {
+    float r[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int first = (s ? oct.y : oct.x) & ~3;
+      float m = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int o = first + j;
+        const bool split = o < 2 * rotated;
+        const int lane = split ? (o < rotated ? o : o - rotated) : o >> 1;
+        const bool slot_b = split ? o >= rotated : (o & 1);
+        const float va = __shfl_sync(0xffffffffu, ma, lane, lanes), vb = __shfl_sync(0xffffffffu, mb, lane, lanes);
+        m = q4::max_nan(m, slot_b ? vb : va);
+      }
+      r[s] = m;
+    }
+    return make_float2(r[0], r[1]);
+  }
+}
+
+__device__ __forceinline__ float octet_max(const float (&x)[8]) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = q4::max_nan(m, fabsf(x[i]));
+  return m;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_q4(uint32_t* codes, T* scales, const float (&x)[8], int o, float amax, int groups) {
+  const float s = q4::scale_of<T>(amax);
+  codes[q4::word_of_octet(o, groups)] = q4::codes_of(x, s);
+  if ((o & 3) == 0) scales[o >> 2] = Elem<T>::from_f(s);
+}
+
+// Head rows of one frame: the queries' (into q_out), then the keys' and the values' (into their page).
+template <typename T, bool kInter, bool kQ4>
+__global__ void __launch_bounds__(256) write_kv_rope_kernel(const WriteArgs a) {
+  ptx::grid_dep_launch();
+  ptx::grid_dep_wait();
+  const int64_t group = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> a.lane_shift;
+  const int u = threadIdx.x & (a.lanes - 1);
+  const int64_t frame = group / a.chunks;
+  const int head0 = static_cast<int>(group - frame * a.chunks) * a.per_lane;
+  const int64_t b = frame / a.T, t = frame - b * a.T;
+  const bool mine = b < a.B && u < a.units;
+  const int rotated = a.half / 8;
+  const int2 oct = unit_octets<kInter>(u, rotated);
+  bool fresh = false, known = false;
+  int64_t page = -1, slot = 0, pos = 0;
+  if (mine) {
+    fresh = !a.new_lens || t < a.new_lens[b];
+    const int64_t at = static_cast<int64_t>(a.offsets[b]) + t;
+    pos = a.rope_offsets ? static_cast<int64_t>(a.rope_offsets[b]) + t : at;
+    known = fresh && pos >= 0 && pos < a.table_rows;
+    const int64_t logical = at / a.block_size;
+    slot = at - logical * a.block_size;
+    if (fresh && at >= 0 && logical < a.blocks_per_seq) page = a.block_table[b * a.blocks_per_seq + logical];
+    if (page >= a.num_blocks) page = -1;             // outside the table or the pool: dropped, never written
+  }
+  const bool turned = known && u < rotated;
+  Turn tn;
+  if (turned) tn = load_turn(a.table + pos * 2 * a.half, a.half, u);
+  const int dims = a.units * 16;
+  for (int i = 0; i < a.per_lane; ++i) {
+    const int head = head0 + i;
+    const int kind = head < a.heads ? 0 : head < a.heads + a.kv_heads ? 1 : 2;
+    const int h = kind == 0 ? head : head - a.heads - (kind - 1) * a.kv_heads;
+    const bool live = mine && head < a.heads + 2 * a.kv_heads;
+    const int2 at = kind == 2 ? make_int2(2 * u, 2 * u + 1) : oct;   // values are not rotated: neighbouring octets
+    const bool read = live && fresh && (kind == 2 || known) && (kind == 0 || page >= 0);
+    float xa[8] = {}, xb[8] = {};
+    if (read) {
+      const T* src = kind == 0   ? static_cast<const T*>(a.q) + b * a.qs_b + h * a.qs_h + t * a.qs_t
+                     : kind == 1 ? static_cast<const T*>(a.k) + b * a.ks_b + h * a.ks_h + t * a.ks_t
+                                 : static_cast<const T*>(a.v) + b * a.vs_b + h * a.vs_h + t * a.vs_t;
+      load8(src + at.x * 8, xa);
+      load8(src + at.y * 8, xb);
+    }
+    if (a.q_weight || a.k_weight) {
+      const T* weight = static_cast<const T*>(kind == 0 ? a.q_weight : kind == 1 ? a.k_weight : nullptr);
+      UnitWeight<T> w;
+      if (weight && read) w.load(weight, at);
+      float na[8], nb[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) na[j] = xa[j], nb[j] = xb[j];
+      norm_row<T>(na, nb, w.w, a.lanes, a.inv_d, a.eps);
+      if (weight && read) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) xa[j] = na[j], xb[j] = nb[j];
+      }
+    }
+    if (turned && kind != 2) rotate<kInter>(xa, xb, tn);
+    float2 gmax;
+    if constexpr (kQ4) {   // uniform: shuffles
+      const float ma = octet_max(xa), mb = octet_max(xb);
+      const float2 pairs = group_max<true>(ma, mb, at, rotated, a.lanes);
+      if constexpr (kInter) {
+        gmax = pairs;
+      } else {
+        const float2 split = group_max<false>(ma, mb, at, rotated, a.lanes);
+        gmax = kind == 2 ? pairs : split;
+      }
+    }
+    if (!live) continue;
+    if (kind == 0) {
+      T* dst = static_cast<T*>(a.q_out) + b * a.qo_b + h * a.qo_h + t * a.qo_t;
+      store8(dst + at.x * 8, xa);
+      store8(dst + at.y * 8, xb);
+    } else if (fresh && page >= 0) {
+      if constexpr (kQ4) {
+        const int64_t row = (page * a.kv_heads + h) * a.block_size + slot;
+        uint32_t* codes = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(kind == 1 ? a.k_pool : a.v_pool) + row * (dims / 2));
+        T* scales = static_cast<T*>(kind == 1 ? a.k_scales : a.v_scales) + row * a.groups;
+        store_q4<T>(codes, scales, xa, at.x, gmax.x, a.groups);
+        store_q4<T>(codes, scales, xb, at.y, gmax.y, a.groups);
+      } else {
+        const int64_t row = (page * a.block_size + slot) * a.kv_heads + h;
+        T* dst = static_cast<T*>(kind == 1 ? a.k_pool : a.v_pool) + row * dims;
+        store8(dst + at.x * 8, xa);
+        store8(dst + at.y * 8, xb);
+      }
+    }
+  }
+}
+
+struct GatherArgs {
+  void *k_out, *v_out;
+  const uint32_t *k_codes, *v_codes;
+  const void *k_scales, *v_scales;
+  const int32_t *block_table, *starts;
+  int64_t B, Hkv, T, blocks_per_seq, block_size, num_blocks;
+  int words, groups;
+};
+
+// out[b, h, i, :] = the values of position starts[b] + i; a word (8 values) of K and of V per thread.
+template <typename T>
+__global__ void __launch_bounds__(256) gather_q4_kernel(const GatherArgs a) {
+  ptx::grid_dep_launch();
+  ptx::grid_dep_wait();
+  const int64_t total = a.B * a.Hkv * a.T * a.words;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += stride) {
+    const int64_t r = i / a.words;
+    const int j = static_cast<int>(i - r * a.words);
+    const int64_t bh = r / a.T, pos = (a.starts ? static_cast<int64_t>(a.starts[bh / a.Hkv]) : 0) + (r - bh * a.T);
+    const int64_t b = bh / a.Hkv, h = bh - b * a.Hkv;
+    const int64_t logical = pos / a.block_size;
+    int64_t page = -1;
+    if (pos >= 0 && logical < a.blocks_per_seq) page = a.block_table[b * a.blocks_per_seq + logical];
+    float k[8] = {}, v[8] = {};
+    const int o = q4::octet_of_word(j, a.groups);
+    if (page >= 0 && page < a.num_blocks) {
+      const int64_t row = (page * a.Hkv + h) * a.block_size + (pos - logical * a.block_size);
+      const uint32_t kw = a.k_codes[row * a.words + j], vw = a.v_codes[row * a.words + j];
+      const float ks = Elem<T>::to_f(static_cast<const T*>(a.k_scales)[row * a.groups + (o >> 2)]);
+      const float vs = Elem<T>::to_f(static_cast<const T*>(a.v_scales)[row * a.groups + (o >> 2)]);
+#pragma unroll
+      for (int d = 0; d < 8; ++d) k[d] = q4::value_of(kw, d, ks), v[d] = q4::value_of(vw, d, vs);
+    }
+    const int64_t dst = (r * a.words + o) * 8;
+    store8(static_cast<T*>(a.k_out) + dst, k);
+    store8(static_cast<T*>(a.v_out) + dst, v);
+  }
+}
+
+// Lanes of a row (a power of two that holds its units), and how many heads a lane walks over: as many as leave every SM
+// eight blocks, since each further head saves a lane its cos / sin loads.
+struct Shape {
+  int units, lanes, lane_shift, per_lane, chunks;
+  int64_t blocks;
+};
+Shape shape_of(int64_t D, int64_t rows, int64_t heads) {
+  Shape s;
+  s.units = static_cast<int>(D / 16);
+  s.lanes = 1, s.lane_shift = 0;
+  while (s.lanes < s.units) s.lanes <<= 1, ++s.lane_shift;
+  if (s.lanes < 2) s.lanes = 2, s.lane_shift = 1;
+  s.per_lane = 8;
+  while (s.per_lane > 1 && rows * ((heads + s.per_lane - 1) / s.per_lane) * s.lanes < static_cast<int64_t>(sm_count()) * 8 * 256) s.per_lane >>= 1;
+  s.chunks = static_cast<int>((heads + s.per_lane - 1) / s.per_lane);
+  s.blocks = (rows * s.chunks * s.lanes + 255) / 256;
+  return s;
+}
+
+bool strides8(int64_t a, int64_t b, int64_t c) { return a % 8 == 0 && b % 8 == 0 && c % 8 == 0; }
+
+int write_common(bool q4, void* q_out, const int64_t* qo, void* k_pool, void* k_scales, void* v_pool, void* v_scales, const void* q,
+                 const int64_t* qs, const void* k, const int64_t* ks, const void* v, const int64_t* vs, const void* q_weight,
+                 const void* k_weight, const float* table, int64_t table_rows, int64_t rotary_dim, const int32_t* block_table,
+                 const int32_t* offsets, const int32_t* rope_offsets, const int32_t* new_lens, int64_t B, int64_t H, int64_t Hkv,
+                 int64_t T, int64_t D, int64_t blocks_per_seq, int64_t block_size, int64_t num_blocks, double eps, int interleaved,
+                 int dtype, void* stream) {
+  OB_REQUIRE(B >= 0 && T >= 0 && H >= 0 && Hkv > 0 && D > 0 && blocks_per_seq >= 0 && block_size > 0 && num_blocks > 0, OASR_ERR_INVALID,
+             "write_kv_rope: bad shape");
+  OB_REQUIRE(H + 2 * Hkv <= 65535, OASR_ERR_INVALID, "write_kv_rope: head count too large");
+  OB_REQUIRE(D % 16 == 0 && D <= 512, OASR_ERR_UNSUPPORTED, "write_kv_rope: head_dim must be a multiple of 16 up to 512 (got %lld)", (long long)D);
+  OB_REQUIRE(!q4 || D % 32 == 0, OASR_ERR_UNSUPPORTED, "write_kv_rope_q4: head_dim must be a multiple of 32 (got %lld)", (long long)D);
+  OB_REQUIRE(rotary_dim > 0 && rotary_dim % 16 == 0 && rotary_dim <= D, OASR_ERR_UNSUPPORTED,
+             "write_kv_rope: rotary_dim must be a multiple of 16 up to head_dim (got %lld)", (long long)rotary_dim);
+  OB_REQUIRE(table_rows > 0, OASR_ERR_INVALID, "write_kv_rope: empty position table");
+  if (B == 0 || T == 0) return OASR_OK;
+  OB_REQUIRE(k_pool && v_pool && k && v && ks && vs && table && block_table && offsets && (!q4 || (k_scales && v_scales)) &&
+                 (H == 0 || (q && q_out && qs && qo)),
+             OASR_ERR_INVALID, "write_kv_rope: null pointer argument");
+  OB_REQUIRE(strides8(ks[0], ks[1], ks[2]) && strides8(vs[0], vs[1], vs[2]) &&
+                 (H == 0 || (strides8(qs[0], qs[1], qs[2]) && strides8(qo[0], qo[1], qo[2]))),
+             OASR_ERR_ALIGN, "write_kv_rope: strides must be multiples of 8 elements");
+  OB_REQUIRE(is_aligned(k_pool, 16) && is_aligned(v_pool, 16) && is_aligned(k, 16) && is_aligned(v, 16) && is_aligned(table, 16) &&
+                 (H == 0 || (is_aligned(q, 16) && is_aligned(q_out, 16))) && is_aligned(q_weight, 16) && is_aligned(k_weight, 16),
+             OASR_ERR_ALIGN, "write_kv_rope: operands must be 16-byte aligned");
+  const Shape s = shape_of(D, B * T, H + 2 * Hkv);
+  OB_REQUIRE(s.blocks <= 0x7fffffff, OASR_ERR_INVALID, "write_kv_rope: too many rows for one call");
+  static const int64_t kNone[3] = {0, 0, 0};
+  if (H == 0) qs = qo = kNone;
+  const WriteArgs a{q_out, k_pool, v_pool, k_scales, v_scales, q, k, v, q_weight, k_weight, table, block_table, offsets, rope_offsets, new_lens,
+                    table_rows, B, T, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], qo[0], qo[1], qo[2],
+                    blocks_per_seq, block_size, num_blocks, static_cast<int>(rotary_dim / 2), static_cast<int>(H), static_cast<int>(Hkv),
+                    s.units, s.lanes, s.lane_shift, s.per_lane, s.chunks, static_cast<int>(D / 32), 1.f / static_cast<float>(D),
+                    static_cast<float>(eps)};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const dim3 grid(static_cast<unsigned>(s.blocks));
+  return OB_DISPATCH_HALF(dtype, T_, [&]() -> int {
+    auto kern = q4 ? (interleaved ? write_kv_rope_kernel<T_, true, true> : write_kv_rope_kernel<T_, false, true>)
+                   : (interleaved ? write_kv_rope_kernel<T_, true, false> : write_kv_rope_kernel<T_, false, false>);
+    launch_pdl(kern, grid, dim3(256), 0, st, a);
+    return check_launch("write_kv_rope launch");
+  });
+}
+
+}  // namespace
+}  // namespace ob
+
+extern "C" {
+
+int oasr_b200_qk_norm_rope(void* q_out, void* k_out, const void* q, const void* k, const void* q_weight, const void* k_weight,
+                           const float* table, int64_t table_rows, int64_t rotary_dim, const void* positions, int pos_i64, int64_t N,
+                           int64_t H, int64_t Hkv, int64_t D, int64_t qs_n, int64_t qs_h, int64_t ks_n, int64_t ks_h, int64_t qo_n,
+                           int64_t qo_h, int64_t ko_n, int64_t ko_h, double eps, int interleaved, int dtype, void* stream) {
+  using namespace ob;
+  OB_REQUIRE(N >= 0 && H > 0 && Hkv >= 0 && D > 0, OASR_ERR_INVALID, "qk_norm_rope: bad shape");
+  OB_REQUIRE(H + Hkv <= 65535, OASR_ERR_INVALID, "qk_norm_rope: head count too large");
+  OB_REQUIRE(D % 16 == 0 && D <= 512, OASR_ERR_UNSUPPORTED, "qk_norm_rope: head_dim must be a multiple of 16 up to 512 (got %lld)", (long long)D);
+  OB_REQUIRE(rotary_dim > 0 && rotary_dim % 16 == 0 && rotary_dim <= D, OASR_ERR_UNSUPPORTED,
+             "qk_norm_rope: rotary_dim must be a multiple of 16 up to head_dim (got %lld)", (long long)rotary_dim);
+  OB_REQUIRE(table_rows > 0, OASR_ERR_INVALID, "qk_norm_rope: empty position table");
+  if (N == 0) return OASR_OK;
+  OB_REQUIRE(q && q_out && table && positions && (Hkv == 0 || (k && k_out)), OASR_ERR_INVALID, "qk_norm_rope: null pointer argument");
+  const int64_t e = dtype == OASR_DT_F32 ? 4 : 8;
+  OB_REQUIRE(qs_n % e == 0 && qs_h % e == 0 && ks_n % e == 0 && ks_h % e == 0 && qo_n % e == 0 && qo_h % e == 0 && ko_n % e == 0 && ko_h % e == 0,
+             OASR_ERR_ALIGN, "qk_norm_rope: strides must be multiples of 16 bytes");
+  OB_REQUIRE(is_aligned(q, 16) && is_aligned(k, 16) && is_aligned(q_out, 16) && is_aligned(k_out, 16) && is_aligned(table, 16) &&
+                 is_aligned(q_weight, 16) && is_aligned(k_weight, 16) && is_aligned(positions, pos_i64 ? 8 : 4),
+             OASR_ERR_ALIGN, "qk_norm_rope: operands must be 16-byte aligned");
+  const Shape s = shape_of(D, N, H + Hkv);
+  OB_REQUIRE(s.blocks <= 0x7fffffff, OASR_ERR_INVALID, "qk_norm_rope: too many rows for one call");
+  const QkArgs a{q_out, k_out, q, k, q_weight, k_weight, table, positions, table_rows, N, qs_n, qs_h, ks_n, ks_h, qo_n, qo_h, ko_n, ko_h,
+                 static_cast<int>(rotary_dim / 2), static_cast<int>(H), static_cast<int>(Hkv), s.units, s.lanes, s.lane_shift, s.per_lane,
+                 s.chunks, pos_i64, 1.f / static_cast<float>(D), static_cast<float>(eps)};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return OB_DISPATCH_FLOAT(dtype, T_, [&]() -> int {
+    launch_pdl(interleaved ? qk_norm_rope_kernel<T_, true> : qk_norm_rope_kernel<T_, false>, dim3(static_cast<unsigned>(s.blocks)), dim3(256), 0, st, a);
+    return check_launch("qk_norm_rope launch");
+  });
+}
+
+int oasr_b200_write_kv_rope(void* q_out, const int64_t* q_out_strides, void* k_pool, void* v_pool, const void* q, const int64_t* q_strides,
+                            const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, const void* q_weight,
+                            const void* k_weight, const float* table, int64_t table_rows, int64_t rotary_dim, const int32_t* block_table,
+                            const int32_t* offsets, const int32_t* rope_offsets, const int32_t* new_lens, int64_t B, int64_t H,
+                            int64_t Hkv, int64_t T, int64_t D, int64_t blocks_per_seq, int64_t block_size, int64_t num_blocks, double eps,
+                            int interleaved, int dtype, void* stream) {
+  return ob::write_common(false, q_out, q_out_strides, k_pool, nullptr, v_pool, nullptr, q, q_strides, k, k_strides, v, v_strides, q_weight,
+                          k_weight, table, table_rows, rotary_dim, block_table, offsets, rope_offsets, new_lens, B, H, Hkv, T, D,
+                          blocks_per_seq, block_size, num_blocks, eps, interleaved, dtype, stream);
+}
+
+int oasr_b200_write_kv_rope_q4(void* q_out, const int64_t* q_out_strides, void* k_codes, void* k_scales, void* v_codes, void* v_scales,
+                               const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                               const int64_t* v_strides, const void* q_weight, const void* k_weight, const float* table,
+                               int64_t table_rows, int64_t rotary_dim, const int32_t* block_table, const int32_t* offsets,
+                               const int32_t* rope_offsets, const int32_t* new_lens, int64_t B, int64_t H, int64_t Hkv, int64_t T,
+                               int64_t D, int64_t blocks_per_seq, int64_t block_size, int64_t num_blocks, double eps, int interleaved,
+                               int dtype, void* stream) {
+  return ob::write_common(true, q_out, q_out_strides, k_codes, k_scales, v_codes, v_scales, q, q_strides, k, k_strides, v, v_strides, q_weight,
+                          k_weight, table, table_rows, rotary_dim, block_table, offsets, rope_offsets, new_lens, B, H, Hkv, T, D,
+                          blocks_per_seq, block_size, num_blocks, eps, interleaved, dtype, stream);
+}
+
+int oasr_b200_paged_kv_gather_q4(void* k_out, void* v_out, const void* k_codes, const void* k_scales, const void* v_codes,
+                                 const void* v_scales, const int32_t* block_table, const int32_t* starts, int64_t B, int64_t Hkv, int64_t T,
+                                 int64_t D, int64_t blocks_per_seq, int64_t block_size, int64_t num_blocks, int dtype, void* stream) {
+  using namespace ob;
+  OB_REQUIRE(B >= 0 && T >= 0 && Hkv > 0 && D > 0 && blocks_per_seq >= 0 && block_size > 0 && num_blocks > 0, OASR_ERR_INVALID,
+             "paged_kv_gather_q4: bad shape");
+  OB_REQUIRE(D % 32 == 0 && D <= 512, OASR_ERR_UNSUPPORTED, "paged_kv_gather_q4: head_dim must be a multiple of 32 up to 512 (got %lld)", (long long)D);
+  if (B == 0 || T == 0) return OASR_OK;
+  OB_REQUIRE(k_out && v_out && k_codes && k_scales && v_codes && v_scales && block_table, OASR_ERR_INVALID,
+             "paged_kv_gather_q4: null pointer argument");
+  OB_REQUIRE(is_aligned(k_out, 16) && is_aligned(v_out, 16) && is_aligned(k_codes, 16) && is_aligned(v_codes, 16), OASR_ERR_ALIGN,
+             "paged_kv_gather_q4: operands must be 16-byte aligned");
+  const GatherArgs a{k_out, v_out, static_cast<const uint32_t*>(k_codes), static_cast<const uint32_t*>(v_codes), k_scales, v_scales, block_table, starts,
+                     B, Hkv, T, blocks_per_seq, block_size, num_blocks, static_cast<int>(D / 8), static_cast<int>(D / 32)};
+  const int64_t items = B * Hkv * T * a.words, cap = static_cast<int64_t>(sm_count()) * 16;
+  const unsigned grid = static_cast<unsigned>(items / 256 + 1 < cap ? items / 256 + 1 : cap);
+  return OB_DISPATCH_HALF(dtype, T_, [&]() -> int {
+    launch_pdl(gather_q4_kernel<T_>, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(stream), a);
+    return check_launch("paged_kv_gather_q4 launch");
+  });
+}
+
+}  // extern "C"

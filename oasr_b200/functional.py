@@ -10,7 +10,7 @@ honoured and returned), kernels run on the current CUDA stream.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple, Union
+from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
@@ -505,6 +505,134 @@ def gemm_log_softmax(A, B, C=None, out=None, *, out_dtype: Optional[torch.dtype]
     _lib.call("oasr_b200_gemm_log_softmax", _p(out), _p(A), _p(B), _p(C), M, N, K, _dt(A), _DTYPE_ID[out_dtype],
               _p(arg), _stream(A))
     return (out, arg) if return_argmax else out
+
+
+# ---------------------------------------------------------------------------
+# Decoding: rotary positions and scores (no reference operators)
+# ---------------------------------------------------------------------------
+def _same_device(ref: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    device = ref.get_device()
+    for t in others:
+        if t is not None and t.get_device() != device:
+            raise RuntimeError(f"all tensors must live on {ref.device}, got one on {t.device}")
+
+
+def rope_table(rows: int, rotary_dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
+    """Position table of the rotary operators, ``(rows, rotary_dim)`` fp32: the cosines of the ``rotary_dim / 2`` angles
+    ``position * base^(-2 i / rotary_dim)``, then their sines, from angles in 64 bits."""
+    if rows <= 0 or rotary_dim <= 0 or rotary_dim % 16:
+        raise ValueError(f"rope_table needs rows > 0 and rotary_dim a positive multiple of 16, got {rows}, {rotary_dim}")
+    rate = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
+    angle = torch.arange(rows, dtype=torch.float64, device=device)[:, None] * rate
+    return torch.cat([angle.cos(), angle.sin()], 1).float()
+
+
+def _check_rope_table(table: torch.Tensor, head_dim: int) -> None:
+    if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous():
+        raise RuntimeError("cos_sin must be a contiguous fp32 (positions, rotary_dim) table (rope_table)")
+    if table.size(1) > head_dim:
+        raise RuntimeError(f"rotary_dim {table.size(1)} is more than the head_dim {head_dim}")
+
+
+def _check_head_weight(ref: torch.Tensor, head_dim: int, **weights) -> None:
+    for name, w in weights.items():
+        if w is not None and (w.shape != (head_dim,) or w.dtype != ref.dtype or not w.is_contiguous()):
+            raise RuntimeError(f"{name} must be a contiguous ({head_dim},) tensor of {ref.dtype}")
+
+
+def qk_norm_rope(q, k, cos_sin, positions, q_weight=None, k_weight=None, *, eps: float = 1e-6, interleaved: bool = False,
+                 q_out=None, k_out=None):
+    """RMS norm of every head of ``q (N, H, D)`` and ``k (N, H_kv, D)``, then their rotation at ``positions (N,)``, in one pass;
+    returns ``(q, k)``.
+
+    ``cos_sin`` is a ``rope_table``; its width says how many leading dims turn, in pairs ``(i, i + R / 2)`` or, ``interleaved``,
+    ``(2 i, 2 i + 1)``.  A weight of None leaves that norm out.  Inputs may be views of one fused projection (unit stride along
+    D); results are new contiguous tensors unless ``q_out`` / ``k_out`` are given, which may be ``q`` / ``k`` themselves.  A
+    position outside the table gives a zero row.  ``k`` may be None."""
+    _need_cuda(q, k, cos_sin, positions, q_weight, k_weight, q_out, k_out)
+    _same_device(q, k, cos_sin, positions, q_weight, k_weight, q_out, k_out)
+    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.size(0) != q.size(0) or k.size(2) != q.size(2))):
+        raise RuntimeError("qk_norm_rope expects q (N, H, D) and k (N, H_kv, D)")
+    N, H, D = q.shape
+    Hkv = 0 if k is None else k.size(1)
+    _check_rope_table(cos_sin, D)
+    if positions.shape != (N,) or positions.dtype not in (torch.int32, torch.int64) or not positions.is_contiguous():
+        raise RuntimeError(f"positions must be a contiguous int32 or int64 ({N},) tensor")
+    _check_head_weight(q, D, q_weight=q_weight, k_weight=k_weight)
+    if k is None and (k_out is not None or k_weight is not None):
+        raise RuntimeError("k_out and k_weight need k")
+    if q_out is None:
+        q_out = torch.empty((N, H, D), dtype=q.dtype, device=q.device)
+    if k_out is None and k is not None:
+        k_out = torch.empty((N, Hkv, D), dtype=q.dtype, device=q.device)
+    _same_dtype(q, k=k, q_out=q_out, k_out=k_out)
+    if q_out.shape != q.shape or (k is not None and k_out.shape != k.shape):
+        raise RuntimeError("q_out and k_out must have the shapes of q and k")
+    for t in (q, k, q_out, k_out):
+        if t is not None and t.stride(2) != 1 and D > 1:
+            raise RuntimeError("qk_norm_rope needs unit stride along head_dim")
+    _check_distinct_rows(q_out=q_out, k_out=k_out)
+    ks_n, ks_h, ko_n, ko_h = (0, 0, 0, 0) if k is None else (k.stride(0), k.stride(1), k_out.stride(0), k_out.stride(1))
+    _lib.call("oasr_b200_qk_norm_rope", _p(q_out), _p(k_out), _p(q), _p(k), _p(q_weight), _p(k_weight), _p(cos_sin),
+              cos_sin.size(0), cos_sin.size(1), _p(positions), int(positions.dtype == torch.int64), N, H, Hkv, D,
+              q.stride(0), q.stride(1), ks_n, ks_h, q_out.stride(0), q_out.stride(1), ko_n, ko_h, float(eps),
+              int(bool(interleaved)), _dt(q), _stream(q))
+    return q_out, k_out
+
+
+def _check_distinct_rows(**outs) -> None:
+    """An output whose rows share memory (an expanded view) has no single result."""
+    for name, t in outs.items():
+        if t is None or t.is_contiguous():
+            continue
+        for extent, stride in sorted(zip(t.shape[:-1], t.stride()[:-1]), key=lambda p: p[1]):
+            if extent > 1 and stride < t.size(-1):
+                raise RuntimeError(f"{name} must not overlap itself")
+
+
+class TokenLogProbs(NamedTuple):
+    """What ``token_log_probs`` returns; None for what was not asked."""
+
+    log_probs: Optional[torch.Tensor]
+    entropy: Optional[torch.Tensor]
+    top_log_probs: Optional[torch.Tensor]
+    top_ids: Optional[torch.Tensor]
+
+
+def token_log_probs(logits, tokens=None, *, top_k: int = 0, entropy: bool = True) -> TokenLogProbs:
+    """Log-probs of given tokens, entropy (nats) and the ``top_k`` likeliest alternatives of every row of ``logits
+    (..., V)``, in one pass over them (fp32 arithmetic and results).
+
+    ``tokens`` is ``(...)`` (one a row) or ``(..., n)``, int32 or int64; a token outside ``[0, V)`` is padding and scores 0.
+    Alternatives are ordered by value, equal values by lowest id (``top_k`` up to 32; NaN ranks first).  Rows may lie apart
+    (``logits[:, :V]`` of a head with padded columns).  -inf logits are impossible tokens; a row of nothing else has
+    log-probs of -inf and entropy 0.  ``V`` is at most 262144."""
+    _need_cuda(logits, tokens)
+    _same_device(logits, tokens)
+    if logits.dim() < 1 or logits.size(-1) < 1:
+        raise RuntimeError("token_log_probs expects logits (..., V)")
+    lead, V = logits.shape[:-1], logits.size(-1)
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    if x.stride(1) != 1 and V > 1 or (x.size(0) > 1 and x.stride(0) < V):
+        x = x.contiguous()
+    rows = x.size(0)
+    n, log_probs = 0, None
+    if tokens is not None:
+        if tokens.dtype not in (torch.int32, torch.int64):
+            raise RuntimeError(f"tokens must be int32 or int64, got {tokens.dtype}")
+        if tokens.shape != lead and (tokens.dim() == 0 or tokens.shape[:-1] != lead):
+            raise RuntimeError(f"tokens must be {tuple(lead)} or {tuple(lead)} + (n,), got {tuple(tokens.shape)}")
+        n = 1 if tokens.shape == lead else tokens.size(-1)
+        tokens = tokens.contiguous()
+        log_probs = torch.empty(tokens.shape, dtype=torch.float32, device=x.device)
+    ent = torch.empty(lead, dtype=torch.float32, device=x.device) if entropy else None
+    top_lp = top_ids = None
+    if top_k:
+        top_lp = torch.empty(lead + (top_k,), dtype=torch.float32, device=x.device)
+        top_ids = torch.empty(lead + (top_k,), dtype=torch.int32, device=x.device)
+    _lib.call("oasr_b200_token_log_probs", _p(log_probs), _p(ent), _p(top_lp), _p(top_ids), _p(x), _p(tokens),
+              int(n > 0 and tokens.dtype == torch.int64), rows, V, x.stride(0) if rows > 1 else V, n, int(top_k), _dt(x), _stream(x))
+    return TokenLogProbs(log_probs, ent, top_lp, top_ids)
 
 
 def device_status(device=None) -> int:
