@@ -375,6 +375,28 @@ def test_fmha_q4_unseen_keys_say_nothing(dtype, T):
     close(got, want, HALF[dt], float(top * (HALF[dt] + 20 * D * 2.0 ** -24)))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [3, 40, 200])
+def test_fmha_q4_nan_reaches_the_rows_that_see_it_and_no_other(T, D):
+    """NaN keys and values inside the length, seen by the later rows of a causal chunk only, and a NaN query."""
+    block, N = 16, T + 70
+    bt, n = pages(3, 1, -(-N // block))
+    pools = q4_pool(10, n, 2, block, D, torch.bfloat16)
+    k, v, _ = dense64(pools, bt)
+    q = rand(12, 1, 4, T, D).bfloat16().cuda()
+    q[0, 1, 0] = math.nan
+    at = N - 2                                           # the last row and the one before it see this key
+    pools[3][bt[0, at // block], 1, at % block, 1] = math.nan     # values of key head 1: dims 32..63
+    pools[1][bt[0, at // block], 0, at % block, 0] = math.nan     # keys of key head 0
+    got = ob.fmha_q4(q, *pools, softmax_scale=0.125, block_table=bt.cuda(), cache_seqlens=torch.tensor([N], device="cuda"), causal=True).cpu().double()
+    want = attend64(q.nan_to_num(0).cpu().double(), k, v, 0.125, [N], None, None, True)
+    want[0, 1, 0] = math.nan
+    want[0, :2, T - 2:] = math.nan
+    want[0, 2:, T - 2:, 32:64] = math.nan
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    close(got.nan_to_num(0), want.nan_to_num(0), 2.0 ** -8, float(v.abs().max() * (2.0 ** -8 + 20 * D * 2.0 ** -24)))
+
+
 @pytest.mark.parametrize("T", [1, 40])
 def test_fmha_q4_of_large_and_small_scores(T):
     """Scores of thousands (one key has all the weight) and of nothing (all have the same)."""
