@@ -9,16 +9,23 @@
 // so a single token wastes 7 of 8 columns and not 15 of 16 rows, and a code needs no transpose: as MMA operands' row, column
 // and contraction orders are free, each lane takes whole 32-bit words of codes of whichever keys and dims its fragment stands
 // for.  Per 32 keys of a warp, with g = lane / 4 and t = lane % 4:
-//   K   the lane holds words t G .. t G + G - 1 (an octet of each group) of keys 4 g .. 4 g + 3.  The operand is the code with
-//       a magic exponent in front, 128 + n in bf16 (1024 + n in fp16): one LOP3 per two codes, exact.  The offset comes off in
-//       the accumulator, which starts at -136 (-1032) sum(q) of the group; a group's sums are scaled in fp32 afterwards.
-//   V   the lane holds words of keys 8 t .. 8 t + 7.  Long sums would drown under such an offset, so here the operand is
-//       (n - 8) * scale, exact in the type (q4.cuh).
+//   K   the lane holds words t G .. t G + G - 1 (an octet of each group) of keys g + 8 x.  The operand, fp16 for either
+//       type, is the code behind a magic exponent: 1024 + n where the nibble lies lowest, 1024 + 16 n where it lies second, one
+//       LOP3 per two codes and a shift per four, exact.  The queries carry what that needs: each row is brought to 2^10 by a power of two (bf16
+//       reaches further than fp16; exact but for what is 2^-34 of the row's largest), every second dim by 1 / 16 more.  The
+//       offsets come off in the accumulator, which starts at -(1032 sum of even + 72 sum of odd q) of the group; a group's
+//       sums are scaled in fp32 afterwards.
+//   V   the lane holds words g D / 64 (+ 1) of keys 8 x + 2 t and 8 x + 2 t + 1.  Long sums would drown under such an offset, so here the operand is
+//       (n - 8) * scale, exact in the type (q4.cuh).  In bf16 the second nibble has no room behind an exponent: left alone it is
+//       the number n 2^-129 (gradual underflow joins the normal numbers at n = 8), which one FMA takes to (n - 8) / 4.
 //   P   the scores' fragment is the transpose of what the second product reads: movmatrix.
+// The ALU (logic, shifts, permutes: half a warp instruction a clock) is the busiest unit; the FMA pipe, which does the rest of the
+// conversion, is not.
 // The running maximum moves only when a score passes it by 2^8 (weights stay below that, exact in either type): most tiles
 // need one vote in the place of a reduction over the lanes.
-// Every warp walks its own tiles with its own maximum, sum and output; the warps of a block, and the blocks of a cluster that
-// share one (sequence, key head, rows), meet in shared memory at the end.
+// Every warp walks its own tiles with its own maximum, sum and output, and has its own ring of tiles in shared memory, filled by
+// asynchronous copies (a tile is two runs of 16 keys of a page): no registers wait for memory, no warp for another.  One, two or four
+// warps of a block, or the blocks of a cluster, share a (sequence, key head, rows) and meet in shared memory at the end.
 #include "common.cuh"
 #include "q4.cuh"
 #include "sm100_ptx.cuh"
@@ -41,24 +48,47 @@ struct Args {
 
 constexpr int kWarps = 4;
 
+constexpr float kEmpty = -3e38f;   // a maximum below every score: differences to it overflow to -inf or are zero, never NaN
+
+__device__ __forceinline__ uint32_t half2_bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+__device__ __forceinline__ uint32_t bf162_bits(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+__device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
+
+constexpr uint32_t kLow = 0x000f000fu, kSecond = 0x00f000f0u, kMagic16 = 0x64006400u;   // 1024 in fp16
+
+// (w & mask) | magic in one instruction
+__device__ __forceinline__ uint32_t behind(uint32_t w, uint32_t mask, uint32_t magic) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
+  return r;
+}
+
+// S = A B + C in fp16 with fp32 accumulators
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t* a, uint32_t b0, uint32_t b1, const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
+// The second product's operands.  `low` / `second`: the codes of two keys (one in each half) at bits 0..3 / 4..7, times the
+// keys' scales; `steep`: what second() wants for the scales.
 template <typename T>
 struct Op;
 template <>
 struct Op<__nv_bfloat16> {
-  static constexpr uint32_t kMagic = 0x43004300u;   // 128
-  static constexpr float kBias = 136.f;
-  static __device__ __forceinline__ uint32_t centred(uint32_t w) {   // (128 + n) - 136
-    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&w), __nv_bfloat162(__float2bfloat16_rn(136.f), __float2bfloat16_rn(136.f)));
-    return *reinterpret_cast<const uint32_t*>(&v);
+  static __device__ __forceinline__ uint32_t low(uint32_t w, uint32_t scale) {   // ((128 + n) - 136) s
+    const __nv_bfloat162 v = __hsub2(as_bf162(behind(w, kLow, 0x43004300u)), as_bf162(0x43084308u));
+    return bf162_bits(__hmul2(v, as_bf162(scale)));
   }
-  static __device__ __forceinline__ uint32_t mul(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&v);
+  static __device__ __forceinline__ uint32_t steep(uint32_t scale) { return bf162_bits(__hmul2(as_bf162(scale), as_bf162(0x40804080u))); }   // 4 s: finite
+  static __device__ __forceinline__ uint32_t second(uint32_t w, uint32_t steep) {   // (n 2^-129 2^127 - 2) 4 s
+    const __nv_bfloat162 v = __hfma2(as_bf162(w & kSecond), as_bf162(0x7f007f00u), as_bf162(0xc000c000u));
+    return bf162_bits(__hmul2(v, as_bf162(steep)));
   }
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
+  static __device__ __forceinline__ float low_f(uint32_t w) { return __uint_as_float(w << 16); }
+  static __device__ __forceinline__ float high_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return bf162_bits(__floats2bfloat162_rn(lo, hi)); }
   static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -66,20 +96,18 @@ struct Op<__nv_bfloat16> {
 };
 template <>
 struct Op<__half> {
-  static constexpr uint32_t kMagic = 0x64006400u;   // 1024
-  static constexpr float kBias = 1032.f;
-  static __device__ __forceinline__ uint32_t centred(uint32_t w) {
-    const __half2 v = __hsub2(*reinterpret_cast<__half2*>(&w), __half2(__float2half_rn(1032.f), __float2half_rn(1032.f)));
-    return *reinterpret_cast<const uint32_t*>(&v);
+  static __device__ __forceinline__ uint32_t low(uint32_t w, uint32_t scale) {   // ((1024 + n) - 1032) s
+    const __half2 v = __hsub2(as_half2(behind(w, kLow, kMagic16)), as_half2(0x64086408u));
+    return half2_bits(__hmul2(v, as_half2(scale)));
   }
-  static __device__ __forceinline__ uint32_t mul(uint32_t a, uint32_t b) {
-    const __half2 v = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&v);
+  static __device__ __forceinline__ uint32_t steep(uint32_t scale) { return scale; }
+  static __device__ __forceinline__ uint32_t second(uint32_t w, uint32_t scale) {   // ((1024 + 16 n) / 16 - 72) s
+    const __half2 v = __hfma2(as_half2(behind(w, kSecond, kMagic16)), as_half2(0x2c002c00u), as_half2(0xd480d480u));
+    return half2_bits(__hmul2(v, as_half2(scale)));
   }
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
+  static __device__ __forceinline__ float low_f(uint32_t w) { return __low2float(as_half2(w)); }
+  static __device__ __forceinline__ float high_f(uint32_t w) { return __high2float(as_half2(w)); }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return half2_bits(__floats2half2_rn(lo, hi)); }
   static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -100,55 +128,56 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
 __device__ __forceinline__ uint32_t lows(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
 __device__ __forceinline__ uint32_t highs(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
 
-template <int G>
-struct KTile {           // keys 4 g .. 4 g + 3
-  uint32_t w[4][G];
-  uint32_t s[4 * G / 2];  // their scales, two to a word
-};
-template <int G>
-struct VTile {           // keys 8 t .. 8 t + 7
-  uint32_t w[8][G / 2];
-  uint32_t s[8 * G / 2];
-};
-
+__device__ __forceinline__ void copy16(uint32_t dst, uint64_t src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 template <int N>
-__device__ __forceinline__ void ldg(const void* p, uint32_t* r) {
-  if constexpr (N == 1) {
-    r[0] = __ldg(static_cast<const uint32_t*>(p));
-  } else if constexpr (N == 2) {
-    const uint2 v = __ldg(static_cast<const uint2*>(p));
-    r[0] = v.x, r[1] = v.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-      const uint4 v = __ldg(static_cast<const uint4*>(p) + i);
-      r[4 * i] = v.x, r[4 * i + 1] = v.y, r[4 * i + 2] = v.z, r[4 * i + 3] = v.w;
-    }
-  }
+__device__ __forceinline__ void copies_but() {   // all but the last N groups of copies have landed
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void lds(uint32_t p, uint32_t* r) {
+  if constexpr (N == 1) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(p));
+  else if constexpr (N == 2) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(p));
+  else asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p));
 }
 
-template <typename T, int D, int NT>
+// A tile of 32 keys in the ring: codes of K and V, then their scales.  In rows of 64 bytes the upper two 16-byte pieces of every
+// second pair of rows change places with the lower two, which halves the V reads' bank conflicts (their rows are 2 t apart).
+template <int D>
+struct Tile {
+  static constexpr int kRow = D / 2, kCodes = 32 * kRow, kScales = 32 * (D / 32) * 2;
+  static constexpr int kK = 0, kV = kCodes, kKs = 2 * kCodes, kVs = 2 * kCodes + kScales, kBytes = 2 * kCodes + 2 * kScales;
+  static constexpr int kStages = D == 64 ? 4 : 3;
+  static __device__ __forceinline__ int at(int row, int byte) { return row * kRow + (D == 128 ? byte ^ ((row & 2) << 4) : byte); }
+};
+
+template <int D, int NT>
 struct Merge {   // a warp's, and then the block's, maxima, sums and outputs
   float m[kWarps][8 * NT], l[kWarps][8 * NT];
   float o[kWarps][8 * NT][D + 4];
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32) fmha_q4_kernel(const Args a, const int parts, const int row_blocks) {
-  constexpr int G = D / 32, W = D / 8, VW = G / 2;   // words of a row, of them a lane's in V
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : NT == 2 ? (D == 64 ? 4 : 3) : 2)
+fmha_q4_kernel(const Args a, const int parts, const int ways, const int row_blocks, const int groups) {
+  constexpr int G = D / 32, VW = G / 2;   // groups of a row; words of a V row that a lane holds
   constexpr int NR = 8 * NT;
+  using Ring = Tile<D>;
   extern __shared__ __align__(16) uint8_t smem[];
-  Merge<T, D, NT>& sh = *reinterpret_cast<Merge<T, D, NT>*>(smem);
+  Merge<D, NT>& sh = *reinterpret_cast<Merge<D, NT>*>(smem);   // after the walk, in the rings' place
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int part = blockIdx.x % parts;
-  int at = blockIdx.x / parts;
+  // `ways` warps of the block share a group (sequence, key head, rows)
+  const int group = static_cast<int>(blockIdx.x / parts) * (kWarps / ways) + warp / ways, way = warp % ways;
+  int at = min(group, groups - 1);
   const int rb = at % row_blocks;
   at /= row_blocks;
   const int hk = at % a.Hkv, b = at / a.Hkv;
   const int share = a.H / a.Hkv;
-  const int rows = share * a.Tq, row0 = rb * NR;
+  const int rows = group < groups ? share * a.Tq : 0, row0 = rb * NR;
   const int len = a.seqlens[b], q_len = a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq;
   const int capacity = static_cast<int>(a.blocks_per_seq * a.block_size);
   const int start = a.seqstarts ? max(a.seqstarts[b], 0) : 0;
@@ -175,128 +204,168 @@ __global__ void __launch_bounds__(kWarps * 32) fmha_q4_kernel(const Args a, cons
 
   // ---- queries as the second operand: column g, dims of octet t of each group
   uint32_t qf[NT][G][4];
-  float bias[NT][G][2];
+  float bias[NT][G][4], unit[NT][2];   // `unit` takes a column's sums to scores in the log2 domain
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int r = row0 + n * 8 + g;
     const T* q = static_cast<const T*>(a.q) + b * a.qs_b + (hk * share + r % share) * a.qs_h + static_cast<int64_t>(r / share) * a.qs_t;
+    Pack<T> x[G];
+    float top = 0.f;
 #pragma unroll
     for (int k = 0; k < G; ++k) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r < rows) v = *reinterpret_cast<const uint4*>(q + k * 32 + t * 8);
-      const T* x = reinterpret_cast<const T*>(&v);
-      float sum = 0.f;
+      if (r < rows) x[k] = ld128(q + k * 32 + t * 8);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += Elem<T>::to_f(x[i]);
+      for (int i = 0; i < 8; ++i) {
+        if (r >= rows) x[k].v[i] = Elem<T>::from_f(0.f);
+        top = q4::max_nan(top, fabsf(Elem<T>::to_f(x[k].v[i])));
+      }
+    }
+    top = q4::max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = q4::max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int e = max(static_cast<int>(__float_as_uint(top) >> 23) & 255, 12);   // biased exponent of the row's largest
+    const float lift = __uint_as_float(static_cast<uint32_t>(264 - e) << 23);     // 2^(137 - e)
+    const float down = __uint_as_float(static_cast<uint32_t>(max(e - 10, 1)) << 23) * fabsf(a.scale_log2);
+    unit[n][0] = fmaxf(__shfl_sync(0xffffffffu, down, 8 * t), 1.2e-38f);           // a scale of zero leaves masked scores at -inf
+    unit[n][1] = fmaxf(__shfl_sync(0xffffffffu, down, 8 * t + 4), 1.2e-38f);
+    const float signed_lift = a.scale_log2 < 0.f ? -lift : lift;
+#pragma unroll
+    for (int k = 0; k < G; ++k) {
+      float y[8], sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        y[i] = __half2float(__float2half_rn(Elem<T>::to_f(x[k].v[i]) * signed_lift));
+        sum = fmaf(y[i], i & 1 ? -72.f : -1032.f, sum);
+      }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      bias[n][k][0] = -Op<T>::kBias * __shfl_sync(0xffffffffu, sum, 8 * t);
-      bias[n][k][1] = -Op<T>::kBias * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
-      qf[n][k][0] = lows(v.x, v.z), qf[n][k][1] = highs(v.x, v.z);   // dims (0, 4), (1, 5) of the octet
-      qf[n][k][2] = lows(v.y, v.w), qf[n][k][3] = highs(v.y, v.w);   // (2, 6), (3, 7)
+      bias[n][k][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+      bias[n][k][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+      // an accumulator of its own, so that it is not put together from two registers for every tile
+      asm("mov.b32 %0, %2;\n\tmov.b32 %1, %3;" : "=f"(bias[n][k][2]), "=f"(bias[n][k][3]) : "f"(bias[n][k][0]), "f"(bias[n][k][1]));
+      qf[n][k][0] = half2_bits(__floats2half2_rn(y[0], y[4]));
+      qf[n][k][1] = half2_bits(__floats2half2_rn(y[1] * 0.0625f, y[5] * 0.0625f));
+      qf[n][k][2] = half2_bits(__floats2half2_rn(y[2], y[6]));
+      qf[n][k][3] = half2_bits(__floats2half2_rn(y[3] * 0.0625f, y[7] * 0.0625f));
     }
   }
 
   float o[NT][VW * 4][4] = {}, m[NT][2], l[NT][2];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
+  for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = kEmpty, l[n][0] = l[n][1] = 0.f;
 
-  const int units = static_cast<int>(a.block_size) / 16;   // halves of a tile are 16 keys of one page
+  // A tile's halves are 16 keys of one page each: half h of tile i is unit 2 i + h, in block (2 i + h) / units of the table.  The
+  // walk keeps quotient and remainder, and looks a block up two tiles ahead.
+  const int units = static_cast<int>(a.block_size) / 16, table_len = static_cast<int>(a.blocks_per_seq);
   const int32_t* table = a.block_table + b * a.blocks_per_seq;
-  const int step = kWarps * parts;
+  const int step = ways * parts, step_blocks = 2 * step / units, step_units = 2 * step - step_blocks * units;
   const int tile_end = (end + 31) / 32;
-  int tile = start / 32 + part * kWarps + warp;
-
-  // pages of a tile's two halves; -1: none
-  auto pages_of = [&](int i, int& p0, int& p1) {
-    p0 = p1 = -1;
-    if (i >= tile_end) return;
-    const int u = 2 * i, blk = u / units;
-    p0 = table[blk];                                                  // u * 16 < end <= capacity
-    const int blk1 = u + 1 - blk * units < units ? blk : blk + 1;
-    if (blk1 < a.blocks_per_seq) p1 = blk1 == blk ? p0 : table[blk1];
-    if (p0 < 0 || p0 >= a.num_blocks) p0 = -1;
-    if (p1 < 0 || p1 >= a.num_blocks) p1 = -1;
+  int tile = start / 32 + part * ways + way;
+  struct Place {
+    int page0, page1;   // as the table has them
+    int unit;           // of the first half in its block; the second's is the next one, or the next block's first
   };
-  // first row of the half's 16 keys; a half without a page reads page 0 and is masked
-  auto row_of = [&](int i, int half, int page) {
-    const int u = 2 * i + half;
-    return (static_cast<int64_t>(max(page, 0)) * a.Hkv + hk) * a.block_size + (u % units) * 16;
+  int ahead_block = 2 * tile / units, ahead_unit = 2 * tile - ahead_block * units;
+  auto look_ahead = [&]() {   // the place of the next tile of the walk
+    Place p;
+    p.unit = ahead_unit;
+    const int block1 = ahead_block + (ahead_unit + 1 == units);
+    p.page0 = ahead_block < table_len ? __ldg(table + ahead_block) : -1;
+    p.page1 = block1 < table_len ? __ldg(table + block1) : -1;
+    ahead_block += step_blocks;
+    ahead_unit += step_units;
+    if (ahead_unit >= units) ahead_unit -= units, ++ahead_block;
+    return p;
   };
-  KTile<G> kt;
-  VTile<G> vt;
-  auto load_k = [&](int i, int p0, int p1) {
-    const int half = g >> 2;
-    const int64_t row = row_of(i, half, half ? p1 : p0) + (g & 3) * 4;
+  auto known = [&](int page) { return static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_blocks); };
+  // copies of a tile: a half's codes are one run of 16 rows, its scales another
+  const uint32_t ring = ptx::smem_u32(smem) + warp * (Ring::kStages * Ring::kBytes);
+  constexpr int kPieces = Ring::kCodes / 2 / 16;      // of a half: 32 or 64
+  const uint32_t to = Ring::at(lane * 16 / Ring::kRow, lane * 16 % Ring::kRow);
+  constexpr int kScalePieces = Ring::kScales / 16;    // of a tile's K or V: 8 or 16 lanes
+  const bool scale_lane = lane < 2 * kScalePieces, scale_half = lane % kScalePieces >= kScalePieces / 2;
+  const uint64_t k_codes = reinterpret_cast<uint64_t>(a.k_codes) + lane * 16, v_codes = reinterpret_cast<uint64_t>(a.v_codes) + lane * 16;
+  const uint64_t scales = reinterpret_cast<uint64_t>(lane >= kScalePieces ? a.v_scales : a.k_scales) + lane % (kScalePieces / 2) * 16;
+  const uint32_t page_bytes = a.Hkv * static_cast<uint32_t>(a.block_size) * Ring::kRow, head_bytes = hk * static_cast<uint32_t>(a.block_size) * Ring::kRow;
+  uint32_t there = 0;   // two bits a tile in the ring: its halves have pages
+  auto fetch = [&](const Place& p, uint32_t stage) {
+    // a half without a page reads page 0 and is masked
+    const bool k0 = known(p.page0), k1 = known(p.page1);
+    const int unit1 = p.unit + 1 == units ? 0 : p.unit + 1;
+    const uint64_t o0 = static_cast<uint64_t>(k0 ? static_cast<uint32_t>(p.page0) : 0u) * page_bytes + (head_bytes + static_cast<uint32_t>(p.unit) * (16 * Ring::kRow));
+    const uint64_t o1 = static_cast<uint64_t>(k1 ? static_cast<uint32_t>(p.page1) : 0u) * page_bytes + (head_bytes + static_cast<uint32_t>(unit1) * (16 * Ring::kRow));
 #pragma unroll
-    for (int x = 0; x < 4; ++x) ldg<G>(a.k_codes + (row + x) * W + t * G, kt.w[x]);
-    ldg<2 * G>(static_cast<const T*>(a.k_scales) + row * G, kt.s);
+    for (int i = 0; i < kPieces / 32; ++i) {          // 512 bytes further: 8 or 16 rows, the same place in the row
+      copy16(stage + Ring::kK + to + i * 512, k_codes + o0 + i * 512);
+      copy16(stage + Ring::kK + to + Ring::kCodes / 2 + i * 512, k_codes + o1 + i * 512);
+      copy16(stage + Ring::kV + to + i * 512, v_codes + o0 + i * 512);
+      copy16(stage + Ring::kV + to + Ring::kCodes / 2 + i * 512, v_codes + o1 + i * 512);
+    }
+    if (scale_lane) copy16(stage + Ring::kKs + lane * 16, scales + ((scale_half ? o1 : o0) >> 3));   // a row has an eighth of its codes' bytes
+    there |= (k0 ? 1u : 0u) << (2 * Ring::kStages - 2) | (k1 ? 2u : 0u) << (2 * Ring::kStages - 2);
   };
-  auto load_v = [&](int i, int p0, int p1) {
-    const int half = t >> 1;
-    const int64_t row = row_of(i, half, half ? p1 : p0) + (t & 1) * 8;
-#pragma unroll
-    for (int x = 0; x < 8; ++x) ldg<VW>(a.v_codes + (row + x) * W + g * VW, vt.w[x]);
-    ldg<4 * G>(static_cast<const T*>(a.v_scales) + row * G, vt.s);
-  };
+  auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
 
-  int p0, p1, n0, n1;
-  pages_of(tile, p0, p1);
-  pages_of(tile + step, n0, n1);
-  if (tile < tile_end) {
-    load_k(tile, p0, p1);
-    load_v(tile, p0, p1);
+  Place next = look_ahead();
+#pragma unroll
+  for (int i = 0; i < Ring::kStages - 1; ++i) {
+    there >>= 2;
+    if (tile + i * step < tile_end) fetch(next, ring + i * Ring::kBytes);
+    commit();
+    next = look_ahead();
   }
+  const uint32_t k_lane = g * Ring::kRow + Ring::at(g, t * (G * 4)) % Ring::kRow;
+  const uint32_t v_lane = 2 * t * Ring::kRow + Ring::at(2 * t, g * (VW * 4)) % Ring::kRow;
+  uint32_t stage = ring, free_stage = ring + (Ring::kStages - 1) * Ring::kBytes;
   for (; tile < tile_end; tile += step) {
+    copies_but<Ring::kStages - 2>();
+    __syncwarp();                                      // the tile is there for all lanes, and the last one is read by all
+    there >>= 2;
+    if (tile + (Ring::kStages - 1) * step < tile_end) fetch(next, free_stage);
+    commit();
+    next = look_ahead();
     const int j0 = tile * 32;
-    const bool whole = j0 >= start && j0 + 32 <= all_end && p0 >= 0 && p1 >= 0;   // nothing to mask
-    int f0, f1;
-    pages_of(tile + 2 * step, f0, f1);
+    const bool whole = j0 >= start && j0 + 32 <= all_end && (there & 3) == 3;   // nothing to mask
 
-    // ---- scores of keys 4 g + 2 i (+ 1), columns 2 t (+ 1)
-    float s[NT][2][4] = {};
+    // ---- scores: m-tile i has keys 16 i + g and 16 i + 8 + g, columns 2 t (+ 1)
+    float s[NT][2][4];
 #pragma unroll
-    for (int k = 0; k < G; ++k) {
+    for (int i = 0; i < 2; ++i) {
+      uint32_t kw[2][G], ks[2][G / 2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float sc[2];   // scales of keys 4 g + 2 i, 4 g + 2 i + 1
+      for (int x = 0; x < 2; ++x) {
+        const int row = 16 * i + 8 * x;
+        lds<G>(stage + k_lane + (Ring::kK + row * Ring::kRow), kw[x]);
+        lds<G / 2>(stage + g * (G * 2) + (Ring::kKs + row * (G * 2)), ks[x]);
+      }
+#pragma unroll
+      for (int k = 0; k < G; ++k) {
+        float sc[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const int e = (2 * i + x) * G + k;
-          const uint32_t w = kt.s[e / 2];
-          const unsigned short h = static_cast<unsigned short>(e & 1 ? w >> 16 : w);
-          sc[x] = Elem<T>::to_f(*reinterpret_cast<const T*>(&h)) * a.scale_log2;
+          sc[x] = k & 1 ? Op<T>::high_f(ks[x][k / 2]) : Op<T>::low_f(ks[x][k / 2]);
         }
-        const uint32_t wa = kt.w[2 * i][k], wb = kt.w[2 * i + 1][k];
-        uint32_t af[8];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          af[2 * n] = ((wa >> (4 * n)) & 0x000f000fu) | Op<T>::kMagic;
-          af[2 * n + 1] = ((wb >> (4 * n)) & 0x000f000fu) | Op<T>::kMagic;
-        }
+        const uint32_t wa = kw[0][k], wb = kw[1][k], ha = wa >> 8, hb = wb >> 8;
+        const uint32_t af[8] = {behind(wa, kLow, kMagic16), behind(wb, kLow, kMagic16), behind(wa, kSecond, kMagic16), behind(wb, kSecond, kMagic16),
+                                behind(ha, kLow, kMagic16), behind(hb, kLow, kMagic16), behind(ha, kSecond, kMagic16), behind(hb, kSecond, kMagic16)};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          float c[4] = {bias[n][k][0], bias[n][k][1], bias[n][k][0], bias[n][k][1]};
-          Op<T>::mma(c, af[0], af[1], af[2], af[3], qf[n][k][0], qf[n][k][1]);
-          Op<T>::mma(c, af[4], af[5], af[6], af[7], qf[n][k][2], qf[n][k][3]);
-          s[n][i][0] = fmaf(sc[0], c[0], s[n][i][0]);
-          s[n][i][1] = fmaf(sc[0], c[1], s[n][i][1]);
-          s[n][i][2] = fmaf(sc[1], c[2], s[n][i][2]);
-          s[n][i][3] = fmaf(sc[1], c[3], s[n][i][3]);
+          float c[4];
+          mma_f16(c, af, qf[n][k][0], qf[n][k][1], bias[n][k]);
+          mma_f16(c, af + 4, qf[n][k][2], qf[n][k][3], c);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[n][i][x] = k == 0 ? sc[x >> 1] * c[x] : fmaf(sc[x >> 1], c[x], s[n][i][x]);
         }
       }
     }
-    if (tile + step < tile_end) load_k(tile + step, n0, n1);
     if (!whole) {
-      const bool page = (g >> 2 ? p1 : p0) >= 0;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
-            const int j = j0 + 4 * g + 2 * i + (x >> 1);
-            if (!page || j < start || j >= limit[n][x & 1]) s[n][i][x] = -INFINITY;
+            const int j = j0 + 16 * i + 8 * (x >> 1) + g;
+            if (!(there >> i & 1) || j < start || j >= limit[n][x & 1]) s[n][i][x] = -INFINITY;
           }
     }
 
@@ -307,7 +376,7 @@ __global__ void __launch_bounds__(kWarps * 32) fmha_q4_kernel(const Args a, cons
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        top[n][c] = fmaxf(fmaxf(s[n][0][c], s[n][0][2 + c]), fmaxf(s[n][1][c], s[n][1][2 + c]));
+        top[n][c] = fmaxf(fmaxf(s[n][0][c], s[n][0][2 + c]), fmaxf(s[n][1][c], s[n][1][2 + c])) * unit[n][c];
         raise |= top[n][c] > m[n][c] + 8.f;
       }
     if (__any_sync(0xffffffffu, raise)) {
@@ -320,55 +389,69 @@ __global__ void __launch_bounds__(kWarps * 32) fmha_q4_kernel(const Args a, cons
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
           v = fmaxf(v, m[n][c]);
-          const float f = v == -INFINITY ? 1.f : ex2(m[n][c] - v);
+          const float f = ex2(m[n][c] - v);
           m[n][c] = v;
           l[n][c] *= f;
 #pragma unroll
           for (int i = 0; i < VW * 4; ++i) o[n][i][c] *= f, o[n][i][2 + c] *= f;
         }
     }
-    uint32_t pf[NT][4];   // block x: keys 4 g + x -> after the transpose columns are rows
+    uint32_t pf[NT][4];   // block x: keys 8 x + g; after the transpose the lane has keys 8 x + 2 t (+ 1) of row g
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        const float e0 = ex2(s[n][x >> 1][(x & 1) * 2] - m0), e1 = ex2(s[n][x >> 1][(x & 1) * 2 + 1] - m1);
+        const float e0 = ex2(fmaf(s[n][x >> 1][(x & 1) * 2], unit[n][0], -m[n][0]));
+        const float e1 = ex2(fmaf(s[n][x >> 1][(x & 1) * 2 + 1], unit[n][1], -m[n][1]));
         l[n][0] += e0;
         l[n][1] += e1;
         pf[n][x] = transpose8x8(Op<T>::pack(e0, e1));
       }
     }
 
-    // ---- output: dims of word(s) g, keys 8 t + x and 8 t + 4 + x of block x
-    uint32_t vs[8 * VW];
-    const int vgroup = (g * VW) % G;   // group of the lane's first word; the next word's group is the next one
+    // ---- output: dims of the lane's words, keys 8 x + 2 t and 8 x + 2 t + 1 of block x
+    uint32_t vw[4][2][VW], sp[VW][4];
+    const uint32_t own = g & 1 ? 0x7632u : 0x5410u;
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      // scales of key 8 t + x in the lane's groups: word x * G / 2 (+ which half)
-      if constexpr (G == 2) vs[x] = vt.s[x];
-      else vs[x] = vgroup ? vt.s[2 * x + 1] : vt.s[2 * x];
+    for (int x = 0; x < 4; ++x) {
+      const int row = 8 * x + 2 * t;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) lds<VW>(stage + v_lane + (Ring::kV + (8 * x + y) * Ring::kRow), vw[x][y]);
+      uint32_t s2[2];
+      if constexpr (G == 2) {   // a key's two scales are a word; the lane's group is g % 2
+        lds<2>(stage + Ring::kVs + row * 4, s2);
+        sp[0][x] = __byte_perm(s2[0], s2[1], own);
+      } else {                  // its words 2 g and 2 g + 1 are of groups 0, 1 (g even) or 2, 3
+        lds<1>(stage + Ring::kVs + row * 8 + (g & 1) * 4, s2);
+        lds<1>(stage + Ring::kVs + row * 8 + 8 + (g & 1) * 4, s2 + 1);
+        sp[0][x] = lows(s2[0], s2[1]);
+        sp[VW - 1][x] = highs(s2[0], s2[1]);
+      }
     }
     if (!whole) {   // a key that some row of the block does not see must not reach it as 0 * NaN: those rows' outputs take it by hand
       bool odd = false;
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const int j = j0 + 8 * t + x;
-        const bool there = (t >> 1 ? p1 : p0) >= 0 && j >= start && j < end;
-        unsigned short lo = static_cast<unsigned short>(vs[x]), hi = static_cast<unsigned short>(vs[x] >> 16);
-        const float flo = Elem<T>::to_f(*reinterpret_cast<T*>(&lo)), fhi = Elem<T>::to_f(*reinterpret_cast<T*>(&hi));
-        if (!there || !(fabsf(flo) < INFINITY)) odd |= there, vs[x] &= 0xffff0000u;
-        if (!there || !(fabsf(fhi) < INFINITY)) odd |= there, vs[x] &= 0x0000ffffu;
-      }
-      if (__any_sync(0xffffffffu, odd)) {
-        for (int x = 0; x < 32; ++x) {
-          const int j = j0 + x, page = x >> 4 ? p1 : p0;
-          if (page < 0 || j < start || j >= end) continue;
-          const T* sc = static_cast<const T*>(a.v_scales) + (row_of(tile, x >> 4, page) + (x & 15)) * G;
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int j = j0 + 8 * x + 2 * t + y;
+          const bool seen = (there >> (x >> 1) & 1) && j >= start && j < end;
 #pragma unroll
           for (int w = 0; w < VW; ++w) {
-            const float v = Elem<T>::to_f(sc[(g * VW + w) % G]);
-            if (fabsf(v) < INFINITY) continue;
+            const unsigned short h = static_cast<unsigned short>(sp[w][x] >> (16 * y));
+            if (seen && fabsf(Elem<T>::to_f(*reinterpret_cast<const T*>(&h))) < INFINITY) continue;
+            odd |= seen;
+            sp[w][x] &= y ? 0x0000ffffu : 0xffff0000u;
+          }
+        }
+      if (__any_sync(0xffffffffu, odd)) {
+        for (int x = 0; x < 32; ++x) {
+          const int j = j0 + x;
+          if (!(there >> (x >> 4) & 1) || j < start || j >= end) continue;
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            const T* sc = reinterpret_cast<const T*>(smem + (stage - ptx::smem_u32(smem)) + Ring::kVs) + x * G + (g * VW + w) % G;
+            if (fabsf(Elem<T>::to_f(*sc)) < INFINITY) continue;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -382,23 +465,17 @@ __global__ void __launch_bounds__(kWarps * 32) fmha_q4_kernel(const Args a, cons
     }
 #pragma unroll
     for (int w = 0; w < VW; ++w) {
-      uint32_t lo[4], hi[4], sp[4];
+      uint32_t st[4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        lo[x] = lows(vt.w[x][w], vt.w[x + 4][w]);
-        hi[x] = highs(vt.w[x][w], vt.w[x + 4][w]);
-        // G = 2: the word's group is g % 2; G = 4: words 2 g, 2 g + 1 are the low and the high scale of the selected pair
-        if constexpr (G == 2) sp[x] = g & 1 ? highs(vs[x], vs[x + 4]) : lows(vs[x], vs[x + 4]);
-        else sp[x] = w ? highs(vs[x], vs[x + 4]) : lows(vs[x], vs[x + 4]);
-      }
+      for (int x = 0; x < 4; ++x) st[x] = Op<T>::steep(sp[w][x]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {   // dims 2 i, 2 i + 1 of the octet
+      for (int i = 0; i < 4; ++i) {   // dims 2 i, 2 i + 1 of the octet: byte i of the words
         uint32_t d0[4], d1[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const uint32_t src = i < 2 ? lo[x] : hi[x];
-          d0[x] = Op<T>::mul(Op<T>::centred(((src >> (8 * (i & 1))) & 0x000f000fu) | Op<T>::kMagic), sp[x]);
-          d1[x] = Op<T>::mul(Op<T>::centred(((src >> (8 * (i & 1) + 4)) & 0x000f000fu) | Op<T>::kMagic), sp[x]);
+          const uint32_t src = __byte_perm(vw[x][0][w], vw[x][1][w], 0x4400 + 0x1111 * i);
+          d0[x] = Op<T>::low(src, sp[w][x]);
+          d1[x] = Op<T>::second(src, st[x]);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -407,11 +484,12 @@ __global__ void __launch_bounds__(kWarps * 32) fmha_q4_kernel(const Args a, cons
         }
       }
     }
-    if (tile + step < tile_end) load_v(tile + step, n0, n1);
-    p0 = n0, p1 = n1, n0 = f0, n1 = f1;
+    free_stage = stage;
+    stage = stage == ring + (Ring::kStages - 1) * Ring::kBytes ? ring : stage + Ring::kBytes;
   }
 
-  // ---- the warps of the block meet, then the blocks of the cluster
+  // ---- the warps of a group meet, then the blocks of the cluster
+  __syncthreads();   // the rings are done with
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -421,7 +499,7 @@ __global__ void __launch_bounds__(kWarps * 32) fmha_q4_kernel(const Args a, cons
       v += __shfl_xor_sync(0xffffffffu, v, 8);
       v += __shfl_xor_sync(0xffffffffu, v, 16);
       const int r = n * 8 + 2 * t + c;
-      if (g == 0) sh.m[warp][r] = v == v ? m[n][c] : 0.f, sh.l[warp][r] = v;   // a NaN never became the maximum, but has a say
+      if (g == 0) sh.m[warp][r] = m[n][c], sh.l[warp][r] = v;
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
         const int dim = q4::octet_of_word(g * VW + w, G) * 8;
@@ -440,9 +518,9 @@ __global__ void __launch_bounds__(kWarps * 32) fmha_q4_kernel(const Args a, cons
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = sh.m[w][r] == -INFINITY ? 0.f : ex2(sh.m[w][r] - top);
+        const float f = ex2(sh.m[w][r] - top);
         const float4 v = *reinterpret_cast<const float4*>(&sh.o[w][r][d]);
-        if (sh.m[w][r] != -INFINITY) acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+        acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
       }
       *reinterpret_cast<float4*>(&sh.o[0][r][d]) = acc;
     }
@@ -453,44 +531,44 @@ __global__ void __launch_bounds__(kWarps * 32) fmha_q4_kernel(const Args a, cons
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sh.m[w][r]);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w)
-        if (sh.m[w][r] != -INFINITY) sum = fmaf(sh.l[w][r], ex2(sh.m[w][r] - top), sum);
+      for (int w = 0; w < kWarps; ++w) sum = fmaf(sh.l[w][r], ex2(sh.m[w][r] - top), sum);
       sh.m[0][r] = top, sh.l[0][r] = sum;
     }
     ptx::cluster_sync();
   }
-  const int ways = parts > 1 ? parts : kWarps;
+  // Rows of the warp's own group, dealt over its warps; with a cluster (the block is one group) over those of all blocks.
+  const int sources = parts > 1 ? parts : ways, first = warp - way;
   auto remote = [&](const float* p, int rank) {
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ptx::map_to_cta(p, rank)) : "memory");
     return v;
   };
-  for (int i = part * kWarps * 32 + threadIdx.x; i < NR * (D / 8); i += parts * kWarps * 32) {
+  for (int i = (part * ways + way) * 32 + lane; i < NR * (D / 8); i += parts * ways * 32) {
     const int n = i / (D / 8), d = i % (D / 8) * 8, r = row0 + n;
     if (r >= rows) continue;
-    float ms[8], top = -INFINITY, sum = 0.f, acc[8] = {};
+    float ms[8], top = kEmpty, sum = 0.f, acc[8] = {};
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
-      if (w < ways) {
-        ms[w] = parts > 1 ? remote(&sh.m[0][n], w) : sh.m[w & (kWarps - 1)][n];
+      if (w < sources) {
+        ms[w] = parts > 1 ? remote(&sh.m[0][n], w) : sh.m[(first + w) & (kWarps - 1)][n];
         top = fmaxf(top, ms[w]);
       }
     }
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
-      if (w < ways && ms[w] != -INFINITY) {
+      if (w < sources) {
         const float f = ex2(ms[w] - top);
-        sum = fmaf(f, parts > 1 ? remote(&sh.l[0][n], w) : sh.l[w & (kWarps - 1)][n], sum);
-        const float* src = parts > 1 ? &sh.o[0][n][d] : &sh.o[w & (kWarps - 1)][n][d];
+        const int from = (first + w) & (kWarps - 1);
+        sum = fmaf(f, parts > 1 ? remote(&sh.l[0][n], w) : sh.l[from][n], sum);
         float v[8];
         if (parts > 1) {
 #pragma unroll
           for (int x = 0; x < 2; ++x)
             asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[4 * x]), "=f"(v[4 * x + 1]), "=f"(v[4 * x + 2]), "=f"(v[4 * x + 3])
-                         : "r"(ptx::map_to_cta(src + 4 * x, w)) : "memory");
+                         : "r"(ptx::map_to_cta(&sh.o[0][n][d + 4 * x], w)) : "memory");
         } else {
 #pragma unroll
-          for (int x = 0; x < 8; ++x) v[x] = src[x];
+          for (int x = 0; x < 8; ++x) v[x] = sh.o[from][n][d + x];
         }
 #pragma unroll
         for (int x = 0; x < 8; ++x) acc[x] = fmaf(f, v[x], acc[x]);
@@ -509,15 +587,22 @@ template <typename T, int D, int NT>
 int launch(const Args& a, cudaStream_t s) {
   const int64_t rows = static_cast<int64_t>(a.H / a.Hkv) * a.Tq, row_blocks = (rows + 8 * NT - 1) / (8 * NT);
   const int64_t groups = static_cast<int64_t>(a.B) * a.Hkv * row_blocks, tiles = (a.blocks_per_seq * a.block_size + 31) / 32;
-  int parts = 1;   // few groups: a cluster each, down to two tiles a warp
-  while (parts < 8 && groups * parts < sm_count() * 3 && tiles > 2 * kWarps * parts) parts *= 2;
-  OB_REQUIRE(groups * parts <= 0x7fffffff, OASR_ERR_INVALID, "fmha_q4: too many rows for one call");
+  // Warps that share a group: until the SMs are full (down to two tiles each), and so many that none walks more than 32 tiles.  Fewer
+  // leave the longest sequences of a ragged batch running alone, more pay a block's start and end (some 8 us of latency) more often:
+  // 128 sequences of 500 to 8191 keys, 8 key heads of 128, take 212 / 187 / 205 / 274 us with 4 / 8 / 16 / 32 warps, 256 chunks of 16
+  // rows over up to 1001 keys, 8 heads of 64, take 68 / 54 / 61 us with 1 / 2 / 4.
+  int splits = 1;
+  while (splits < 32 && (tiles > 32 * splits || (groups * splits < sm_count() * 16 && tiles > 2 * splits))) splits *= 2;
+  const int ways = splits < kWarps ? splits : kWarps, parts = splits / ways;
+  const int64_t blocks = (groups + kWarps / ways - 1) / (kWarps / ways) * parts;
+  OB_REQUIRE(groups <= 0x7fffffff && blocks <= 0x7fffffff, OASR_ERR_INVALID, "fmha_q4: too many rows for one call");
   static SmemLimit limit;
-  constexpr int kSmem = sizeof(Merge<T, D, NT>);
+  constexpr int kRings = kWarps * Tile<D>::kStages * Tile<D>::kBytes, kMerge = sizeof(Merge<D, NT>);
+  constexpr int kSmem = kRings > kMerge ? kRings : kMerge;
   cudaError_t e = limit.raise(fmha_q4_kernel<T, D, NT>, kSmem);
   if (e != cudaSuccess) return set_error(OASR_ERR_CUDA, "fmha_q4: shared memory limit: %s", cudaGetErrorString(e));
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(groups * parts));
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(kWarps * 32);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = s;
@@ -528,7 +613,7 @@ int launch(const Args& a, cudaStream_t s) {
   at[1].val.clusterDim = {static_cast<unsigned>(parts), 1, 1};
   cfg.attrs = at;
   cfg.numAttrs = parts > 1 ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, fmha_q4_kernel<T, D, NT>, a, parts, static_cast<int>(row_blocks));
+  cudaLaunchKernelEx(&cfg, fmha_q4_kernel<T, D, NT>, a, parts, ways, static_cast<int>(row_blocks), static_cast<int>(groups));
   return check_launch("fmha_q4 launch");
 }
 
@@ -555,6 +640,7 @@ extern "C" int oasr_b200_fmha_q4(void* out, const int64_t* out_strides, const vo
   OB_REQUIRE(D == 64 || D == 128, OASR_ERR_UNSUPPORTED, "fmha_q4: head_dim %lld is not supported (64 and 128 are)", (long long)D);
   OB_REQUIRE(block_size > 0 && block_size % 16 == 0, OASR_ERR_UNSUPPORTED, "fmha_q4: the block size must be a multiple of 16 (got %lld)",
              (long long)block_size);
+  OB_REQUIRE(Hkv * block_size * D <= 0x7fffffff, OASR_ERR_INVALID, "fmha_q4: pages too large");
   OB_REQUIRE(B <= 65535 && H <= 65535 && Tq <= 0x7fffff && blocks_per_seq * block_size <= 0x7fffffff, OASR_ERR_INVALID,
              "fmha_q4: batch, head count or length too large");
   if (B == 0 || Tq == 0) return OASR_OK;
