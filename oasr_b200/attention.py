@@ -7,7 +7,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .functional import _DTYPE_ID, _check_distinct_rows, _need_cuda, _p, _same_device, _stream
+from .functional import _DTYPE_ID, _check_distinct_rows, _need_cuda, _one_device, _p, _stream
 
 _HALF = (torch.float16, torch.bfloat16)
 _Strides = ctypes.c_int64 * 3
@@ -208,12 +208,31 @@ def fmha_varlen(q, k, v, *, softmax_scale: float, cu_seqlens_q: torch.Tensor, cu
     return out
 
 
+def _index32(name: str, t: Optional[torch.Tensor], B: int) -> Optional[torch.Tensor]:
+    """A number for each sequence as the kernels take it."""
+    if t is None:
+        return None
+    if t.shape != (B,):
+        raise ValueError(f"{name} must be ({B},), got {tuple(t.shape)}")
+    if t.dtype != torch.int32:
+        t = t.to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _table32(table: torch.Tensor, B: int) -> torch.Tensor:
+    if table.dim() != 2 or table.shape[0] != B:
+        raise ValueError("block_table must be (B, max_blocks_per_seq)")
+    if table.dtype != torch.int32:
+        table = table.to(torch.int32)
+    return table if table.is_contiguous() else table.contiguous()
+
+
 def _check_q4_pools(k_codes, k_scales, v_codes, v_scales, dtype):
     """``(num_blocks, H_kv, block_size, D)`` of 4-bit pools, or an error."""
-    _need_cuda(k_codes, k_scales, v_codes, v_scales)
-    if k_codes.dim() != 4 or k_codes.dtype != torch.uint8 or v_codes.dtype != torch.uint8 or v_codes.shape != k_codes.shape:
+    shape = k_codes.shape
+    if len(shape) != 4 or k_codes.dtype != torch.uint8 or v_codes.dtype != torch.uint8 or v_codes.shape != shape:
         raise ValueError("codes must be uint8 (num_blocks, H_kv, block_size, D / 2) and match")
-    num_blocks, Hkv, block_size, half = k_codes.shape
+    num_blocks, Hkv, block_size, half = shape
     if half % 16 or half == 0:
         raise ValueError(f"head_dim must be a multiple of 32, got {2 * half}")
     want = (num_blocks, Hkv, block_size, half // 16)
@@ -233,22 +252,17 @@ def gather_paged_kv_q4(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: t
     """The values of ``length`` positions from ``start[b]`` on (None: from 0) out of 4-bit pages, as dense
     ``(B, H_kv, length, D)`` tensors in the scales' type (exact).  A position without a page gives zeros."""
     num_blocks, Hkv, block_size, D = _check_q4_pools(k_codes, k_scales, v_codes, v_scales, k_scales.dtype)
-    if block_table.dim() != 2:
-        raise ValueError("block_table must be (B, max_blocks_per_seq)")
-    B, length = block_table.size(0), int(length)
-    if length < 0:
-        raise ValueError(f"length must not be negative, got {length}")
-    if start is not None:
-        if start.shape != (B,):
-            raise ValueError(f"start must be ({B},), got {tuple(start.shape)}")
-        start = (start if start.dtype == torch.int32 else start.to(torch.int32)).contiguous()
-    _need_cuda(block_table, start)
-    _same_device(k_codes, k_scales, v_codes, v_scales, block_table, start)
-    block_table = (block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)).contiguous()
+    length = int(length)
+    if block_table.dim() != 2 or length < 0:
+        raise ValueError("gather_paged_kv_q4 expects a (B, max_blocks_per_seq) block table and length >= 0")
+    B = block_table.shape[0]
+    block_table, start = _table32(block_table, B), _index32("start", start, B)
+    _one_device(k_codes, k_scales, v_codes, v_scales, block_table, start)
     k = torch.empty(B, Hkv, length, D, device=k_codes.device, dtype=k_scales.dtype)
     v = torch.empty_like(k)
-    _lib.call("oasr_b200_paged_kv_gather_q4", _p(k), _p(v), _p(k_codes), _p(k_scales), _p(v_codes), _p(v_scales), _p(block_table),
-              _p(start), B, Hkv, length, D, block_table.size(1), block_size, num_blocks, _DTYPE_ID[k.dtype], _stream(k))
+    _lib.call("oasr_b200_paged_kv_gather_q4", k.data_ptr(), v.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+              v_scales.data_ptr(), block_table.data_ptr(), _p(start), B, Hkv, length, D, block_table.shape[1], block_size, num_blocks,
+              _DTYPE_ID[k.dtype], _stream(k))
     return k, v
 
 
@@ -271,28 +285,29 @@ def fmha_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_co
         raise ValueError("q and k head_dim must match")
     if Hkv == 0 or H % Hkv:
         raise ValueError(f"H ({H}) must be divisible by H_kv ({Hkv})")
-    if block_table.dim() != 2 or block_table.size(0) != B:
-        raise ValueError("block_table must be (B, max_blocks_per_seq)")
-    lens = []
-    for name, t in (("cache_seqlens", cache_seqlens), ("cache_seqstarts", cache_seqstarts), ("q_lens", q_lens)):
-        if t is not None:
-            if t.shape != (B,):
-                raise ValueError(f"{name} must be (B,) = ({B},); got {tuple(t.shape)}")
-            t = (t if t.dtype == torch.int32 else t.to(torch.int32)).contiguous()
-        lens.append(t)
-    _need_cuda(q, block_table, *lens, out)
-    _same_device(q, k_codes, k_scales, v_codes, v_scales, block_table, *lens, out)
-    block_table = (block_table if block_table.dtype == torch.int32 else block_table.to(torch.int32)).contiguous()
-    want = (B, T, H, D) if token_major else (B, H, T, D)
+    block_table = _table32(block_table, B)
+    lens, starts = _index32("cache_seqlens", cache_seqlens, B), _index32("cache_seqstarts", cache_seqstarts, B)
+    q_lens = _index32("q_lens", q_lens, B)
+    _one_device(q, k_codes, k_scales, v_codes, v_scales, block_table, lens, starts, q_lens, out)
+    sb, sh, st, unit = q.stride()
+    if unit != 1 or sb % 8 or sh % 8 or st % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+        sb, sh, st, unit = q.stride()
     if out is None:
-        out = torch.empty(want, dtype=q.dtype, device=q.device)
-    elif tuple(out.shape) != want or out.dtype != q.dtype or out.stride(3) != 1:
-        raise ValueError(f"out must be {want} in q's dtype, with unit stride along D")
-    _check_distinct_rows(out=out)
-    q, qs = _canon(q)
-    os = out.stride()
-    os = _Strides(os[0], os[2], os[1]) if token_major else _Strides(*os[:3])
-    _lib.call("oasr_b200_fmha_q4", _p(out), os, _p(q), qs, _p(k_codes), _p(k_scales), _p(v_codes), _p(v_scales), _p(block_table),
-              _p(lens[0]), _p(lens[1]), _p(lens[2]), block_table.size(1), block_size, num_blocks, B, H, Hkv, T, D, float(softmax_scale),
-              int(bool(causal)), _DTYPE_ID[q.dtype], _stream(q))
+        if token_major:
+            out = torch.empty(B, T, H, D, dtype=q.dtype, device=q.device)
+            os = _Strides(T * H * D, D, H * D)
+        else:
+            out = torch.empty(B, H, T, D, dtype=q.dtype, device=q.device)
+            os = _Strides(H * T * D, T * D, D)
+    else:
+        want = (B, T, H, D) if token_major else (B, H, T, D)
+        if tuple(out.shape) != want or out.dtype != q.dtype or out.stride(3) != 1:
+            raise ValueError(f"out must be {want} in q's dtype, with unit stride along D")
+        _check_distinct_rows(out=out)
+        ob, oh, ot = (out.stride(0), out.stride(2), out.stride(1)) if token_major else out.stride()[:3]
+        os = _Strides(ob, oh, ot)
+    _lib.call("oasr_b200_fmha_q4", out.data_ptr(), os, q.data_ptr(), _Strides(sb, sh, st), k_codes.data_ptr(), k_scales.data_ptr(),
+              v_codes.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(), lens.data_ptr(), _p(starts), _p(q_lens), block_table.shape[1],
+              block_size, num_blocks, B, H, Hkv, T, D, softmax_scale, bool(causal), _DTYPE_ID[q.dtype], _stream(q))
     return out

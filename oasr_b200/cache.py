@@ -9,8 +9,8 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .attention import _HALF, _Strides, _check_q4_pools, fmha_q4, gather_paged_kv, gather_paged_kv_q4  # noqa: F401  (re-exported)
-from .functional import _DTYPE_ID, _check_distinct_rows, _check_head_weight, _check_rope_table, _need_cuda, _p, _same_device, _stream
+from .attention import _HALF, _Strides, _check_q4_pools, _index32, _table32, fmha_q4, gather_paged_kv, gather_paged_kv_q4  # noqa: F401  (re-exported)
+from .functional import _DTYPE_ID, _check_distinct_rows, _check_head_weight, _check_rope_table, _need_cuda, _one_device, _p, _stream
 
 
 def write_kv_chunk(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, new_k: torch.Tensor,
@@ -74,61 +74,54 @@ class PagedKVCache:
         return k[:, :, :max_total_kv], v[:, :, :max_total_kv]
 
 
-def _index32(name: str, t: Optional[torch.Tensor], B: int) -> Optional[torch.Tensor]:
-    if t is None:
-        return None
-    if t.shape != (B,):
-        raise ValueError(f"{name} must be ({B},), got {tuple(t.shape)}")
-    return (t if t.dtype == torch.int32 else t.to(torch.int32)).contiguous()
+def _heads(name: str, x: torch.Tensor):
+    """``x`` with unit stride along D, and its (batch, head, frame) strides."""
+    sb, sh, st, unit = x.stride()
+    if unit != 1:
+        x = x.contiguous()
+        sb, sh, st, unit = x.stride()
+    return x, _Strides(sb, sh, st)
 
 
-def _write_rope(q4, pools, page_shape, block_table, new_k, new_v, offset, cos_sin, q, q_weight, k_weight, eps, interleaved,
-                rope_offset, new_lens, q_out):
-    _need_cuda(*pools, block_table, new_k, new_v, cos_sin, q, q_weight, k_weight, q_out)
+def _write_rope(entry, pools, num_blocks, block_size, pool_heads, pool_dim, block_table, new_k, new_v, offset, cos_sin, q, q_weight,
+                k_weight, eps, interleaved, rope_offset, new_lens, q_out):
     if new_k.dim() != 4 or new_k.shape != new_v.shape:
         raise ValueError("new_k / new_v must be (B, H_kv, T, D) and match")
     B, Hkv, T, D = new_k.shape
-    num_blocks, block_size, pool_heads, pool_dim = page_shape
-    if new_k.dtype not in _HALF or new_v.dtype != new_k.dtype:
-        raise ValueError(f"new_k / new_v must share fp16 or bf16, got {new_k.dtype} / {new_v.dtype}")
+    dtype = new_k.dtype
+    if dtype not in _HALF or new_v.dtype != dtype:
+        raise ValueError(f"new_k / new_v must share fp16 or bf16, got {dtype} / {new_v.dtype}")
     if pool_heads != Hkv or pool_dim != D:
         raise ValueError(f"pools hold {pool_heads} heads of {pool_dim}, the chunk has {Hkv} of {D}")
-    if block_table.dim() != 2 or block_table.size(0) != B:
-        raise ValueError("block_table must be (B, max_blocks_per_seq)")
+    block_table = _table32(block_table, B)
     if isinstance(offset, int):
         offset = torch.full((B,), offset, dtype=torch.int32, device=new_k.device)
     offset, rope_offset, new_lens = _index32("offset", offset, B), _index32("rope_offset", rope_offset, B), _index32("new_lens", new_lens, B)
-    if block_table.dtype != torch.int32:
-        block_table = block_table.to(torch.int32)
-    block_table = block_table.contiguous()
-    _same_device(new_k, *pools, block_table, new_v, offset, rope_offset, new_lens, cos_sin, q, q_weight, k_weight, q_out)
-    _check_rope_table(cos_sin, D)
-    _check_head_weight(new_k, D, q_weight=q_weight, k_weight=k_weight)
-    H = 0
+    _one_device(new_k, *pools, block_table, new_v, offset, rope_offset, new_lens, cos_sin, q, q_weight, k_weight, q_out)
+    rows, rotary = _check_rope_table(cos_sin, D)
+    new_k, ks = _heads("new_k", new_k)
+    new_v, vs = _heads("new_v", new_v)
+    H, src, dst, qs, qo = 0, None, None, None, None
     if q is not None:
-        if q.dim() != 4 or q.size(0) != B or q.size(2) != T or q.size(3) != D or q.dtype != new_k.dtype:
-            raise ValueError(f"q must be ({B}, H, {T}, {D}) {new_k.dtype}, got {tuple(q.shape)} {q.dtype}")
-        H = q.size(1)
+        if q.dim() != 4 or q.dtype != dtype or q.shape[0] != B or q.shape[2:] != (T, D):
+            raise ValueError(f"q must be ({B}, H, {T}, {D}) {dtype}, got {tuple(q.shape)} {q.dtype}")
+        H = q.shape[1]
         if q_out is None:
             q_out = torch.empty_like(q)
-        elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(3) != 1:
-            raise ValueError("q_out must have q's shape and dtype, with unit stride along D")
-        _check_distinct_rows(q_out=q_out)
+        else:
+            if q_out.shape != q.shape or q_out.dtype != dtype:
+                raise ValueError("q_out must have q's shape and dtype")
+            _check_distinct_rows(q_out=q_out)
+        if q_out.stride(3) != 1:
+            raise ValueError("q and q_out need unit stride along D")
+        q, qs = _heads("q", q)
+        src, dst, qo = q.data_ptr(), q_out.data_ptr(), _Strides(*q_out.stride()[:3])
     elif q_out is not None or q_weight is not None:
         raise ValueError("q_out and q_weight need q")
-    if new_k.stride(3) != 1:
-        new_k = new_k.contiguous()
-    if new_v.stride(3) != 1:
-        new_v = new_v.contiguous()
-    qs = qo = None
-    if q is not None:
-        if q.stride(3) != 1:
-            q = q.contiguous()
-        qs, qo = _Strides(*q.stride()[:3]), _Strides(*q_out.stride()[:3])
-    _lib.call("oasr_b200_write_kv_rope_q4" if q4 else "oasr_b200_write_kv_rope", _p(q_out), qo, *map(_p, pools), _p(q), qs,
-              _p(new_k), _Strides(*new_k.stride()[:3]), _p(new_v), _Strides(*new_v.stride()[:3]), _p(q_weight), _p(k_weight),
-              _p(cos_sin), cos_sin.size(0), cos_sin.size(1), _p(block_table), _p(offset), _p(rope_offset), _p(new_lens), B, H, Hkv, T, D,
-              block_table.size(1), block_size, num_blocks, float(eps), int(bool(interleaved)), _DTYPE_ID[new_k.dtype], _stream(new_k))
+    _lib.call(entry, dst, qo, *[p.data_ptr() for p in pools], src, qs, new_k.data_ptr(), ks, new_v.data_ptr(), vs,
+              _check_head_weight("q_weight", q_weight, D, dtype), _check_head_weight("k_weight", k_weight, D, dtype), cos_sin.data_ptr(),
+              rows, rotary, block_table.data_ptr(), offset.data_ptr(), _p(rope_offset), _p(new_lens), B, H, Hkv, T, D,
+              block_table.shape[1], block_size, num_blocks, eps, bool(interleaved), _DTYPE_ID[dtype], _stream(new_k))
     return q_out
 
 
@@ -151,7 +144,7 @@ def write_kv_rope(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: tor
         raise ValueError("pools must be contiguous")
     if k_cache.dtype != new_k.dtype or v_cache.dtype != new_k.dtype:
         raise ValueError("chunk and pool dtypes must match")
-    return _write_rope(False, (k_cache, v_cache), tuple(k_cache.shape), block_table, new_k, new_v, offset, cos_sin, q, q_weight,
+    return _write_rope("oasr_b200_write_kv_rope", (k_cache, v_cache), *k_cache.shape, block_table, new_k, new_v, offset, cos_sin, q, q_weight,
                        k_weight, eps, interleaved, rope_offset, new_lens, q_out)
 
 
@@ -164,8 +157,8 @@ def write_kv_rope_q4(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: tor
     """``write_kv_rope`` into 4-bit pages (``PagedKVCacheQ4`` describes them): the turned keys and the values are rounded to
     codes and scales from fp32."""
     num_blocks, Hkv, block_size, D = _check_q4_pools(k_codes, k_scales, v_codes, v_scales, new_k.dtype)
-    return _write_rope(True, (k_codes, k_scales, v_codes, v_scales), (num_blocks, block_size, Hkv, D), block_table, new_k, new_v, offset,
-                       cos_sin, q, q_weight, k_weight, eps, interleaved, rope_offset, new_lens, q_out)
+    return _write_rope("oasr_b200_write_kv_rope_q4", (k_codes, k_scales, v_codes, v_scales), num_blocks, block_size, Hkv, D, block_table,
+                       new_k, new_v, offset, cos_sin, q, q_weight, k_weight, eps, interleaved, rope_offset, new_lens, q_out)
 
 
 @dataclass

@@ -510,10 +510,14 @@ def gemm_log_softmax(A, B, C=None, out=None, *, out_dtype: Optional[torch.dtype]
 # ---------------------------------------------------------------------------
 # Decoding: rotary positions and scores (no reference operators)
 # ---------------------------------------------------------------------------
-def _same_device(ref: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+def _one_device(ref: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    """All tensors on ``ref``'s GPU, in one walk (calls of a few tokens are as long as their checks)."""
     device = ref.get_device()
+    if device < 0:
+        _need_cuda(ref)
     for t in others:
         if t is not None and t.get_device() != device:
+            _need_cuda(t)
             raise RuntimeError(f"all tensors must live on {ref.device}, got one on {t.device}")
 
 
@@ -527,17 +531,23 @@ def rope_table(rows: int, rotary_dim: int, base: float = 10000.0, device="cuda")
     return torch.cat([angle.cos(), angle.sin()], 1).float()
 
 
-def _check_rope_table(table: torch.Tensor, head_dim: int) -> None:
-    if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous():
+def _check_rope_table(table: torch.Tensor, head_dim: int):
+    """``(rows, rotary_dim)`` of a position table, or an error."""
+    shape = table.shape
+    if len(shape) != 2 or table.dtype != torch.float32 or not table.is_contiguous():
         raise RuntimeError("cos_sin must be a contiguous fp32 (positions, rotary_dim) table (rope_table)")
-    if table.size(1) > head_dim:
-        raise RuntimeError(f"rotary_dim {table.size(1)} is more than the head_dim {head_dim}")
+    if shape[1] > head_dim:
+        raise RuntimeError(f"rotary_dim {shape[1]} is more than the head_dim {head_dim}")
+    return shape
 
 
-def _check_head_weight(ref: torch.Tensor, head_dim: int, **weights) -> None:
-    for name, w in weights.items():
-        if w is not None and (w.shape != (head_dim,) or w.dtype != ref.dtype or not w.is_contiguous()):
-            raise RuntimeError(f"{name} must be a contiguous ({head_dim},) tensor of {ref.dtype}")
+def _check_head_weight(name: str, w: Optional[torch.Tensor], head_dim: int, dtype) -> Optional[int]:
+    """Address of a norm weight (None without one), or an error."""
+    if w is None:
+        return None
+    if w.shape != (head_dim,) or w.dtype != dtype or not w.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous ({head_dim},) tensor of {dtype}")
+    return w.data_ptr()
 
 
 def qk_norm_rope(q, k, cos_sin, positions, q_weight=None, k_weight=None, *, eps: float = 1e-6, interleaved: bool = False,
@@ -549,35 +559,49 @@ def qk_norm_rope(q, k, cos_sin, positions, q_weight=None, k_weight=None, *, eps:
     ``(2 i, 2 i + 1)``.  A weight of None leaves that norm out.  Inputs may be views of one fused projection (unit stride along
     D); results are new contiguous tensors unless ``q_out`` / ``k_out`` are given, which may be ``q`` / ``k`` themselves.  A
     position outside the table gives a zero row.  ``k`` may be None."""
-    _need_cuda(q, k, cos_sin, positions, q_weight, k_weight, q_out, k_out)
-    _same_device(q, k, cos_sin, positions, q_weight, k_weight, q_out, k_out)
-    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.size(0) != q.size(0) or k.size(2) != q.size(2))):
+    _one_device(q, k, cos_sin, positions, q_weight, k_weight, q_out, k_out)
+    dtype = q.dtype
+    if q.dim() != 3:
         raise RuntimeError("qk_norm_rope expects q (N, H, D) and k (N, H_kv, D)")
     N, H, D = q.shape
-    Hkv = 0 if k is None else k.size(1)
-    _check_rope_table(cos_sin, D)
-    if positions.shape != (N,) or positions.dtype not in (torch.int32, torch.int64) or not positions.is_contiguous():
-        raise RuntimeError(f"positions must be a contiguous int32 or int64 ({N},) tensor")
-    _check_head_weight(q, D, q_weight=q_weight, k_weight=k_weight)
-    if k is None and (k_out is not None or k_weight is not None):
+    qs_n, qs_h, unit = q.stride()
+    if unit != 1:
+        raise RuntimeError("qk_norm_rope needs unit stride along head_dim")
+    q_dst, qo_n, qo_h, q_out = _turned("q", q, q_out, N, H, D)
+    Hkv = ks_n = ks_h = ko_n = ko_h = 0
+    k_src = k_dst = None
+    if k is not None:
+        if k.dim() != 3 or k.dtype != dtype:
+            raise RuntimeError(f"k must be (N, H_kv, D) of {dtype}, got {tuple(k.shape)} {k.dtype}")
+        n, Hkv, d = k.shape
+        ks_n, ks_h, unit = k.stride()
+        if n != N or d != D or unit != 1:
+            raise RuntimeError("qk_norm_rope expects q (N, H, D) and k (N, H_kv, D) with unit stride along head_dim")
+        k_dst, ko_n, ko_h, k_out = _turned("k", k, k_out, N, Hkv, D)
+        k_src = k.data_ptr()
+    elif k_out is not None or k_weight is not None:
         raise RuntimeError("k_out and k_weight need k")
-    if q_out is None:
-        q_out = torch.empty((N, H, D), dtype=q.dtype, device=q.device)
-    if k_out is None and k is not None:
-        k_out = torch.empty((N, Hkv, D), dtype=q.dtype, device=q.device)
-    _same_dtype(q, k=k, q_out=q_out, k_out=k_out)
-    if q_out.shape != q.shape or (k is not None and k_out.shape != k.shape):
-        raise RuntimeError("q_out and k_out must have the shapes of q and k")
-    for t in (q, k, q_out, k_out):
-        if t is not None and t.stride(2) != 1 and D > 1:
-            raise RuntimeError("qk_norm_rope needs unit stride along head_dim")
-    _check_distinct_rows(q_out=q_out, k_out=k_out)
-    ks_n, ks_h, ko_n, ko_h = (0, 0, 0, 0) if k is None else (k.stride(0), k.stride(1), k_out.stride(0), k_out.stride(1))
-    _lib.call("oasr_b200_qk_norm_rope", _p(q_out), _p(k_out), _p(q), _p(k), _p(q_weight), _p(k_weight), _p(cos_sin),
-              cos_sin.size(0), cos_sin.size(1), _p(positions), int(positions.dtype == torch.int64), N, H, Hkv, D,
-              q.stride(0), q.stride(1), ks_n, ks_h, q_out.stride(0), q_out.stride(1), ko_n, ko_h, float(eps),
-              int(bool(interleaved)), _dt(q), _stream(q))
+    rows, rotary = _check_rope_table(cos_sin, D)
+    wide = positions.dtype == torch.int64
+    if not (wide or positions.dtype == torch.int32) or positions.shape != (N,) or not positions.is_contiguous():
+        raise RuntimeError(f"positions must be a contiguous int32 or int64 ({N},) tensor")
+    _lib.call("oasr_b200_qk_norm_rope", q_dst, k_dst, q.data_ptr(), k_src, _check_head_weight("q_weight", q_weight, D, dtype),
+              _check_head_weight("k_weight", k_weight, D, dtype), cos_sin.data_ptr(), rows, rotary, positions.data_ptr(), wide, N, H,
+              Hkv, D, qs_n, qs_h, ks_n, ks_h, qo_n, qo_h, ko_n, ko_h, eps, bool(interleaved), _dt(q), _stream(q))
     return q_out, k_out
+
+
+def _turned(name, x, out, N, H, D):
+    """Address, strides and tensor of the result for ``x (N, H, D)``."""
+    if out is None:
+        out = torch.empty_like(x)
+        if out.is_contiguous():
+            return out.data_ptr(), H * D, D, out
+        out = torch.empty(N, H, D, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.stride(2) != 1:
+        raise RuntimeError(f"{name}_out must have the shape and dtype of {name}, with unit stride along head_dim")
+    _check_distinct_rows(**{name + "_out": out})
+    return out.data_ptr(), out.stride(0), out.stride(1), out
 
 
 def _check_distinct_rows(**outs) -> None:
@@ -607,31 +631,40 @@ def token_log_probs(logits, tokens=None, *, top_k: int = 0, entropy: bool = True
     Alternatives are ordered by value, equal values by lowest id (``top_k`` up to 32; NaN ranks first).  Rows may lie apart
     (``logits[:, :V]`` of a head with padded columns).  -inf logits are impossible tokens; a row of nothing else has
     log-probs of -inf and entropy 0.  ``V`` is at most 262144."""
-    _need_cuda(logits, tokens)
-    _same_device(logits, tokens)
-    if logits.dim() < 1 or logits.size(-1) < 1:
+    _one_device(logits, tokens)
+    lead, V = logits.shape[:-1], logits.shape[-1] if logits.dim() else 0
+    if V < 1:
         raise RuntimeError("token_log_probs expects logits (..., V)")
-    lead, V = logits.shape[:-1], logits.size(-1)
     x = logits if logits.dim() == 2 else logits.reshape(-1, V)
-    if x.stride(1) != 1 and V > 1 or (x.size(0) > 1 and x.stride(0) < V):
+    rows = x.shape[0]
+    stride, unit = x.stride()
+    if unit != 1 and V > 1 or (rows > 1 and stride < V):
         x = x.contiguous()
-    rows = x.size(0)
-    n, log_probs = 0, None
+        stride = V
+    n = ids = log_probs = ent = top_lp = top_ids = None
+    wide = False
     if tokens is not None:
-        if tokens.dtype not in (torch.int32, torch.int64):
+        wide = tokens.dtype == torch.int64
+        if not (wide or tokens.dtype == torch.int32):
             raise RuntimeError(f"tokens must be int32 or int64, got {tokens.dtype}")
-        if tokens.shape != lead and (tokens.dim() == 0 or tokens.shape[:-1] != lead):
-            raise RuntimeError(f"tokens must be {tuple(lead)} or {tuple(lead)} + (n,), got {tuple(tokens.shape)}")
-        n = 1 if tokens.shape == lead else tokens.size(-1)
-        tokens = tokens.contiguous()
-        log_probs = torch.empty(tokens.shape, dtype=torch.float32, device=x.device)
-    ent = torch.empty(lead, dtype=torch.float32, device=x.device) if entropy else None
-    top_lp = top_ids = None
+        shape = tokens.shape
+        if shape == lead:
+            n = 1
+        elif len(shape) == len(lead) + 1 and shape[:-1] == lead:
+            n = shape[-1]
+        else:
+            raise RuntimeError(f"tokens must be {tuple(lead)} or {tuple(lead)} + (n,), got {tuple(shape)}")
+        if not tokens.is_contiguous():
+            tokens = tokens.contiguous()
+        log_probs = torch.empty_like(tokens, dtype=torch.float32)
+        ids, lp = tokens.data_ptr(), log_probs.data_ptr()
+    if entropy:
+        ent = torch.empty_like(log_probs) if n == 1 and shape == lead else torch.empty(lead, dtype=torch.float32, device=x.device)
     if top_k:
-        top_lp = torch.empty(lead + (top_k,), dtype=torch.float32, device=x.device)
-        top_ids = torch.empty(lead + (top_k,), dtype=torch.int32, device=x.device)
-    _lib.call("oasr_b200_token_log_probs", _p(log_probs), _p(ent), _p(top_lp), _p(top_ids), _p(x), _p(tokens),
-              int(n > 0 and tokens.dtype == torch.int64), rows, V, x.stride(0) if rows > 1 else V, n, int(top_k), _dt(x), _stream(x))
+        top_lp = torch.empty(*lead, top_k, dtype=torch.float32, device=x.device)
+        top_ids = torch.empty_like(top_lp, dtype=torch.int32)
+    _lib.call("oasr_b200_token_log_probs", None if n is None else lp, _p(ent), _p(top_lp), _p(top_ids), x.data_ptr(), ids, wide, rows, V,
+              stride if rows > 1 else V, n or 0, top_k, _dt(x), _stream(x))
     return TokenLogProbs(log_probs, ent, top_lp, top_ids)
 
 
