@@ -142,7 +142,7 @@ __device__ __forceinline__ void merge_lists(const uint64_t (*lists)[kMaxTop], in
 
 // W warps of a block share a row's slice; `parts` blocks of a cluster share a row.
 template <typename T, int W, int NV>
-__global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_log_probs_kernel(const Args a, const int parts) {
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? (NV == 20 ? 3 : 4) : 1) token_log_probs_kernel(const Args a, const int parts) {
   constexpr int VE = Elem<T>::kVec;
   constexpr int kRows = W == 1 ? 4 : 1;                 // rows of a block
   __shared__ Shared<W * kRows> sh;
@@ -154,34 +154,31 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_l
   const int64_t row = W == 1 ? static_cast<int64_t>(blockIdx.x) * kRows + warp : blockIdx.x / parts;
   if (W == 1 && row >= a.rows) return;
   const T* x0 = static_cast<const T*>(a.logits) + row * a.stride;
-  // granules start at the 16-byte boundary at or before the row; what lies outside the row is never read
-  const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));
-  const int granules = (a.vocab + lead + VE - 1) / VE;
+  // The row is `head` elements up to a 16-byte boundary, whole granules, and a tail; head and tail (fewer than 2 VE elements) lie
+  // one to a lane in the first warp, so that every other load is a granule without a branch.
+  const int head = min(static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x0) & 15)) % 16 / sizeof(T)), a.vocab);
+  const int granules = (a.vocab - head) / VE;
   const int first = W == 1 ? lane : part * W * 32 + threadIdx.x;
   const int step = W == 1 ? 32 : parts * W * 32;
+  const T* x1 = x0 + head;
 
   uint4 g[NV];
   const uint32_t low = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;   // -inf
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int gi = first + i * step, e0 = gi * VE - lead;
+    const int gi = first + i * step;
     g[i] = make_uint4(low, low, low, low);
-    if (gi < granules) {
-      if (e0 >= 0 && e0 + VE <= a.vocab) {
-        g[i] = *reinterpret_cast<const uint4*>(ld128_stream(x0 + e0).v);
-      } else {
-        T* p = reinterpret_cast<T*>(&g[i]);
-#pragma unroll
-        for (int j = 0; j < VE; ++j)
-          if (e0 + j >= 0 && e0 + j < a.vocab) p[j] = x0[e0 + j];
-      }
-    }
+    if (gi < granules) g[i] = *reinterpret_cast<const uint4*>(ld128_stream(x1 + gi * VE).v);
   }
+  const bool has_edge = first < a.vocab - granules * VE;
+  const int edge_at = first < head ? first : first + granules * VE;
+  const float edge = has_edge ? Elem<T>::to_f(x0[edge_at]) : -INFINITY;
 
   // ---- maximum and sums of the warp's part
   float lane_max = granule_max<T>(g[0]);
 #pragma unroll
   for (int i = 1; i < NV; ++i) lane_max = max_nan(lane_max, granule_max<T>(g[i]));
+  lane_max = max_nan(lane_max, edge);
   float m = lane_max;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -189,7 +186,8 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_l
   // size that differ at all differ by 2^102 or more, so any factor gives exponents of 0 or below kFar.
   const float unit = fabsf(m) > 1e38f ? 0x1p-90f : kLog2e;
   const float m2 = m == -INFINITY ? 0.f : m * unit;
-  float s = 0.f, w = 0.f;
+  const float edge_d = max_nan(fmaf(edge, unit, -m2), kFar);
+  float s = ex2(edge_d), w = edge_d * s;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     float x[VE];
@@ -228,19 +226,28 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_l
       threshold = from_ordered(top);
       if (lane == 0) sh.count[warp] = 0;
       __syncwarp();
-      if (threshold != -INFINITY && lane_max >= threshold) {
+      auto take = [&](float x, int index) {
+        const int at = atomicAdd(&sh.count[warp], 1);
+        if (at < kList) sh.list[warp][at] = key_of(x, index);
+      };
+      if (threshold != -INFINITY) {
+        if (edge >= threshold) take(edge, edge_at);
+        // granules that reach it; few, at places of their own in every lane: read again (from the caches) and not picked out of
+        // registers, which would take the whole warp through each
+        uint32_t reach = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          if (granule_max<T>(g[i]) >= threshold) {
-            float x[VE];
-            unpack<T>(g[i], x);
+          asm("" : "+r"(g[i].x), "+r"(g[i].y), "+r"(g[i].z), "+r"(g[i].w));   // not kept unpacked from the sums until here
+          if (granule_max<T>(g[i]) >= threshold) reach |= 1u << i;
+        }
+        while (reach) {
+          const int gi = first + (__ffs(reach) - 1) * step;
+          reach &= reach - 1;
+          const Pack<T> again = ld128(x1 + gi * VE);
 #pragma unroll
-            for (int j = 0; j < VE; ++j) {
-              if (x[j] >= threshold) {
-                const int at = atomicAdd(&sh.count[warp], 1);
-                if (at < kList) sh.list[warp][at] = key_of(x[j], (first + i * step) * VE - lead + j);
-              }
-            }
+          for (int j = 0; j < VE; ++j) {
+            const float x = Elem<T>::to_f(again.v[j]);
+            if (x >= threshold) take(x, head + gi * VE + j);
           }
         }
       }
@@ -249,6 +256,12 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_l
       fast = threshold != -INFINITY && found <= kList;
     }
     if (fast) {
+      if (found <= 32) {   // the usual case: every lane counts what is above its own
+        const uint64_t mine = lane < found ? sh.list[warp][lane] : 0;
+        int above = 0;
+        for (int i = 0; i < found; ++i) above += sh.list[warp][i] > mine;
+        if (lane < found && above < k) sorted[above] = mine;
+      } else {
       uint64_t best = 0;
       for (int i = lane; i < found; i += 32) best = max(best, sh.list[warp][i]);
       for (int r = 0; r < k; ++r) {
@@ -262,14 +275,16 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_l
           }
         }
       }
+      }
     } else {
       // rounds over the warp's part of the row, from memory again (a copy in the caches): rare, and without a limit on equal values
       uint64_t last = ~0ull;
       for (int r = 0; r < k; ++r) {
         uint64_t best = 0;
+        if (has_edge && key_of(edge, edge_at) < last) best = key_of(edge, edge_at);
         for (int gi = first; gi < granules; gi += step) {
-          for (int e = max(gi * VE - lead, 0); e < min(gi * VE - lead + VE, a.vocab); ++e) {
-            const uint64_t c = key_of(Elem<T>::to_f(x0[e]), e);
+          for (int e = 0; e < VE; ++e) {
+            const uint64_t c = key_of(Elem<T>::to_f(x1[gi * VE + e]), head + gi * VE + e);
             if (c < last) best = max(best, c);
           }
         }
@@ -352,7 +367,7 @@ int launch(const Args& a, int parts, cudaStream_t s) {
 template <typename T>
 int run(const Args& a, cudaStream_t s) {
   constexpr int VE = Elem<T>::kVec;
-  const int64_t granules = (a.vocab + 2 * VE - 2) / VE;   // at the worst alignment
+  const int64_t granules = a.vocab / VE;   // at most
   const int64_t sms = sm_count();
   // many rows: a warp each, without a block's barriers
   if (a.rows >= sms * 4 && granules <= 32 * 20) {
