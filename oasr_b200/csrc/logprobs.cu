@@ -142,7 +142,7 @@ __device__ __forceinline__ void merge_lists(const uint64_t (*lists)[kMaxTop], in
 
 // W warps of a block share a row's slice; `parts` blocks of a cluster share a row.
 template <typename T, int W, int NV>
-__global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? (NV == 20 ? 3 : 4) : 1) token_log_probs_kernel(const Args a, const int parts) {
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_log_probs_kernel(const Args a, const int parts) {
   constexpr int VE = Elem<T>::kVec;
   constexpr int kRows = W == 1 ? 4 : 1;                 // rows of a block
   __shared__ Shared<W * kRows> sh;
