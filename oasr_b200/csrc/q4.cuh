@@ -33,13 +33,32 @@ __device__ __forceinline__ float scale_of(float amax) {
   return fminf(fmaxf(__uint_as_float(up), Limits<T>::kMin), Limits<T>::kMax);
 }
 
+// rint(x / scale) of eight values as nibbles, exactly (ties to even), without a division each: the product with an approximate
+// reciprocal is within 2^-18 of the quotient, so its rounding is off by one at most, and where it is, or where the quotient lies
+// halfway, the remainder x - c scale says so, which is exact (a code and a scale have eight bits together, and it is at most half a
+// scale).
+template <typename T>
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float scale) {
-  uint32_t w = 0;
+  constexpr float kMagic = 12582912.f;   // 1.5 * 2^23: adding it rounds to whole numbers, ties to even, into the low bits
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+  const int half = __float_as_int(0.5f * scale);
+  int c[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int c = min(max(__float2int_rn(__fdiv_rn(x[i], scale)), -7), 7);
-    w |= static_cast<uint32_t>(c + 8) << (4 * i);
+    const float t = fmaf(x[i], inv, kMagic);
+    const float d = fmaf(kMagic - t, scale, x[i]);
+    c[i] = __float_as_int(t) - __float_as_int(kMagic);
+    // further than half a step, or exactly half a step from an odd number: the neighbour
+    if (fabsf(d) > __int_as_float(half - (c[i] & 1))) c[i] += d < 0.f ? -1 : 1;
   }
+  if (!(scale < Limits<T>::kMax)) {      // a scale at its limit: what is beyond saturates (and a NaN scale has some code)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = min(max(c[i], -7), 7);
+  }
+  uint32_t w = 0x88888888u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w += static_cast<uint32_t>(c[i]) << (4 * i);
   return w;
 }
 

@@ -3,13 +3,13 @@
 //   n(x) = x * rsqrt(mean(x^2) + eps) * w                         per head row, skipped without a weight
 //   y_a  = x_a cos - x_b sin,  y_b = x_b cos + x_a sin            pairs (a, b) of the first R dims: (i, i + R / 2), or (2 i, 2 i + 1)
 //
-// cos | sin come from an fp32 table row per position.  All arithmetic is fp32; the products and sums of the rotation are
-// rounded one by one (no contraction), so that a 4-bit code or a 16-bit rounding does not depend on how the compiler fuses
-// them.  Everything is read once and written once: HBM-bound from some thousand rows on, launch-bound below.
+// cos | sin come from an fp32 table row per position.  All arithmetic is fp32; on the way to 4-bit codes the products and sums of
+// the rotation are rounded one by one (no contraction), so that a code is a matter of the formula alone.  Everything is read once and written once: HBM-bound from some thousand rows on, launch-bound below.
 //
 // A lane owns a unit of 16 dims: the two octets whose dims pair up (u and u + R / 16), or two neighbouring octets where pairs
-// are neighbours or nothing is rotated.  So a lane reads what it writes and nothing else (rows may be turned in place), the
-// row sum is a shuffle over D / 16 lanes, and cos / sin are loaded once for the heads that a lane walks over.
+// are neighbours or nothing is rotated.  So a lane reads what it writes and nothing else (rows may be turned in place), and the
+// row sum is a shuffle over D / 16 lanes.  Heads are the fast index of the grid: neighbouring lanes read neighbouring memory, and the heads
+// of a token find its cosines and sines in L1.
 #include "common.cuh"
 #include "q4.cuh"
 #include "sm100_ptx.cuh"
@@ -63,11 +63,11 @@ __device__ __forceinline__ Turn load_turn(const float* row, int half, int u) {
   return t;
 }
 
-template <bool kInter>
+template <bool kInter, bool kRounded>
 __device__ __forceinline__ void rotate(float (&a)[8], float (&b)[8], const Turn& t) {
   auto turn = [](float& x, float& y, float c, float s) {
-    const float nx = __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s));
-    y = __fadd_rn(__fmul_rn(y, c), __fmul_rn(x, s));
+    const float nx = kRounded ? __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s)) : fmaf(x, c, -y * s);
+    y = kRounded ? __fadd_rn(__fmul_rn(y, c), __fmul_rn(x, s)) : fmaf(y, c, x * s);
     x = nx;
   };
   if constexpr (kInter) {
@@ -82,35 +82,43 @@ __device__ __forceinline__ void rotate(float (&a)[8], float (&b)[8], const Turn&
   }
 }
 
-// x * rsqrt(mean(x^2) + eps) * w over the `lanes` lanes of a row; every lane of the warp calls it (idle ones with zeros).
+// The two octets of a lane in a row, as loaded.
 template <typename T>
-__device__ __forceinline__ void norm_row(float (&a)[8], float (&b)[8], const Pack<T>* w, int lanes, float inv_d, float eps) {
+struct Unit {
+  static constexpr int kPacks = 8 / Elem<T>::kVec;
+  Pack<T> a[kPacks], b[kPacks];
+  __device__ __forceinline__ void load(const T* row, int2 oct) {
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i) a[i] = ld128(row + oct.x * 8 + i * Elem<T>::kVec), b[i] = ld128(row + oct.y * 8 + i * Elem<T>::kVec);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i) *reinterpret_cast<uint4*>(&a[i]) = *reinterpret_cast<uint4*>(&b[i]) = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void values(float (&xa)[8], float (&xb)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      xa[i] = Elem<T>::to_f(a[i / Elem<T>::kVec].v[i % Elem<T>::kVec]);
+      xb[i] = Elem<T>::to_f(b[i / Elem<T>::kVec].v[i % Elem<T>::kVec]);
+    }
+  }
+};
+
+// x * rsqrt(mean(x^2) + eps) * w over the `lanes` lanes of a row; every lane of the warp calls it, idle ones with zeros, and rows
+// that are not normed (a NaN weight does not reach a row that has no position) with `on` false.
+template <typename T>
+__device__ __forceinline__ void norm_row(float (&a)[8], float (&b)[8], const Unit<T>& w, bool on, int lanes, float inv_d, float eps) {
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum = fmaf(a[i], a[i], fmaf(b[i], b[i], sum));
   for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (!on) return;
   const float r = rsqrtf(fmaf(sum, inv_d, eps));
-  const T* wa = reinterpret_cast<const T*>(w);
+  float wa[8], wb[8];
+  w.values(wa, wb);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    a[i] = a[i] * r * Elem<T>::to_f(wa[i]);
-    b[i] = b[i] * r * Elem<T>::to_f(wa[8 + i]);
-  }
+  for (int i = 0; i < 8; ++i) a[i] = a[i] * r * wa[i], b[i] = b[i] * r * wb[i];
 }
-
-// 16 values of a weight row as a lane holds them
-template <typename T>
-struct UnitWeight {
-  static constexpr int kPacks = 16 / Elem<T>::kVec;
-  Pack<T> w[kPacks];
-  __device__ void load(const T* row, int2 oct) {
-#pragma unroll
-    for (int i = 0; i < kPacks / 2; ++i) {
-      w[i] = ld128_nc(row + oct.x * 8 + i * Elem<T>::kVec);
-      w[kPacks / 2 + i] = ld128_nc(row + oct.y * 8 + i * Elem<T>::kVec);
-    }
-  }
-};
 
 struct QkArgs {
   void *q_out, *k_out;
@@ -118,63 +126,42 @@ struct QkArgs {
   const float* table;
   const void* positions;
   int64_t table_rows, tokens, qs_n, qs_h, ks_n, ks_h, qo_n, qo_h, ko_n, ko_h;
-  int half, heads, kv_heads, units, lanes, lane_shift, per_lane, chunks, pos_i64;
+  int half, heads, kv_heads, units, lanes, lane_shift, pos_i64;
   float inv_d, eps;
 };
 
 template <typename T, bool kInter>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkArgs a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) qk_norm_rope_kernel(const QkArgs a) {
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
-  const int64_t group = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> a.lane_shift;
+  const uint32_t group = static_cast<uint32_t>((static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> a.lane_shift);   // fewer than 2^31
   const int u = threadIdx.x & (a.lanes - 1);
-  const int64_t n = group / a.chunks;
-  const int head0 = static_cast<int>(group - n * a.chunks) * a.per_lane;
-  const bool mine = n < a.tokens && u < a.units;
+  const uint32_t all = a.heads + a.kv_heads, n32 = group / all;
+  const int64_t n = n32;
+  const int at = static_cast<int>(group - n32 * all);
+  const bool mine = n < a.tokens && u < a.units, is_q = at < a.heads;
+  const int head = is_q ? at : at - a.heads;
   const int rotated = a.half / 8;
   const int2 oct = unit_octets<kInter>(u, rotated);
   int64_t pos = -1;
   if (mine) pos = a.pos_i64 ? static_cast<const int64_t*>(a.positions)[n] : static_cast<const int32_t*>(a.positions)[n];
   const bool known = pos >= 0 && pos < a.table_rows;   // other positions: a zero row
   const bool turned = known && u < rotated;
+  const T* weight = static_cast<const T*>(is_q ? a.q_weight : a.k_weight);
+  Unit<T> x, w;
+  x.zero();
+  if (known) x.load(is_q ? static_cast<const T*>(a.q) + n * a.qs_n + head * a.qs_h : static_cast<const T*>(a.k) + n * a.ks_n + head * a.ks_h, oct);
+  if (weight && known) w.load(weight, oct);
   Turn t;
   if (turned) t = load_turn(a.table + pos * 2 * a.half, a.half, u);
-  for (int i = 0; i < a.per_lane; ++i) {
-    const int head = head0 + i;
-    const bool is_q = head < a.heads;
-    const int h = is_q ? head : head - a.heads;
-    const bool live = mine && head < a.heads + a.kv_heads;
-    float xa[8] = {}, xb[8] = {};
-    if (live && known) {
-      const T* src = is_q ? static_cast<const T*>(a.q) + n * a.qs_n + h * a.qs_h : static_cast<const T*>(a.k) + n * a.ks_n + h * a.ks_h;
-      load8(src + oct.x * 8, xa);
-      load8(src + oct.y * 8, xb);
-    }
-    const T* weight = static_cast<const T*>(is_q ? a.q_weight : a.k_weight);
-    if (a.q_weight || a.k_weight) {   // uniform: the shuffles inside take every lane
-      UnitWeight<T> w;
-      if (weight && live) {
-        w.load(weight, oct);
-      }
-      float na[8], nb[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) na[j] = xa[j], nb[j] = xb[j];
-      norm_row<T>(na, nb, w.w, a.lanes, a.inv_d, a.eps);
-      if (weight) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) xa[j] = na[j], xb[j] = nb[j];
-      }
-    }
-    if (turned) rotate<kInter>(xa, xb, t);
-    if (live) {
-      if (!known) {   // a NaN weight must not reach a row that has no position
-#pragma unroll
-        for (int j = 0; j < 8; ++j) xa[j] = xb[j] = 0.f;
-      }
-      T* dst = is_q ? static_cast<T*>(a.q_out) + n * a.qo_n + h * a.qo_h : static_cast<T*>(a.k_out) + n * a.ko_n + h * a.ko_h;
-      store8(dst + oct.x * 8, xa);
-      store8(dst + oct.y * 8, xb);
-    }
+  float xa[8], xb[8];
+  x.values(xa, xb);
+  if (a.q_weight || a.k_weight) norm_row<T>(xa, xb, w, weight && known, a.lanes, a.inv_d, a.eps);
+  if (turned) rotate<kInter, false>(xa, xb, t);
+  if (mine) {
+    T* dst = is_q ? static_cast<T*>(a.q_out) + n * a.qo_n + head * a.qo_h : static_cast<T*>(a.k_out) + n * a.ko_n + head * a.ko_h;
+    store8(dst + oct.x * 8, xa);
+    store8(dst + oct.y * 8, xb);
   }
 }
 
@@ -186,36 +173,39 @@ struct WriteArgs {
   const int32_t *block_table, *offsets, *rope_offsets, *new_lens;
   int64_t table_rows, B, T, qs_b, qs_h, qs_t, ks_b, ks_h, ks_t, vs_b, vs_h, vs_t, qo_b, qo_h, qo_t;
   int64_t blocks_per_seq, block_size, num_blocks;
-  int half, heads, kv_heads, units, lanes, lane_shift, per_lane, chunks, groups;
+  int half, heads, kv_heads, units, lanes, lane_shift, groups;
   float inv_d, eps;
 };
 
-// Largest magnitude of each of the lane's two octets' groups.  `owner` of an octet: the lane and slot that hold it.
-template <bool kPairs>
-__device__ __forceinline__ float2 group_max(float ma, float mb, int2 oct, int rotated, int lanes) {
-  if constexpr (kPairs) {
-    float m = q4::max_nan(ma, mb);
-    m = q4::max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    return make_float2(m, m);
-  } else {
-    float r[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int first = (s ? oct.y : oct.x) & ~3;
-      float m = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int o = first + j;
-        const bool split = o < 2 * rotated;
-        const int lane = split ? (o < rotated ? o : o - rotated) : o >> 1;
-        const bool slot_b = split ? o >= rotated : (o & 1);
-        const float va = __shfl_sync(0xffffffffu, ma, lane, lanes), vb = __shfl_sync(0xffffffffu, mb, lane, lanes);
-        m = q4::max_nan(m, slot_b ? vb : va);
-      }
-      r[s] = m;
-    }
-    return make_float2(r[0], r[1]);
+// Largest magnitudes of the groups that a lane's two octets lie in.
+template <bool kInter>
+__device__ __forceinline__ float2 group_max(float ma, float mb, int2 oct, int u, int rotated, int lanes, bool pairs) {
+  const float both = q4::max_nan(ma, mb), pair = q4::max_nan(both, __shfl_xor_sync(0xffffffffu, both, 1));
+  if (kInter || pairs) return make_float2(pair, pair);   // neighbouring octets: a group is two lanes
+  if (rotated % 4 == 0) {                                 // octets u and u + rotated: each in a group of four lanes
+    ma = q4::max_nan(ma, __shfl_xor_sync(0xffffffffu, ma, 1));
+    mb = q4::max_nan(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
+    ma = q4::max_nan(ma, __shfl_xor_sync(0xffffffffu, ma, 2));
+    mb = q4::max_nan(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
+    return u < rotated ? make_float2(ma, mb) : make_float2(pair, pair);
   }
+  float r[2];                                             // a group holds octets of both kinds: ask each octet's lane
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int first = (s ? oct.y : oct.x) & ~3;
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int o = first + j;
+      const bool split = o < 2 * rotated;
+      const int lane = split ? (o < rotated ? o : o - rotated) : o >> 1;
+      const bool slot_b = split ? o >= rotated : (o & 1);
+      const float va = __shfl_sync(0xffffffffu, ma, lane, lanes), vb = __shfl_sync(0xffffffffu, mb, lane, lanes);
+      m = q4::max_nan(m, slot_b ? vb : va);
+    }
+    r[s] = m;
+  }
+  return make_float2(r[0], r[1]);
 }
 
 __device__ __forceinline__ float octet_max(const float (&x)[8]) {
@@ -228,23 +218,25 @@ __device__ __forceinline__ float octet_max(const float (&x)[8]) {
 template <typename T>
 __device__ __forceinline__ void store_q4(uint32_t* codes, T* scales, const float (&x)[8], int o, float amax, int groups) {
   const float s = q4::scale_of<T>(amax);
-  codes[q4::word_of_octet(o, groups)] = q4::codes_of(x, s);
+  codes[q4::word_of_octet(o, groups)] = q4::codes_of<T>(x, s);
   if ((o & 3) == 0) scales[o >> 2] = Elem<T>::from_f(s);
 }
 
 // Head rows of one frame: the queries' (into q_out), then the keys' and the values' (into their page).
 template <typename T, bool kInter, bool kQ4>
-__global__ void __launch_bounds__(256) write_kv_rope_kernel(const WriteArgs a) {
+__global__ void __launch_bounds__(256, 4) write_kv_rope_kernel(const WriteArgs a) {
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
-  const int64_t group = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> a.lane_shift;
+  const uint32_t group = static_cast<uint32_t>((static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> a.lane_shift);   // fewer than 2^31
   const int u = threadIdx.x & (a.lanes - 1);
-  const int64_t frame = group / a.chunks;
-  const int head0 = static_cast<int>(group - frame * a.chunks) * a.per_lane;
-  const int64_t b = frame / a.T, t = frame - b * a.T;
+  const uint32_t all = a.heads + 2 * a.kv_heads, frame = group / all, T32 = static_cast<uint32_t>(a.T);
+  const int64_t b = frame / T32, t = frame - static_cast<uint32_t>(b) * T32;
+  const int index = static_cast<int>(group - frame * all);
+  const int kind = index < a.heads ? 0 : index < a.heads + a.kv_heads ? 1 : 2;
+  const int head = index - (kind > 0 ? a.heads : 0) - (kind > 1 ? a.kv_heads : 0);
   const bool mine = b < a.B && u < a.units;
   const int rotated = a.half / 8;
-  const int2 oct = unit_octets<kInter>(u, rotated);
+  const int2 oct = kind == 2 ? make_int2(2 * u, 2 * u + 1) : unit_octets<kInter>(u, rotated);   // values are not rotated
   bool fresh = false, known = false;
   int64_t page = -1, slot = 0, pos = 0;
   if (mine) {
@@ -252,73 +244,53 @@ __global__ void __launch_bounds__(256) write_kv_rope_kernel(const WriteArgs a) {
     const int64_t at = static_cast<int64_t>(a.offsets[b]) + t;
     pos = a.rope_offsets ? static_cast<int64_t>(a.rope_offsets[b]) + t : at;
     known = fresh && pos >= 0 && pos < a.table_rows;
-    const int64_t logical = at / a.block_size;
-    slot = at - logical * a.block_size;
-    if (fresh && at >= 0 && logical < a.blocks_per_seq) page = a.block_table[b * a.blocks_per_seq + logical];
-    if (page >= a.num_blocks) page = -1;             // outside the table or the pool: dropped, never written
+    if (fresh && at >= 0) {                             // below 2^32
+      const uint32_t size = static_cast<uint32_t>(a.block_size), logical = static_cast<uint32_t>(at) / size;
+      slot = static_cast<uint32_t>(at) - logical * size;
+      if (logical < a.blocks_per_seq) page = a.block_table[b * a.blocks_per_seq + logical];
+    }
+    if (page >= a.num_blocks) page = -1;                // outside the table or the pool: dropped, never written
   }
-  const bool turned = known && u < rotated;
+  const bool there = kind == 0 ? known : page >= 0 && (kind == 2 || known);   // a key of no known position is zeros
+  const T* weight = static_cast<const T*>(kind == 0 ? a.q_weight : kind == 1 ? a.k_weight : nullptr);
+  const bool turned = known && kind != 2 && u < rotated;
+  Unit<T> x, w;
+  x.zero();
+  if (there)
+    x.load(kind == 0   ? static_cast<const T*>(a.q) + b * a.qs_b + head * a.qs_h + t * a.qs_t
+           : kind == 1 ? static_cast<const T*>(a.k) + b * a.ks_b + head * a.ks_h + t * a.ks_t
+                       : static_cast<const T*>(a.v) + b * a.vs_b + head * a.vs_h + t * a.vs_t,
+           oct);
+  if (weight && there) w.load(weight, oct);
   Turn tn;
   if (turned) tn = load_turn(a.table + pos * 2 * a.half, a.half, u);
+  float xa[8], xb[8];
+  x.values(xa, xb);
+  if (a.q_weight || a.k_weight) norm_row<T>(xa, xb, w, weight && there, a.lanes, a.inv_d, a.eps);
+  if (turned) {
+    if (kQ4 && kind == 1) rotate<kInter, true>(xa, xb, tn);
+    else rotate<kInter, false>(xa, xb, tn);
+  }
+  float2 gmax = make_float2(0.f, 0.f);
+  if (kQ4 && __any_sync(0xffffffffu, kind != 0)) gmax = group_max<kInter>(octet_max(xa), octet_max(xb), oct, u, rotated, a.lanes, kind == 2);
+  if (!mine) return;
   const int dims = a.units * 16;
-  for (int i = 0; i < a.per_lane; ++i) {
-    const int head = head0 + i;
-    const int kind = head < a.heads ? 0 : head < a.heads + a.kv_heads ? 1 : 2;
-    const int h = kind == 0 ? head : head - a.heads - (kind - 1) * a.kv_heads;
-    const bool live = mine && head < a.heads + 2 * a.kv_heads;
-    const int2 at = kind == 2 ? make_int2(2 * u, 2 * u + 1) : oct;   // values are not rotated: neighbouring octets
-    const bool read = live && fresh && (kind == 2 || known) && (kind == 0 || page >= 0);
-    float xa[8] = {}, xb[8] = {};
-    if (read) {
-      const T* src = kind == 0   ? static_cast<const T*>(a.q) + b * a.qs_b + h * a.qs_h + t * a.qs_t
-                     : kind == 1 ? static_cast<const T*>(a.k) + b * a.ks_b + h * a.ks_h + t * a.ks_t
-                                 : static_cast<const T*>(a.v) + b * a.vs_b + h * a.vs_h + t * a.vs_t;
-      load8(src + at.x * 8, xa);
-      load8(src + at.y * 8, xb);
-    }
-    if (a.q_weight || a.k_weight) {
-      const T* weight = static_cast<const T*>(kind == 0 ? a.q_weight : kind == 1 ? a.k_weight : nullptr);
-      UnitWeight<T> w;
-      if (weight && read) w.load(weight, at);
-      float na[8], nb[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) na[j] = xa[j], nb[j] = xb[j];
-      norm_row<T>(na, nb, w.w, a.lanes, a.inv_d, a.eps);
-      if (weight && read) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) xa[j] = na[j], xb[j] = nb[j];
-      }
-    }
-    if (turned && kind != 2) rotate<kInter>(xa, xb, tn);
-    float2 gmax;
-    if constexpr (kQ4) {   // uniform: shuffles
-      const float ma = octet_max(xa), mb = octet_max(xb);
-      const float2 pairs = group_max<true>(ma, mb, at, rotated, a.lanes);
-      if constexpr (kInter) {
-        gmax = pairs;
-      } else {
-        const float2 split = group_max<false>(ma, mb, at, rotated, a.lanes);
-        gmax = kind == 2 ? pairs : split;
-      }
-    }
-    if (!live) continue;
-    if (kind == 0) {
-      T* dst = static_cast<T*>(a.q_out) + b * a.qo_b + h * a.qo_h + t * a.qo_t;
-      store8(dst + at.x * 8, xa);
-      store8(dst + at.y * 8, xb);
-    } else if (fresh && page >= 0) {
-      if constexpr (kQ4) {
-        const int64_t row = (page * a.kv_heads + h) * a.block_size + slot;
-        uint32_t* codes = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(kind == 1 ? a.k_pool : a.v_pool) + row * (dims / 2));
-        T* scales = static_cast<T*>(kind == 1 ? a.k_scales : a.v_scales) + row * a.groups;
-        store_q4<T>(codes, scales, xa, at.x, gmax.x, a.groups);
-        store_q4<T>(codes, scales, xb, at.y, gmax.y, a.groups);
-      } else {
-        const int64_t row = (page * a.block_size + slot) * a.kv_heads + h;
-        T* dst = static_cast<T*>(kind == 1 ? a.k_pool : a.v_pool) + row * dims;
-        store8(dst + at.x * 8, xa);
-        store8(dst + at.y * 8, xb);
-      }
+  if (kind == 0) {
+    T* dst = static_cast<T*>(a.q_out) + b * a.qo_b + head * a.qo_h + t * a.qo_t;
+    store8(dst + oct.x * 8, xa);
+    store8(dst + oct.y * 8, xb);
+  } else if (page >= 0) {
+    if constexpr (kQ4) {
+      const int64_t row = (page * a.kv_heads + head) * a.block_size + slot;
+      uint32_t* codes = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(kind == 1 ? a.k_pool : a.v_pool) + row * (dims / 2));
+      T* scales = static_cast<T*>(kind == 1 ? a.k_scales : a.v_scales) + row * a.groups;
+      store_q4<T>(codes, scales, xa, oct.x, gmax.x, a.groups);
+      store_q4<T>(codes, scales, xb, oct.y, gmax.y, a.groups);
+    } else {
+      const int64_t row = (page * a.block_size + slot) * a.kv_heads + head;
+      T* dst = static_cast<T*>(kind == 1 ? a.k_pool : a.v_pool) + row * dims;
+      store8(dst + oct.x * 8, xa);
+      store8(dst + oct.y * 8, xb);
     }
   }
 }
@@ -329,56 +301,54 @@ struct GatherArgs {
   const void *k_scales, *v_scales;
   const int32_t *block_table, *starts;
   int64_t B, Hkv, T, blocks_per_seq, block_size, num_blocks;
-  int words, groups;
+  int words, groups, rows, span;
+  uint32_t chunks;
 };
 
-// out[b, h, i, :] = the values of position starts[b] + i; a word (8 values) of K and of V per thread.
+// out[b, h, i, :] = the values of position starts[b] + i; a word (8 values) of K and of V per thread.  A block takes `span`
+// positions of one (b, h), `rows` of them at a time.
 template <typename T>
 __global__ void __launch_bounds__(256) gather_q4_kernel(const GatherArgs a) {
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
-  const int64_t total = a.B * a.Hkv * a.T * a.words;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += stride) {
-    const int64_t r = i / a.words;
-    const int j = static_cast<int>(i - r * a.words);
-    const int64_t bh = r / a.T, pos = (a.starts ? static_cast<int64_t>(a.starts[bh / a.Hkv]) : 0) + (r - bh * a.T);
-    const int64_t b = bh / a.Hkv, h = bh - b * a.Hkv;
-    const int64_t logical = pos / a.block_size;
+  const uint32_t bh = blockIdx.x / a.chunks, chunk = blockIdx.x - bh * a.chunks;
+  const uint32_t b = bh / static_cast<uint32_t>(a.Hkv), h = bh - b * static_cast<uint32_t>(a.Hkv);
+  const int row0 = threadIdx.x / a.words, j = threadIdx.x - row0 * a.words;
+  if (row0 >= a.rows) return;
+  const int o = q4::octet_of_word(j, a.groups);
+  const int64_t start = a.starts ? a.starts[b] : 0;
+  const uint32_t size = static_cast<uint32_t>(a.block_size);
+  const int64_t end = min(static_cast<int64_t>(chunk + 1) * a.span, a.T);
+  for (int64_t i = static_cast<int64_t>(chunk) * a.span + row0; i < end; i += a.rows) {
+    const int64_t pos = start + i;
+    const uint32_t logical = static_cast<uint32_t>(pos) / size;     // of positions from 0 on, below 2^32
     int64_t page = -1;
     if (pos >= 0 && logical < a.blocks_per_seq) page = a.block_table[b * a.blocks_per_seq + logical];
     float k[8] = {}, v[8] = {};
-    const int o = q4::octet_of_word(j, a.groups);
     if (page >= 0 && page < a.num_blocks) {
-      const int64_t row = (page * a.Hkv + h) * a.block_size + (pos - logical * a.block_size);
+      const int64_t row = (page * a.Hkv + h) * a.block_size + (static_cast<uint32_t>(pos) - logical * size);
       const uint32_t kw = a.k_codes[row * a.words + j], vw = a.v_codes[row * a.words + j];
       const float ks = Elem<T>::to_f(static_cast<const T*>(a.k_scales)[row * a.groups + (o >> 2)]);
       const float vs = Elem<T>::to_f(static_cast<const T*>(a.v_scales)[row * a.groups + (o >> 2)]);
 #pragma unroll
       for (int d = 0; d < 8; ++d) k[d] = q4::value_of(kw, d, ks), v[d] = q4::value_of(vw, d, vs);
     }
-    const int64_t dst = (r * a.words + o) * 8;
+    const int64_t dst = ((bh * a.T + i) * a.words + o) * 8;
     store8(static_cast<T*>(a.k_out) + dst, k);
     store8(static_cast<T*>(a.v_out) + dst, v);
   }
 }
 
-// Lanes of a row (a power of two that holds its units), and how many heads a lane walks over: as many as leave every SM
-// eight blocks, since each further head saves a lane its cos / sin loads.
 struct Shape {
-  int units, lanes, lane_shift, per_lane, chunks;
+  int units, lanes, lane_shift;   // lanes: a power of two that holds a row's units
   int64_t blocks;
 };
-Shape shape_of(int64_t D, int64_t rows, int64_t heads) {
+Shape shape_of(int64_t D, int64_t rows) {
   Shape s;
   s.units = static_cast<int>(D / 16);
-  s.lanes = 1, s.lane_shift = 0;
+  s.lanes = 2, s.lane_shift = 1;
   while (s.lanes < s.units) s.lanes <<= 1, ++s.lane_shift;
-  if (s.lanes < 2) s.lanes = 2, s.lane_shift = 1;
-  s.per_lane = 8;
-  while (s.per_lane > 1 && rows * ((heads + s.per_lane - 1) / s.per_lane) * s.lanes < static_cast<int64_t>(sm_count()) * 8 * 256) s.per_lane >>= 1;
-  s.chunks = static_cast<int>((heads + s.per_lane - 1) / s.per_lane);
-  s.blocks = (rows * s.chunks * s.lanes + 255) / 256;
+  s.blocks = (rows * s.lanes + 255) / 256;
   return s;
 }
 
@@ -408,14 +378,15 @@ int write_common(bool q4, void* q_out, const int64_t* qo, void* k_pool, void* k_
   OB_REQUIRE(is_aligned(k_pool, 16) && is_aligned(v_pool, 16) && is_aligned(k, 16) && is_aligned(v, 16) && is_aligned(table, 16) &&
                  (H == 0 || (is_aligned(q, 16) && is_aligned(q_out, 16))) && is_aligned(q_weight, 16) && is_aligned(k_weight, 16),
              OASR_ERR_ALIGN, "write_kv_rope: operands must be 16-byte aligned");
-  const Shape s = shape_of(D, B * T, H + 2 * Hkv);
-  OB_REQUIRE(s.blocks <= 0x7fffffff, OASR_ERR_INVALID, "write_kv_rope: too many rows for one call");
+  const Shape s = shape_of(D, B * T * (H + 2 * Hkv));
+  OB_REQUIRE(block_size <= 0x7fffffff && B * T * (H + 2 * Hkv) <= 0x7fffff00 && s.blocks <= 0x7fffffff, OASR_ERR_INVALID,
+             "write_kv_rope: too many rows for one call");
   static const int64_t kNone[3] = {0, 0, 0};
   if (H == 0) qs = qo = kNone;
   const WriteArgs a{q_out, k_pool, v_pool, k_scales, v_scales, q, k, v, q_weight, k_weight, table, block_table, offsets, rope_offsets, new_lens,
                     table_rows, B, T, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], qo[0], qo[1], qo[2],
                     blocks_per_seq, block_size, num_blocks, static_cast<int>(rotary_dim / 2), static_cast<int>(H), static_cast<int>(Hkv),
-                    s.units, s.lanes, s.lane_shift, s.per_lane, s.chunks, static_cast<int>(D / 32), 1.f / static_cast<float>(D),
+                    s.units, s.lanes, s.lane_shift, static_cast<int>(D / 32), 1.f / static_cast<float>(D),
                     static_cast<float>(eps)};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(s.blocks));
@@ -451,11 +422,10 @@ int oasr_b200_qk_norm_rope(void* q_out, void* k_out, const void* q, const void* 
   OB_REQUIRE(is_aligned(q, 16) && is_aligned(k, 16) && is_aligned(q_out, 16) && is_aligned(k_out, 16) && is_aligned(table, 16) &&
                  is_aligned(q_weight, 16) && is_aligned(k_weight, 16) && is_aligned(positions, pos_i64 ? 8 : 4),
              OASR_ERR_ALIGN, "qk_norm_rope: operands must be 16-byte aligned");
-  const Shape s = shape_of(D, N, H + Hkv);
-  OB_REQUIRE(s.blocks <= 0x7fffffff, OASR_ERR_INVALID, "qk_norm_rope: too many rows for one call");
+  const Shape s = shape_of(D, N * (H + Hkv));
+  OB_REQUIRE(N * (H + Hkv) <= 0x7fffff00 && s.blocks <= 0x7fffffff, OASR_ERR_INVALID, "qk_norm_rope: too many rows for one call");
   const QkArgs a{q_out, k_out, q, k, q_weight, k_weight, table, positions, table_rows, N, qs_n, qs_h, ks_n, ks_h, qo_n, qo_h, ko_n, ko_h,
-                 static_cast<int>(rotary_dim / 2), static_cast<int>(H), static_cast<int>(Hkv), s.units, s.lanes, s.lane_shift, s.per_lane,
-                 s.chunks, pos_i64, 1.f / static_cast<float>(D), static_cast<float>(eps)};
+                 static_cast<int>(rotary_dim / 2), static_cast<int>(H), static_cast<int>(Hkv), s.units, s.lanes, s.lane_shift, pos_i64, 1.f / static_cast<float>(D), static_cast<float>(eps)};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return OB_DISPATCH_FLOAT(dtype, T_, [&]() -> int {
     launch_pdl(interleaved ? qk_norm_rope_kernel<T_, true> : qk_norm_rope_kernel<T_, false>, dim3(static_cast<unsigned>(s.blocks)), dim3(256), 0, st, a);
@@ -498,12 +468,15 @@ int oasr_b200_paged_kv_gather_q4(void* k_out, void* v_out, const void* k_codes, 
              "paged_kv_gather_q4: null pointer argument");
   OB_REQUIRE(is_aligned(k_out, 16) && is_aligned(v_out, 16) && is_aligned(k_codes, 16) && is_aligned(v_codes, 16), OASR_ERR_ALIGN,
              "paged_kv_gather_q4: operands must be 16-byte aligned");
+  OB_REQUIRE(T <= 0x7fffffff && block_size <= 0x7fffffff, OASR_ERR_INVALID, "paged_kv_gather_q4: too long");
+  const int words = static_cast<int>(D / 8), rows = 256 / words;
+  const int span = rows * 4;   // four rounds a block where the sequence is that long
+  const int64_t chunks = (T + span - 1) / span, grid = B * Hkv * chunks;
+  OB_REQUIRE(grid <= 0x7fffffff, OASR_ERR_INVALID, "paged_kv_gather_q4: too many rows for one call");
   const GatherArgs a{k_out, v_out, static_cast<const uint32_t*>(k_codes), static_cast<const uint32_t*>(v_codes), k_scales, v_scales, block_table, starts,
-                     B, Hkv, T, blocks_per_seq, block_size, num_blocks, static_cast<int>(D / 8), static_cast<int>(D / 32)};
-  const int64_t items = B * Hkv * T * a.words, cap = static_cast<int64_t>(sm_count()) * 16;
-  const unsigned grid = static_cast<unsigned>(items / 256 + 1 < cap ? items / 256 + 1 : cap);
+                     B, Hkv, T, blocks_per_seq, block_size, num_blocks, words, static_cast<int>(D / 32), rows, span, static_cast<uint32_t>(chunks)};
   return OB_DISPATCH_HALF(dtype, T_, [&]() -> int {
-    launch_pdl(gather_q4_kernel<T_>, dim3(grid), dim3(256), 0, static_cast<cudaStream_t>(stream), a);
+    launch_pdl(gather_q4_kernel<T_>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, static_cast<cudaStream_t>(stream), a);
     return check_launch("paged_kv_gather_q4 launch");
   });
 }
