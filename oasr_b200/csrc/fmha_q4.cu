@@ -27,42 +27,16 @@
 // asynchronous copies (a tile is two runs of 16 keys of a page): no registers wait for memory, no warp for another.  One, two or four
 // warps of a block, or the blocks of a cluster, share a (sequence, key head, rows) and meet in shared memory at the end.
 #include "common.cuh"
+#include "fmha_q4.cuh"
 #include "q4.cuh"
 #include "sm100_ptx.cuh"
 #include "smem_limit.cuh"
 
 namespace ob {
+namespace fmha_q4 {
 namespace {
 
-struct Args {
-  void* out;
-  const void* q;
-  const uint32_t *k_codes, *v_codes;
-  const void *k_scales, *v_scales;
-  const int32_t *block_table, *seqlens, *seqstarts, *q_lens;
-  int64_t qs_b, qs_h, qs_t, os_b, os_h, os_t;
-  int64_t blocks_per_seq, block_size, num_blocks;
-  int B, H, Hkv, Tq, causal;
-  float scale_log2;
-};
-
 constexpr int kWarps = 4;
-
-constexpr float kEmpty = -3e38f;   // a maximum below every score: differences to it overflow to -inf or are zero, never NaN
-
-__device__ __forceinline__ uint32_t half2_bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
-__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
-__device__ __forceinline__ uint32_t bf162_bits(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t*>(&v); }
-__device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162*>(&v); }
-
-constexpr uint32_t kLow = 0x000f000fu, kSecond = 0x00f000f0u, kMagic16 = 0x64006400u;   // 1024 in fp16
-
-// (w & mask) | magic in one instruction
-__device__ __forceinline__ uint32_t behind(uint32_t w, uint32_t mask, uint32_t magic) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
-  return r;
-}
 
 // S = A B + C in fp16 with fp32 accumulators
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t* a, uint32_t b0, uint32_t b1, const float (&c)[4]) {
@@ -71,63 +45,11 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t* a, uint32
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// The second product's operands.  `low` / `second`: the codes of two keys (one in each half) at bits 0..3 / 4..7, times the
-// keys' scales; `steep`: what second() wants for the scales.
-template <typename T>
-struct Op;
-template <>
-struct Op<__nv_bfloat16> {
-  static __device__ __forceinline__ uint32_t low(uint32_t w, uint32_t scale) {   // ((128 + n) - 136) s
-    const __nv_bfloat162 v = __hsub2(as_bf162(behind(w, kLow, 0x43004300u)), as_bf162(0x43084308u));
-    return bf162_bits(__hmul2(v, as_bf162(scale)));
-  }
-  static __device__ __forceinline__ uint32_t steep(uint32_t scale) { return bf162_bits(__hmul2(as_bf162(scale), as_bf162(0x40804080u))); }   // 4 s: finite
-  static __device__ __forceinline__ uint32_t second(uint32_t w, uint32_t steep) {   // (n 2^-129 2^127 - 2) 4 s
-    const __nv_bfloat162 v = __hfma2(as_bf162(w & kSecond), as_bf162(0x7f007f00u), as_bf162(0xc000c000u));
-    return bf162_bits(__hmul2(v, as_bf162(steep)));
-  }
-  static __device__ __forceinline__ float low_f(uint32_t w) { return __uint_as_float(w << 16); }
-  static __device__ __forceinline__ float high_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return bf162_bits(__floats2bfloat162_rn(lo, hi)); }
-  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-};
-template <>
-struct Op<__half> {
-  static __device__ __forceinline__ uint32_t low(uint32_t w, uint32_t scale) {   // ((1024 + n) - 1032) s
-    const __half2 v = __hsub2(as_half2(behind(w, kLow, kMagic16)), as_half2(0x64086408u));
-    return half2_bits(__hmul2(v, as_half2(scale)));
-  }
-  static __device__ __forceinline__ uint32_t steep(uint32_t scale) { return scale; }
-  static __device__ __forceinline__ uint32_t second(uint32_t w, uint32_t scale) {   // ((1024 + 16 n) / 16 - 72) s
-    const __half2 v = __hfma2(as_half2(behind(w, kSecond, kMagic16)), as_half2(0x2c002c00u), as_half2(0xd480d480u));
-    return half2_bits(__hmul2(v, as_half2(scale)));
-  }
-  static __device__ __forceinline__ float low_f(uint32_t w) { return __low2float(as_half2(w)); }
-  static __device__ __forceinline__ float high_f(uint32_t w) { return __high2float(as_half2(w)); }
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return half2_bits(__floats2half2_rn(lo, hi)); }
-  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-// two 16-bit values (the low halves or the high halves of two words) as one
-__device__ __forceinline__ uint32_t lows(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
-__device__ __forceinline__ uint32_t highs(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
-
 __device__ __forceinline__ void copy16(uint32_t dst, uint64_t src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -627,6 +549,7 @@ int run(const Args& a, cudaStream_t s) {
 }
 
 }  // namespace
+}  // namespace fmha_q4
 }  // namespace ob
 
 extern "C" int oasr_b200_fmha_q4(void* out, const int64_t* out_strides, const void* q, const int64_t* q_strides, const void* k_codes,
@@ -635,6 +558,7 @@ extern "C" int oasr_b200_fmha_q4(void* out, const int64_t* out_strides, const vo
                                  int64_t block_size, int64_t num_blocks, int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t D,
                                  double scale, int causal, int dtype, void* stream) {
   using namespace ob;
+  using namespace ob::fmha_q4;
   OB_REQUIRE(B >= 0 && H > 0 && Hkv > 0 && Tq >= 0 && D > 0 && blocks_per_seq >= 0 && num_blocks > 0, OASR_ERR_INVALID, "fmha_q4: bad shape");
   OB_REQUIRE(H % Hkv == 0, OASR_ERR_INVALID, "fmha_q4: H (%lld) must be divisible by H_kv (%lld)", (long long)H, (long long)Hkv);
   OB_REQUIRE(D == 64 || D == 128, OASR_ERR_UNSUPPORTED, "fmha_q4: head_dim %lld is not supported (64 and 128 are)", (long long)D);
@@ -656,5 +580,6 @@ extern "C" int oasr_b200_fmha_q4(void* out, const int64_t* out_strides, const vo
                block_size, num_blocks, static_cast<int>(B), static_cast<int>(H), static_cast<int>(Hkv), static_cast<int>(Tq), causal != 0,
                static_cast<float>(scale * 1.4426950408889634)};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (H / Hkv * Tq > 64) return run_prompt(a, static_cast<int>(D), dtype, st);
   return OB_DISPATCH_HALF(dtype, T_, [&]() -> int { return D == 64 ? run<T_, 64>(a, st) : run<T_, 128>(a, st); });
 }
