@@ -65,6 +65,7 @@ int g_pdl = 1;  // programmatic stream serialisation for the kernels launched th
                 // previous one drains): offline step 6.29 against 6.38 ms with every GEMM-shaped kernel on it; neutral on the
                 // graph-replayed streaming step (2.91 ms) and on the FastConformer step (51.5 ms)
 extern int g_fmha_chunk_path;
+namespace fmha_q4 { extern int g_path; }
 extern int g_fused_addnorm;
 extern int g_qkv_dup;
 namespace conv1_mma { extern int g_enabled; }
@@ -91,6 +92,11 @@ int oasr_b200_set_tunable(const char* name, int value) {
   }
   if (name && std::strcmp(name, "fmha_chunk_path") == 0) {
     ob::g_fmha_chunk_path = value != 0;
+    return OASR_OK;
+  }
+  if (name && std::strcmp(name, "fmha_q4_path") == 0) {
+    if (value < 0 || value > 2) return ob::set_error(OASR_ERR_INVALID, "fmha_q4_path must be 0, 1 or 2 (got %d)", value);
+    ob::fmha_q4::g_path = value;
     return OASR_OK;
   }
   if (name && std::strcmp(name, "fmha_relpos_path") == 0) {

@@ -34,6 +34,9 @@
 
 namespace ob {
 namespace fmha_q4 {
+
+int g_path = 0;   // tunable "fmha_q4_path": 0 by size, 1 the few-row form, 2 the prompt form
+
 namespace {
 
 constexpr int kWarps = 4;
@@ -548,6 +551,19 @@ int run(const Args& a, cudaStream_t s) {
   return launch<T, D, 2>(a, s);
 }
 
+// Which form: measured times, as far as sizes tell.  The few-row form takes 3.66 ps (head_dim 128; 64: 1.46 ps) a row and key when it
+// fills the GPU, up to twice that when it does not; the prompt form 2.5 us for 128 keys of a block of 256 rows, however many of them
+// are there.  In us, few-row against prompt form, bf16: 64 rows over 1000 keys, 128 groups of 128: 56 / 28, 8 groups: 14 / 26; 1024 groups of
+// 64: 109 / 150; 512 rows over 1000 keys, 8 groups of 128: 45 / 37, 1024 groups: 1686 / 558; 64 rows over 8000 keys, 8 groups: 34 / 151.
+bool prompt_is_faster(int64_t rows, int64_t heads, int64_t keys, int64_t D) {
+  if (g_path != 0) return g_path == 2;
+  if (rows <= 16) return false;
+  const double few = 8e-6 + 1.3 * (D == 64 ? 1.46e-12 : 3.66e-12) * static_cast<double>(rows) * static_cast<double>(keys) * static_cast<double>(heads);
+  const int64_t waves = ((rows + 255) / 256 * heads + sm_count() - 1) / sm_count();
+  const double prompt = 6e-6 + 2.5e-6 * static_cast<double>(waves) * static_cast<double>((keys + 127) / 128);
+  return prompt < few;
+}
+
 }  // namespace
 }  // namespace fmha_q4
 }  // namespace ob
@@ -580,6 +596,6 @@ extern "C" int oasr_b200_fmha_q4(void* out, const int64_t* out_strides, const vo
                block_size, num_blocks, static_cast<int>(B), static_cast<int>(H), static_cast<int>(Hkv), static_cast<int>(Tq), causal != 0,
                static_cast<float>(scale * 1.4426950408889634)};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (H / Hkv * Tq > 64) return run_prompt(a, static_cast<int>(D), dtype, st);
+  if (prompt_is_faster(H / Hkv * Tq, B * Hkv, blocks_per_seq * block_size, D)) return run_prompt(a, static_cast<int>(D), dtype, st);
   return OB_DISPATCH_HALF(dtype, T_, [&]() -> int { return D == 64 ? run<T_, 64>(a, st) : run<T_, 128>(a, st); });
 }

@@ -1,16 +1,19 @@
 // Attention of long chunks over 4-bit pages (fmha_q4.cu has the formula, and the form for few rows): tcgen05 products.
 //
 // A block owns 256 query rows of one (sequence, key head), two tiles of 128, and walks the keys 128 at a time.  13 warps:
-//   0-3, 4-7  softmax of the two tiles: a thread owns a row, reads its scores from tensor memory, writes weights to shared memory;
+//   0-3, 4-7  softmax of the two tiles: a thread owns a row, reads its scores from tensor memory and writes its weights there;
 //   8         issues the products: S = Q K^T into 128 columns of tensor memory per tile, O += P V into D columns per tile;
 //   9-12      turn codes into 16-bit rows of K and V in shared memory (128-byte swizzle).
 // The tiles run half a step apart: while one's softmax works, the tensor cores have the other's products.  Both share the
 // converted keys and values, so a code is converted once for 256 rows.  Output stays in tensor memory; a row's maximum moves only
 // when a score passes it by 2^8, and only then is the output scaled again.
+// Weights take the place of the scores they were made of (16 bits for 32) and are the A operand of the second product from
+// there: a product with both operands in shared memory reads 128 bytes a clock, all there is, and the weights' way through it
+// was a third of that traffic.  So S of step j + 1 waits for O of step j to be complete; the other tile's products fill the gap.
 //
 // Converted rows hold the exact values (q4.cuh).  Within an octet the dims lie in the order 0 4 1 5 2 6 3 7, the pairs that one mask
 // of a code word gives; queries are stored in the same order, and the output's columns are put right when they are read.
-// Shared memory at D = 128: Q and P 64 KB each, K and V in three slots of 32 KB that follow one another K V K V.
+// Shared memory at D = 128: Q 64 KB, K and V in five slots of 32 KB that follow one another K V K V.
 #include <cuda.h>
 
 #include <type_traits>
@@ -26,16 +29,37 @@ namespace ob {
 namespace fmha_q4 {
 namespace {
 
-constexpr int kThreads = 13 * 32;
-constexpr int kMmaWarp = 8, kProducer = 9, kProducers = 4;
+constexpr int kMmaWarp = 8, kProducer = 9, kProducers = 4, kThreads = (kProducer + kProducers) * 32;
 constexpr int kAtom = 128 * 128;   // 128 rows of 128 bytes
 constexpr int kKeys = 128;
 
+// two fp32 operations in one instruction
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 template <int D>
 struct Smem {
-  static constexpr int kAtoms = D / 64, kSlots = D == 128 ? 3 : 4;
-  static constexpr int kQ = 0, kP = kQ + 2 * kAtoms * kAtom, kRing = kP + 2 * 2 * kAtom, kBars = kRing + kSlots * kAtoms * kAtom;
-  static constexpr int kNumBars = 2 * kSlots + 8;
+  static constexpr int kAtoms = D / 64, kSlots = D == 128 ? 5 : 8;
+  static constexpr int kQ = 0, kRing = kQ + 2 * kAtoms * kAtom, kBars = kRing + kSlots * kAtoms * kAtom;
+  static constexpr int kNumBars = 2 * kSlots + 6;
   static constexpr int kTotal = kBars + kNumBars * 8 + 16, kDynamic = kTotal + 1024;
 };
 
@@ -76,11 +100,10 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_q4_prompt_kernel(const Args 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t* empty = full + S::kSlots;
-  uint64_t* s_full = empty + S::kSlots;   // [2]  scores are there
-  uint64_t* s_free = s_full + 2;          // [2]  scores are read
-  uint64_t* p_full = s_full + 4;          // [2]  weights are there, output is scaled
-  uint64_t* po_done = s_full + 6;         // [2]  output has them
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 8);
+  uint64_t* s_full = empty + S::kSlots;   // [2]  scores are there (and the output has all weights before)
+  uint64_t* p_full = s_full + 2;          // [2]  weights are there, output is scaled
+  uint64_t* o_done = s_full + 4;          // [2]  output has the weights
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 6);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   volatile uint32_t* odd_values = tmem_slot + 2;   // some value scale is not finite
 
@@ -92,9 +115,8 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_q4_prompt_kernel(const Args 
     }
     for (int x = 0; x < 2; ++x) {
       ptx::mbar_init(&s_full[x], 1);
-      ptx::mbar_init(&s_free[x], 128);
       ptx::mbar_init(&p_full[x], 128);
-      ptx::mbar_init(&po_done[x], 1);
+      ptx::mbar_init(&o_done[x], 1);
     }
     *abort_flag = 0;
     *odd_values = 0;
@@ -137,41 +159,43 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_q4_prompt_kernel(const Args 
     const uint32_t base = ptx::smem_u32(smem);
     auto slot_of = [&](int h) { return base + S::kRing + (h % S::kSlots) * S::kAtoms * kAtom; };
     auto wait_full = [&](int h) { return ptx::mbar_wait(&full[h % S::kSlots], (h / S::kSlots) & 1, abort_flag); };
-    auto pv = [&](int x, int j) {   // tile x's weights of step j
-      const uint64_t ad = ptx::smem_desc_kmajor_sw128(base + S::kP + x * 2 * kAtom);
-      const uint64_t bd = ptx::smem_desc_mnmajor_sw128(slot_of(2 * j + 1), kAtom, 1024);
-      if (issuer) {
+    auto scores = [&](int x, int j) {
+      if (!issuer) return;
+      const uint64_t ad = ptx::smem_desc_kmajor_sw128(base + S::kQ + x * S::kAtoms * kAtom), bd = ptx::smem_desc_kmajor_sw128(slot_of(2 * j));
 #pragma unroll
-        for (int kk = 0; kk < kKeys / 16; ++kk)
-          ptx::umma_f16(tmem + kColO + x * 128, ad + (((kk / 4) * kAtom + (kk % 4) * 32) >> 4), bd + ((kk * 2048) >> 4), kIdescPV, j > 0 || kk > 0);
-        ptx::umma_commit(&po_done[x]);
+      for (int kk = 0; kk < S::kAtoms * 4; ++kk) {
+        const uint32_t off = ((kk / 4) * kAtom + (kk % 4) * 32) >> 4;
+        ptx::umma_f16(tmem + kColS + x * 128, ad + off, bd + off, kIdescQK, kk > 0);
       }
+      ptx::umma_commit(&s_full[x]);
+      if (x == streams - 1) ptx::umma_commit(&empty[(2 * j) % S::kSlots]);
     };
-    for (int j = 0; ok && j <= tiles; ++j) {
-      if (j < tiles) ok = wait_full(2 * j);
-      for (int x = 0; ok && x < streams; ++x) {
-        if (j < tiles) {
-          if (j > 0) ok = ptx::mbar_wait(&s_free[x], (j - 1) & 1, abort_flag);
-          if (!ok) break;
-          ptx::tc_fence_after_sync();
-          if (issuer) {
-            const uint64_t ad = ptx::smem_desc_kmajor_sw128(base + S::kQ + x * S::kAtoms * kAtom), bd = ptx::smem_desc_kmajor_sw128(slot_of(2 * j));
+    auto output = [&](int x, int j) {
+      if (!issuer) return;
+      const uint64_t bd = ptx::smem_desc_mnmajor_sw128(slot_of(2 * j + 1), kAtom, 1024);
 #pragma unroll
-            for (int kk = 0; kk < S::kAtoms * 4; ++kk) {
-              const uint32_t off = ((kk / 4) * kAtom + (kk % 4) * 32) >> 4;
-              ptx::umma_f16(tmem + kColS + x * 128, ad + off, bd + off, kIdescQK, kk > 0);
-            }
-            ptx::umma_commit(&s_full[x]);
-            if (x == streams - 1) ptx::umma_commit(&empty[(2 * j) % S::kSlots]);
-          }
-        }
-        if (j > 0) {
-          if (x == 0) ok = wait_full(2 * j - 1);
-          ok = ok && ptx::mbar_wait(&p_full[x], (j - 1) & 1, abort_flag);
+      for (int kk = 0; kk < kKeys / 16; ++kk)
+        ptx::umma_f16_ts(tmem + kColO + x * 128, tmem + kColS + x * 128 + kk * 8, bd + ((kk * 2048) >> 4), kIdescPV, j > 0 || kk > 0);
+      ptx::umma_commit(&o_done[x]);
+      if (x == streams - 1) ptx::umma_commit(&empty[(2 * j + 1) % S::kSlots]);
+    };
+    ok = wait_full(0);
+    ptx::tc_fence_after_sync();
+    for (int x = 0; ok && x < streams; ++x) scores(x, 0);
+    for (int j = 0; ok && j < tiles; ++j) {
+      for (int x = 0; ok && x < streams; ++x) {
+        if (x == 0) ok = wait_full(2 * j + 1);
+        ok = ok && ptx::mbar_wait(&p_full[x], j & 1, abort_flag);
+        if (!ok) break;
+        ptx::tc_fence_after_sync();
+        output(x, j);
+        if (j + 1 < tiles) {
+          if (x == 0) ok = wait_full(2 * j + 2);
+          // products into other columns are not bound to stay in order: the weights go only once they are used
+          ok = ok && ptx::mbar_wait(&o_done[x], j & 1, abort_flag);
           if (!ok) break;
           ptx::tc_fence_after_sync();
-          pv(x, j - 1);
-          if (issuer && x == streams - 1) ptx::umma_commit(&empty[(2 * j - 1) % S::kSlots]);
+          scores(x, j + 1);
         }
       }
     }
@@ -182,13 +206,32 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_q4_prompt_kernel(const Args 
     constexpr int kLanes = D / 32, kPassRows = kProducers * 32 / kLanes, kPasses = kKeys / kPassRows;
     const int row_in_pass = (warp - kProducer) * (32 / kLanes) + lane / kLanes, piece = lane % kLanes;
     const uint32_t page_rows = static_cast<uint32_t>(a.Hkv * a.block_size), head_rows = static_cast<uint32_t>(hk * a.block_size);
-    int64_t row[kPasses];    // of the pools; -1: no page, reads row 0
-    auto look_up = [&](int j) {
+    // Pages are asked for two tiles ahead and rows made of them one tile ahead, so that no load waits for another.  A lane's rows
+    // of pass p lie in unit (16 keys of a page) 8 tile + unit0 + p * kPassRows / 16; quotient and remainder by the units of a
+    // page are kept from tile to tile.
+    const int first_unit = tile0 * 8 + (row_in_pass >> 4), step_blocks = 8 / units, step_units = 8 - step_blocks * units;
+    int block[kPasses], unit[kPasses], page[kPasses];
+    int64_t row[kPasses];      // of the pools
+    uint32_t known = 0;        // bit p: that row has a page (one without reads row 0)
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      block[p] = (first_unit + p * (kPassRows / 16)) / units;
+      unit[p] = first_unit + p * (kPassRows / 16) - block[p] * units;
+    }
+    auto ask = [&] {           // the pages of the next tile
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) page[p] = block[p] < table_len ? __ldg(table + block[p]) : -1;
+    };
+    auto resolve = [&] {       // rows of the pages asked for, and on to the next tile
+      known = 0;
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
-        const int key = (tile0 + j) * kKeys + p * kPassRows + row_in_pass, unit = key >> 4;
-        const int page = page_of(unit);
-        row[p] = page < 0 ? -1 : static_cast<int64_t>(page) * page_rows + (head_rows + static_cast<uint32_t>(unit % units * 16 + (key & 15)));
+        const bool there = static_cast<uint32_t>(page[p]) < static_cast<uint32_t>(a.num_blocks);
+        known |= (there ? 1u : 0u) << p;
+        row[p] = there ? static_cast<int64_t>(page[p]) * page_rows + (head_rows + static_cast<uint32_t>(unit[p] * 16 + (row_in_pass & 15))) : 0;
+        block[p] += step_blocks;
+        unit[p] += step_units;
+        if (unit[p] >= units) unit[p] -= units, ++block[p];
       }
     };
     struct Rows {
@@ -198,9 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_q4_prompt_kernel(const Args 
     auto load = [&](Rows& r, const uint32_t* codes, const void* scales) {
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
-        const int64_t at = row[p] < 0 ? 0 : row[p];
-        r.w[p] = __ldg(reinterpret_cast<const uint4*>(codes) + at * kLanes + piece);
-        const uint32_t* sc = static_cast<const uint32_t*>(scales) + at * (G / 2);
+        r.w[p] = __ldg(reinterpret_cast<const uint4*>(codes) + row[p] * kLanes + piece);
+        const uint32_t* sc = static_cast<const uint32_t*>(scales) + row[p] * (G / 2);
 #pragma unroll
         for (int i = 0; i < G / 2; ++i) r.s[p][i] = __ldg(sc + i);
       }
@@ -230,9 +272,11 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_q4_prompt_kernel(const Args 
       ptx::mbar_arrive(&full[s]);
       return true;
     };
-    look_up(0);
+    ask();
+    resolve();
     load(kr, a.k_codes, a.k_scales);
     load(vr, a.v_codes, a.v_scales);
+    ask();
     for (int j = 0; ok && j < tiles; ++j) {
       // values that no row may see are zeros: a weight of zero does not undo a NaN; a NaN that some row sees is marked
       const int key0 = (tile0 + j) * kKeys;
@@ -240,13 +284,14 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_q4_prompt_kernel(const Args 
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
         const int key = key0 + p * kPassRows + row_in_pass;
-        usable |= (row[p] >= 0 && key >= start && key < end ? 1u : 0u) << p;
+        usable |= key >= start && key < end ? known & (1u << p) : 0u;
       }
       ok = hand_over(2 * j, kr);
       if (!ok) break;
       if (j + 1 < tiles) {
-        look_up(j + 1);
+        resolve();
         load(kr, a.k_codes, a.k_scales);
+        ask();
       }
 #pragma unroll
       for (int p = 0; p < kPasses; ++p)
@@ -271,39 +316,39 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_q4_prompt_kernel(const Args 
     const float unit = fmaxf(fabsf(a.scale_log2), 1.2e-38f);   // a scale of zero leaves masked scores at -inf
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + lanes + kColS + x * 128, t_o = tmem + lanes + kColO + x * 128;
-    uint8_t* p_row = smem + S::kP + x * 2 * kAtom + r * 128;
-    int next_page = lane < 8 ? page_of(tile0 * 8 + lane) : 0;
+    auto ask = [&](int tile) {   // lane i < 8: the page of 16 keys, as the table has it (looked at a tile later)
+      const int blk = (tile * 8 + lane) / units;
+      return lane < 8 && blk < table_len ? __ldg(table + blk) : -1;
+    };
+    int next_page = ask(tile0);
     for (int j = 0; j < tiles; ++j) {
       const int key0 = (tile0 + j) * kKeys;
-      const uint32_t pages = __ballot_sync(0xffffffffu, next_page >= 0) & 0xffu;   // 16 keys each
-      if (lane < 8 && j + 1 < tiles) next_page = page_of((tile0 + j + 1) * 8 + lane);
+      const uint32_t pages = __ballot_sync(0xffffffffu, static_cast<uint32_t>(next_page) < static_cast<uint32_t>(a.num_blocks)) & 0xffu;   // 16 keys each
+      next_page = ask(tile0 + j + 1);
       ok = ptx::mbar_wait(&s_full[x], j & 1, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       ptx::tc_fence_after_sync();
       const bool whole = __all_sync(0xffffffffu, key0 + kKeys <= limit) && key0 >= start && pages == 0xffu;
-      auto mask = [&](uint32_t (&v)[32], int c0) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int key = key0 + c0 + i;
-          if (key < start || key >= limit || !(pages >> ((c0 + i) >> 4) & 1)) v[i] = 0xff800000u;
-        }
+      auto seen = [&](int c) {
+        const int key = key0 + c;
+        return key >= start && key < limit && (pages >> (c >> 4) & 1);
       };
-      float top = -INFINITY;
+      float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll 1
-      for (int c0 = 0; c0 < kKeys; c0 += 32) {
-        uint32_t v[32];
-        ptx::tmem_ld_32x32(t_s + c0, v);
+      for (int c0 = 0; c0 < kKeys; c0 += 64) {
+        uint32_t v[64];
+        ptx::tmem_ld_32x64(t_s + c0, v);
         ptx::tmem_ld_wait();
-        if (!whole) mask(v, c0);
+        if (whole) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(v[i]));
+          for (int i = 0; i < 64; i += 2) t0 = fmaxf(t0, __uint_as_float(v[i])), t1 = fmaxf(t1, __uint_as_float(v[i + 1]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (seen(c0 + i)) t0 = fmaxf(t0, __uint_as_float(v[i]));
+        }
       }
-      top *= unit;
-      if (j > 0) {   // the weights' place is free, and the output at rest
-        ok = ptx::mbar_wait(&po_done[x], (j - 1) & 1, abort_flag);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        ptx::tc_fence_after_sync();
-      }
+      const float top = fmaxf(t0, t1) * unit;
       const bool raise = top > m + 8.f;
       if (__any_sync(0xffffffffu, raise)) {
         const float f = raise ? ex2(m - top) : 1.f;
@@ -319,34 +364,35 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_q4_prompt_kernel(const Args 
             for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
             ptx::tmem_st_32x32(t_o + c0, v);
           }
-          ptx::tmem_st_wait();
         }
       }
-      float sum = 0.f;
+      const uint64_t unit2 = pair(unit, unit), minus_m = pair(-m, -m);
+      uint64_t s0 = 0, s1 = 0;   // sums of two at a time
 #pragma unroll 1
       for (int c0 = 0; c0 < kKeys; c0 += 32) {
         uint32_t v[32], packed[16];
         ptx::tmem_ld_32x32(t_s + c0, v);
         ptx::tmem_ld_wait();
-        if (!whole) mask(v, c0);
+        if (!whole) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float p0 = ex2(fmaf(__uint_as_float(v[i]), unit, -m)), p1 = ex2(fmaf(__uint_as_float(v[i + 1]), unit, -m));
-          sum += p0 + p1;
-          packed[i / 2] = Op<T>::pack(p0, p1);
+          for (int i = 0; i < 32; ++i) v[i] = seen(c0 + i) ? v[i] : 0xff800000u;
         }
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<uint4*>(p_row + (c0 / 64) * kAtom + (((c0 % 64) / 8 + q) ^ (r & 7)) * 16) =
-              make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
+        for (int i = 0; i < 32; i += 2) {
+          const float2 e = unpair(fma2(pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), unit2, minus_m));
+          const float p0 = ex2(e.x), p1 = ex2(e.y);
+          (i & 2 ? s1 : s0) = add2(i & 2 ? s1 : s0, pair(p0, p1));
+          packed[i / 2] = Op<T>::pack(p0, p1);
+        }
+        ptx::tmem_st_32x16(t_s + c0 / 2, packed);   // columns whose scores are read
       }
-      l += sum;
+      const float2 both = unpair(add2(s0, s1));
+      l += both.x + both.y;
+      ptx::tmem_st_wait();
       ptx::tc_fence_before_sync();
-      ptx::mbar_arrive(&s_free[x]);
-      ptx::fence_proxy_async_smem();
       ptx::mbar_arrive(&p_full[x]);
     }
-    if (ok) ok = ptx::mbar_wait(&po_done[x], (tiles - 1) & 1, abort_flag);
+    if (ok) ok = ptx::mbar_wait(&o_done[x], (tiles - 1) & 1, abort_flag);
     ok = __all_sync(0xffffffffu, ok);
     ptx::tc_fence_after_sync();
     if (!ok && lane == 0 && status) atomicOr(status, kStatusFmhaSoftmax);

@@ -10,6 +10,8 @@ up to 15 on the run-at-once register-streaming kernel), 0 all of them on the run
 ``fmha_chunk_path``: 1 (default) runs paged rel-pos attention with <= 16 query frames on the streaming-chunk kernel: a warp
 per (stream, head), or inside the Conformer's step of few streams a block that also appends the chunk to its pages; 0 on the
 128-row tcgen05 kernel behind a page write (fp8 pages: the warp-per-(stream, head) form behind one).
+``fmha_q4_path``: attention over 4-bit pages - 0 (default) chooses by size, 1 always the few-row kernel, 2 always the tcgen05
+kernel of long chunks.
 ``fmha_relpos_path``: 1 (default) runs packed relative-position attention on the two-CTAs-per-SM kernel, 0 on the general one.
 ``conv1_mma``: 1 (default) runs the first subsampling convolution (parity-split output, 256 / 512 channels) as a K = 32
 split-bf16 GEMM on the tensor cores, 0 as the fp32 stencil kernel.

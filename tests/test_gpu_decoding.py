@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import oasr_b200 as ob
+import oasr_b200.tunables
 
 pytestmark = pytest.mark.gpu
 DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
@@ -301,6 +302,14 @@ def test_write_kv_rope_refusals():
             ob.write_kv_rope_q4(**(good | how))
 
 
+@pytest.fixture(params=[0, 1, 2], ids=["by_size", "few_rows", "prompt"])
+def form(request):
+    """Both kernels of fmha_q4, and the choice between them."""
+    ob.tunables.set("fmha_q4_path", request.param)
+    yield request.param
+    ob.tunables.set("fmha_q4_path", 0)
+
+
 # ---- attention over 4-bit pages -----------------------------------------------------------------------------------------
 def q4_pool(seed, n, Hkv, block, D, dt):
     out = []
@@ -327,7 +336,7 @@ ATTEND = [  # B, H, Hkv, T, D, block, lens, starts, q_lens, causal
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("B,H,Hkv,T,D,block,lens,starts,q_lens,causal", ATTEND)
-def test_fmha_q4(dtype, B, H, Hkv, T, D, block, lens, starts, q_lens, causal):
+def test_fmha_q4(form, dtype, B, H, Hkv, T, D, block, lens, starts, q_lens, causal):
     dt = DTYPES[dtype]
     bt, n = pages(3, B, -(-max(max(lens), 1) // block) + 1)
     pools = q4_pool(10, n, Hkv, block, D, dt)
@@ -351,7 +360,7 @@ def test_fmha_q4(dtype, B, H, Hkv, T, D, block, lens, starts, q_lens, causal):
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("T", [1, 20, 200])
-def test_fmha_q4_unseen_keys_say_nothing(dtype, T):
+def test_fmha_q4_unseen_keys_say_nothing(form, dtype, T):
     """NaN scales behind the length and before the start, pages outside the pool, and a table wider than the length."""
     dt, block, D = DTYPES[dtype], 16, 64
     bt, n = pages(3, 2, 8)
@@ -377,7 +386,7 @@ def test_fmha_q4_unseen_keys_say_nothing(dtype, T):
 
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("T", [3, 40, 200])
-def test_fmha_q4_nan_reaches_the_rows_that_see_it_and_no_other(T, D):
+def test_fmha_q4_nan_reaches_the_rows_that_see_it_and_no_other(form, T, D):
     """NaN keys and values inside the length, seen by the later rows of a causal chunk only, and a NaN query."""
     block, N = 16, T + 70
     bt, n = pages(3, 1, -(-N // block))
@@ -398,7 +407,7 @@ def test_fmha_q4_nan_reaches_the_rows_that_see_it_and_no_other(T, D):
 
 
 @pytest.mark.parametrize("T", [1, 40])
-def test_fmha_q4_of_large_and_small_scores(T):
+def test_fmha_q4_of_large_and_small_scores(form, T):
     """Scores of thousands (one key has all the weight) and of nothing (all have the same)."""
     D, N = 64, 96
     bt, n = pages(3, 1, 6)
