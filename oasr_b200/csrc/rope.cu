@@ -126,42 +126,56 @@ struct QkArgs {
   const float* table;
   const void* positions;
   int64_t table_rows, tokens, qs_n, qs_h, ks_n, ks_h, qo_n, qo_h, ko_n, ko_h;
-  int half, heads, kv_heads, units, lanes, lane_shift, pos_i64;
+  int half, heads, kv_heads, q_chunks, units, lanes, lane_shift, pos_i64;
   float inv_d, eps;
 };
 
-template <typename T, bool kInter>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 3 : 4) qk_norm_rope_kernel(const QkArgs a) {
+// A lane takes one head, or two neighbouring ones (HB) that share weights, cosines and sines.
+template <typename T, bool kInter, int HB>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : HB == 1 ? 4 : 3) qk_norm_rope_kernel(const QkArgs a) {
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
   const uint32_t group = static_cast<uint32_t>((static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> a.lane_shift);   // fewer than 2^31
   const int u = threadIdx.x & (a.lanes - 1);
-  const uint32_t all = a.heads + a.kv_heads, n32 = group / all;
-  const int64_t n = n32;
-  const int at = static_cast<int>(group - n32 * all);
-  const bool mine = n < a.tokens && u < a.units, is_q = at < a.heads;
-  const int head = is_q ? at : at - a.heads;
+  const uint32_t tokens = static_cast<uint32_t>(a.tokens), at32 = group / tokens;
+  const int64_t n = group - at32 * tokens;
+  const int at = static_cast<int>(at32);
+  const bool is_q = at < a.q_chunks;
+  const int head = (is_q ? at : at - a.q_chunks) * HB;
+  const int heads = u < a.units ? (is_q ? a.heads : a.kv_heads) - head : 0;   // <= 0: an idle lane
   const int rotated = a.half / 8;
   const int2 oct = unit_octets<kInter>(u, rotated);
-  int64_t pos = -1;
-  if (mine) pos = a.pos_i64 ? static_cast<const int64_t*>(a.positions)[n] : static_cast<const int32_t*>(a.positions)[n];
-  const bool known = pos >= 0 && pos < a.table_rows;   // other positions: a zero row
-  const bool turned = known && u < rotated;
   const T* weight = static_cast<const T*>(is_q ? a.q_weight : a.k_weight);
-  Unit<T> x, w;
-  x.zero();
-  if (known) x.load(is_q ? static_cast<const T*>(a.q) + n * a.qs_n + head * a.qs_h : static_cast<const T*>(a.k) + n * a.ks_n + head * a.ks_h, oct);
-  if (weight && known) w.load(weight, oct);
+  const int64_t in_stride = is_q ? a.qs_h : a.ks_h, out_stride = is_q ? a.qo_h : a.ko_h;
+  const T* src = (is_q ? static_cast<const T*>(a.q) + n * a.qs_n : static_cast<const T*>(a.k) + n * a.ks_n) + head * in_stride;
+  T* dst = (is_q ? static_cast<T*>(a.q_out) + n * a.qo_n : static_cast<T*>(a.k_out) + n * a.ko_n) + head * out_stride;
+  Unit<T> x[HB], w;
+  int64_t pos = -1;
+  if (heads > 0) pos = a.pos_i64 ? static_cast<const int64_t*>(a.positions)[n] : static_cast<const int32_t*>(a.positions)[n];
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {   // none of these waits for the position
+    x[i].zero();
+    if (i < heads) x[i].load(src + i * in_stride, oct);
+  }
+  if (weight && heads > 0) w.load(weight, oct);
+  const bool known = pos >= 0 && pos < a.table_rows;
+  const bool turned = known && u < rotated;
   Turn t;
   if (turned) t = load_turn(a.table + pos * 2 * a.half, a.half, u);
-  float xa[8], xb[8];
-  x.values(xa, xb);
-  if (a.q_weight || a.k_weight) norm_row<T>(xa, xb, w, weight && known, a.lanes, a.inv_d, a.eps);
-  if (turned) rotate<kInter, false>(xa, xb, t);
-  if (mine) {
-    T* dst = is_q ? static_cast<T*>(a.q_out) + n * a.qo_n + head * a.qo_h : static_cast<T*>(a.k_out) + n * a.ko_n + head * a.ko_h;
-    store8(dst + oct.x * 8, xa);
-    store8(dst + oct.y * 8, xb);
+#pragma unroll
+  for (int i = 0; i < HB; ++i) {
+    float xa[8], xb[8];
+    x[i].values(xa, xb);
+    if (a.q_weight || a.k_weight) norm_row<T>(xa, xb, w, weight, a.lanes, a.inv_d, a.eps);
+    if (turned) rotate<kInter, false>(xa, xb, t);
+    if (!known) {                  // no such position: a zero row
+#pragma unroll
+      for (int j = 0; j < 8; ++j) xa[j] = xb[j] = 0.f;
+    }
+    if (i < heads) {
+      store8(dst + i * out_stride + oct.x * 8, xa);
+      store8(dst + i * out_stride + oct.y * 8, xb);
+    }
   }
 }
 
@@ -229,18 +243,28 @@ __global__ void __launch_bounds__(256, 4) write_kv_rope_kernel(const WriteArgs a
   ptx::grid_dep_wait();
   const uint32_t group = static_cast<uint32_t>((static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> a.lane_shift);   // fewer than 2^31
   const int u = threadIdx.x & (a.lanes - 1);
-  const uint32_t all = a.heads + 2 * a.kv_heads, frame = group / all, T32 = static_cast<uint32_t>(a.T);
+  const uint32_t frames = static_cast<uint32_t>(a.B * a.T), index32 = group / frames, frame = group - index32 * frames, T32 = static_cast<uint32_t>(a.T);
   const int64_t b = frame / T32, t = frame - static_cast<uint32_t>(b) * T32;
-  const int index = static_cast<int>(group - frame * all);
+  const int index = static_cast<int>(index32);
   const int kind = index < a.heads ? 0 : index < a.heads + a.kv_heads ? 1 : 2;
   const int head = index - (kind > 0 ? a.heads : 0) - (kind > 1 ? a.kv_heads : 0);
-  const bool mine = b < a.B && u < a.units;
+  const bool mine = index < a.heads + 2 * a.kv_heads && u < a.units;
   const int rotated = a.half / 8;
   const int2 oct = kind == 2 ? make_int2(2 * u, 2 * u + 1) : unit_octets<kInter>(u, rotated);   // values are not rotated
+  const T* weight = static_cast<const T*>(kind == 0 ? a.q_weight : kind == 1 ? a.k_weight : nullptr);
+  Unit<T> x, w;
+  x.zero();
   bool fresh = false, known = false;
   int64_t page = -1, slot = 0, pos = 0;
   if (mine) {
     fresh = !a.new_lens || t < a.new_lens[b];
+    if (fresh) {   // not waiting for the page or the position
+      x.load(kind == 0   ? static_cast<const T*>(a.q) + b * a.qs_b + head * a.qs_h + t * a.qs_t
+             : kind == 1 ? static_cast<const T*>(a.k) + b * a.ks_b + head * a.ks_h + t * a.ks_t
+                         : static_cast<const T*>(a.v) + b * a.vs_b + head * a.vs_h + t * a.vs_t,
+             oct);
+      if (weight) w.load(weight, oct);
+    }
     const int64_t at = static_cast<int64_t>(a.offsets[b]) + t;
     pos = a.rope_offsets ? static_cast<int64_t>(a.rope_offsets[b]) + t : at;
     known = fresh && pos >= 0 && pos < a.table_rows;
@@ -251,25 +275,19 @@ __global__ void __launch_bounds__(256, 4) write_kv_rope_kernel(const WriteArgs a
     }
     if (page >= a.num_blocks) page = -1;                // outside the table or the pool: dropped, never written
   }
-  const bool there = kind == 0 ? known : page >= 0 && (kind == 2 || known);   // a key of no known position is zeros
-  const T* weight = static_cast<const T*>(kind == 0 ? a.q_weight : kind == 1 ? a.k_weight : nullptr);
   const bool turned = known && kind != 2 && u < rotated;
-  Unit<T> x, w;
-  x.zero();
-  if (there)
-    x.load(kind == 0   ? static_cast<const T*>(a.q) + b * a.qs_b + head * a.qs_h + t * a.qs_t
-           : kind == 1 ? static_cast<const T*>(a.k) + b * a.ks_b + head * a.ks_h + t * a.ks_t
-                       : static_cast<const T*>(a.v) + b * a.vs_b + head * a.vs_h + t * a.vs_t,
-           oct);
-  if (weight && there) w.load(weight, oct);
   Turn tn;
   if (turned) tn = load_turn(a.table + pos * 2 * a.half, a.half, u);
   float xa[8], xb[8];
   x.values(xa, xb);
-  if (a.q_weight || a.k_weight) norm_row<T>(xa, xb, w, weight && there, a.lanes, a.inv_d, a.eps);
+  if (a.q_weight || a.k_weight) norm_row<T>(xa, xb, w, weight && fresh, a.lanes, a.inv_d, a.eps);
   if (turned) {
     if (kQ4 && kind == 1) rotate<kInter, true>(xa, xb, tn);
     else rotate<kInter, false>(xa, xb, tn);
+  }
+  if (!known && kind != 2) {   // no such position: a zero query or key
+#pragma unroll
+    for (int i = 0; i < 8; ++i) xa[i] = xb[i] = 0.f;
   }
   float2 gmax = make_float2(0.f, 0.f);
   if (kQ4 && __any_sync(0xffffffffu, kind != 0)) gmax = group_max<kInter>(octet_max(xa), octet_max(xb), oct, u, rotated, a.lanes, kind == 2);
@@ -422,13 +440,18 @@ int oasr_b200_qk_norm_rope(void* q_out, void* k_out, const void* q, const void* 
   OB_REQUIRE(is_aligned(q, 16) && is_aligned(k, 16) && is_aligned(q_out, 16) && is_aligned(k_out, 16) && is_aligned(table, 16) &&
                  is_aligned(q_weight, 16) && is_aligned(k_weight, 16) && is_aligned(positions, pos_i64 ? 8 : 4),
              OASR_ERR_ALIGN, "qk_norm_rope: operands must be 16-byte aligned");
-  const Shape s = shape_of(D, N * (H + Hkv));
-  OB_REQUIRE(N * (H + Hkv) <= 0x7fffff00 && s.blocks <= 0x7fffffff, OASR_ERR_INVALID, "qk_norm_rope: too many rows for one call");
+  // two heads a lane where that leaves every SM eight blocks
+  const int batch = shape_of(D, N * ((H + Hkv) / 2)).blocks >= static_cast<int64_t>(sm_count()) * 8 ? 2 : 1;
+  const int64_t q_chunks = (H + batch - 1) / batch, chunks = q_chunks + (Hkv + batch - 1) / batch;
+  const Shape s = shape_of(D, N * chunks);
+  OB_REQUIRE(N * chunks <= 0x7fffff00 && s.blocks <= 0x7fffffff, OASR_ERR_INVALID, "qk_norm_rope: too many rows for one call");
   const QkArgs a{q_out, k_out, q, k, q_weight, k_weight, table, positions, table_rows, N, qs_n, qs_h, ks_n, ks_h, qo_n, qo_h, ko_n, ko_h,
-                 static_cast<int>(rotary_dim / 2), static_cast<int>(H), static_cast<int>(Hkv), s.units, s.lanes, s.lane_shift, pos_i64, 1.f / static_cast<float>(D), static_cast<float>(eps)};
+                 static_cast<int>(rotary_dim / 2), static_cast<int>(H), static_cast<int>(Hkv), static_cast<int>(q_chunks), s.units, s.lanes, s.lane_shift, pos_i64, 1.f / static_cast<float>(D), static_cast<float>(eps)};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return OB_DISPATCH_FLOAT(dtype, T_, [&]() -> int {
-    launch_pdl(interleaved ? qk_norm_rope_kernel<T_, true> : qk_norm_rope_kernel<T_, false>, dim3(static_cast<unsigned>(s.blocks)), dim3(256), 0, st, a);
+    auto kern = batch == 2 ? (interleaved ? qk_norm_rope_kernel<T_, true, 2> : qk_norm_rope_kernel<T_, false, 2>)
+                           : (interleaved ? qk_norm_rope_kernel<T_, true, 1> : qk_norm_rope_kernel<T_, false, 1>);
+    launch_pdl(kern, dim3(static_cast<unsigned>(s.blocks)), dim3(256), 0, st, a);
     return check_launch("qk_norm_rope launch");
   });
 }
