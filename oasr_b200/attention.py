@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -11,6 +12,12 @@ from .functional import _DTYPE_ID, _check_distinct_rows, _need_cuda, _one_device
 
 _HALF = (torch.float16, torch.bfloat16)
 _Strides = ctypes.c_int64 * 3
+
+
+@functools.lru_cache(maxsize=4096)
+def _stride_array(a: int, b: int, c: int):
+    """Three strides as the host array that the entry points read (one for each combination of values)."""
+    return _Strides(a, b, c)
 
 
 def _strides3(t: torch.Tensor):
@@ -296,18 +303,18 @@ def fmha_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_co
     if out is None:
         if token_major:
             out = torch.empty(B, T, H, D, dtype=q.dtype, device=q.device)
-            os = _Strides(T * H * D, D, H * D)
+            os = _stride_array(T * H * D, D, H * D)
         else:
             out = torch.empty(B, H, T, D, dtype=q.dtype, device=q.device)
-            os = _Strides(H * T * D, T * D, D)
+            os = _stride_array(H * T * D, T * D, D)
     else:
         want = (B, T, H, D) if token_major else (B, H, T, D)
         if tuple(out.shape) != want or out.dtype != q.dtype or out.stride(3) != 1:
             raise ValueError(f"out must be {want} in q's dtype, with unit stride along D")
         _check_distinct_rows(out=out)
         ob, oh, ot = (out.stride(0), out.stride(2), out.stride(1)) if token_major else out.stride()[:3]
-        os = _Strides(ob, oh, ot)
-    _lib.call("oasr_b200_fmha_q4", out.data_ptr(), os, q.data_ptr(), _Strides(sb, sh, st), k_codes.data_ptr(), k_scales.data_ptr(),
+        os = _stride_array(ob, oh, ot)
+    _lib.call("oasr_b200_fmha_q4", out.data_ptr(), os, q.data_ptr(), _stride_array(sb, sh, st), k_codes.data_ptr(), k_scales.data_ptr(),
               v_codes.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(), lens.data_ptr(), _p(starts), _p(q_lens), block_table.shape[1],
               block_size, num_blocks, B, H, Hkv, T, D, softmax_scale, bool(causal), _DTYPE_ID[q.dtype], _stream(q))
     return out

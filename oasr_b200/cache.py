@@ -9,7 +9,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .attention import _HALF, _Strides, _check_q4_pools, _index32, _table32, fmha_q4, gather_paged_kv, gather_paged_kv_q4  # noqa: F401  (re-exported)
+from .attention import _HALF, _check_q4_pools, _stride_array, _index32, _table32, fmha_q4, gather_paged_kv, gather_paged_kv_q4  # noqa: F401  (re-exported)
 from .functional import _DTYPE_ID, _check_distinct_rows, _check_head_weight, _check_rope_table, _need_cuda, _one_device, _p, _stream
 
 
@@ -74,13 +74,13 @@ class PagedKVCache:
         return k[:, :, :max_total_kv], v[:, :, :max_total_kv]
 
 
-def _heads(name: str, x: torch.Tensor):
+def _heads(x: torch.Tensor):
     """``x`` with unit stride along D, and its (batch, head, frame) strides."""
     sb, sh, st, unit = x.stride()
     if unit != 1:
         x = x.contiguous()
         sb, sh, st, unit = x.stride()
-    return x, _Strides(sb, sh, st)
+    return x, _stride_array(sb, sh, st)
 
 
 def _write_rope(entry, pools, num_blocks, block_size, pool_heads, pool_dim, block_table, new_k, new_v, offset, cos_sin, q, q_weight,
@@ -96,11 +96,15 @@ def _write_rope(entry, pools, num_blocks, block_size, pool_heads, pool_dim, bloc
     block_table = _table32(block_table, B)
     if isinstance(offset, int):
         offset = torch.full((B,), offset, dtype=torch.int32, device=new_k.device)
-    offset, rope_offset, new_lens = _index32("offset", offset, B), _index32("rope_offset", rope_offset, B), _index32("new_lens", new_lens, B)
+    offset = _index32("offset", offset, B)
+    if rope_offset is not None:
+        rope_offset = _index32("rope_offset", rope_offset, B)
+    if new_lens is not None:
+        new_lens = _index32("new_lens", new_lens, B)
     _one_device(new_k, *pools, block_table, new_v, offset, rope_offset, new_lens, cos_sin, q, q_weight, k_weight, q_out)
     rows, rotary = _check_rope_table(cos_sin, D)
-    new_k, ks = _heads("new_k", new_k)
-    new_v, vs = _heads("new_v", new_v)
+    new_k, ks = _heads(new_k)
+    new_v, vs = _heads(new_v)
     H, src, dst, qs, qo = 0, None, None, None, None
     if q is not None:
         if q.dim() != 4 or q.dtype != dtype or q.shape[0] != B or q.shape[2:] != (T, D):
@@ -108,14 +112,17 @@ def _write_rope(entry, pools, num_blocks, block_size, pool_heads, pool_dim, bloc
         H = q.shape[1]
         if q_out is None:
             q_out = torch.empty_like(q)
+            if q_out.stride(3) != 1:
+                q_out = torch.empty(q.shape, dtype=dtype, device=q.device)
         else:
             if q_out.shape != q.shape or q_out.dtype != dtype:
                 raise ValueError("q_out must have q's shape and dtype")
+            if q_out.stride(3) != 1:
+                raise ValueError("q_out needs unit stride along D")
             _check_distinct_rows(q_out=q_out)
-        if q_out.stride(3) != 1:
-            raise ValueError("q and q_out need unit stride along D")
-        q, qs = _heads("q", q)
-        src, dst, qo = q.data_ptr(), q_out.data_ptr(), _Strides(*q_out.stride()[:3])
+        q, qs = _heads(q)
+        sb, sh, st, _ = q_out.stride()
+        src, dst, qo = q.data_ptr(), q_out.data_ptr(), _stride_array(sb, sh, st)
     elif q_out is not None or q_weight is not None:
         raise ValueError("q_out and q_weight need q")
     _lib.call(entry, dst, qo, *[p.data_ptr() for p in pools], src, qs, new_k.data_ptr(), ks, new_v.data_ptr(), vs,
