@@ -39,8 +39,6 @@ int g_path = 0;   // tunable "fmha_q4_path": 0 by size, 1 the few-row form, 2 th
 
 namespace {
 
-constexpr int kWarps = 4;
-
 // S = A B + C in fp16 with fp32 accumulators
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t* a, uint32_t b0, uint32_t b1, const float (&c)[4]) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
@@ -67,6 +65,8 @@ __device__ __forceinline__ void lds(uint32_t p, uint32_t* r) {
   else asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p));
 }
 
+constexpr int kMaxParts = 4;   // blocks of a cluster
+
 // A tile of 32 keys in the ring: codes of K and V, then their scales.  In rows of 64 bytes the upper two 16-byte pieces of every
 // second pair of rows change places with the lower two, which halves the V reads' bank conflicts (their rows are 2 t apart).
 template <int D>
@@ -77,20 +77,20 @@ struct Tile {
   static __device__ __forceinline__ int at(int row, int byte) { return row * kRow + (D == 128 ? byte ^ ((row & 2) << 4) : byte); }
 };
 
-template <int D, int NT>
+template <int D, int NT, int kWarps>
 struct Merge {   // a warp's, and then the block's, maxima, sums and outputs
   float m[kWarps][8 * NT], l[kWarps][8 * NT];
   float o[kWarps][8 * NT][D + 4];
 };
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? (D == 64 ? 5 : 4) : NT == 2 ? (D == 64 ? 4 : 3) : 2)
+template <typename T, int D, int NT, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, (NT == 1 ? (D == 64 ? 20 : 16) : NT == 2 ? (D == 64 ? 16 : 12) : 8) / kWarps)
 fmha_q4_kernel(const Args a, const int parts, const int ways, const int row_blocks, const int groups) {
   constexpr int G = D / 32, VW = G / 2;   // groups of a row; words of a V row that a lane holds
   constexpr int NR = 8 * NT;
   using Ring = Tile<D>;
   extern __shared__ __align__(16) uint8_t smem[];
-  Merge<D, NT>& sh = *reinterpret_cast<Merge<D, NT>*>(smem);   // after the walk, in the rings' place
+  Merge<D, NT, kWarps>& sh = *reinterpret_cast<Merge<D, NT, kWarps>*>(smem);   // after the walk, in the rings' place
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -106,6 +106,32 @@ fmha_q4_kernel(const Args a, const int parts, const int ways, const int row_bloc
   const int len = a.seqlens[b], q_len = a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq;
   const int capacity = static_cast<int>(a.blocks_per_seq * a.block_size);
   const int start = a.seqstarts ? max(a.seqstarts[b], 0) : 0;
+
+  // A tile's halves are 16 keys of one page each: half h of tile i is unit 2 i + h, in block (2 i + h) / units of the table.  The
+  // walk keeps quotient and remainder, and looks a block up two tiles ahead.
+  const int units = static_cast<int>(a.block_size) / 16, table_len = static_cast<int>(a.blocks_per_seq);
+  const int32_t* table = a.block_table + b * a.blocks_per_seq;
+  const int step = ways * parts, step_blocks = 2 * step / units, step_units = 2 * step - step_blocks * units;
+  int tile = start / 32 + part * ways + way;
+  struct Place {
+    int page0, page1;   // as the table has them
+    int unit;           // of the first half in its block; the second's is the next one, or the next block's first
+  };
+  int ahead_block = 2 * tile / units, ahead_unit = 2 * tile - ahead_block * units;
+  auto look_ahead = [&]() {   // the place of the next tile of the walk
+    Place p;
+    p.unit = ahead_unit;
+    const int block1 = ahead_block + (ahead_unit + 1 == units);
+    p.page0 = ahead_block < table_len ? __ldg(table + ahead_block) : -1;
+    p.page1 = block1 < table_len ? __ldg(table + block1) : -1;
+    ahead_block += step_blocks;
+    ahead_unit += step_units;
+    if (ahead_unit >= units) ahead_unit -= units, ++ahead_block;
+    return p;
+  };
+  Place first[Ring::kStages];   // the look-ups of the first tiles are on their way while the lengths are
+#pragma unroll
+  for (int i = 0; i < Ring::kStages; ++i) first[i] = look_ahead();
 
   // keys that a row may see: [start, limit)
   auto limit_of = [&](int r) {
@@ -127,6 +153,43 @@ fmha_q4_kernel(const Args a, const int parts, const int ways, const int row_bloc
   const int end = last_row >= row0 ? limit_of(last_row) : 0;
   const int all_end = last_row >= row0 ? limit_of(row0) : 0;   // padding rows see nothing, and nobody reads what they hold
 
+  const int tile_end = (end + 31) / 32;
+  auto known = [&](int page) { return static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_blocks); };
+  // copies of a tile: a half's codes are one run of 16 rows, its scales another
+  const uint32_t ring = ptx::smem_u32(smem) + warp * (Ring::kStages * Ring::kBytes);
+  constexpr int kPieces = Ring::kCodes / 2 / 16;      // of a half: 32 or 64
+  const uint32_t to = Ring::at(lane * 16 / Ring::kRow, lane * 16 % Ring::kRow);
+  constexpr int kScalePieces = Ring::kScales / 16;    // of a tile's K or V: 8 or 16 lanes
+  const bool scale_lane = lane < 2 * kScalePieces, scale_half = lane % kScalePieces >= kScalePieces / 2;
+  const uint64_t k_codes = reinterpret_cast<uint64_t>(a.k_codes) + lane * 16, v_codes = reinterpret_cast<uint64_t>(a.v_codes) + lane * 16;
+  const uint64_t scales = reinterpret_cast<uint64_t>(lane >= kScalePieces ? a.v_scales : a.k_scales) + lane % (kScalePieces / 2) * 16;
+  const uint32_t page_bytes = a.Hkv * static_cast<uint32_t>(a.block_size) * Ring::kRow, head_bytes = hk * static_cast<uint32_t>(a.block_size) * Ring::kRow;
+  uint32_t there = 0;   // two bits a tile in the ring: its halves have pages
+  auto fetch = [&](const Place& p, uint32_t stage) {
+    // a half without a page reads page 0 and is masked
+    const bool k0 = known(p.page0), k1 = known(p.page1);
+    const int unit1 = p.unit + 1 == units ? 0 : p.unit + 1;
+    const uint64_t o0 = static_cast<uint64_t>(k0 ? static_cast<uint32_t>(p.page0) : 0u) * page_bytes + (head_bytes + static_cast<uint32_t>(p.unit) * (16 * Ring::kRow));
+    const uint64_t o1 = static_cast<uint64_t>(k1 ? static_cast<uint32_t>(p.page1) : 0u) * page_bytes + (head_bytes + static_cast<uint32_t>(unit1) * (16 * Ring::kRow));
+#pragma unroll
+    for (int i = 0; i < kPieces / 32; ++i) {          // 512 bytes further: 8 or 16 rows, the same place in the row
+      copy16(stage + Ring::kK + to + i * 512, k_codes + o0 + i * 512);
+      copy16(stage + Ring::kK + to + Ring::kCodes / 2 + i * 512, k_codes + o1 + i * 512);
+      copy16(stage + Ring::kV + to + i * 512, v_codes + o0 + i * 512);
+      copy16(stage + Ring::kV + to + Ring::kCodes / 2 + i * 512, v_codes + o1 + i * 512);
+    }
+    if (scale_lane) copy16(stage + Ring::kKs + lane * 16, scales + ((scale_half ? o1 : o0) >> 3));   // a row has an eighth of its codes' bytes
+    there |= (k0 ? 1u : 0u) << (2 * Ring::kStages - 2) | (k1 ? 2u : 0u) << (2 * Ring::kStages - 2);
+  };
+  auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+
+#pragma unroll
+  for (int i = 0; i < Ring::kStages - 1; ++i) {
+    there >>= 2;
+    if (tile + i * step < tile_end) fetch(first[i], ring + i * Ring::kBytes);
+    commit();
+  }
+  Place next = first[Ring::kStages - 1];
   // ---- queries as the second operand: column g, dims of octet t of each group
   uint32_t qf[NT][G][4];
   float bias[NT][G][4], unit[NT][2];   // `unit` takes a column's sums to scores in the log2 domain
@@ -178,66 +241,6 @@ fmha_q4_kernel(const Args a, const int parts, const int ways, const int row_bloc
 #pragma unroll
   for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = kEmpty, l[n][0] = l[n][1] = 0.f;
 
-  // A tile's halves are 16 keys of one page each: half h of tile i is unit 2 i + h, in block (2 i + h) / units of the table.  The
-  // walk keeps quotient and remainder, and looks a block up two tiles ahead.
-  const int units = static_cast<int>(a.block_size) / 16, table_len = static_cast<int>(a.blocks_per_seq);
-  const int32_t* table = a.block_table + b * a.blocks_per_seq;
-  const int step = ways * parts, step_blocks = 2 * step / units, step_units = 2 * step - step_blocks * units;
-  const int tile_end = (end + 31) / 32;
-  int tile = start / 32 + part * ways + way;
-  struct Place {
-    int page0, page1;   // as the table has them
-    int unit;           // of the first half in its block; the second's is the next one, or the next block's first
-  };
-  int ahead_block = 2 * tile / units, ahead_unit = 2 * tile - ahead_block * units;
-  auto look_ahead = [&]() {   // the place of the next tile of the walk
-    Place p;
-    p.unit = ahead_unit;
-    const int block1 = ahead_block + (ahead_unit + 1 == units);
-    p.page0 = ahead_block < table_len ? __ldg(table + ahead_block) : -1;
-    p.page1 = block1 < table_len ? __ldg(table + block1) : -1;
-    ahead_block += step_blocks;
-    ahead_unit += step_units;
-    if (ahead_unit >= units) ahead_unit -= units, ++ahead_block;
-    return p;
-  };
-  auto known = [&](int page) { return static_cast<uint32_t>(page) < static_cast<uint32_t>(a.num_blocks); };
-  // copies of a tile: a half's codes are one run of 16 rows, its scales another
-  const uint32_t ring = ptx::smem_u32(smem) + warp * (Ring::kStages * Ring::kBytes);
-  constexpr int kPieces = Ring::kCodes / 2 / 16;      // of a half: 32 or 64
-  const uint32_t to = Ring::at(lane * 16 / Ring::kRow, lane * 16 % Ring::kRow);
-  constexpr int kScalePieces = Ring::kScales / 16;    // of a tile's K or V: 8 or 16 lanes
-  const bool scale_lane = lane < 2 * kScalePieces, scale_half = lane % kScalePieces >= kScalePieces / 2;
-  const uint64_t k_codes = reinterpret_cast<uint64_t>(a.k_codes) + lane * 16, v_codes = reinterpret_cast<uint64_t>(a.v_codes) + lane * 16;
-  const uint64_t scales = reinterpret_cast<uint64_t>(lane >= kScalePieces ? a.v_scales : a.k_scales) + lane % (kScalePieces / 2) * 16;
-  const uint32_t page_bytes = a.Hkv * static_cast<uint32_t>(a.block_size) * Ring::kRow, head_bytes = hk * static_cast<uint32_t>(a.block_size) * Ring::kRow;
-  uint32_t there = 0;   // two bits a tile in the ring: its halves have pages
-  auto fetch = [&](const Place& p, uint32_t stage) {
-    // a half without a page reads page 0 and is masked
-    const bool k0 = known(p.page0), k1 = known(p.page1);
-    const int unit1 = p.unit + 1 == units ? 0 : p.unit + 1;
-    const uint64_t o0 = static_cast<uint64_t>(k0 ? static_cast<uint32_t>(p.page0) : 0u) * page_bytes + (head_bytes + static_cast<uint32_t>(p.unit) * (16 * Ring::kRow));
-    const uint64_t o1 = static_cast<uint64_t>(k1 ? static_cast<uint32_t>(p.page1) : 0u) * page_bytes + (head_bytes + static_cast<uint32_t>(unit1) * (16 * Ring::kRow));
-#pragma unroll
-    for (int i = 0; i < kPieces / 32; ++i) {          // 512 bytes further: 8 or 16 rows, the same place in the row
-      copy16(stage + Ring::kK + to + i * 512, k_codes + o0 + i * 512);
-      copy16(stage + Ring::kK + to + Ring::kCodes / 2 + i * 512, k_codes + o1 + i * 512);
-      copy16(stage + Ring::kV + to + i * 512, v_codes + o0 + i * 512);
-      copy16(stage + Ring::kV + to + Ring::kCodes / 2 + i * 512, v_codes + o1 + i * 512);
-    }
-    if (scale_lane) copy16(stage + Ring::kKs + lane * 16, scales + ((scale_half ? o1 : o0) >> 3));   // a row has an eighth of its codes' bytes
-    there |= (k0 ? 1u : 0u) << (2 * Ring::kStages - 2) | (k1 ? 2u : 0u) << (2 * Ring::kStages - 2);
-  };
-  auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
-
-  Place next = look_ahead();
-#pragma unroll
-  for (int i = 0; i < Ring::kStages - 1; ++i) {
-    there >>= 2;
-    if (tile + i * step < tile_end) fetch(next, ring + i * Ring::kBytes);
-    commit();
-    next = look_ahead();
-  }
   const uint32_t k_lane = g * Ring::kRow + Ring::at(g, t * (G * 4)) % Ring::kRow;
   const uint32_t v_lane = 2 * t * Ring::kRow + Ring::at(2 * t, g * (VW * 4)) % Ring::kRow;
   uint32_t stage = ring, free_stage = ring + (Ring::kStages - 1) * Ring::kBytes;
@@ -462,69 +465,62 @@ fmha_q4_kernel(const Args a, const int parts, const int ways, const int row_bloc
     ptx::cluster_sync();
   }
   // Rows of the warp's own group, dealt over its warps; with a cluster (the block is one group) over those of all blocks.
-  const int sources = parts > 1 ? parts : ways, first = warp - way;
-  auto remote = [&](const float* p, int rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ptx::map_to_cta(p, rank)) : "memory");
-    return v;
-  };
+  const int first_warp = warp - way;
   for (int i = (part * ways + way) * 32 + lane; i < NR * (D / 8); i += parts * ways * 32) {
     const int n = i / (D / 8), d = i % (D / 8) * 8, r = row0 + n;
     if (r >= rows) continue;
-    float ms[8], top = kEmpty, sum = 0.f, acc[8] = {};
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      if (w < sources) {
-        ms[w] = parts > 1 ? remote(&sh.m[0][n], w) : sh.m[(first + w) & (kWarps - 1)][n];
-        top = fmaxf(top, ms[w]);
+    float top = kEmpty, sum = 0.f, acc[8] = {};
+    if (parts == 1) {
+      for (int w = first_warp; w < first_warp + ways; ++w) top = fmaxf(top, sh.m[w][n]);
+      for (int w = first_warp; w < first_warp + ways; ++w) {
+        const float f = ex2(sh.m[w][n] - top);
+        const float4 a0 = *reinterpret_cast<const float4*>(&sh.o[w][n][d]), a1 = *reinterpret_cast<const float4*>(&sh.o[w][n][d + 4]);
+        sum = fmaf(f, sh.l[w][n], sum);
+        acc[0] = fmaf(f, a0.x, acc[0]), acc[1] = fmaf(f, a0.y, acc[1]), acc[2] = fmaf(f, a0.z, acc[2]), acc[3] = fmaf(f, a0.w, acc[3]);
+        acc[4] = fmaf(f, a1.x, acc[4]), acc[5] = fmaf(f, a1.y, acc[5]), acc[6] = fmaf(f, a1.z, acc[6]), acc[7] = fmaf(f, a1.w, acc[7]);
       }
-    }
+    } else {   // all loads from the other blocks on their way before the first is used; ranks past the last one read it again
+      float ms[kMaxParts], ls[kMaxParts], v[kMaxParts][8];
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      if (w < sources) {
-        const float f = ex2(ms[w] - top);
-        const int from = (first + w) & (kWarps - 1);
-        sum = fmaf(f, parts > 1 ? remote(&sh.l[0][n], w) : sh.l[from][n], sum);
-        float v[8];
-        if (parts > 1) {
+      for (int w = 0; w < kMaxParts; ++w) {
+        const int rank = min(w, parts - 1);
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(ms[w]) : "r"(ptx::map_to_cta(&sh.m[0][n], rank)));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(ls[w]) : "r"(ptx::map_to_cta(&sh.l[0][n], rank)));
+        const uint32_t src = ptx::map_to_cta(&sh.o[0][n][d], rank);
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-            asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[4 * x]), "=f"(v[4 * x + 1]), "=f"(v[4 * x + 2]), "=f"(v[4 * x + 3])
-                         : "r"(ptx::map_to_cta(&sh.o[0][n][d + 4 * x], w)) : "memory");
-        } else {
+        for (int x = 0; x < 8; x += 4)
+          asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[w][x]), "=f"(v[w][x + 1]), "=f"(v[w][x + 2]), "=f"(v[w][x + 3]) : "r"(src + 4 * x));
+      }
 #pragma unroll
-          for (int x = 0; x < 8; ++x) v[x] = sh.o[from][n][d + x];
+      for (int w = 0; w < kMaxParts; ++w) top = fmaxf(top, ms[w]);
+#pragma unroll
+      for (int w = 0; w < kMaxParts; ++w) {
+        if (w < parts) {
+          const float f = ex2(ms[w] - top);
+          sum = fmaf(f, ls[w], sum);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) acc[x] = fmaf(f, v[w][x], acc[x]);
         }
-#pragma unroll
-        for (int x = 0; x < 8; ++x) acc[x] = fmaf(f, v[x], acc[x]);
       }
     }
     const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;   // NaN stays
+    const int tq = r / share;
     Pack<T> out;
 #pragma unroll
-    for (int x = 0; x < 8; ++x) out.v[x] = Elem<T>::from_f(r / share < q_len ? acc[x] * inv : 0.f);
-    st128(static_cast<T*>(a.out) + b * a.os_b + (hk * share + r % share) * a.os_h + static_cast<int64_t>(r / share) * a.os_t + d, out);
+    for (int x = 0; x < 8; ++x) out.v[x] = Elem<T>::from_f(tq < q_len ? acc[x] * inv : 0.f);
+    st128(static_cast<T*>(a.out) + b * a.os_b + (hk * share + r - tq * share) * a.os_h + static_cast<int64_t>(tq) * a.os_t + d, out);
   }
   if (parts > 1) ptx::cluster_sync();   // nobody leaves while its sums are read
 }
 
-template <typename T, int D, int NT>
-int launch(const Args& a, cudaStream_t s) {
-  const int64_t rows = static_cast<int64_t>(a.H / a.Hkv) * a.Tq, row_blocks = (rows + 8 * NT - 1) / (8 * NT);
-  const int64_t groups = static_cast<int64_t>(a.B) * a.Hkv * row_blocks, tiles = (a.blocks_per_seq * a.block_size + 31) / 32;
-  // Warps that share a group: until the SMs are full (down to two tiles each), and so many that none walks more than 32 tiles.  Fewer
-  // leave the longest sequences of a ragged batch running alone, more pay a block's start and end (some 8 us of latency) more often:
-  // 128 sequences of 500 to 8191 keys, 8 key heads of 128, take 212 / 187 / 205 / 274 us with 4 / 8 / 16 / 32 warps, 256 chunks of 16
-  // rows over up to 1001 keys, 8 heads of 64, take 68 / 54 / 61 us with 1 / 2 / 4.
-  int splits = 1;
-  while (splits < 32 && (tiles > 32 * splits || (groups * splits < sm_count() * 16 && tiles > 2 * splits))) splits *= 2;
-  const int ways = splits < kWarps ? splits : kWarps, parts = splits / ways;
+template <typename T, int D, int NT, int kWarps>
+int launch(const Args& a, int ways, int parts, int64_t row_blocks, int64_t groups, cudaStream_t s) {
   const int64_t blocks = (groups + kWarps / ways - 1) / (kWarps / ways) * parts;
   OB_REQUIRE(groups <= 0x7fffffff && blocks <= 0x7fffffff, OASR_ERR_INVALID, "fmha_q4: too many rows for one call");
   static SmemLimit limit;
-  constexpr int kRings = kWarps * Tile<D>::kStages * Tile<D>::kBytes, kMerge = sizeof(Merge<D, NT>);
+  constexpr int kRings = kWarps * Tile<D>::kStages * Tile<D>::kBytes, kMerge = sizeof(Merge<D, NT, kWarps>);
   constexpr int kSmem = kRings > kMerge ? kRings : kMerge;
-  cudaError_t e = limit.raise(fmha_q4_kernel<T, D, NT>, kSmem);
+  cudaError_t e = limit.raise(fmha_q4_kernel<T, D, NT, kWarps>, kSmem);
   if (e != cudaSuccess) return set_error(OASR_ERR_CUDA, "fmha_q4: shared memory limit: %s", cudaGetErrorString(e));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
@@ -538,8 +534,22 @@ int launch(const Args& a, cudaStream_t s) {
   at[1].val.clusterDim = {static_cast<unsigned>(parts), 1, 1};
   cfg.attrs = at;
   cfg.numAttrs = parts > 1 ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, fmha_q4_kernel<T, D, NT>, a, parts, ways, static_cast<int>(row_blocks), static_cast<int>(groups));
+  cudaLaunchKernelEx(&cfg, fmha_q4_kernel<T, D, NT, kWarps>, a, parts, ways, static_cast<int>(row_blocks), static_cast<int>(groups));
   return check_launch("fmha_q4 launch");
+}
+
+template <typename T, int D, int NT>
+int launch(const Args& a, cudaStream_t s) {
+  const int64_t rows = static_cast<int64_t>(a.H / a.Hkv) * a.Tq, row_blocks = (rows + 8 * NT - 1) / (8 * NT);
+  const int64_t groups = static_cast<int64_t>(a.B) * a.Hkv * row_blocks, tiles = (a.blocks_per_seq * a.block_size + 31) / 32;
+  // Warps that share a group: until the SMs are full (down to two tiles each), and so many that none walks more than 32 tiles.  Fewer
+  // leave the longest sequences of a ragged batch running alone, more pay a block's start and end (some 6 us of latency) more often:
+  // 128 sequences of 500 to 8191 keys, 8 key heads of 128, take 186 / 176 / 189 us with 4 / 8 / 16 warps, 256 chunks of 16 rows over up
+  // to 1001 keys, 8 heads of 64, take 60 / 50 / 52 us with 1 / 2 / 4.  Beyond eight, blocks of eight in a cluster.
+  int splits = 1;
+  while (splits < 8 * kMaxParts && (tiles > 32 * splits || (groups * splits < sm_count() * 16 && tiles > 2 * splits))) splits *= 2;
+  if (splits <= 4) return launch<T, D, NT, 4>(a, splits, 1, row_blocks, groups, s);
+  return launch<T, D, NT, 8>(a, 8, splits / 8, row_blocks, groups, s);
 }
 
 template <typename T, int D>
