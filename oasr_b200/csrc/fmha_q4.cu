@@ -14,7 +14,7 @@
 //       LOP3 per two codes and a shift per four, exact.  The queries carry what that needs: each row is brought to 2^10 by a power of two (bf16
 //       reaches further than fp16; exact but for what is 2^-34 of the row's largest), every second dim by 1 / 16 more.  The
 //       offsets come off in the accumulator, which starts at -(1032 sum of even + 72 sum of odd q) of the group; a group's
-//       sums are scaled in fp32 afterwards.
+//       sums are scaled in fp32 afterwards.  What fp32 sums of that size round is at most 2^-13 of sum |q| times the largest code.
 //   V   the lane holds words g D / 64 (+ 1) of keys 8 x + 2 t and 8 x + 2 t + 1.  Long sums would drown under such an offset, so here the operand is
 //       (n - 8) * scale, exact in the type (q4.cuh).  In bf16 the second nibble has no room behind an exponent: left alone it is
 //       the number n 2^-129 (gradual underflow joins the normal numbers at n = 8), which one FMA takes to (n - 8) / 4.
@@ -594,7 +594,7 @@ extern "C" int oasr_b200_fmha_q4(void* out, const int64_t* out_strides, const vo
   OB_REQUIRE(B <= 65535 && H <= 65535 && Tq <= 0x7fffff && blocks_per_seq * block_size <= 0x7fffffff, OASR_ERR_INVALID,
              "fmha_q4: batch, head count or length too large");
   if (B == 0 || Tq == 0) return OASR_OK;
-  OB_REQUIRE(out && out_strides && q && q_strides && k_codes && k_scales && v_codes && v_scales && block_table && seqlens, OASR_ERR_INVALID,
+  OB_REQUIRE(out && out_strides && q && q_strides && k_codes && k_scales && v_codes && v_scales && (block_table || blocks_per_seq == 0) && seqlens, OASR_ERR_INVALID,
              "fmha_q4: null pointer argument");
   for (int i = 0; i < 3; ++i)
     OB_REQUIRE(out_strides[i] % 8 == 0 && q_strides[i] % 8 == 0, OASR_ERR_ALIGN, "fmha_q4: strides must be multiples of 8 elements");

@@ -187,7 +187,8 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_l
   const float unit = fabsf(m) > 1e38f ? 0x1p-90f : kLog2e;
   const float m2 = m == -INFINITY ? 0.f : m * unit;
   const float edge_d = max_nan(fmaf(edge, unit, -m2), kFar);
-  float s = ex2(edge_d), w = edge_d * s;
+  // four sums of each: shorter chains, and the likeliest token's 1 costs fewer of the small terms their last bits
+  float s4[4] = {ex2(edge_d)}, w4[4] = {edge_d * s4[0]};
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     float x[VE];
@@ -196,12 +197,11 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_l
     for (int j = 0; j < VE; ++j) {
       const float d = max_nan(fmaf(x[j], unit, -m2), kFar);
       const float e = ex2(d);
-      s += e;
-      w = fmaf(d, e, w);
+      s4[j & 3] += e;
+      w4[j & 3] = fmaf(d, e, w4[j & 3]);
     }
   }
-  s = warp_sum(s);
-  w = warp_sum(w);
+  float s = warp_sum((s4[0] + s4[1]) + (s4[2] + s4[3])), w = warp_sum((w4[0] + w4[1]) + (w4[2] + w4[3]));
   if (m != -INFINITY) {
     const float shift = fmaf(m, unit, -m2), f = ex2(-shift);   // m2 + shift is m * unit
     w = fmaf(-shift, s, w) * f;

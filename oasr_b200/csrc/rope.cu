@@ -387,7 +387,7 @@ int write_common(bool q4, void* q_out, const int64_t* qo, void* k_pool, void* k_
              "write_kv_rope: rotary_dim must be a multiple of 16 up to head_dim (got %lld)", (long long)rotary_dim);
   OB_REQUIRE(table_rows > 0, OASR_ERR_INVALID, "write_kv_rope: empty position table");
   if (B == 0 || T == 0) return OASR_OK;
-  OB_REQUIRE(k_pool && v_pool && k && v && ks && vs && table && block_table && offsets && (!q4 || (k_scales && v_scales)) &&
+  OB_REQUIRE(k_pool && v_pool && k && v && ks && vs && table && (block_table || blocks_per_seq == 0) && offsets && (!q4 || (k_scales && v_scales)) &&
                  (H == 0 || (q && q_out && qs && qo)),
              OASR_ERR_INVALID, "write_kv_rope: null pointer argument");
   OB_REQUIRE(strides8(ks[0], ks[1], ks[2]) && strides8(vs[0], vs[1], vs[2]) &&
@@ -487,7 +487,7 @@ int oasr_b200_paged_kv_gather_q4(void* k_out, void* v_out, const void* k_codes, 
              "paged_kv_gather_q4: bad shape");
   OB_REQUIRE(D % 32 == 0 && D <= 512, OASR_ERR_UNSUPPORTED, "paged_kv_gather_q4: head_dim must be a multiple of 32 up to 512 (got %lld)", (long long)D);
   if (B == 0 || T == 0) return OASR_OK;
-  OB_REQUIRE(k_out && v_out && k_codes && k_scales && v_codes && v_scales && block_table, OASR_ERR_INVALID,
+  OB_REQUIRE(k_out && v_out && k_codes && k_scales && v_codes && v_scales && (block_table || blocks_per_seq == 0), OASR_ERR_INVALID,
              "paged_kv_gather_q4: null pointer argument");
   OB_REQUIRE(is_aligned(k_out, 16) && is_aligned(v_out, 16) && is_aligned(k_codes, 16) && is_aligned(v_codes, 16), OASR_ERR_ALIGN,
              "paged_kv_gather_q4: operands must be 16-byte aligned");

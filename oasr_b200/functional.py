@@ -609,9 +609,12 @@ def _check_distinct_rows(**outs) -> None:
     for name, t in outs.items():
         if t is None or t.is_contiguous():
             continue
-        for extent, stride in sorted(zip(t.shape[:-1], t.stride()[:-1]), key=lambda p: p[1]):
-            if extent > 1 and stride < t.size(-1):
-                raise RuntimeError(f"{name} must not overlap itself")
+        span = t.size(-1)
+        for stride, extent in sorted(zip(t.stride()[:-1], t.shape[:-1])):
+            if extent > 1:
+                if stride < span:
+                    raise RuntimeError(f"{name} must not overlap itself")
+                span += (extent - 1) * stride
 
 
 class TokenLogProbs(NamedTuple):

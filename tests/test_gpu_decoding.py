@@ -433,6 +433,14 @@ def test_fmha_q4_refusals():
         x, p = args.pop("q", q), args.pop("pools", pools)
         with pytest.raises((RuntimeError, ValueError)):
             ob.fmha_q4(x, *p, **args)
+    packed = torch.zeros(2 * 4 * 64 + 64, device="cuda").bfloat16()
+    with pytest.raises(RuntimeError):                     # heads one row apart, sequences two: some rows are the same memory
+        ob.fmha_q4(q, *pools, out=packed.as_strided((2, 4, 1, 64), (128, 64, 64, 1)), **good)
+    for form in (1, 2):                                   # no pages at all
+        ob.tunables.set("fmha_q4_path", form)
+        assert not ob.fmha_q4(q + 1, *pools, softmax_scale=1.0, block_table=bt[:, :0], cache_seqlens=lens).any()
+    ob.tunables.set("fmha_q4_path", 0)
+    assert not any(x.any() for x in ob.gather_paged_kv_q4(*pools, bt[:, :0], None, 3))
     assert ob.fmha_q4(q[:, :, :0], *pools, **good).shape == (2, 4, 0, 64)
     assert ob.fmha_q4(q[:0], *pools, softmax_scale=1.0, block_table=bt[:0], cache_seqlens=lens[:0]).shape == (0, 4, 1, 64)
 
