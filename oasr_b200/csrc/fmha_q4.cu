@@ -11,21 +11,25 @@
 // for.  Per 32 keys of a warp, with g = lane / 4 and t = lane % 4:
 //   K   the lane holds words t G .. t G + G - 1 (an octet of each group) of keys g + 8 x.  The operand, fp16 for either
 //       type, is the code behind a magic exponent: 1024 + n where the nibble lies lowest, 1024 + 16 n where it lies second, one
-//       LOP3 per two codes and a shift per four, exact.  The queries carry what that needs: each row is brought to 2^10 by a power of two (bf16
-//       reaches further than fp16; exact but for what is 2^-34 of the row's largest), every second dim by 1 / 16 more.  The
-//       offsets come off in the accumulator, which starts at -(1032 sum of even + 72 sum of odd q) of the group; a group's
+//       LOP3 per two codes and a shift per four, exact.  The queries carry what that needs: each row is brought to 2^10 by a
+//       power of two (bf16 reaches further than fp16; exact but for what is 2^-34 of the row's largest), every second dim by
+//       1 / 16 more.  The offsets come off in the accumulator, which starts at -(1032 sum of even + 72 sum of odd q) of the group; a group's
 //       sums are scaled in fp32 afterwards.  What fp32 sums of that size round is at most 2^-13 of sum |q| times the largest code.
-//   V   the lane holds words g D / 64 (+ 1) of keys 8 x + 2 t and 8 x + 2 t + 1.  Long sums would drown under such an offset, so here the operand is
-//       (n - 8) * scale, exact in the type (q4.cuh).  In bf16 the second nibble has no room behind an exponent: left alone it is
+//   V   the lane holds words g D / 64 (+ 1) of keys 8 x + 2 t and 8 x + 2 t + 1.  Long sums would drown under such an offset, so
+//       here the operand is (n - 8) * scale, exact in the type (q4.cuh).  In bf16 the second nibble has no room behind an exponent: left alone it is
 //       the number n 2^-129 (gradual underflow joins the normal numbers at n = 8), which one FMA takes to (n - 8) / 4.
 //   P   the scores' fragment is the transpose of what the second product reads: movmatrix.
 // The ALU (logic, shifts, permutes: half a warp instruction a clock) is the busiest unit; the FMA pipe, which does the rest of the
 // conversion, is not.
-// The running maximum moves only when a score passes it by 2^8 (weights stay below that, exact in either type): most tiles
+// The running maximum moves only when a score passes it by 2^8 (weights stay below that, finite in either type): most tiles
 // need one vote in the place of a reduction over the lanes.
 // Every warp walks its own tiles with its own maximum, sum and output, and has its own ring of tiles in shared memory, filled by
-// asynchronous copies (a tile is two runs of 16 keys of a page): no registers wait for memory, no warp for another.  One, two or four
+// asynchronous copies (a tile is two runs of 16 keys of a page): no registers wait for memory, no warp for another.  One to eight
 // warps of a block, or the blocks of a cluster, share a (sequence, key head, rows) and meet in shared memory at the end.
+//
+// B200: 64 sequences of 6000 keys, 32 heads of 128 over 8 key heads, one token each: 117-121 us (442 MB, 3.7 TB/s), bound by
+// instructions (some 700 of a warp for 32 keys; ALU 0.55 busy, issue slots 0.64).  256 chunks of 16 rows over up to 1001 keys, 8 heads of
+// 64: 51 us, a third of it a block's start (lengths, pages, first tile) and end.
 #include "common.cuh"
 #include "fmha_q4.cuh"
 #include "q4.cuh"
@@ -122,8 +126,8 @@ fmha_q4_kernel(const Args a, const int parts, const int ways, const int row_bloc
     Place p;
     p.unit = ahead_unit;
     const int block1 = ahead_block + (ahead_unit + 1 == units);
-    p.page0 = ahead_block < table_len ? __ldg(table + ahead_block) : -1;
-    p.page1 = block1 < table_len ? __ldg(table + block1) : -1;
+    p.page0 = ahead_block < table_len ? table[ahead_block] : -1;
+    p.page1 = block1 < table_len ? table[block1] : -1;
     ahead_block += step_blocks;
     ahead_unit += step_units;
     if (ahead_unit >= units) ahead_unit -= units, ++ahead_block;

@@ -13,6 +13,9 @@
 //
 // Converted rows hold the exact values (q4.cuh).  Within an octet the dims lie in the order 0 4 1 5 2 6 3 7, the pairs that one mask
 // of a code word gives; queries are stored in the same order, and the output's columns are put right when they are read.
+// B200: 4001 rows over 4098 keys, causal, 32 heads of 128 over 8 key heads: 224 us (614 TFLOP/s; 236 us with the weights through shared
+// memory).  A step of 128 keys takes 4.5k clocks: products 2.1k, a tile's softmax 2.9k, which its two warps a scheduler and 128
+// registers a thread set.
 // Shared memory at D = 128: Q 64 KB, K and V in five slots of 32 KB that follow one another K V K V.
 #include <cuda.h>
 
@@ -148,7 +151,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_q4_prompt_kernel(const Args 
   const int32_t* table = a.block_table + b * a.blocks_per_seq;
   auto page_of = [&](int unit) {   // of 16 keys; -1: none
     const int blk = unit / units;
-    const int page = blk < table_len ? __ldg(table + blk) : -1;
+    const int page = blk < table_len ? table[blk] : -1;
     return page < a.num_blocks ? page : -1;
   };
   bool ok = true;
@@ -220,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_q4_prompt_kernel(const Args 
     }
     auto ask = [&] {           // the pages of the next tile
 #pragma unroll
-      for (int p = 0; p < kPasses; ++p) page[p] = block[p] < table_len ? __ldg(table + block[p]) : -1;
+      for (int p = 0; p < kPasses; ++p) page[p] = block[p] < table_len ? table[block[p]] : -1;
     };
     auto resolve = [&] {       // rows of the pages asked for, and on to the next tile
       known = 0;
@@ -241,10 +244,10 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_q4_prompt_kernel(const Args 
     auto load = [&](Rows& r, const uint32_t* codes, const void* scales) {
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
-        r.w[p] = __ldg(reinterpret_cast<const uint4*>(codes) + row[p] * kLanes + piece);
+        r.w[p] = reinterpret_cast<const uint4*>(codes)[row[p] * kLanes + piece];
         const uint32_t* sc = static_cast<const uint32_t*>(scales) + row[p] * (G / 2);
 #pragma unroll
-        for (int i = 0; i < G / 2; ++i) r.s[p][i] = __ldg(sc + i);
+        for (int i = 0; i < G / 2; ++i) r.s[p][i] = sc[i];
       }
     };
     auto convert = [&](const Rows& r, uint8_t* slot) {
@@ -318,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_q4_prompt_kernel(const Args 
     const uint32_t t_s = tmem + lanes + kColS + x * 128, t_o = tmem + lanes + kColO + x * 128;
     auto ask = [&](int tile) {   // lane i < 8: the page of 16 keys, as the table has it (looked at a tile later)
       const int blk = (tile * 8 + lane) / units;
-      return lane < 8 && blk < table_len ? __ldg(table + blk) : -1;
+      return lane < 8 && blk < table_len ? table[blk] : -1;
     };
     int next_page = ask(tile0);
     for (int j = 0; j < tiles; ++j) {

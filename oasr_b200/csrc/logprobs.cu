@@ -8,9 +8,9 @@
 //
 // A warp owns up to 32 * NV granules of 16 bytes of one row and holds them in registers: they are read from memory once, and the
 // maximum, the sums and the selection all run on that copy.  Selection: the k-th largest of the 32 lane maxima is a lower bound
-// of the k-th largest value, so only what reaches it (a little over k values) goes to a list in shared memory, from which k
-// rounds of a warp-wide maximum take the alternatives in order.  A row whose list overflows (many equal values: a mask that
-// leaves fewer than k tokens) or that holds a NaN takes its rounds over the registers instead; the result is the same.
+// of the k-th largest value, so only what reaches it (a little over k values) goes to a list in shared memory, where every
+// lane counts how many are above its own.  A row whose list overflows (many equal values: a mask that leaves fewer than k tokens)
+// or that holds a NaN takes k rounds of a warp-wide maximum over the row instead; the result is the same.
 // Larger rows are split over the warps of a block, and over a cluster of blocks where the rows are few: the parts' statistics
 // and sorted lists meet in shared memory (the first block's, written through the cluster).
 #include <type_traits>
