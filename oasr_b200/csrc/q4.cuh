@@ -62,10 +62,6 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float scale) {
   return w;
 }
 
-__device__ __forceinline__ float value_of(uint32_t word, int i, float scale) {
-  return static_cast<float>(static_cast<int>((word >> (4 * i)) & 15u) - 8) * scale;
-}
-
 // word of octet o (dims 8 o .. 8 o + 7), and the octet of word j
 __device__ __forceinline__ int word_of_octet(int o, int groups) { return (o & 3) * groups + (o >> 2); }
 __device__ __forceinline__ int octet_of_word(int j, int groups) { return (j % groups) * 4 + j / groups; }

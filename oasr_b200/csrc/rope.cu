@@ -16,6 +16,7 @@
 // the copy rate; 0.61 of the issue slots); 20016 frames of 48 heads of 128 of which half are padding, into 4-bit pages, 106 us, bound by
 // instructions (0.76 of the issue slots: an exact code costs some 15); calls of a few tokens by their launch.
 #include "common.cuh"
+#include "fmha_q4.cuh"
 #include "q4.cuh"
 #include "sm100_ptx.cuh"
 
@@ -328,6 +329,15 @@ struct GatherArgs {
   uint32_t chunks;
 };
 
+// The eight values of a word in order; each is one product in T, rounded once where the scale has more than its five bits.
+template <typename T>
+__device__ __forceinline__ uint4 values_of(uint32_t w, uint32_t scale) {
+  using Op = fmha_q4::Op<T>;
+  const uint32_t s2 = scale | (scale << 16), s4 = Op::steep(s2), h = w >> 8;
+  const uint32_t a = Op::low(w, s2), b = Op::second(w, s4), c = Op::low(h, s2), d = Op::second(h, s4);   // dims (0, 4), (1, 5), (2, 6), (3, 7)
+  return make_uint4(fmha_q4::lows(a, b), fmha_q4::lows(c, d), fmha_q4::highs(a, b), fmha_q4::highs(c, d));
+}
+
 // out[b, h, i, :] = the values of position starts[b] + i; a word (8 values) of K and of V per thread.  A block takes `span`
 // positions of one (b, h), `rows` of them at a time.
 template <typename T>
@@ -347,18 +357,16 @@ __global__ void __launch_bounds__(256) gather_q4_kernel(const GatherArgs a) {
     const uint32_t logical = static_cast<uint32_t>(pos) / size;     // of positions from 0 on, below 2^32
     int64_t page = -1;
     if (pos >= 0 && logical < a.blocks_per_seq) page = a.block_table[b * a.blocks_per_seq + logical];
-    float k[8] = {}, v[8] = {};
+    uint4 k = make_uint4(0, 0, 0, 0), v = k;
     if (page >= 0 && page < a.num_blocks) {
       const int64_t row = (page * a.Hkv + h) * a.block_size + (static_cast<uint32_t>(pos) - logical * size);
       const uint32_t kw = a.k_codes[row * a.words + j], vw = a.v_codes[row * a.words + j];
-      const float ks = Elem<T>::to_f(static_cast<const T*>(a.k_scales)[row * a.groups + (o >> 2)]);
-      const float vs = Elem<T>::to_f(static_cast<const T*>(a.v_scales)[row * a.groups + (o >> 2)]);
-#pragma unroll
-      for (int d = 0; d < 8; ++d) k[d] = q4::value_of(kw, d, ks), v[d] = q4::value_of(vw, d, vs);
+      k = values_of<T>(kw, static_cast<const uint16_t*>(a.k_scales)[row * a.groups + (o >> 2)]);
+      v = values_of<T>(vw, static_cast<const uint16_t*>(a.v_scales)[row * a.groups + (o >> 2)]);
     }
     const int64_t dst = ((bh * a.T + i) * a.words + o) * 8;
-    store8(static_cast<T*>(a.k_out) + dst, k);
-    store8(static_cast<T*>(a.v_out) + dst, v);
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.k_out) + dst) = k;
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.v_out) + dst) = v;
   }
 }
 
