@@ -7,10 +7,10 @@
 // What the rounding of m2 shifts all of them by is taken out of the two sums afterwards.
 //
 // A warp owns up to 32 * NV granules of 16 bytes of one row and holds them in registers: they are read from memory once, and the
-// maximum, the sums and the selection all run on that copy.  Selection: the k-th largest of the 32 lane maxima is a lower bound
-// of the k-th largest value, so only what reaches it (a little over k values) goes to a list in shared memory, where every
-// lane counts how many are above its own.  A row whose list overflows (many equal values: a mask that leaves fewer than k tokens)
-// or that holds a NaN takes k rounds of a warp-wide maximum over the row instead; the result is the same.
+// maximum, the sums and the selection all run on that copy.  Selection: the k-th largest of 64 to 128 maxima of parts of the row is a
+// lower bound of its k-th largest value, so only what reaches it (a little over k values) goes to a list in shared memory, where
+// every lane counts how many are above its own.  A row whose list overflows (many equal values: a mask that leaves fewer than k
+// tokens) or that holds a NaN takes k rounds of a warp-wide maximum over the row instead; the result is the same.
 // Larger rows are split over the warps of a block, and over a cluster of blocks where the rows are few: the parts' statistics
 // and sorted lists meet in shared memory (the first block's, written through the cluster).
 #include <type_traits>
@@ -22,7 +22,7 @@ namespace ob {
 namespace {
 
 constexpr int kMaxTop = 32;
-constexpr int kList = 128;          // candidates a warp can hold
+constexpr int kList = 192;          // candidates a row can hold
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 constexpr float kFar = -200.f;      // 2^-200 is zero in fp32: the exponent of a masked (-inf) logit, which keeps d * exp2(d) at zero
 
@@ -118,16 +118,36 @@ __device__ __forceinline__ Stats warp_merge(Stats v) {
   return v;
 }
 
-template <int W>
+template <int W, int kRows>
 struct Shared {
-  uint64_t list[W][kList];
-  uint64_t sorted[W][kMaxTop];
-  int count[W];
+  uint64_t list[kRows][kList];          // candidates
+  int granule[kRows][kList];            // granules they are in (a warp to a row)
+  uint64_t sorted[W * kRows][kMaxTop];  // a warp's alternatives
+  uint64_t merged[kMaxTop];
+  int count;
   Stats stats[W];
+  alignas(16) uint32_t maxima[128];     // of parts of the block's slice
+  uint32_t bound;                       // the k-th largest of them
   // written by the other blocks of the cluster, read by the first
   uint64_t part_sorted[8][kMaxTop];
   Stats part_stats[8];
 };
+
+// The k largest of `found` (>= k) keys, in order: a key's place is the number of keys above it.
+__device__ __forceinline__ void rank_list(const uint64_t* list, int found, int k, uint64_t* out, int lane) {
+  for (int base = lane; base < found; base += 64) {
+    const uint64_t k0 = list[base], k1 = base + 32 < found ? list[base + 32] : 0;
+    int above0 = 0, above1 = 0;
+#pragma unroll 4
+    for (int i = 0; i < found; ++i) {
+      const uint64_t o = list[i];
+      above0 += o > k0;
+      above1 += o > k1;
+    }
+    if (above0 < k) out[above0] = k0;
+    if (base + 32 < found && above1 < k) out[above1] = k1;
+  }
+}
 
 // k rounds over `lists` sorted lists of k keys each (lane l walks list l); the result is sorted into `out`.
 __device__ __forceinline__ void merge_lists(const uint64_t (*lists)[kMaxTop], int n, int k, uint64_t* out, int lane) {
@@ -145,7 +165,7 @@ template <typename T, int W, int NV>
 __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_log_probs_kernel(const Args a, const int parts) {
   constexpr int VE = Elem<T>::kVec;
   constexpr int kRows = W == 1 ? 4 : 1;                 // rows of a block
-  __shared__ Shared<W * kRows> sh;
+  __shared__ Shared<W, kRows> sh;
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
   if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // waited for before the first remote write
@@ -175,10 +195,10 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_l
   const float edge = has_edge ? Elem<T>::to_f(x0[edge_at]) : -INFINITY;
 
   // ---- maximum and sums of the warp's part
-  float lane_max = granule_max<T>(g[0]);
+  float max0 = max_nan(edge, granule_max<T>(g[0])), max1 = -INFINITY;
 #pragma unroll
-  for (int i = 1; i < NV; ++i) lane_max = max_nan(lane_max, granule_max<T>(g[i]));
-  lane_max = max_nan(lane_max, edge);
+  for (int i = 1; i < NV; ++i) (i & 1 ? max1 : max0) = max_nan(i & 1 ? max1 : max0, granule_max<T>(g[i]));
+  const float lane_max = max_nan(max0, max1);
   float m = lane_max;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -209,38 +229,121 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_l
   }
   Stats st{m, s, w};
 
-  // ---- the warp's top k
+  // ---- the k largest
   const int k = a.top_k;
-  uint64_t* sorted = sh.sorted[warp];
-  if (k > 0) {
-    bool fast = m == m && m != -INFINITY;
-    float threshold = 0.f;
-    int found = 0;
-    if (fast) {
-      uint32_t cur = ordered(lane_max), top = 0;
-      for (int n = 0; n < k;) {
-        top = __reduce_max_sync(0xffffffffu, cur);
-        n += __popc(__ballot_sync(0xffffffffu, cur == top));
-        if (cur == top) cur = 0;
+  uint64_t* const list = sh.list[W == 1 ? warp : 0];
+  // rounds over the warp's part of the row, from memory again (a copy in the caches): rare, and without a limit on equal values
+  auto rounds = [&](uint64_t* out) {
+    uint64_t last = ~0ull;
+    for (int r = 0; r < k; ++r) {
+      uint64_t best = 0;
+      if (has_edge && key_of(edge, edge_at) < last) best = key_of(edge, edge_at);
+      for (int gi = first; gi < granules; gi += step) {
+        for (int e = 0; e < VE; ++e) {
+          const uint64_t c = key_of(Elem<T>::to_f(x1[gi * VE + e]), head + gi * VE + e);
+          if (c < last) best = max(best, c);
+        }
       }
-      threshold = from_ordered(top);
-      if (lane == 0) sh.count[warp] = 0;
+      last = warp_max_key(best);
+      if (lane == 0) out[r] = last;
+    }
+  };
+  const uint64_t* sorted = nullptr;
+  if constexpr (W == 1) {
+    const uint32_t below = (1u << lane) - 1;
+    sorted = sh.sorted[warp];
+    if (k > 0) {
+      int found = kList + 1;
+      if (m == m && m != -INFINITY) {
+        // k-th largest of the lanes' two maxima each
+        uint32_t cur = ordered(fmaxf(max0, max1)), next = ordered(fminf(max0, max1)), top = 0;
+        for (int n = 0; n < k;) {
+          top = __reduce_max_sync(0xffffffffu, cur);
+          n += __popc(__ballot_sync(0xffffffffu, cur == top));
+          if (cur == top) cur = next, next = 0;
+        }
+        const float threshold = from_ordered(top);
+        if (threshold != -INFINITY) {
+          // what reaches it: first the granules, then, a granule to a lane, the values.  The granules are read again (from the
+          // caches): picking them out of registers would take the whole warp through each.
+          int* const hits = sh.granule[warp];
+          int n = 0;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            asm("" : "+r"(g[i].x), "+r"(g[i].y), "+r"(g[i].z), "+r"(g[i].w));   // not kept unpacked from the sums until here
+            const bool hit = granule_max<T>(g[i]) >= threshold;
+            const uint32_t all = __ballot_sync(0xffffffffu, hit);
+            const int at = n + __popc(all & below);
+            if (hit && at < kList) hits[at] = first + i * step;
+            n += __popc(all);
+          }
+          __syncwarp();
+          found = 0;
+          auto take = [&](bool hit, float x, int index) {
+            const uint32_t all = __ballot_sync(0xffffffffu, hit);
+            const int at = found + __popc(all & below);
+            if (hit && at < kList) list[at] = key_of(x, index);
+            found += __popc(all);
+          };
+          take(edge >= threshold, edge, edge_at);
+          for (int base = 0; base < min(n, kList); base += 32) {
+            const bool any = base + lane < min(n, kList);
+            const int gi = any ? hits[base + lane] : first;
+            Pack<T> again;
+            if (any) again = ld128(x1 + gi * VE);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {
+              const float x = any ? Elem<T>::to_f(again.v[j]) : -INFINITY;
+              take(x >= threshold, x, head + gi * VE + j);
+            }
+          }
+          if (n > kList) found = kList + 1;
+          __syncwarp();
+        }
+      }
+      if (found <= kList) rank_list(list, found, k, sh.sorted[warp], lane);
+      else rounds(sh.sorted[warp]);
       __syncwarp();
-      auto take = [&](float x, int index) {
-        const int at = atomicAdd(&sh.count[warp], 1);
-        if (at < kList) sh.list[warp][at] = key_of(x, index);
-      };
-      if (threshold != -INFINITY) {
+    }
+  } else {
+    constexpr int kGroup = W == 16 ? 4 : 2, kMaxima = W * 32 / kGroup;   // lanes behind a maximum; 128 or 64 of them
+    float gm = lane_max;
+#pragma unroll
+    for (int o = 1; o < kGroup; o <<= 1) gm = max_nan(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+    if (lane % kGroup == 0) sh.maxima[(warp * 32 + lane) / kGroup] = ordered(gm);
+    if (lane == 0) sh.stats[warp] = st;
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    if (parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    st = warp_merge(lane < W ? sh.stats[lane] : Stats{-INFINITY, 0.f, 0.f});   // the block's, in every warp
+    if (k > 0) {
+      if (threadIdx.x < kMaxima) {   // the k-th largest maximum; several threads write the same number if it is there more often
+        const uint32_t mine = sh.maxima[threadIdx.x];
+        int above = 0, reach = 0;
+#pragma unroll 4
+        for (int i = 0; i < kMaxima; i += 4) {
+          const uint4 o = *reinterpret_cast<const uint4*>(&sh.maxima[i]);
+          above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+          reach += (o.x >= mine) + (o.y >= mine) + (o.z >= mine) + (o.w >= mine);
+        }
+        if (above < k && reach >= k) sh.bound = mine;
+      }
+      __syncthreads();
+      const bool try_list = st.m == st.m && sh.bound > ordered(-INFINITY);
+      if (try_list) {
+        const float threshold = from_ordered(sh.bound);
+        auto take = [&](float x, int index) {
+          const int at = atomicAdd(&sh.count, 1);
+          if (at < kList) list[at] = key_of(x, index);
+        };
         if (edge >= threshold) take(edge, edge_at);
-        // granules that reach it; few, at places of their own in every lane: read again (from the caches) and not picked out of
-        // registers, which would take the whole warp through each
         uint32_t reach = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           asm("" : "+r"(g[i].x), "+r"(g[i].y), "+r"(g[i].z), "+r"(g[i].w));   // not kept unpacked from the sums until here
           if (granule_max<T>(g[i]) >= threshold) reach |= 1u << i;
         }
-        while (reach) {
+        while (reach) {   // few, at places of their own in every lane: read again (from the caches)
           const int gi = first + (__ffs(reach) - 1) * step;
           reach &= reach - 1;
           const Pack<T> again = ld128(x1 + gi * VE);
@@ -251,64 +354,21 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_l
           }
         }
       }
-      __syncwarp();
-      found = sh.count[warp];
-      fast = threshold != -INFINITY && found <= kList;
-    }
-    if (fast) {
-      if (found <= 32) {   // the usual case: every lane counts what is above its own
-        const uint64_t mine = lane < found ? sh.list[warp][lane] : 0;
-        int above = 0;
-        for (int i = 0; i < found; ++i) above += sh.list[warp][i] > mine;
-        if (lane < found && above < k) sorted[above] = mine;
+      __syncthreads();
+      if (try_list && sh.count <= kList) {
+        if (warp == 0) rank_list(list, sh.count, k, sh.merged, lane);
       } else {
-      uint64_t best = 0;
-      for (int i = lane; i < found; i += 32) best = max(best, sh.list[warp][i]);
-      for (int r = 0; r < k; ++r) {
-        const uint64_t won = warp_max_key(best);
-        if (lane == 0) sorted[r] = won;
-        if (best == won) {
-          best = 0;
-          for (int i = lane; i < found; i += 32) {
-            const uint64_t c = sh.list[warp][i];
-            if (c < won) best = max(best, c);
-          }
-        }
-      }
-      }
-    } else {
-      // rounds over the warp's part of the row, from memory again (a copy in the caches): rare, and without a limit on equal values
-      uint64_t last = ~0ull;
-      for (int r = 0; r < k; ++r) {
-        uint64_t best = 0;
-        if (has_edge && key_of(edge, edge_at) < last) best = key_of(edge, edge_at);
-        for (int gi = first; gi < granules; gi += step) {
-          for (int e = 0; e < VE; ++e) {
-            const uint64_t c = key_of(Elem<T>::to_f(x1[gi * VE + e]), head + gi * VE + e);
-            if (c < last) best = max(best, c);
-          }
-        }
-        last = warp_max_key(best);
-        if (lane == 0) sorted[r] = last;
+        rounds(sh.sorted[warp]);
+        __syncthreads();
+        if (warp == 0) merge_lists(sh.sorted, W, k, sh.merged, lane);
       }
     }
-    __syncwarp();
-  }
-
-  // ---- the row's: parts meet
-  if constexpr (W > 1) {
-    if (lane == 0) sh.stats[warp] = st;
-    __syncthreads();
-    if (parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    if (warp == 0) {
-      st = warp_merge(lane < W ? sh.stats[lane] : Stats{-INFINITY, 0.f, 0.f});
-      uint64_t* dst = parts > 1 ? sh.list[0] : sh.list[1];   // lists of the warps are done with
-      if (k > 0) merge_lists(sh.sorted, W, k, dst, lane);
-      __syncwarp();
-      if (parts > 1) {   // into the first block's shared memory
-        if (k > 0 && lane < k) {
+    if (warp == 0) __syncwarp();
+    if (parts > 1) {
+      if (warp == 0) {   // into the first block's shared memory
+        if (lane < k) {
           const uint32_t to = ptx::map_to_cta(&sh.part_sorted[part][lane], 0);
-          asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(dst[lane]) : "memory");
+          asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(sh.merged[lane]) : "memory");
         }
         if (lane < 3) {
           const float v = lane == 0 ? st.m : lane == 1 ? st.s : st.w;
@@ -316,18 +376,16 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_l
           asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(v) : "memory");
         }
       }
-    }
-    if (parts > 1) {
       ptx::cluster_sync();
       if (part != 0) return;
       if (warp == 0) {
         st = warp_merge(lane < parts ? sh.part_stats[lane] : Stats{-INFINITY, 0.f, 0.f});
-        if (k > 0) merge_lists(sh.part_sorted, parts, k, sh.list[1], lane);
+        if (k > 0) merge_lists(sh.part_sorted, parts, k, sh.merged, lane);
         __syncwarp();
       }
     }
     if (warp != 0) return;
-    sorted = sh.list[1];
+    sorted = sh.merged;
   }
   const bool none = st.m == -INFINITY;             // a row of -inf: every log-prob is -inf, the entropy 0
   const float log_s = logf(st.s);
@@ -376,7 +434,8 @@ int run(const Args& a, cudaStream_t s) {
     return launch<T, 1, 20>(a, 1, s);
   }
   if (granules <= 128 * 5) return launch<T, 4, 5>(a, 1, s);
-  if (a.rows >= sms * 2 && granules <= 128 * 10) return launch<T, 4, 10>(a, 1, s);
+  if (a.rows >= sms * 2 && granules <= 128 * 7) return launch<T, 4, 7>(a, 1, s);
+  if (a.rows >= sms * 2 && granules <= 128 * 10 * 8) return launch<T, 4, 10>(a, static_cast<int>((granules + 1279) / 1280), s);
   int parts = 1;   // few rows: a cluster each
   while (parts < 8 && (a.rows * parts < sms || granules > 512 * 16 * parts) && granules > 512 * parts) parts *= 2;
   const int64_t per = (granules + 512 * parts - 1) / (512 * parts);

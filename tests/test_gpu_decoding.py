@@ -521,6 +521,29 @@ def test_token_log_probs_of_odd_rows(dtype, rows, V):
     check_scores(x.cuda(), tokens.cuda(), 3)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,V,k", [(300, 7001, 32), (303, 24001, 30), (297, 52345, 32), (298, 81923, 16), (620, 5002, 30)])
+def test_token_log_probs_of_many_long_rows(dtype, rows, V, k):
+    test_token_log_probs(dtype, rows, V, 3, k)                 # clusters of other than a power of two among them
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_token_log_probs_of_many_long_odd_rows(dtype):
+    test_token_log_probs_of_odd_rows(dtype, 601, 23999)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,V", [(601, 4000), (300, 6000), (4, 6000), (4, 60000)])
+def test_token_log_probs_of_values_in_one_place(dtype, rows, V):
+    """Likely tokens all next to one another, more of them than parts of a row hold a maximum of, and many equal ones."""
+    x = 0.1 * rand(V, rows, V)
+    x[:, 100:260] += 8 + 4 * rand(V + 1, rows, 160)
+    x[1, 300:1500] = 30.0
+    x[2, 300:492] = 30.0                                       # as many as are listed, and one more
+    x[3, 300:493] = 30.0
+    check_scores(x.to(DTYPES[dtype]).cuda(), torch.randint(0, V, (rows,), generator=torch.Generator().manual_seed(3)).cuda(), 32)
+
+
 def test_token_log_probs_shapes_and_refusals():
     x = rand(1, 2, 3, 50).cuda()
     x32 = x.float()
