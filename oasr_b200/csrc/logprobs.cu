@@ -106,9 +106,11 @@ __device__ __forceinline__ Stats merge(Stats a, Stats b) {
   return r;
 }
 
+// N statistics, lane l's being number l % N
+template <int N>
 __device__ __forceinline__ Stats warp_merge(Stats v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int o = N / 2; o > 0; o >>= 1) {
     Stats b;
     b.m = __shfl_xor_sync(0xffffffffu, v.m, o);
     b.s = __shfl_xor_sync(0xffffffffu, v.s, o);
@@ -162,7 +164,7 @@ __device__ __forceinline__ void merge_lists(const uint64_t (*lists)[kMaxTop], in
 
 // W warps of a block share a row's slice; `parts` blocks of a cluster share a row.
 template <typename T, int W, int NV>
-__global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_log_probs_kernel(const Args a, const int parts) {
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W > 4 ? 1 : NV <= 5 ? 7 : NV <= 10 ? 5 : 4) token_log_probs_kernel(const Args a, const int parts) {
   constexpr int VE = Elem<T>::kVec;
   constexpr int kRows = W == 1 ? 4 : 1;                 // rows of a block
   __shared__ Shared<W, kRows> sh;
@@ -315,7 +317,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_l
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
     if (parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    st = warp_merge(lane < W ? sh.stats[lane] : Stats{-INFINITY, 0.f, 0.f});   // the block's, in every warp
+    if (warp == 0) st = warp_merge<W>(sh.stats[lane % W]);   // the block's
     if (k > 0) {
       if (threadIdx.x < kMaxima) {   // the k-th largest maximum; several threads write the same number if it is there more often
         const uint32_t mine = sh.maxima[threadIdx.x];
@@ -327,9 +329,10 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_l
           reach += (o.x >= mine) + (o.y >= mine) + (o.z >= mine) + (o.w >= mine);
         }
         if (above < k && reach >= k) sh.bound = mine;
+        if (mine == 0xffffffffu) sh.count = kList + 1;   // a NaN
       }
       __syncthreads();
-      const bool try_list = st.m == st.m && sh.bound > ordered(-INFINITY);
+      const bool try_list = sh.bound > ordered(-INFINITY);
       if (try_list) {
         const float threshold = from_ordered(sh.bound);
         auto take = [&](float x, int index) {
@@ -379,7 +382,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 1 ? 4 : 1) token_l
       ptx::cluster_sync();
       if (part != 0) return;
       if (warp == 0) {
-        st = warp_merge(lane < parts ? sh.part_stats[lane] : Stats{-INFINITY, 0.f, 0.f});
+        st = warp_merge<8>(lane % 8 < parts ? sh.part_stats[lane % 8] : Stats{-INFINITY, 0.f, 0.f});
         if (k > 0) merge_lists(sh.part_sorted, parts, k, sh.merged, lane);
         __syncwarp();
       }
