@@ -9,8 +9,9 @@
 // A warp owns up to 32 * NV granules of 16 bytes of one row and holds them in registers: they are read from memory once, and the
 // maximum, the sums and the selection all run on that copy.  Selection: the k-th largest of 64 to 128 maxima of parts of the row is a
 // lower bound of its k-th largest value, so only what reaches it (a little over k values) goes to a list in shared memory, where
-// every lane counts how many are above its own.  A row whose list overflows (many equal values: a mask that leaves fewer than k
-// tokens) or that holds a NaN takes k rounds of a warp-wide maximum over the row instead; the result is the same.
+// every lane counts how many are above its own.  Where that is too many (a mask that leaves fewer than k tokens makes the bound the
+// mask's value) the list takes what is above the bound, and the lowest indices of the bound's value fill it up.  A row whose list
+// still overflows, or that holds a NaN, takes k rounds of a warp-wide maximum over the row instead; the result is the same.
 // Larger rows are split over the warps of a block, and over a cluster of blocks where the rows are few: the parts' statistics
 // and sorted lists meet in shared memory (the first block's, written through the cluster).
 #include <type_traits>
@@ -126,7 +127,7 @@ struct Shared {
   int granule[kRows][kList];            // granules they are in (a warp to a row)
   uint64_t sorted[W * kRows][kMaxTop];  // a warp's alternatives
   uint64_t merged[kMaxTop];
-  int count;
+  int count, nan;
   Stats stats[W];
   alignas(16) uint32_t maxima[128];     // of parts of the block's slice
   uint32_t bound;                       // the k-th largest of them
@@ -234,6 +235,19 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W > 4 ? 1 : NV <= 5 ? 7
   // ---- the k largest
   const int k = a.top_k;
   uint64_t* const list = sh.list[W == 1 ? warp : 0];
+  const uint32_t below = (1u << lane) - 1;
+  // entries `found` to k - 1 of the list: the lowest indices in [lo, hi) whose logit is v
+  auto fill = [&](int lo, int hi, float v, int found) {
+    for (int base = lo; base < hi && found < k; base += 32) {
+      const int j = base + lane;
+      const bool hit = j < hi && Elem<T>::to_f(x0[min(j, hi - 1)]) == v;
+      const uint32_t all = __ballot_sync(0xffffffffu, hit);
+      const int at = found + __popc(all & below);
+      if (hit && at < k) list[at] = key_of(v, j);
+      found = min(found + __popc(all), k);
+    }
+    return found;
+  };
   // rounds over the warp's part of the row, from memory again (a copy in the caches): rare, and without a limit on equal values
   auto rounds = [&](uint64_t* out) {
     uint64_t last = ~0ull;
@@ -252,11 +266,10 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W > 4 ? 1 : NV <= 5 ? 7
   };
   const uint64_t* sorted = nullptr;
   if constexpr (W == 1) {
-    const uint32_t below = (1u << lane) - 1;
     sorted = sh.sorted[warp];
     if (k > 0) {
       int found = kList + 1;
-      if (m == m && m != -INFINITY) {
+      if (m == m) {
         // k-th largest of the lanes' two maxima each
         uint32_t cur = ordered(fmaxf(max0, max1)), next = ordered(fminf(max0, max1)), top = 0;
         for (int n = 0; n < k;) {
@@ -264,8 +277,12 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W > 4 ? 1 : NV <= 5 ? 7
           n += __popc(__ballot_sync(0xffffffffu, cur == top));
           if (cur == top) cur = next, next = 0;
         }
-        const float threshold = from_ordered(top);
-        if (threshold != -INFINITY) {
+        const float bound = from_ordered(top);
+        bool over = bound == -INFINITY;                                   // take what is above the bound, not all that reaches it
+#pragma unroll 1
+        for (int pass = over; pass < 2 && found > kList; ++pass) {
+          over = pass == 1;
+          const float threshold = over ? from_ordered(top + 1) : bound;   // (NaN behind +inf: nothing)
           // what reaches it: first the granules, then, a granule to a lane, the values.  The granules are read again (from the
           // caches): picking them out of registers would take the whole warp through each.
           int* const hits = sh.granule[warp];
@@ -302,6 +319,10 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W > 4 ? 1 : NV <= 5 ? 7
           if (n > kList) found = kList + 1;
           __syncwarp();
         }
+        if (over && found < k) {
+          found = fill(0, a.vocab, bound, found);
+          __syncwarp();
+        }
       }
       if (found <= kList) rank_list(list, found, k, sh.sorted[warp], lane);
       else rounds(sh.sorted[warp]);
@@ -314,7 +335,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W > 4 ? 1 : NV <= 5 ? 7
     for (int o = 1; o < kGroup; o <<= 1) gm = max_nan(gm, __shfl_xor_sync(0xffffffffu, gm, o));
     if (lane % kGroup == 0) sh.maxima[(warp * 32 + lane) / kGroup] = ordered(gm);
     if (lane == 0) sh.stats[warp] = st;
-    if (threadIdx.x == 0) sh.count = 0;
+    if (threadIdx.x == 0) sh.count = sh.nan = 0;
     __syncthreads();
     if (parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (warp == 0) st = warp_merge<W>(sh.stats[lane % W]);   // the block's
@@ -329,12 +350,17 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W > 4 ? 1 : NV <= 5 ? 7
           reach += (o.x >= mine) + (o.y >= mine) + (o.z >= mine) + (o.w >= mine);
         }
         if (above < k && reach >= k) sh.bound = mine;
-        if (mine == 0xffffffffu) sh.count = kList + 1;   // a NaN
+        if (mine == 0xffffffffu) sh.nan = 1;
       }
       __syncthreads();
-      const bool try_list = sh.bound > ordered(-INFINITY);
-      if (try_list) {
-        const float threshold = from_ordered(sh.bound);
+      const uint32_t top = sh.bound;
+      const float bound = from_ordered(top);
+      bool over = bound == -INFINITY;                                   // take what is above the bound, not all that reaches it
+      int found = kList + 1;
+#pragma unroll 1
+      for (int pass = over; pass < 2 && !sh.nan; ++pass) {
+        over = pass == 1;
+        const float threshold = over ? from_ordered(top + 1) : bound;   // (NaN behind +inf: nothing)
         auto take = [&](float x, int index) {
           const int at = atomicAdd(&sh.count, 1);
           if (at < kList) list[at] = key_of(x, index);
@@ -356,10 +382,26 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W > 4 ? 1 : NV <= 5 ? 7
             if (x >= threshold) take(x, head + gi * VE + j);
           }
         }
+        __syncthreads();
+        found = sh.count;
+        if (found <= kList || over) break;
+        __syncthreads();
+        if (threadIdx.x == 0) sh.count = 0;
+        __syncthreads();
       }
-      __syncthreads();
-      if (try_list && sh.count <= kList) {
-        if (warp == 0) rank_list(list, sh.count, k, sh.merged, lane);
+      if (found <= kList) {
+        if (warp == 0) {
+          if (over && found < k) {
+            if (part == 0) found = fill(0, head, bound, found);
+            for (int gi = part * W * 32; gi < granules && found < k; gi += step) {
+              found = fill(head + gi * VE, head + min(gi + W * 32, granules) * VE, bound, found);
+            }
+            if (part == 0) found = fill(head + granules * VE, a.vocab, bound, found);
+            if (lane >= found && lane < k) sh.merged[lane] = 0;         // a part of fewer than k
+            __syncwarp();
+          }
+          rank_list(list, found, k, sh.merged, lane);
+        }
       } else {
         rounds(sh.sorted[warp]);
         __syncthreads();

@@ -453,7 +453,6 @@ def score64(x, k):
     lp[none] = -math.inf
     ent = -(lp.exp() * torch.where(lp == -math.inf, torch.zeros_like(lp), lp)).sum(-1)
     rank = torch.where(torch.isnan(x), torch.full_like(x, math.inf), x)
-    order = sorted  # noqa: F841
     ids = torch.sort(torch.stack([torch.isnan(x).double(), rank], 0)[1] + 0.0, descending=True, stable=True, dim=-1).indices
     for r in torch.isnan(x).any(-1).nonzero().flatten().tolist():      # NaN before +inf
         ids[r] = torch.tensor(sorted(range(x.shape[1]), key=lambda i: (not math.isnan(x[r, i]), -rank[r, i].item(), i)))
@@ -542,6 +541,25 @@ def test_token_log_probs_of_values_in_one_place(dtype, rows, V):
     x[2, 300:492] = 30.0                                       # as many as are listed, and one more
     x[3, 300:493] = 30.0
     check_scores(x.to(DTYPES[dtype]).cuda(), torch.randint(0, V, (rows,), generator=torch.Generator().manual_seed(3)).cuda(), 32)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,V", [(601, 4001), (600, 77), (3, 999), (300, 24001), (4, 60001), (2, 200003)])
+def test_token_log_probs_of_masked_rows(dtype, rows, V):
+    """Masks that leave fewer tokens than alternatives are asked for: the rest are the lowest masked ids."""
+    dt = DTYPES[dtype]
+    x = rand(V + 2, rows, V).to(dt)
+    g = torch.Generator().manual_seed(V)
+    for r in range(min(rows, 40)):
+        left = torch.randperm(V, generator=g)[:r % 34]
+        if r % 3 == 0:
+            left = torch.cat([left, torch.tensor([0, 1, 5, V - 1])])
+        y = torch.full((V,), (-math.inf, torch.finfo(dt).min, 0.0, math.inf)[r % 4], dtype=dt)
+        y[left] = x[r, left]
+        x[r] = y
+    tokens = torch.randint(0, V, (rows,), generator=g)
+    for k in (1, 32):
+        check_scores(x.cuda(), tokens.cuda(), k)
 
 
 def test_token_log_probs_shapes_and_refusals():
