@@ -197,17 +197,19 @@ struct WriteArgs {
   float inv_d, eps;
 };
 
-// Largest magnitudes of the groups that a lane's two octets lie in.
+// Largest magnitudes of the groups that a lane's two octets lie in.  The rows of a warp may be of different kinds (`pairs`: of
+// values, whose groups are always two lanes), and a shuffle names the whole warp: every branch here goes the same way in all of its
+// lanes, and lanes choose among the results afterwards.
 template <bool kInter>
 __device__ __forceinline__ float2 group_max(float ma, float mb, int2 oct, int u, int rotated, int lanes, bool pairs) {
   const float both = q4::max_nan(ma, mb), pair = q4::max_nan(both, __shfl_xor_sync(0xffffffffu, both, 1));
-  if (kInter || pairs) return make_float2(pair, pair);   // neighbouring octets: a group is two lanes
+  if (kInter || __all_sync(0xffffffffu, pairs)) return make_float2(pair, pair);   // neighbouring octets: a group is two lanes
   if (rotated % 4 == 0) {                                 // octets u and u + rotated: each in a group of four lanes
     ma = q4::max_nan(ma, __shfl_xor_sync(0xffffffffu, ma, 1));
     mb = q4::max_nan(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
     ma = q4::max_nan(ma, __shfl_xor_sync(0xffffffffu, ma, 2));
     mb = q4::max_nan(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
-    return u < rotated ? make_float2(ma, mb) : make_float2(pair, pair);
+    return !pairs && u < rotated ? make_float2(ma, mb) : make_float2(pair, pair);
   }
   float r[2];                                             // a group holds octets of both kinds: ask each octet's lane
 #pragma unroll
@@ -225,7 +227,7 @@ __device__ __forceinline__ float2 group_max(float ma, float mb, int2 oct, int u,
     }
     r[s] = m;
   }
-  return make_float2(r[0], r[1]);
+  return pairs ? make_float2(pair, pair) : make_float2(r[0], r[1]);
 }
 
 __device__ __forceinline__ float octet_max(const float (&x)[8]) {
