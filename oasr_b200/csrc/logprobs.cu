@@ -4,7 +4,8 @@
 //   top k by (value, then lowest index)
 //
 // Sums run in fp32 and in the log2 domain, d_j = x_j log2(e) - m2 with m2 = M log2(e) rounded: one fused multiply-add a value.
-// What the rounding of m2 shifts all of them by is taken out of the two sums afterwards.
+// What the rounding of m2 shifts all of them by is taken out of the two sums afterwards.  Rows whose maximum is beyond 2^20 (a mask
+// that leaves nothing, of whatever size) take d_j = (x_j - M) log2(e).
 //
 // A warp owns up to 32 * NV granules of 16 bytes of one row and holds them in registers: they are read from memory once, and the
 // maximum, the sums and the selection all run on that copy.  Selection: the k-th largest of 64 to 128 maxima of parts of the row is a
@@ -210,28 +211,37 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W > 4 ? 1 : NV <= 5 ? 7
   float m = lane_max;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-  // Logits near the type's limit (a mask of its lowest value that leaves nothing) would overflow when multiplied.  Two of that
-  // size that differ at all differ by 2^102 or more, so any factor gives exponents of 0 or below kFar.
-  const float unit = fabsf(m) > 1e38f ? 0x1p-90f : kLog2e;
-  const float m2 = m == -INFINITY ? 0.f : m * unit;
-  const float edge_d = max_nan(fmaf(edge, unit, -m2), kFar);
-  // four sums of each: shorter chains, and the likeliest token's 1 costs fewer of the small terms their last bits
-  float s4[4] = {ex2(edge_d)}, w4[4] = {edge_d * s4[0]};
+  // Exponents d_j = (x_j - m) log2(e).  Rows up to 2^20 form them with one multiply-add, x_j log2(e) - m2, and what the rounding of
+  // m2 shifts all of them by (2^-4 at most) is taken out of the sums.  That shift grows with |m| (2^-24 of it) until the sums overflow
+  // or vanish, so that larger rows subtract first: exactly where the two are within a factor of two, and to below kFar where they are not.
+  const bool large = !(fabsf(m) <= 0x1p20f);
+  const float base = m == -INFINITY ? 0.f : m, m2 = base * kLog2e;
+  float s = 0.f, w = 0.f;
+  auto sums = [&](auto exponent) {
+    const float edge_d = max_nan(exponent(edge), kFar);
+    // four sums of each: shorter chains, and the likeliest token's 1 costs fewer of the small terms their last bits
+    float s4[4] = {ex2(edge_d)}, w4[4] = {edge_d * s4[0]};
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    float x[VE];
-    unpack<T>(g[i], x);
+    for (int i = 0; i < NV; ++i) {
+      float x[VE];
+      unpack<T>(g[i], x);
 #pragma unroll
-    for (int j = 0; j < VE; ++j) {
-      const float d = max_nan(fmaf(x[j], unit, -m2), kFar);
-      const float e = ex2(d);
-      s4[j & 3] += e;
-      w4[j & 3] = fmaf(d, e, w4[j & 3]);
+      for (int j = 0; j < VE; ++j) {
+        const float d = max_nan(exponent(x[j]), kFar);
+        const float e = ex2(d);
+        s4[j & 3] += e;
+        w4[j & 3] = fmaf(d, e, w4[j & 3]);
+      }
     }
-  }
-  float s = warp_sum((s4[0] + s4[1]) + (s4[2] + s4[3])), w = warp_sum((w4[0] + w4[1]) + (w4[2] + w4[3]));
-  if (m != -INFINITY) {
-    const float shift = fmaf(m, unit, -m2), f = ex2(-shift);   // m2 + shift is m * unit
+    s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+    w = (w4[0] + w4[1]) + (w4[2] + w4[3]);
+  };
+  if (large) sums([&](float x) { return (x - base) * kLog2e; });
+  else sums([&](float x) { return fmaf(x, kLog2e, -m2); });
+  s = warp_sum(s);
+  w = warp_sum(w);
+  if (!large) {
+    const float shift = fmaf(m, kLog2e, -m2), f = ex2(-shift);   // m2 + shift is m log2(e)
     w = fmaf(-shift, s, w) * f;
     s *= f;
   }

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import oasr_b200 as ob
-from tests.test_gpu_decoding import EPS, chunk, rand
+from tests.test_gpu_decoding import DTYPES, EPS, check_scores, chunk, rand, score64
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +27,39 @@ def test_codes_do_not_depend_on_the_rows_beside_them(frames, H, Hkv, D, R, inter
         out = ob.write_kv_rope_q4(*pools, bt[:n], k[:n], v[:n], off[:n], table, q=q[:n] if H else None, k_weight=kw, eps=EPS, interleaved=inter)
         got.append([p[:frames] for p in pools] + ([out[:frames]] if H else []))
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+# ---- scores -------------------------------------------------------------------------------------------------------------
+LARGE = [1e6, 3e7, 2.0 ** 30, 1e9, 5e9, 1e10, 1e12, 1e15, 1e20, 1e30, 3e37, 9.9e37, 1.1e38, 3e38]
+FORMS = [(600, 1000), (5, 2000), (300, 6000), (300, 24001), (3, 9000), (4, 60001)]   # a warp a row, blocks and clusters of four and of sixteen warps
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows,V", FORMS)
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_token_log_probs_of_large_logits(dtype, rows, V, sign):
+    """Finite rows of every size: one value alone, neighbours of it, a mask of it with likely tokens left."""
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(V)
+    near = sign * (1 + torch.finfo(dt).eps * torch.randint(0, 5, (V,), generator=g).double())
+    left = torch.randperm(V, generator=g)[:40]
+    tokens = torch.randint(0, V, (min(rows, 32),), generator=g)
+    for size in LARGE:
+        x = torch.empty(rows, V, dtype=torch.float64)
+        x[0::4] = sign * size
+        x[1::4] = (size * near).clamp(-3.3e38, 3.3e38)
+        x[2::4] = -size
+        x[2::4, left] = 3 * rand(5, 40)
+        x[3::4] = sign * size * 0.5
+        x[3::4, left[:9]] = sign * size
+        # equal rows have equal results: one of each kind is compared with 64 bits, the others with that one
+        x = x.to(dt).cuda()
+        check_scores(x[:4].contiguous(), tokens[:len(x[:4])].cuda(), 32)
+        first, all_ = ob.token_log_probs(x[:4], top_k=32), ob.token_log_probs(x, top_k=32)
+        lp, ent, ids = score64(x[:4].cpu().double(), 32)
+        tol = (2.0 ** -24 * (V / 32 + 20) + 2.0 ** -20) * (1 + ent.max())      # as in check_scores
+        for r in range(len(ids)):
+            assert (all_.top_ids[r::4].cpu() == ids[r].int()).all() and (all_.top_ids[r::4] == first.top_ids[r]).all()
+            assert ((all_.entropy[r::4].cpu() - ent[r]).abs() <= 2.0 ** -22 * ent[r] + tol).all(), size
+            want = lp[r, ids[r]]
+            assert ((all_.top_log_probs[r::4].cpu() - want).abs() <= 2.0 ** -22 * want.abs() + tol).all(), size
