@@ -51,14 +51,16 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Order of the values as unsigned numbers; a NaN ranks above everything.
+// Order of the values as unsigned numbers; a NaN ranks above everything, and below all ones: no element's key is the one above
+// all keys that a walk through them starts from.
+constexpr uint32_t kNan = 0xfffffffeu;
 __device__ __forceinline__ uint32_t ordered(float x) {
-  if (x != x) return 0xffffffffu;
+  if (x != x) return kNan;
   const uint32_t b = __float_as_uint(x + 0.f);   // -0 ranks with +0
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float from_ordered(uint32_t o) {
-  if (o == 0xffffffffu) return __uint_as_float(0x7fffffffu);
+  if (o == kNan) return __uint_as_float(0x7fffffffu);
   return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 // (value, lowest index first) as one unsigned number; 0 is below every element
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W > 4 ? 1 : NV <= 5 ? 7
   };
   // rounds over the warp's part of the row, from memory again (a copy in the caches): rare, and without a limit on equal values
   auto rounds = [&](uint64_t* out) {
-    uint64_t last = ~0ull;
+    uint64_t last = ~0ull;   // above every key
     for (int r = 0; r < k; ++r) {
       uint64_t best = 0;
       if (has_edge && key_of(edge, edge_at) < last) best = key_of(edge, edge_at);
@@ -365,7 +367,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W > 4 ? 1 : NV <= 5 ? 7
           reach += (o.x >= mine) + (o.y >= mine) + (o.z >= mine) + (o.w >= mine);
         }
         if (above < k && reach >= k) sh.bound = mine;
-        if (mine == 0xffffffffu) sh.nan = 1;
+        if (mine == kNan) sh.nan = 1;
       }
       __syncthreads();
       const uint32_t top = sh.bound;

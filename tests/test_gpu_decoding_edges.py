@@ -1,4 +1,6 @@
 """The decoding operators where they can go wrong."""
+import math
+
 import pytest
 import torch
 
@@ -63,3 +65,21 @@ def test_token_log_probs_of_large_logits(dtype, rows, V, sign):
             assert ((all_.entropy[r::4].cpu() - ent[r]).abs() <= 2.0 ** -22 * ent[r] + tol).all(), size
             want = lp[r, ids[r]]
             assert ((all_.top_log_probs[r::4].cpu() - want).abs() <= 2.0 ** -22 * want.abs() + tol).all(), size
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,V", FORMS + [(3, 8), (700, 8), (2, 1)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_token_log_probs_ranks_a_nan_first_wherever_it_is(dtype, rows, V, shift):
+    x = (3 * rand(V, rows, V + shift)).to(DTYPES[dtype])[:, shift:]
+    x[0, 0] = math.nan                                     # the first token alone
+    if rows > 1:
+        x[1] = math.nan                                    # nothing else: ids in order
+    if rows > 2:
+        x[2, 0] = x[2, V - 1] = math.nan
+    if rows > 3:
+        x[3, 0], x[3, V // 2] = math.inf, math.nan
+    tokens = torch.zeros(rows, dtype=torch.int64)
+    x = x.cuda() if not shift else torch.empty(rows, V + shift, dtype=x.dtype, device="cuda")[:, shift:].copy_(x)
+    for k in {1, min(V, 32)}:
+        check_scores(x, tokens.cuda(), k)
