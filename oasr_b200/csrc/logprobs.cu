@@ -114,7 +114,8 @@ __device__ __forceinline__ Stats merge(Stats a, Stats b) {
   return r;
 }
 
-// N statistics, lane l's being number l % N
+// N statistics, lane l's being number l % N.  A merge rounds by the order of its arguments, so that lanes could end a bit apart: all
+// get the first lane's, and with it a token the same log-prob wherever it is asked for.
 template <int N>
 __device__ __forceinline__ Stats warp_merge(Stats v) {
 #pragma unroll
@@ -125,7 +126,7 @@ __device__ __forceinline__ Stats warp_merge(Stats v) {
     b.w = __shfl_xor_sync(0xffffffffu, v.w, o);
     v = merge(v, b);
   }
-  return v;
+  return Stats{__shfl_sync(0xffffffffu, v.m, 0), __shfl_sync(0xffffffffu, v.s, 0), __shfl_sync(0xffffffffu, v.w, 0)};
 }
 
 template <int W, int kRows>

@@ -83,3 +83,16 @@ def test_token_log_probs_ranks_a_nan_first_wherever_it_is(dtype, rows, V, shift)
     x = x.cuda() if not shift else torch.empty(rows, V + shift, dtype=x.dtype, device="cuda")[:, shift:].copy_(x)
     for k in {1, min(V, 32)}:
         check_scores(x, tokens.cuda(), k)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,V", FORMS + [(2000, 6000), (500, 60001)])
+def test_token_log_probs_of_one_token_are_one_number(dtype, rows, V):
+    """A token scores the same among the given ones and among the alternatives, and equal logits score the same."""
+    x = (3 * rand(V + 9, min(rows, 600), V)).to(DTYPES[dtype]).cuda()
+    x = x[torch.arange(rows) % len(x)]
+    x[:, -1] = x[:, 0] = x[:, V // 3] = 20.0
+    ids = ob.token_log_probs(x, top_k=32).top_ids
+    got = ob.token_log_probs(x, ids, top_k=32)
+    assert torch.equal(got.top_ids, ids) and torch.equal(got.log_probs, got.top_log_probs)
+    assert (got.top_log_probs[:, :3] == got.top_log_probs[:, :1]).all() and got.top_ids[0, :3].tolist() == [0, V // 3, V - 1]
