@@ -10,14 +10,13 @@
 // and contraction orders are free, each lane takes whole 32-bit words of codes of whichever keys and dims its fragment stands
 // for.  Per 32 keys of a warp, with g = lane / 4 and t = lane % 4:
 //   K   the lane holds words t G .. t G + G - 1 (an octet of each group) of keys g + 8 x.  The operand, fp16 for either
-//       type, is the code behind a magic exponent: 1024 + n where the nibble lies lowest, 1024 + 16 n where it lies second, one
-//       LOP3 per two codes and a shift per four, exact.  The queries carry what that needs: each row is brought to 2^10 by a
-//       power of two (bf16 reaches further than fp16; exact but for what is 2^-34 of the row's largest), every second dim by
-//       1 / 16 more.  The offsets come off in the accumulator, which starts at -(1032 sum of even + 72 sum of odd q) of the group; a group's
-//       sums are scaled in fp32 afterwards.  What fp32 sums of that size round is at most 2^-13 of sum |q| times the largest code.
-//   V   the lane holds words g D / 64 (+ 1) of keys 8 x + 2 t and 8 x + 2 t + 1.  Long sums would drown under such an offset, so
-//       here the operand is (n - 8) * scale, exact in the type (q4.cuh).  In bf16 the second nibble has no room behind an exponent: left alone it is
-//       the number n 2^-129 (gradual underflow joins the normal numbers at n = 8), which one FMA takes to (n - 8) / 4.
+//       type, is the code n - 8 itself: a LOP3 puts two of them behind an exponent, a half2 subtraction or multiply-add takes the offset
+//       off (left in the products, to be taken off in their sums, it costs the scores 2^-13 of sum |q| times the largest code).  Each
+//       row of queries is brought to 2^10 by a power of two (bf16 reaches further than fp16; exact but for what is 2^-34 of the
+//       row's largest); a group's sums are scaled in fp32 afterwards.  So a score is a sum of exact products in fp32.
+//   V   the lane holds words g D / 64 (+ 1) of keys 8 x + 2 t and 8 x + 2 t + 1.  Here the operand is (n - 8) * scale, exact in the
+//       type (q4.cuh).  In bf16 the second nibble has no room behind an exponent: left alone it is the number n 2^-129 (gradual
+//       underflow joins the normal numbers at n = 8), which one FMA takes to (n - 8) / 4.
 //   P   the scores' fragment is the transpose of what the second product reads: movmatrix.
 // The ALU (logic, shifts, permutes: half a warp instruction a clock) is the busiest unit; the FMA pipe, which does the rest of the
 // conversion, is not.
@@ -43,7 +42,7 @@ int g_path = 0;   // tunable "fmha_q4_path": 0 by size, 1 the few-row form, 2 th
 
 namespace {
 
-// S = A B + C in fp16 with fp32 accumulators
+// D = A B + C in fp16 with fp32 accumulators
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t* a, uint32_t b0, uint32_t b1, const float (&c)[4]) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
@@ -196,7 +195,7 @@ fmha_q4_kernel(const Args a, const int parts, const int ways, const int row_bloc
   Place next = first[Ring::kStages - 1];
   // ---- queries as the second operand: column g, dims of octet t of each group
   uint32_t qf[NT][G][4];
-  float bias[NT][G][4], unit[NT][2];   // `unit` takes a column's sums to scores in the log2 domain
+  float unit[NT][2];   // takes a column's sums to scores in the log2 domain
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int r = row0 + n * 8 + g;
@@ -222,22 +221,11 @@ fmha_q4_kernel(const Args a, const int parts, const int ways, const int row_bloc
     const float signed_lift = a.scale_log2 < 0.f ? -lift : lift;
 #pragma unroll
     for (int k = 0; k < G; ++k) {
-      float y[8], sum = 0.f;
+      float y[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        y[i] = __half2float(__float2half_rn(Elem<T>::to_f(x[k].v[i]) * signed_lift));
-        sum = fmaf(y[i], i & 1 ? -72.f : -1032.f, sum);
-      }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      bias[n][k][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
-      bias[n][k][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
-      // an accumulator of its own, so that it is not put together from two registers for every tile
-      asm("mov.b32 %0, %2;\n\tmov.b32 %1, %3;" : "=f"(bias[n][k][2]), "=f"(bias[n][k][3]) : "f"(bias[n][k][0]), "f"(bias[n][k][1]));
-      qf[n][k][0] = half2_bits(__floats2half2_rn(y[0], y[4]));
-      qf[n][k][1] = half2_bits(__floats2half2_rn(y[1] * 0.0625f, y[5] * 0.0625f));
-      qf[n][k][2] = half2_bits(__floats2half2_rn(y[2], y[6]));
-      qf[n][k][3] = half2_bits(__floats2half2_rn(y[3] * 0.0625f, y[7] * 0.0625f));
+      for (int i = 0; i < 8; ++i) y[i] = Elem<T>::to_f(x[k].v[i]) * signed_lift;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qf[n][k][i] = half2_bits(__floats2half2_rn(y[i], y[i + 4]));
     }
   }
 
@@ -277,12 +265,11 @@ fmha_q4_kernel(const Args a, const int parts, const int ways, const int row_bloc
           sc[x] = k & 1 ? Op<T>::high_f(ks[x][k / 2]) : Op<T>::low_f(ks[x][k / 2]);
         }
         const uint32_t wa = kw[0][k], wb = kw[1][k], ha = wa >> 8, hb = wb >> 8;
-        const uint32_t af[8] = {behind(wa, kLow, kMagic16), behind(wb, kLow, kMagic16), behind(wa, kSecond, kMagic16), behind(wb, kSecond, kMagic16),
-                                behind(ha, kLow, kMagic16), behind(hb, kLow, kMagic16), behind(ha, kSecond, kMagic16), behind(hb, kSecond, kMagic16)};
+        const uint32_t af[8] = {low_codes(wa), low_codes(wb), second_codes(wa), second_codes(wb), low_codes(ha), low_codes(hb), second_codes(ha), second_codes(hb)};
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          float c[4];
-          mma_f16(c, af, qf[n][k][0], qf[n][k][1], bias[n][k]);
+          float c[4] = {};
+          mma_f16(c, af, qf[n][k][0], qf[n][k][1], c);
           mma_f16(c, af + 4, qf[n][k][2], qf[n][k][3], c);
 #pragma unroll
           for (int x = 0; x < 4; ++x) s[n][i][x] = k == 0 ? sc[x >> 1] * c[x] : fmaf(sc[x >> 1], c[x], s[n][i][x]);

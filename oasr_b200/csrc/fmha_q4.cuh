@@ -45,6 +45,12 @@ __device__ __forceinline__ uint32_t behind(uint32_t w, uint32_t mask, uint32_t m
   return r;
 }
 
+// The codes n - 8 of two keys (one in each half) at bits 0..3 / 4..7, in fp16 and exact: behind an exponent where a step is 1 / 16.
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return half2_bits(__hsub2(as_half2(behind(w, kLow, kMagic16)), as_half2(0x64086408u))); }   // (1024 + n) - 1032
+__device__ __forceinline__ uint32_t second_codes(uint32_t w) {                                                                                           // (1024 + 16 n) / 16 - 72
+  return half2_bits(__hfma2(as_half2(behind(w, kSecond, kMagic16)), as_half2(0x2c002c00u), as_half2(0xd480d480u)));
+}
+
 // Codes times scales as operands.  `low` / `second`: the codes of two keys (one in each half) at bits 0..3 / 4..7, times the
 // keys' scales; `steep`: what second() wants for the scales.
 template <typename T>
@@ -70,15 +76,9 @@ struct Op<__nv_bfloat16> {
 };
 template <>
 struct Op<__half> {
-  static __device__ __forceinline__ uint32_t low(uint32_t w, uint32_t scale) {   // ((1024 + n) - 1032) s
-    const __half2 v = __hsub2(as_half2(behind(w, kLow, kMagic16)), as_half2(0x64086408u));
-    return half2_bits(__hmul2(v, as_half2(scale)));
-  }
+  static __device__ __forceinline__ uint32_t low(uint32_t w, uint32_t scale) { return half2_bits(__hmul2(as_half2(low_codes(w)), as_half2(scale))); }
   static __device__ __forceinline__ uint32_t steep(uint32_t scale) { return scale; }
-  static __device__ __forceinline__ uint32_t second(uint32_t w, uint32_t scale) {   // ((1024 + 16 n) / 16 - 72) s
-    const __half2 v = __hfma2(as_half2(behind(w, kSecond, kMagic16)), as_half2(0x2c002c00u), as_half2(0xd480d480u));
-    return half2_bits(__hmul2(v, as_half2(scale)));
-  }
+  static __device__ __forceinline__ uint32_t second(uint32_t w, uint32_t scale) { return half2_bits(__hmul2(as_half2(second_codes(w)), as_half2(scale))); }
   static __device__ __forceinline__ float low_f(uint32_t w) { return __low2float(as_half2(w)); }
   static __device__ __forceinline__ float high_f(uint32_t w) { return __high2float(as_half2(w)); }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return half2_bits(__floats2half2_rn(lo, hi)); }

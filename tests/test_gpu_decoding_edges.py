@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import oasr_b200 as ob
-from tests.test_gpu_decoding import DTYPES, EPS, check_scores, chunk, rand, score64
+from tests.test_gpu_decoding import DTYPES, EPS, HALF, check_scores, chunk, form, pages, pack, quantise64, rand, score64  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +96,78 @@ def test_token_log_probs_of_one_token_are_one_number(dtype, rows, V):
     got = ob.token_log_probs(x, ids, top_k=32)
     assert torch.equal(got.top_ids, ids) and torch.equal(got.log_probs, got.top_log_probs)
     assert (got.top_log_probs[:, :3] == got.top_log_probs[:, :1]).all() and got.top_ids[0, :3].tolist() == [0, V // 3, V - 1]
+
+
+# ---- attention over 4-bit pages -----------------------------------------------------------------------------------------
+def attend_bound(q, k, v, scale, lens, partial, dt):
+    """``q (B, H, T, D)`` over the first ``lens`` of ``k``, ``v (B, Hkv, N, D)`` in 64 bits: the result, and how far an element may be off.
+
+    A score is a sum of D exact products in steps of 16 on the tensor cores; each of the 17 addends of a step is cut at 2^-23 of the
+    largest of them, a product or a partial sum (``partial``: a bound of what that reaches, (B, H, T, N)).  Scores off by at most e
+    move weights by a factor within exp(+-2 e), which moves the result by (exp(2 e) - 1) sum p |v - result|.  Weights are rounded to the
+    type (their sum is not), and so is the result; 2^-16 is for the exponentials (2^-22 each, their arguments 2^-24 of 126 at most) and sums.
+    What a type cannot hold: weights are relative to a maximum that is the row's or up to 2^8 below it, so the largest is 1 or more, and an
+    fp16 one below 2^-14 is off by 2^-25 (so is a result); in bf16 exponentials below 2^-126 are zero, relative to a warp's own maximum, whose
+    weights may reach 2^8 times that."""
+    share = q.shape[1] // k.shape[1]
+    k, v = (x.repeat_interleave(share, 1) for x in (k, v))
+    seen = torch.arange(k.shape[2]) < torch.tensor(lens)[:, None]
+    s = (q @ k.transpose(2, 3) * scale).masked_fill(~seen[:, None, None], -math.inf)
+    p = torch.softmax(s, -1)
+    want = p @ v
+    off = 17 * (q.shape[3] // 16) * 2.0 ** -23 * abs(scale) * (partial * seen[:, None, None]).amax(-1, keepdim=True)
+    spread = torch.stack([(p[..., j, None] * (v[:, :, None, j] - want).abs()) for j in range(k.shape[2])]).sum(0)
+    least = 2.0 ** -25 if dt == torch.float16 else 2.0 ** -118
+    tiny = least * (1 + (v.abs() * seen[:, None, :, None]).sum(2, keepdim=True))
+    return want, HALF[dt] * want.abs() + (HALF[dt] + 2.0 ** -16) * (p @ v.abs()) + torch.expm1(2 * off) * spread + tiny
+
+
+def check_attention(q, pools, bt, lens, scale, partial=None):
+    """Attention over pools, whose values the gather gives exactly, within the bound above."""
+    k, v = (x.cpu().double() for x in ob.gather_paged_kv_q4(*pools, bt.cuda(), None, max(lens)))
+    x = q.cpu().double()
+    if partial is None:                                    # in whatever order: no partial sum is larger than the sum of magnitudes
+        partial = x.abs() @ k.abs().repeat_interleave(x.shape[1] // k.shape[1], 1).transpose(2, 3)
+    want, tol = attend_bound(x, k, v, scale, lens, partial, q.dtype)
+    got = ob.fmha_q4(q, *pools, softmax_scale=scale, block_table=bt.cuda(), cache_seqlens=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    off = (got.cpu().double() - want).abs()
+    assert (off <= tol).all(), f"{int((off > tol).sum())} of {off.numel()} off, the worst {float((off / tol).max()):.2f} times its bound"
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [1, 5, 20, 130])
+def test_fmha_q4_scores_of_products_that_cancel(form, dtype, D, T):
+    """Queries with a large common offset against keys whose neighbouring dims nearly cancel: moderate scores out of large products."""
+    dt, B, H, Hkv, block = DTYPES[dtype], 16, 4, 2, 16
+    g = torch.Generator().manual_seed(D + T)
+    bt, n = pages(3, B, 1)
+    shape = (n, Hkv, block, D // 2)
+    even = torch.randint(3, 7, shape, generator=g) * (2 * torch.randint(0, 2, shape, generator=g) - 1)
+    few = torch.where(torch.rand(shape, generator=g) < 4 / (D // 2), 2 * torch.randint(0, 2, shape, generator=g) - 1, 0)   # some four pairs of a row
+    codes = torch.stack([even, -even + few], -1).flatten(-2)
+    v_codes, v_scales = quantise64(rand(4, n, Hkv, block, D), dt)
+    k_scales = torch.full((n, Hkv, block, D // 32), 0.375, dtype=dt)
+    pools = [pack(codes).cuda(), k_scales.cuda(), pack(v_codes).cuda(), v_scales.to(dt).cuda()]
+    q = (256 * 2.0 ** (-6 * torch.rand(B, H, T, D // 2, generator=g, dtype=torch.float64))).repeat_interleave(2, -1).to(dt).cuda()
+    lens = torch.randint(2, 7, (B,), generator=g).tolist()
+    # a step of 16 holds both dims of a pair in either kernel: partial sums are of pairs, four of which are not zero (or one product)
+    k = ob.gather_paged_kv_q4(*pools, bt.cuda(), None, max(lens))[0].cpu().double().repeat_interleave(H // Hkv, 1)
+    x = q.cpu().double()
+    single = (x[..., None, :] * k[:, :, None]).abs().amax(-1)
+    pairs = (x[..., None, :] * k[:, :, None]).unflatten(-1, (-1, 2)).sum(-1).abs().sum(-1)
+    check_attention(q, pools, bt, lens, D ** -0.5, torch.maximum(single, pairs))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("size", [300.0, 17.0, 1.0, 1e-3])
+def test_fmha_q4_of_scores_of_any_size(form, dtype, D, T, size):
+    dt, B, H, Hkv = DTYPES[dtype], 3, 4, 2
+    bt, n = pages(5, B, 6)
+    pools = []
+    for i in range(2):
+        codes, scales = quantise64(rand(20 + i, n, Hkv, 16, D), dt)
+        pools += [pack(codes).cuda(), scales.to(dt).cuda()]
+    check_attention((size * rand(22, B, H, T, D)).to(dt).cuda(), pools, bt, [96, 50, 2], D ** -0.5)
