@@ -20,6 +20,11 @@ def _stride_array(a: int, b: int, c: int):
     return _Strides(a, b, c)
 
 
+def _used_strides(n0: int, n1: int, n2: int, s0: int, s1: int, s2: int):
+    """Strides of three dimensions as the kernels use them: that of a dimension of size 1 may be any number, and is none."""
+    return s0 if n0 > 1 else 0, s1 if n1 > 1 else 0, s2 if n2 > 1 else 0
+
+
 def _strides3(t: torch.Tensor):
     """(batch, head, row) element strides of a (B, H, T, D) view as a host int64[3]; None if the
     view cannot be addressed by the kernel (unit stride along D, the rest multiples of 8)."""
@@ -296,10 +301,11 @@ def fmha_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_co
     lens, starts = _index32("cache_seqlens", cache_seqlens, B), _index32("cache_seqstarts", cache_seqstarts, B)
     q_lens = _index32("q_lens", q_lens, B)
     _one_device(q, k_codes, k_scales, v_codes, v_scales, block_table, lens, starts, q_lens, out)
-    sb, sh, st, unit = q.stride()
-    if unit != 1 or sb % 8 or sh % 8 or st % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
-        sb, sh, st, unit = q.stride()
+    qs = q.stride()
+    sb, sh, st = _used_strides(B, H, T, *qs[:3])
+    if qs[3] != 1 or sb % 8 or sh % 8 or st % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)   # (contiguous() would keep one that is merely misaligned)
+        sb, sh, st = H * T * D, T * D, D
     if out is None:
         if token_major:
             out = torch.empty(B, T, H, D, dtype=q.dtype, device=q.device)
@@ -313,7 +319,7 @@ def fmha_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_co
             raise ValueError(f"out must be {want} in q's dtype, with unit stride along D")
         _check_distinct_rows(out=out)
         ob, oh, ot = (out.stride(0), out.stride(2), out.stride(1)) if token_major else out.stride()[:3]
-        os = _stride_array(ob, oh, ot)
+        os = _stride_array(*_used_strides(B, H, T, ob, oh, ot))
     _lib.call("oasr_b200_fmha_q4", out.data_ptr(), os, q.data_ptr(), _stride_array(sb, sh, st), k_codes.data_ptr(), k_scales.data_ptr(),
               v_codes.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(), lens.data_ptr(), _p(starts), _p(q_lens), block_table.shape[1],
               block_size, num_blocks, B, H, Hkv, T, D, softmax_scale, bool(causal), _DTYPE_ID[q.dtype], _stream(q))

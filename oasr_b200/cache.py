@@ -9,7 +9,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .attention import _HALF, _check_q4_pools, _stride_array, _index32, _table32, fmha_q4, gather_paged_kv, gather_paged_kv_q4  # noqa: F401  (re-exported)
+from .attention import _HALF, _check_q4_pools, _stride_array, _index32, _table32, _used_strides, fmha_q4, gather_paged_kv, gather_paged_kv_q4  # noqa: F401  (re-exported)
 from .functional import _DTYPE_ID, _check_distinct_rows, _check_head_weight, _check_rope_table, _need_cuda, _one_device, _p, _stream
 
 
@@ -80,7 +80,7 @@ def _heads(x: torch.Tensor):
     if unit != 1:
         x = x.contiguous()
         sb, sh, st, unit = x.stride()
-    return x, _stride_array(sb, sh, st)
+    return x, _stride_array(*_used_strides(*x.shape[:3], sb, sh, st))
 
 
 def _write_rope(entry, pools, num_blocks, block_size, pool_heads, pool_dim, block_table, new_k, new_v, offset, cos_sin, q, q_weight,
@@ -122,7 +122,7 @@ def _write_rope(entry, pools, num_blocks, block_size, pool_heads, pool_dim, bloc
             _check_distinct_rows(q_out=q_out)
         q, qs = _heads(q)
         sb, sh, st, _ = q_out.stride()
-        src, dst, qo = q.data_ptr(), q_out.data_ptr(), _stride_array(sb, sh, st)
+        src, dst, qo = q.data_ptr(), q_out.data_ptr(), _stride_array(*_used_strides(B, H, T, sb, sh, st))
     elif q_out is not None or q_weight is not None:
         raise ValueError("q_out and q_weight need q")
     _lib.call(entry, dst, qo, *[p.data_ptr() for p in pools], src, qs, new_k.data_ptr(), ks, new_v.data_ptr(), vs,

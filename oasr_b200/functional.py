@@ -567,6 +567,10 @@ def qk_norm_rope(q, k, cos_sin, positions, q_weight=None, k_weight=None, *, eps:
     qs_n, qs_h, unit = q.stride()
     if unit != 1:
         raise RuntimeError("qk_norm_rope needs unit stride along head_dim")
+    if N == 1:
+        qs_n = 0                          # the stride of a dimension of size 1 may be any number
+    if H == 1:
+        qs_h = 0
     q_dst, qo_n, qo_h, q_out = _turned("q", q, q_out, N, H, D)
     Hkv = ks_n = ks_h = ko_n = ko_h = 0
     k_src = k_dst = None
@@ -577,6 +581,10 @@ def qk_norm_rope(q, k, cos_sin, positions, q_weight=None, k_weight=None, *, eps:
         ks_n, ks_h, unit = k.stride()
         if n != N or d != D or unit != 1:
             raise RuntimeError("qk_norm_rope expects q (N, H, D) and k (N, H_kv, D) with unit stride along head_dim")
+        if N == 1:
+            ks_n = 0
+        if Hkv == 1:
+            ks_h = 0
         k_dst, ko_n, ko_h, k_out = _turned("k", k, k_out, N, Hkv, D)
         k_src = k.data_ptr()
     elif k_out is not None or k_weight is not None:
@@ -601,7 +609,7 @@ def _turned(name, x, out, N, H, D):
     elif out.shape != x.shape or out.dtype != x.dtype or out.stride(2) != 1:
         raise RuntimeError(f"{name}_out must have the shape and dtype of {name}, with unit stride along head_dim")
     _check_distinct_rows(**{name + "_out": out})
-    return out.data_ptr(), out.stride(0), out.stride(1), out
+    return out.data_ptr(), out.stride(0) if N > 1 else 0, out.stride(1) if H > 1 else 0, out
 
 
 def _check_distinct_rows(**outs) -> None:

@@ -171,3 +171,61 @@ def test_fmha_q4_of_scores_of_any_size(form, dtype, D, T, size):
         codes, scales = quantise64(rand(20 + i, n, Hkv, 16, D), dt)
         pools += [pack(codes).cuda(), scales.to(dt).cuda()]
     check_attention((size * rand(22, B, H, T, D)).to(dt).cuda(), pools, bt, [96, 50, 2], D ** -0.5)
+
+
+# ---- views --------------------------------------------------------------------------------------------------------------
+def odd_view(x, dims):
+    """The values of ``x`` behind strides that no kernel may ask for, in dimensions of size 1."""
+    buf = torch.empty(x.numel() + 8 * x.dim(), dtype=x.dtype, device=x.device)
+    strides = [7 if d in dims else s for d, s in enumerate(x.stride())]
+    assert all(x.shape[d] == 1 for d in dims)
+    return buf.as_strided(x.shape, strides).copy_(x)
+
+
+def late(x):
+    """The values of ``x``, contiguous, at an address that is a multiple of the element alone."""
+    return torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)[1:].view(x.shape).copy_(x)
+
+
+def test_fmha_q4_takes_any_query_view():
+    bt, n = pages(3, 3, 2)
+    codes, scales = quantise64(rand(7, n, 1, 16, 64), torch.bfloat16)
+    pools = [pack(codes).cuda(), scales.bfloat16().cuda()] * 2
+    for B, H, T in ((1, 1, 1), (3, 2, 1), (1, 4, 5), (3, 1, 2)):
+        q = rand(5, B, H, T, 64).bfloat16().cuda()
+        how = dict(softmax_scale=0.125, block_table=bt[:B].cuda(), cache_seqlens=torch.full((B,), 20, dtype=torch.int32, device="cuda"))
+        want = ob.fmha_q4(q, *pools, **how)
+        ones = [d for d in range(3) if q.shape[d] == 1]
+        for x in (odd_view(q, ones), late(q), late(q).transpose(1, 2).contiguous().transpose(1, 2)):
+            assert torch.equal(ob.fmha_q4(x, *pools, **how), want)
+        out = odd_view(torch.empty_like(q), ones)
+        assert ob.fmha_q4(q, *pools, out=out, **how) is out and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("q4", [False, True])
+def test_write_kv_rope_takes_any_stride_of_one(q4):
+    table = ob.rope_table(64, 64)
+    for B, H, T in ((1, 1, 1), (2, 1, 1), (1, 2, 3), (1, 1, 4)):
+        q, k, v = (rand(s, B, H, T, 64).bfloat16().cuda() for s in (1, 2, 3))
+        bt = torch.arange(B, dtype=torch.int32, device="cuda")[:, None]
+        ones = [d for d in range(3) if q.shape[d] == 1]
+        got = []
+        for view in (lambda x: x, lambda x: odd_view(x, ones)):
+            pools = ob.PagedKVCacheQ4.empty_pools(B, H, 16, 64) if q4 else [torch.zeros(B, 16, H, 64, device="cuda").bfloat16() for _ in range(2)]
+            out = view(torch.empty_like(q))
+            write = ob.write_kv_rope_q4 if q4 else ob.write_kv_rope
+            assert write(*pools, bt, view(k), view(v), 2, table, q=view(q), q_out=out) is out
+            got.append([out, *pools])
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_qk_norm_rope_takes_any_stride_of_one():
+    table = ob.rope_table(64, 64)
+    for N, H in ((1, 1), (1, 3), (4, 1)):
+        q, pos = rand(1, N, H, 64).bfloat16().cuda(), torch.arange(N, device="cuda") + 3
+        want = ob.qk_norm_rope(q, q, table, pos)
+        ones = [d for d in range(2) if q.shape[d] == 1]
+        outs = [odd_view(torch.empty_like(q), ones) for _ in range(2)]
+        for how in ({}, dict(q_out=outs[0], k_out=outs[1])):
+            got = ob.qk_norm_rope(odd_view(q, ones), odd_view(q, ones), table, pos, **how)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
