@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import oasr_b200 as ob
-from tests.test_gpu_decoding import DTYPES, EPS, HALF, check_scores, chunk, form, pages, pack, quantise64, rand, score64  # noqa: F401
+from tests.test_gpu_decoding import DTYPES, EPS, HALF, check_scores, chunk, form, norm64, pages, pack, quantise64, rand, rope64, score64  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -229,3 +229,60 @@ def test_qk_norm_rope_takes_any_stride_of_one():
         for how in ({}, dict(q_out=outs[0], k_out=outs[1])):
             got = ob.qk_norm_rope(odd_view(q, ones), odd_view(q, ones), table, pos, **how)
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- 4-bit codes, each within its bound ---------------------------------------------------------------------------------
+def five_bits(x, dt):
+    """The scale of a group whose largest magnitude is ``x``, in 64 bits."""
+    m, e = torch.frexp(x / 7)
+    lo, hi = (2.0 ** -20, 9216.0) if dt == torch.float16 else (2.0 ** -120, 1.125 * 2.0 ** 125)
+    return torch.ldexp(torch.ceil(m * 32) / 32, e).clamp(lo, hi)
+
+
+def unpacked(codes):
+    """(..., D / 2) bytes -> (..., D) codes."""
+    D = 2 * codes.shape[-1]
+    nib = torch.stack([codes.long() & 15, codes.long() >> 4], -1).flatten(-2) - 8
+    d = torch.arange(D)
+    return nib[..., ((d % 32) // 8 * (D // 32) + d // 32) * 8 + d % 8].double()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("B,H,Hkv,T,D,R,block,inter", [
+    (1, 8, 8, 1, 64, 64, 16, False), (5, 16, 4, 1, 128, 128, 16, False), (3, 4, 1, 17, 64, 32, 16, False), (4, 2, 2, 33, 64, 64, 32, True), (3, 3, 1, 5, 96, 32, 16, False),
+    (37, 8, 2, 16, 64, 64, 16, False), (2, 2, 1, 3, 32, 16, 16, False), (2, 1, 1, 9, 256, 128, 16, True), (2, 1, 3, 40, 128, 96, 16, False), (3, 1, 1, 30, 512, 512, 16, False)])
+def test_every_code_is_as_near_as_fp32_can_tell(dtype, norm, B, H, Hkv, T, D, R, block, inter):
+    dt = DTYPES[dtype]
+    _, k, v = chunk(15, B, H, Hkv, T, D, dt, T % 2 == 1)
+    kw = (1 + 0.2 * rand(3, D)).to(dt).cuda() if norm else None
+    table = ob.rope_table(400, R)
+    g = torch.Generator().manual_seed(16)
+    off, lens = torch.randint(0, 60, (B,), generator=g), torch.randint((T + 1) // 2, T + 1, (B,), generator=g)
+    bt, n = pages(17, B, -(-(60 + T) // block))
+    before = [torch.randint(1, 255, p.shape, generator=g, dtype=torch.uint8) if p.dtype == torch.uint8 else rand(9, *p.shape).abs().to(dt)
+              for p in ob.PagedKVCacheQ4.empty_pools(n, Hkv, block, D, dt, device="cpu")]
+    after = [p.clone().cuda() for p in before]
+    ob.write_kv_rope_q4(*after, bt.cuda(), k, v, off.cuda(), table, k_weight=kw, eps=EPS, interleaved=inter, new_lens=lens.cuda())
+    after = [p.cpu() for p in after]
+    written = torch.zeros(n, block, dtype=torch.bool)
+    for b in range(B):
+        m = int(lens[b])
+        pos = int(off[b]) + torch.arange(m)
+        page, slot = bt[b].long()[pos // block], pos % block
+        written[page, slot] = True
+        kn = norm64(k[b].transpose(0, 1)[:m].cpu().double(), None if kw is None else kw.cpu())
+        for i, x, e in ((0, rope64(kn, table.cpu(), pos, inter), None), (2, v[b].transpose(0, 1)[:m].cpu().double(), 0.0)):
+            if e is None:
+                # in fp32: the sum of squares 16 + 5 steps, mean and eps 3 more, all halved by the root, the root 4, two products; a rotation's
+                # two products and sum, each of at most sqrt(2) of the row's largest
+                e = (18 + 2) * 2.0 ** -24 * 1.42 * kn.abs().amax(-1, keepdim=True) if norm else 2 * 2.0 ** -24 * 1.42 * kn.abs().amax(-1, keepdim=True)
+            e = torch.as_tensor(e, dtype=torch.float64).expand(*x.shape[:-1], 1)
+            codes, scales = unpacked(after[i][page, :, slot]), after[i + 1][page, :, slot].double()
+            top = x.unflatten(-1, (-1, 32)).abs().amax(-1)
+            near = e + 2.0 ** -24 * top if i == 0 else e      # (and its quotient by 7 rounds)
+            assert ((scales == five_bits(top - near, dt)) | (scales == five_bits(top + near, dt))).all()
+            quotient = x / scales.repeat_interleave(32, -1)
+            assert (codes.abs() <= 7).all() and ((codes - quotient.clamp(-7, 7)).abs() <= 0.5 + e / scales.repeat_interleave(32, -1)).all()
+    for a, b in zip(after, before):
+        assert torch.equal(a.transpose(1, 2)[~written], b.transpose(1, 2)[~written])
