@@ -29,6 +29,8 @@
 // B200: 64 sequences of 6000 keys, 32 heads of 128 over 8 key heads, one token each: 117-121 us (442 MB, 3.7 TB/s), bound by
 // instructions (some 700 of a warp for 32 keys; ALU 0.55 busy, issue slots 0.64).  256 chunks of 16 rows over up to 1001 keys, 8 heads of
 // 64: 51 us, a third of it a block's start (lengths, pages, first tile) and end.
+#include <cmath>
+
 #include "common.cuh"
 #include "fmha_q4.cuh"
 #include "q4.cuh"
@@ -584,6 +586,8 @@ extern "C" int oasr_b200_fmha_q4(void* out, const int64_t* out_strides, const vo
   OB_REQUIRE(Hkv * block_size * D <= 0x7fffffff, OASR_ERR_INVALID, "fmha_q4: pages too large");
   OB_REQUIRE(B <= 65535 && H <= 65535 && Tq <= 0x7fffff && blocks_per_seq * block_size <= 0x7fffffff, OASR_ERR_INVALID,
              "fmha_q4: batch, head count or length too large");
+  // (a scale that is no number would pass for one of zero: scores and scale meet in fmaxf)
+  OB_REQUIRE(std::isfinite(static_cast<float>(scale * 1.4426950408889634)), OASR_ERR_INVALID, "fmha_q4: softmax_scale must be a finite number");
   if (B == 0 || Tq == 0) return OASR_OK;
   OB_REQUIRE(out && out_strides && q && q_strides && k_codes && k_scales && v_codes && v_scales && (block_table || blocks_per_seq == 0) && seqlens, OASR_ERR_INVALID,
              "fmha_q4: null pointer argument");
