@@ -220,6 +220,13 @@ def fmha_varlen(q, k, v, *, softmax_scale: float, cu_seqlens_q: torch.Tensor, cu
     return out
 
 
+def _narrow(t: torch.Tensor) -> torch.Tensor:
+    """As int32; what 32 bits do not hold goes to the nearest number that they do, and not round to one that means something."""
+    if t.dtype == torch.int64:
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1)
+    return t.to(torch.int32)
+
+
 def _index32(name: str, t: Optional[torch.Tensor], B: int) -> Optional[torch.Tensor]:
     """A number for each sequence as the kernels take it."""
     if t is None:
@@ -227,7 +234,7 @@ def _index32(name: str, t: Optional[torch.Tensor], B: int) -> Optional[torch.Ten
     if t.shape != (B,):
         raise ValueError(f"{name} must be ({B},), got {tuple(t.shape)}")
     if t.dtype != torch.int32:
-        t = t.to(torch.int32)
+        t = _narrow(t)
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -235,7 +242,7 @@ def _table32(table: torch.Tensor, B: int) -> torch.Tensor:
     if table.dim() != 2 or table.shape[0] != B:
         raise ValueError("block_table must be (B, max_blocks_per_seq)")
     if table.dtype != torch.int32:
-        table = table.to(torch.int32)
+        table = _narrow(table)
     return table if table.is_contiguous() else table.contiguous()
 
 

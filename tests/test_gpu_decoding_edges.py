@@ -286,3 +286,32 @@ def test_every_code_is_as_near_as_fp32_can_tell(dtype, norm, B, H, Hkv, T, D, R,
             assert (codes.abs() <= 7).all() and ((codes - quotient.clamp(-7, 7)).abs() <= 0.5 + e / scales.repeat_interleave(32, -1)).all()
     for a, b in zip(after, before):
         assert torch.equal(a.transpose(1, 2)[~written], b.transpose(1, 2)[~written])
+
+
+# ---- wide indices -------------------------------------------------------------------------------------------------------
+def test_64_bit_indices_outside_32_bits_are_outside():
+    """int64 tables and numbers: 2^32 more than a page is no page, and what lies beyond 32 bits counts as far."""
+    B, H, D = 6, 2, 64
+    bt, n = pages(3, B, 2)
+    bt = bt.long()
+    far = bt.clone()
+    far[0, 0] += 2 ** 32
+    far[1, 1], far[2, 0], far[2, 1] = -2 ** 63, 2 ** 63 - 1, -2 ** 32
+    none = far.where((far >= 0) & (far < n), torch.tensor(-1)).int().cuda()
+    far, table = far.cuda(), ob.rope_table(64, D)
+    q, k, v = (rand(s, B, H, 3, D).bfloat16().cuda() for s in (1, 2, 3))
+    off = torch.tensor([0, 14, 0, 2 ** 32, -2 ** 32, 5], device="cuda")
+    off32 = torch.tensor([0, 14, 0, 2 ** 31 - 1, -2 ** 31, 5], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([20, 20, 20, 2 ** 32 + 5, 2 ** 33, -2 ** 40], device="cuda")
+    lens32 = torch.tensor([20, 20, 20, 2 ** 31 - 1, 2 ** 31 - 1, 0], dtype=torch.int32, device="cuda")
+    start = torch.tensor([0, 0, 0, -2 ** 40, 2 ** 32, 0], device="cuda")
+    start32 = torch.tensor([0, 0, 0, 0, 2 ** 31 - 1, 0], dtype=torch.int32, device="cuda")
+    got = []
+    for t, o, length, s in ((far, off, lens, start), (none, off32, lens32, start32)):
+        pools = ob.PagedKVCacheQ4.empty_pools(n, H, 16, D)
+        plain = [torch.zeros(n, 16, H, D, device="cuda").bfloat16() for _ in range(2)]
+        for p, write in ((pools, ob.write_kv_rope_q4), (plain, ob.write_kv_rope)):
+            write(*p, t, k, v, o, table, new_lens=length.clamp(0, 3))
+        att = ob.fmha_q4(q, *pools, softmax_scale=0.125, block_table=t, cache_seqlens=length, cache_seqstarts=s)
+        got.append([*pools, *plain, att, *ob.gather_paged_kv_q4(*pools, t, o, 9)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
