@@ -584,7 +584,8 @@ extern "C" int oasr_b200_fmha_q4(void* out, const int64_t* out_strides, const vo
   OB_REQUIRE(block_size > 0 && block_size % 16 == 0, OASR_ERR_UNSUPPORTED, "fmha_q4: the block size must be a multiple of 16 (got %lld)",
              (long long)block_size);
   OB_REQUIRE(Hkv * block_size * D <= 0x7fffffff, OASR_ERR_INVALID, "fmha_q4: pages too large");
-  OB_REQUIRE(B <= 65535 && H <= 65535 && Tq <= 0x7fffff && blocks_per_seq * block_size <= 0x7fffffff, OASR_ERR_INVALID,
+  // (a position and a whole tile more fit 32 bits)
+  OB_REQUIRE(B <= 65535 && H <= 65535 && Tq <= 0x7fffff && blocks_per_seq * block_size <= 0x7fffff00, OASR_ERR_INVALID,
              "fmha_q4: batch, head count or length too large");
   // (a scale that is no number would pass for one of zero: scores and scale meet in fmaxf)
   OB_REQUIRE(std::isfinite(static_cast<float>(scale * 1.4426950408889634)), OASR_ERR_INVALID, "fmha_q4: softmax_scale must be a finite number");
