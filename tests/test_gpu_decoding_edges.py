@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import oasr_b200 as ob
-from tests.test_gpu_decoding import DTYPES, EPS, HALF, check_scores, chunk, form, norm64, pages, pack, quantise64, rand, rope64, score64  # noqa: F401
+from tests.test_gpu_decoding import DTYPES, EPS, HALF, attend64, check_scores, chunk, close, form, norm64, pages, pack, quantise64, rand, rope64, score64  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -315,3 +315,29 @@ def test_64_bit_indices_outside_32_bits_are_outside():
         att = ob.fmha_q4(q, *pools, softmax_scale=0.125, block_table=t, cache_seqlens=length, cache_seqstarts=s)
         got.append([*pools, *plain, att, *ob.gather_paged_kv_q4(*pools, t, o, 9)])
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+# ---- tables wider than the sequences, windows ---------------------------------------------------------------------------
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [1, 6, 40])
+@pytest.mark.parametrize("wide", [1, 4, 32])
+@pytest.mark.parametrize("window", [False, True])
+def test_fmha_q4_in_a_table_wider_than_its_sequences(form, D, T, wide, window):
+    """As a cache of (slots, most pages) hands it out; entries behind the length are of other sequences' pages or none."""
+    B, H, Hkv, dt = 3, 4, 2, torch.bfloat16
+    lens = [300, 47, 130]
+    starts = [250, 0, 129] if window else None
+    bt, n = pages(5, B, 19)
+    table = torch.randint(-1, n + 1, (B, 19 * wide), generator=torch.Generator().manual_seed(wide)).int()
+    table[:, :19] = bt
+    pools = []
+    for i in range(2):
+        codes, scales = quantise64(rand(20 + i, n, Hkv, 16, D), dt)
+        pools += [pack(codes).cuda(), scales.to(dt).cuda()]
+    q = rand(22, B, H, T, D).to(dt).cuda()
+    cuda = lambda x: None if x is None else torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    got = ob.fmha_q4(q, *pools, softmax_scale=D ** -0.5, block_table=table.cuda(), cache_seqlens=cuda(lens), cache_seqstarts=cuda(starts), causal=True)
+    k, v = (x.cpu().double() for x in ob.gather_paged_kv_q4(*pools, bt.cuda(), None, max(lens)))
+    want = attend64(q.cpu().double(), k, v, D ** -0.5, lens, starts, None, True)
+    # half a step of the weights and of the result, and a score's fp32 sum: D products of at most 30 in all, 2^-23 of that for each of D / 16 steps of 17
+    close(got, want, HALF[dt], float(v.abs().max()) * (HALF[dt] + 2 * 17 * (D // 16) * 2.0 ** -23 * 30))
