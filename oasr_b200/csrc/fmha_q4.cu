@@ -108,7 +108,7 @@ fmha_q4_kernel(const Args a, const int parts, const int ways, const int row_bloc
   const int hk = at % a.Hkv, b = at / a.Hkv;
   const int share = a.H / a.Hkv;
   const int rows = group < groups ? share * a.Tq : 0, row0 = rb * NR;
-  const int len = a.seqlens[b], q_len = a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq;
+  const int len = max(a.seqlens[b], 0), q_len = a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq;
   const int capacity = static_cast<int>(a.blocks_per_seq * a.block_size);
   const int start = a.seqstarts ? max(a.seqstarts[b], 0) : 0;
 

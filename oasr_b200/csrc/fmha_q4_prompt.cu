@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_q4_prompt_kernel(const Args 
   const int heads = a.B * a.Hkv, rb = row_blocks - 1 - static_cast<int>(blockIdx.x) / heads;
   const int bh = static_cast<int>(blockIdx.x) % heads, b = bh / a.Hkv, hk = bh - b * a.Hkv;
   const int share = a.H / a.Hkv, rows = share * a.Tq, row0 = rb * 256;
-  const int len = a.seqlens[b], q_len = a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq;
+  const int len = max(a.seqlens[b], 0), q_len = a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq;
   const int capacity = static_cast<int>(a.blocks_per_seq * a.block_size);
   const int start = a.seqstarts ? max(a.seqstarts[b], 0) : 0;
   auto limit_of = [&](int r) {   // keys that row r may see: [start, limit)

@@ -341,3 +341,19 @@ def test_fmha_q4_in_a_table_wider_than_its_sequences(form, D, T, wide, window):
     want = attend64(q.cpu().double(), k, v, D ** -0.5, lens, starts, None, True)
     # half a step of the weights and of the result, and a score's fp32 sum: D products of at most 30 in all, 2^-23 of that for each of D / 16 steps of 17
     close(got, want, HALF[dt], float(v.abs().max()) * (HALF[dt] + 2 * 17 * (D // 16) * 2.0 ** -23 * 30))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("T", [1, 9, 150])
+def test_fmha_q4_of_negative_lengths(form, causal, T):
+    """A length below zero is one of zero, down to the type's lowest, from which no more can be taken."""
+    bt, n = pages(3, 5, 4)
+    codes, scales = quantise64(rand(7, n, 1, 16, 64), torch.bfloat16)
+    pools = [pack(codes).cuda(), scales.bfloat16().cuda()] * 2
+    q = rand(5, 5, 2, T, 64).bfloat16().cuda()
+    how = dict(softmax_scale=0.125, block_table=bt.cuda(), causal=causal)
+    lens = torch.tensor([-2 ** 31, -2 ** 31 + 3, -1, 0, 60], device="cuda")
+    for kind in (torch.int32, torch.int64):
+        out = ob.fmha_q4(q, *pools, cache_seqlens=lens.to(kind), **how)
+        assert not out[:4].any() and out[4].any()
+    assert torch.equal(ob.fmha_q4(q, *pools, cache_seqlens=torch.tensor([-2 ** 40, -2 ** 63, -7, 0, 60], device="cuda"), **how), out)
