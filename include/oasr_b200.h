@@ -760,8 +760,10 @@ OASR_API int oasr_b200_paged_kv_gather_q4(void* k_out, void* v_out, const void* 
                                           void* stream);
 /* Attention of q (B, H, Tq, D) over 4-bit pages: out[t] = softmax(scale q_t . k_j) v over the keys j with
  * seqstarts[b] <= j < seqlens[b] (seqstarts NULL: 0) whose page lies in the pool, and with `causal`
- * j <= seqlens[b] - q_lens[b] + t (q_lens NULL: Tq).  Rows t >= q_lens[b] and rows that see nothing are zeros.  Strides are host
- * int64[3] (batch, head, row) in elements, multiples of 8.  D 64 or 128, H a multiple of Hkv, block_size of 16. */
+ * j <= seqlens[b] - q_lens[b] + t (q_lens NULL: Tq).  Rows t >= q_lens[b] and rows that see nothing are zeros; a length below zero
+ * is zero.  Strides are host int64[3] (batch, head, row) in elements, multiples of 8.  D 64 or 128, H a multiple of Hkv, block_size
+ * of 16, blocks_per_seq * block_size up to 2^31 - 256, a finite scale.  fp32 scores, sums and output; the weights are rounded to the
+ * element type before the second product.  The work is split by blocks_per_seq: a table much wider than the sequences costs time. */
 OASR_API int oasr_b200_fmha_q4(void* out, const int64_t* out_strides, const void* q, const int64_t* q_strides,
                                const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
                                const int32_t* block_table, const int32_t* seqlens, const int32_t* seqstarts,
@@ -770,7 +772,8 @@ OASR_API int oasr_b200_fmha_q4(void* out, const int64_t* out_strides, const void
 /* Scores of logits (rows, vocab), rows `stride` elements apart, vocab up to 262144, fp32 / fp16 / bf16; all outputs fp32.
  * log_probs (rows, num_tokens): of tokens (rows, num_tokens) (int64 with tokens_i64, else int32), 0 for a token outside the
  * vocabulary.  entropy (rows), NULL: not wanted.  top_log_probs / top_ids (rows, top_k), top_k up to 32: by value, equal values
- * by lowest id, NaN above everything.  A row of nothing but -inf has log-probs of -inf and entropy 0. */
+ * by lowest id, NaN above everything.  A row of nothing but -inf has log-probs of -inf and entropy 0; finite logits may have any
+ * size.  fp32 sums. */
 OASR_API int oasr_b200_token_log_probs(float* log_probs, float* entropy, float* top_log_probs, int32_t* top_ids,
                                        const void* logits, const void* tokens, int tokens_i64, int64_t rows, int64_t vocab,
                                        int64_t stride, int64_t num_tokens, int64_t top_k, int dtype, void* stream);

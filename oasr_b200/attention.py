@@ -295,7 +295,11 @@ def fmha_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_co
     it stands at position ``cache_seqlens[b] - q_lens[b] + t`` and sees none behind that (``q_lens`` None: T_q), so the same
     call serves a prompt, a chunk and a single token whose keys have been written.  (``fmha``'s ``causal`` counts rows from key
     0.)  Rows ``t >= q_lens[b]`` are padding; those and rows that see nothing are zeros, and so is a sequence of length 0.  Keys
-    whose page lies outside the pool are not seen.  ``token_major=True`` returns ``(B, T_q, H, D)``."""
+    whose page lies outside the pool are not seen.  ``token_major=True`` returns ``(B, T_q, H, D)``.
+
+    Scores, their maximum and sum and the output are fp32; the weights are rounded to ``q``'s type before they meet the values
+    (``fmha`` does the same), and the result once more.  How the work is split goes by the width of ``block_table``, as lengths are
+    on the GPU: over a table many times wider than the longest sequence pass ``block_table[:, :blocks]`` of what is in use."""
     if q.dim() != 4:
         raise ValueError(f"q must be (B, H, T_q, D); got {tuple(q.shape)}")
     B, H, T, D = q.shape

@@ -17,18 +17,22 @@
 //   V   the lane holds words g D / 64 (+ 1) of keys 8 x + 2 t and 8 x + 2 t + 1.  Here the operand is (n - 8) * scale, exact in the
 //       type (q4.cuh).  In bf16 the second nibble has no room behind an exponent: left alone it is the number n 2^-129 (gradual
 //       underflow joins the normal numbers at n = 8), which one FMA takes to (n - 8) / 4.
-//   P   the scores' fragment is the transpose of what the second product reads: movmatrix.
+//   P   the scores' fragment is the transpose of what the second product reads: movmatrix.  Weights are rounded to the type (their
+//       sum, the maximum and the output are fp32), as in the package's attention over 16-bit pages: each is off by half a step at
+//       most, which with the result's own rounding makes an error of 1.2 to 1.35 times that of rounding the result alone.  Exact
+//       weights would be a second operand and as many products again.
 // The ALU (logic, shifts, permutes: half a warp instruction a clock) is the busiest unit; the FMA pipe, which does the rest of the
 // conversion, is not.
-// The running maximum moves only when a score passes it by 2^8 (weights stay below that, finite in either type): most tiles
-// need one vote in the place of a reduction over the lanes.
+// The running maximum moves only when a score passes it by 2^8: numerator and denominator hold the same factor whatever is
+// subtracted, so that only their range counts (weights stay below 2^8, finite in either type).  Most tiles need one vote in the place
+// of a reduction over the lanes.
 // Every warp walks its own tiles with its own maximum, sum and output, and has its own ring of tiles in shared memory, filled by
 // asynchronous copies (a tile is two runs of 16 keys of a page): no registers wait for memory, no warp for another.  One to eight
 // warps of a block, or the blocks of a cluster, share a (sequence, key head, rows) and meet in shared memory at the end.
 //
-// B200: 64 sequences of 6000 keys, 32 heads of 128 over 8 key heads, one token each: 117-121 us (442 MB, 3.7 TB/s), bound by
-// instructions (some 700 of a warp for 32 keys; ALU 0.55 busy, issue slots 0.64).  256 chunks of 16 rows over up to 1001 keys, 8 heads of
-// 64: 51 us, a third of it a block's start (lengths, pages, first tile) and end.
+// B200: 64 sequences of 6000 keys, 32 heads of 128 over 8 key heads, one token each: 112-120 us (442 MB, 3.8 TB/s), bound by
+// instructions (some 730 of a warp for 32 keys; ALU 0.55 busy, FMA 0.48, issue slots 0.68).  256 chunks of 16 rows over up to 1001 keys,
+// 8 heads of 64: 49 us, a third of it a block's start (lengths, pages, first tile) and end.
 #include <cmath>
 
 #include "common.cuh"
@@ -535,7 +539,10 @@ template <typename T, int D, int NT>
 int launch(const Args& a, cudaStream_t s) {
   const int64_t rows = static_cast<int64_t>(a.H / a.Hkv) * a.Tq, row_blocks = (rows + 8 * NT - 1) / (8 * NT);
   const int64_t groups = static_cast<int64_t>(a.B) * a.Hkv * row_blocks, tiles = (a.blocks_per_seq * a.block_size + 31) / 32;
-  // Warps that share a group: until the SMs are full (down to two tiles each), and so many that none walks more than 32 tiles.  Fewer
+  // Warps that share a group: until the SMs are full (down to two tiles each), and so many that none walks more than 32 tiles.  `tiles`
+  // are the block table's, the only bound of the lengths that the host has: in a table wider than its sequences most warps find
+  // nothing, and their blocks' start and end are what a call then takes (the two cases below in tables four times as wide: 179 ->
+  // 228 us and 49 -> 49 us, 32 times: 228 and 238 us).  Fewer
   // leave the longest sequences of a ragged batch running alone, more pay a block's start and end (some 6 us of latency) more often:
   // 128 sequences of 500 to 8191 keys, 8 key heads of 128, take 186 / 176 / 189 us with 4 / 8 / 16 warps, 256 chunks of 16 rows over up
   // to 1001 keys, 8 heads of 64, take 60 / 50 / 52 us with 1 / 2 / 4.  Beyond eight, blocks of eight in a cluster.
@@ -556,7 +563,7 @@ int run(const Args& a, cudaStream_t s) {
 
 // Which form: measured times, as far as sizes tell.  The few-row form takes 3.66 ps (head_dim 128; 64: 1.46 ps) a row and key when it
 // fills the GPU, up to twice that when it does not; the prompt form 2.5 us for 128 keys of a block of 256 rows, however many of them
-// are there.  In us, few-row against prompt form, bf16: 64 rows over 1000 keys, 128 groups of 128: 56 / 28, 8 groups: 14 / 26; 1024 groups of
+// are there.  `keys` is the block table's width, as above.  In us, few-row against prompt form, bf16: 64 rows over 1000 keys, 128 groups of 128: 56 / 28, 8 groups: 14 / 26; 1024 groups of
 // 64: 109 / 150; 512 rows over 1000 keys, 8 groups of 128: 45 / 37, 1024 groups: 1686 / 558; 64 rows over 8000 keys, 8 groups: 34 / 151.
 bool prompt_is_faster(int64_t rows, int64_t heads, int64_t keys, int64_t D) {
   if (g_path != 0) return g_path == 2;

@@ -45,6 +45,9 @@ __device__ __forceinline__ uint32_t behind(uint32_t w, uint32_t mask, uint32_t m
   return r;
 }
 
+// A code behind a magic exponent (a 4-bit number under the bits of 1024 is 1024 + n, and one subtraction takes 1024 off) is the
+// conversion of Kim, Henry, Fahim and Awadalla, "Who Says Elephants Can't Run: Bringing Large Scale MoE Models into Cloud Scale
+// Production" (2022); the constants follow from the formats.
 // The codes n - 8 of two keys (one in each half) at bits 0..3 / 4..7, in fp16 and exact: behind an exponent where a step is 1 / 16.
 __device__ __forceinline__ uint32_t low_codes(uint32_t w) { return half2_bits(__hsub2(as_half2(behind(w, kLow, kMagic16)), as_half2(0x64086408u))); }   // (1024 + n) - 1032
 __device__ __forceinline__ uint32_t second_codes(uint32_t w) {                                                                                           // (1024 + 16 n) / 16 - 72

@@ -7,9 +7,10 @@
 // The tiles run half a step apart: while one's softmax works, the tensor cores have the other's products.  Both share the
 // converted keys and values, so a code is converted once for 256 rows.  Output stays in tensor memory; a row's maximum moves only
 // when a score passes it by 2^8, and only then is the output scaled again.
-// Weights take the place of the scores they were made of (16 bits for 32) and are the A operand of the second product from
-// there: a product with both operands in shared memory reads 128 bytes a clock, all there is, and the weights' way through it
-// was a third of that traffic.  So S of step j + 1 waits for O of step j to be complete; the other tile's products fill the gap.
+// Weights take the place of the scores they were made of (16 bits for 32: the rounding that fmha_q4.cu explains) and are the A
+// operand of the second product from there: a product with both operands in shared memory reads 128 bytes a clock, all there is,
+// and the weights' way through it was a third of that traffic.  So S of step j + 1 waits for O of step j to be complete; the other
+// tile's products fill the gap.
 //
 // Converted rows hold the exact values (q4.cuh).  Within an octet the dims lie in the order 0 4 1 5 2 6 3 7, the pairs that one mask
 // of a code word gives; queries are stored in the same order, and the output's columns are put right when they are read.
