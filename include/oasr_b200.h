@@ -778,6 +778,58 @@ OASR_API int oasr_b200_token_log_probs(float* log_probs, float* entropy, float* 
                                        const void* logits, const void* tokens, int tokens_i64, int64_t rows, int64_t vocab,
                                        int64_t stride, int64_t num_tokens, int64_t top_k, int dtype, void* stream);
 
+/* ---- drafted tokens over paged caches (no reference counterparts) ----------------------------
+ * A tree of T nodes a sequence: node 0 is the last token that stands, node i > 0 a drafted one that continues node
+ * parents[i] < i.  A node that is not connected with node 0 in this way is padding. */
+
+/* mask (B, T, words), words = ceil(T / 32): bit j of row i is set where node j is i or lies on the way from node 0 to it;
+ * depth (B, T): steps from node 0.  Padding has no bits and depth -1.  T up to 1024. */
+OASR_API int oasr_b200_draft_tree(uint32_t* mask, int32_t* depth, const int32_t* parents, int64_t B, int64_t T, int64_t words,
+                                  void* stream);
+/* Attention of q (B, H, Tq, D) over 16-bit pages (num_blocks, block_size, Hkv, D) whose last q_lens[b] positions are the rows' own
+ * (q_lens NULL: Tq): row t sees the keys seqstarts[b] <= j < P = seqlens[b] - q_lens[b] (seqstarts NULL: 0) and the key P + u where
+ * bit u of its mask is set (mask NULL: u <= t), if its page lies in the pool.  Rows t >= q_lens[b] and rows that see nothing are
+ * zeros; a length below zero is zero.  mask: sequence b's rows of mask_words words each, mask_stride words further for the next
+ * sequence (0: one mask for all).  Strides are host int64[3] (batch, head, row) in elements, multiples of 8.  D 64 or 128, H a multiple
+ * of Hkv, block_size of 16, blocks_per_seq * block_size up to 2^31 - 2^16, a finite scale.  fp32 scores, sums and output; the weights are
+ * rounded to the element type before the second product.  The workspace (16-byte aligned; its size from the function below, which may be 0) is
+ * this call's alone until it has run.  The work is split by blocks_per_seq: a table much wider than the sequences costs time. */
+OASR_API int64_t oasr_b200_fmha_tree_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t D,
+                                                     int64_t blocks_per_seq, int64_t block_size);
+OASR_API int oasr_b200_fmha_tree(void* out, const int64_t* out_strides, const void* q, const int64_t* q_strides,
+                                 const void* k_pool, const void* v_pool, const int32_t* block_table, const int32_t* seqlens,
+                                 const int32_t* seqstarts, const int32_t* q_lens, const uint32_t* mask, int64_t mask_stride,
+                                 int64_t mask_words, void* workspace, int64_t workspace_bytes, int64_t blocks_per_seq,
+                                 int64_t block_size, int64_t num_blocks, int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t D,
+                                 double scale, int dtype, void* stream);
+/* Which drafts stand.  From node 0 on: p = softmax(logits[n] / temperature) (temperature <= 0: 1 at the first maximum); the children c
+ * of n in order, x = drafts[c]: accepted iff uniforms[c] q(x) < p(x), which makes c the next n; else p <- max(p - q, 0), normalised.  q is
+ * draft_probs[n] (fp32), or with draft_probs NULL 1 at x.  With no child accepted the next token is the first whose cumulative p passes
+ * uniforms[0].  Outputs (B, T): path the nodes from node 0 on, tokens the token behind each of them (the last one is the new one), both -1
+ * behind counts (B) entries.  A child whose draft lies outside [0, V) is not accepted.  A row with a NaN, or whose maximum is not finite, has
+ * no distribution: the walk ends there with token -1, as it does where nothing of p is left.  Decisions are taken in 64 bits; weights
+ * below 2^-300 of the row's largest may count as zero.
+ * logits (B, T, V) fp32 / fp16 / bf16 and draft_probs with strides in elements, unit stride along V; parents_stride 0: one tree for all;
+ * temperatures (B) fp32, or NULL and one for all.  T up to 1024. */
+OASR_API int oasr_b200_verify_drafts(int32_t* tokens, int32_t* path, int32_t* counts, const void* logits,
+                                     int64_t logits_stride_b, int64_t logits_stride_n, const int32_t* drafts,
+                                     const int32_t* parents, int64_t parents_stride, const float* uniforms,
+                                     const float* draft_probs, int64_t probs_stride_b, int64_t probs_stride_n,
+                                     const float* temperatures, double temperature, int64_t B, int64_t T, int64_t V, int dtype,
+                                     void* stream);
+/* Pages of `layers` layers that follow one another: (layers, num_blocks, outer, block_size) rows of row_bytes (outer 1 for 16-bit pages,
+ * whose rows hold all heads; the heads for 4-bit codes and scales). */
+typedef struct oasr_b200_draft_pool {
+  void* data;
+  int64_t layers, outer, row_bytes;
+} oasr_b200_draft_pool;
+/* In every pool (a host array), the row of position offset[b] + path[b, i] moves to offset[b] + i for i < counts[b].  A path (B, T) ascends from
+ * 0 on or more; it ends at the first entry that does not.  A position without a page moves nothing.  The sequences
+ * of a call share no page that is written.  Any number of pools; one launch for each 64. */
+OASR_API int oasr_b200_commit_drafts(const oasr_b200_draft_pool* pools, int64_t num_pools, const int32_t* block_table,
+                                     const int32_t* offset, const int32_t* path, const int32_t* counts, int64_t B, int64_t T,
+                                     int64_t blocks_per_seq, int64_t block_size, int64_t num_blocks, void* stream);
+
 /* ---- packed-layout glue ------------------------------------------------ */
 /* out[i, :] = in[index[i], :] for i < n_out (rows of `row_bytes` bytes,
  * multiple of 16; index int64; `in` has `in_rows` rows and an index outside

@@ -9,16 +9,19 @@ reference package so its layers, models and engine run on these kernels.
 from __future__ import annotations
 
 from . import _lib
-from .attention import fmha, fmha_q4, fmha_varlen, gather_paged_kv, gather_paged_kv_q4  # noqa: F401
+from .attention import fmha, fmha_q4, fmha_tree, fmha_varlen, gather_paged_kv, gather_paged_kv_q4  # noqa: F401
 from .cache import (  # noqa: F401
     PagedKVCache,
     PagedKVCacheQ4,
+    commit_drafts,
+    commit_drafts_q4,
     gather_rows,
     scatter_rows,
     write_kv_chunk,
     write_kv_rope,
     write_kv_rope_q4,
 )
+from .drafts import DraftTree, VerifiedDrafts, draft_tree, verify_drafts  # noqa: F401
 from .functional import (  # noqa: F401
     add_layer_norm,
     add_layer_norm_residual,

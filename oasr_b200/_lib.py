@@ -105,6 +105,9 @@ _SIGNATURES = {
     "oasr_b200_paged_kv_gather_q4": [P] * 8 + [I] * 7 + [c_int, P],
     "oasr_b200_fmha_q4": [P] * 12 + [I] * 8 + [c_double, c_int, c_int, P],
     "oasr_b200_token_log_probs": [P] * 6 + [c_int] + [I] * 5 + [c_int, P],
+    "oasr_b200_draft_tree": [P, P, P, I, I, I, P],
+    "oasr_b200_fmha_tree": [P] * 11 + [I, I, P] + [I] * 9 + [c_double, c_int, P],
+    "oasr_b200_verify_drafts": [P] * 4 + [I, I, P, P, I, P, P, I, I, P, c_double, I, I, I, c_int, P],
     "oasr_b200_gather_rows": [P, P, P, I, I, I, P],
     "oasr_b200_scatter_rows": [P, P, P, I, I, I, P],
 }
@@ -152,6 +155,13 @@ class FastConformerModel(ctypes.Structure):
         ("rel_window", c_void_p)]
 
 
+class DraftPool(ctypes.Structure):
+    """struct oasr_b200_draft_pool (include/oasr_b200.h)."""
+
+    _fields_ = [("data", c_void_p), ("layers", c_int64), ("outer", c_int64), ("row_bytes", c_int64)]
+
+
+_SIGNATURES["oasr_b200_commit_drafts"] = [POINTER(DraftPool), I, P, P, P, P, I, I, I, I, I, P]
 _SIGNATURES["oasr_b200_fastconformer_layers_packed"] = [POINTER(FastConformerModel), P, c_int, P, P, I, P, P, I, I, I, I, P, I, P]
 _SIGNATURES["oasr_b200_fastconformer_chunk_paged"] = [POINTER(FastConformerModel), P, c_int, P, I, I, POINTER(c_void_p), POINTER(c_void_p),
                                                      P, P, P, I, I, I, P, I, P, P, I, P]
@@ -199,6 +209,8 @@ def load() -> ctypes.CDLL:
     lib.oasr_b200_conformer_workspace_bytes.argtypes = [POINTER(ConformerModel), I, I]
     lib.oasr_b200_fmha_relpos_plan_bytes.restype = c_int64
     lib.oasr_b200_fmha_relpos_plan_bytes.argtypes = [I, I, I]
+    lib.oasr_b200_fmha_tree_workspace_bytes.restype = c_int64
+    lib.oasr_b200_fmha_tree_workspace_bytes.argtypes = [I] * 7
     lib.oasr_b200_fastconformer_workspace_bytes.restype = c_int64
     lib.oasr_b200_fastconformer_workspace_bytes.argtypes = [POINTER(FastConformerModel), I, I, I]
     lib.oasr_b200_fastconformer_chunk_workspace_bytes.restype = c_int64
@@ -217,7 +229,7 @@ def exported_names() -> list[str]:
     return list(_STRING_FUNCS) + ["oasr_b200_launch_count", "oasr_b200_conformer_workspace_bytes", "oasr_b200_profile_count",
                                   "oasr_b200_conformer_noalloc_capacity_bytes", "oasr_b200_conformer_chunk_workspace_bytes",
                                   "oasr_b200_fastconformer_workspace_bytes", "oasr_b200_fastconformer_chunk_workspace_bytes",
-                                  "oasr_b200_fmha_relpos_plan_bytes"] + list(_SIGNATURES)
+                                  "oasr_b200_fmha_relpos_plan_bytes", "oasr_b200_fmha_tree_workspace_bytes"] + list(_SIGNATURES)
 
 
 def launch_count() -> int:

@@ -335,3 +335,77 @@ def fmha_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_co
               v_codes.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(), lens.data_ptr(), _p(starts), _p(q_lens), block_table.shape[1],
               block_size, num_blocks, B, H, Hkv, T, D, softmax_scale, bool(causal), _DTYPE_ID[q.dtype], _stream(q))
     return out
+
+
+def _tree_mask(mask: torch.Tensor, B: int, T: int):
+    """``(mask, stride from sequence to sequence in words, words of a row)``."""
+    words = (T + 31) // 32
+    if mask.dtype != torch.int32 or mask.dim() not in (2, 3) or tuple(mask.shape) != ((B, T, words) if mask.dim() == 3 else (T, words)):
+        raise ValueError(f"tree_mask must be int32 ({B}, {T}, {words}) or ({T}, {words}) (draft_tree), got {tuple(mask.shape)} {mask.dtype}")
+    if not mask.is_contiguous():
+        mask = mask.contiguous()
+    return mask, T * words if mask.dim() == 3 else 0, words
+
+
+def fmha_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *, softmax_scale: float, block_table: torch.Tensor,
+              cache_seqlens: torch.Tensor, tree_mask: Optional[torch.Tensor] = None, cache_seqstarts: Optional[torch.Tensor] = None,
+              q_lens: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, token_major: bool = False) -> torch.Tensor:
+    """Attention of a tree of drafted tokens ``q (B, H, T, D)`` over 16-bit pages ``(num_blocks, block_size, H_kv, D)``
+    (``PagedKVCache``), D 64 or 128, pages of a multiple of 16 rows.
+
+    The rows' own keys have been written: they are the last ``q_lens[b]`` positions of the ``cache_seqlens[b]`` (``q_lens`` None: T).
+    Row ``t`` sees all keys before those, from ``cache_seqstarts[b]`` on (None: 0), and of its tree the nodes ``u`` whose bit is set in row
+    ``t`` of ``tree_mask``: int32 words ``(B, T, ceil(T / 32))`` or, for one tree of all sequences, ``(T, ceil(T / 32))``, as ``draft_tree``
+    makes them.  Without a mask row ``t`` sees the nodes ``0 .. t``: a chunk, or a single token.  Rows ``t >= q_lens[b]`` are padding; those
+    and rows that see nothing are zeros.  Keys whose page lies outside the pool are not seen.  ``token_major=True`` returns ``(B, T, H, D)``.
+
+    Scores, their maximum and sum and the output are fp32; the weights are rounded to ``q``'s type before they meet the values (``fmha``
+    does the same), and the result once more.  How the work is split goes by the width of ``block_table``, as lengths are on the GPU: over a
+    table many times wider than the longest sequence pass ``block_table[:, :blocks]`` of what is in use."""
+    if q.dim() != 4:
+        raise ValueError(f"q must be (B, H, T_q, D); got {tuple(q.shape)}")
+    B, H, T, D = q.shape
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+        raise ValueError("pools must be (num_blocks, block_size, H_kv, D) and match")
+    num_blocks, block_size, Hkv, pool_dim = k_cache.shape
+    if q.dtype not in _HALF or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise ValueError(f"fmha_tree supports fp16/bf16 with one dtype for q and pools, got {q.dtype}, {k_cache.dtype}, {v_cache.dtype}")
+    if pool_dim != D:
+        raise ValueError("q and k head_dim must match")
+    if Hkv == 0 or H % Hkv:
+        raise ValueError(f"H ({H}) must be divisible by H_kv ({Hkv})")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("pools must be contiguous")
+    block_table = _table32(block_table, B)
+    lens, starts = _index32("cache_seqlens", cache_seqlens, B), _index32("cache_seqstarts", cache_seqstarts, B)
+    q_lens = _index32("q_lens", q_lens, B)
+    mask_stride = words = 0
+    if tree_mask is not None:
+        tree_mask, mask_stride, words = _tree_mask(tree_mask, B, T)
+    _one_device(q, k_cache, v_cache, block_table, lens, starts, q_lens, tree_mask, out)
+    qs = q.stride()
+    sb, sh, st = _used_strides(B, H, T, *qs[:3])
+    if qs[3] != 1 or sb % 8 or sh % 8 or st % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+        sb, sh, st = H * T * D, T * D, D
+    if out is None:
+        if token_major:
+            out = torch.empty(B, T, H, D, dtype=q.dtype, device=q.device)
+            os = _stride_array(T * H * D, D, H * D)
+        else:
+            out = torch.empty(B, H, T, D, dtype=q.dtype, device=q.device)
+            os = _stride_array(H * T * D, T * D, D)
+    else:
+        want = (B, T, H, D) if token_major else (B, H, T, D)
+        if tuple(out.shape) != want or out.dtype != q.dtype or out.stride(3) != 1:
+            raise ValueError(f"out must be {want} in q's dtype, with unit stride along D")
+        _check_distinct_rows(out=out)
+        ob, oh, ot = (out.stride(0), out.stride(2), out.stride(1)) if token_major else out.stride()[:3]
+        os = _stride_array(*_used_strides(B, H, T, ob, oh, ot))
+    per = block_table.shape[1]
+    need = _lib.load().oasr_b200_fmha_tree_workspace_bytes(B, H, Hkv, T, D, per, block_size)
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _lib.call("oasr_b200_fmha_tree", out.data_ptr(), os, q.data_ptr(), _stride_array(sb, sh, st), k_cache.data_ptr(), v_cache.data_ptr(),
+              block_table.data_ptr(), lens.data_ptr(), _p(starts), _p(q_lens), _p(tree_mask), mask_stride, words, _p(work), need, per, block_size,
+              num_blocks, B, H, Hkv, T, D, softmax_scale, _DTYPE_ID[q.dtype], _stream(q))
+    return out

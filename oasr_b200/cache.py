@@ -4,12 +4,12 @@ oasr/cache/block_pool.py:33-41): per-layer pools ``(num_blocks, block_size, H_kv
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional, Union
+from typing import Optional, Sequence, Union
 
 import torch
 
 from . import _lib
-from .attention import _HALF, _check_q4_pools, _stride_array, _index32, _table32, _used_strides, fmha_q4, gather_paged_kv, gather_paged_kv_q4  # noqa: F401  (re-exported)
+from .attention import _HALF, _check_q4_pools, _stride_array, _index32, _narrow, _table32, _used_strides, fmha_q4, fmha_tree, gather_paged_kv, gather_paged_kv_q4  # noqa: F401  (re-exported)
 from .functional import _DTYPE_ID, _check_distinct_rows, _check_head_weight, _check_rope_table, _need_cuda, _one_device, _p, _stream
 
 
@@ -62,6 +62,12 @@ class PagedKVCache:
 
     def write_kv_chunk(self, new_k: torch.Tensor, new_v: torch.Tensor, *, offset: Union[int, torch.Tensor]) -> None:
         write_kv_chunk(self.k_cache, self.v_cache, self.block_table, new_k, new_v, offset)
+
+    def fmha_tree(self, q: torch.Tensor, *, softmax_scale: float, **how) -> torch.Tensor:
+        return fmha_tree(q, self.k_cache, self.v_cache, softmax_scale=softmax_scale, block_table=self.block_table, cache_seqlens=self.cache_seqlens, **how)
+
+    def commit_drafts(self, offset: Union[int, torch.Tensor], path: torch.Tensor, counts: torch.Tensor) -> None:
+        commit_drafts((self.k_cache, self.v_cache), self.block_table, offset, path, counts)
 
     def gather_full_kv(self, max_total_kv: int):
         B = self.block_table.size(0)
@@ -209,8 +215,61 @@ class PagedKVCacheQ4:
     def fmha(self, q: torch.Tensor, *, softmax_scale: float, **how) -> torch.Tensor:
         return fmha_q4(q, *self.pools, softmax_scale=softmax_scale, block_table=self.block_table, cache_seqlens=self.cache_seqlens, **how)
 
+    def commit_drafts(self, offset: Union[int, torch.Tensor], path: torch.Tensor, counts: torch.Tensor) -> None:
+        commit_drafts_q4(self.pools, self.block_table, offset, path, counts)
+
     def gather_full_kv(self, max_total_kv: int):
         return gather_paged_kv_q4(*self.pools, self.block_table, None, max_total_kv)
+
+
+def _commit(pools, geometry, block_table, offset, path, counts):
+    """``geometry(shape)``: (num_blocks, block_size, outer) of one layer's pages, and which of its dimensions a row has."""
+    if path.dim() != 2:
+        raise ValueError(f"path must be (B, T), got {tuple(path.shape)}")
+    B, T = path.shape
+    table = (_lib.DraftPool * len(pools))()
+    shape = None
+    for entry, pool in zip(table, pools):
+        if pool.dim() not in (4, 5) or not pool.is_contiguous():
+            raise ValueError(f"pools must be contiguous pages of one layer or of (layers, ...), got {tuple(pool.shape)}")
+        layers = pool.shape[0] if pool.dim() == 5 else 1
+        num_blocks, block_size, outer, row = geometry(pool.shape[-4:])
+        if shape is None:
+            shape = num_blocks, block_size
+        elif shape != (num_blocks, block_size):
+            raise ValueError(f"pools must have the same pages: {shape} and {(num_blocks, block_size)}")
+        entry.data, entry.layers, entry.outer, entry.row_bytes = pool.data_ptr(), layers, outer, row * pool.element_size()
+    if shape is None:
+        raise ValueError("no pools")
+    block_table = _table32(block_table, B)
+    if isinstance(offset, int):
+        offset = torch.full((B,), offset, dtype=torch.int32, device=path.device)
+    offset, counts = _index32("offset", offset, B), _index32("counts", counts, B)
+    path = _narrow(path) if path.dtype != torch.int32 else path
+    if not path.is_contiguous():
+        path = path.contiguous()
+    _one_device(path, *pools, block_table, offset, counts)
+    _lib.call("oasr_b200_commit_drafts", table, len(pools), block_table.data_ptr(), offset.data_ptr(), path.data_ptr(), counts.data_ptr(), B, T,
+              block_table.shape[1], shape[1], shape[0], _stream(path))
+
+
+def commit_drafts(pools: Sequence[torch.Tensor], block_table: torch.Tensor, offset: Union[int, torch.Tensor], path: torch.Tensor,
+                  counts: torch.Tensor) -> None:
+    """Moves the accepted drafts' rows together in the pages, in place: the row of position ``offset[b] + path[b, i]`` goes to ``offset[b] +
+    i`` for ``i < counts[b]`` (``verify_drafts`` gives ``path (B, T)`` and ``counts (B,)``; ``offset`` is where the tree's node 0 lies).
+
+    ``pools`` are the keys and values, of any element type, of one layer ``(num_blocks, block_size, H_kv, D)`` or of several
+    ``(layers, num_blocks, block_size, H_kv, D)``; all of them are done in one launch (for each 64).  A path ascends; it ends at the first
+    entry that does not.  Positions without a page move nothing.  Rows behind the path stay as they are.  The
+    sequences of a call must not share pages that are written."""
+    _commit(pools, lambda s: (s[0], s[1], 1, s[2] * s[3]), block_table, offset, path, counts)
+
+
+def commit_drafts_q4(pools: Sequence[torch.Tensor], block_table: torch.Tensor, offset: Union[int, torch.Tensor], path: torch.Tensor,
+                     counts: torch.Tensor) -> None:
+    """``commit_drafts`` in 4-bit pages: codes and scales of ``PagedKVCacheQ4``, ``(num_blocks, H_kv, block_size, ...)`` or with the layers
+    before them."""
+    _commit(pools, lambda s: (s[0], s[2], s[1], s[3]), block_table, offset, path, counts)
 
 
 def gather_rows(src: torch.Tensor, index: torch.Tensor, out: torch.Tensor = None) -> torch.Tensor:

@@ -1,0 +1,57 @@
+// What the kernels of attention over 16-bit pages with a tree of drafted tokens share.
+#pragma once
+#include "common.cuh"
+
+namespace ob {
+namespace fmha_tree {
+
+struct Args {
+  void* out;
+  const void *q, *k, *v;
+  const int32_t *block_table, *seqlens, *seqstarts, *q_lens;
+  const uint32_t* mask;          // null: row t sees the drafted keys 0 .. t
+  float* parts;                  // null, or the partial results of `splits` blocks a group
+  int64_t qs_b, qs_h, qs_t, os_b, os_h, os_t;
+  int64_t mask_b;                // words from one sequence's mask to the next one's; 0: one for all
+  int64_t blocks_per_seq, block_size, num_blocks;
+  int B, H, Hkv, Tq, mask_words, splits;
+  float scale_log2;
+};
+
+constexpr float kEmpty = -3e38f;   // a maximum below every score: differences to it overflow to -inf or are zero, never NaN
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A sequence as every block of it sees it.
+struct Sequence {
+  int start, end, prefix, live;   // keys [start, end); the first drafted key (may be below zero); rows that count
+
+  __device__ __forceinline__ Sequence(const Args& a, int b) {
+    const int len = max(a.seqlens[b], 0), capacity = static_cast<int>(a.blocks_per_seq * a.block_size);
+    live = a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq;
+    start = a.seqstarts ? max(a.seqstarts[b], 0) : 0;
+    end = min(len, capacity);
+    prefix = len - live;
+  }
+};
+
+// Whether row t sees drafted key u (u >= 0)
+__device__ __forceinline__ bool sees(const Args& a, const uint32_t* words, int t, int u, int live) {
+  if (u >= live) return false;
+  if (words == nullptr) return u <= t;
+  return u < a.mask_words * 32 && (words[u >> 5] >> (u & 31) & 1u);
+}
+__device__ __forceinline__ const uint32_t* mask_row(const Args& a, int b, int t) {
+  return a.mask ? a.mask + b * a.mask_b + static_cast<int64_t>(t) * a.mask_words : nullptr;
+}
+
+// Partial results of one (split, group, row block of `rows` rows): rows x (maximum, sum), then rows x D of output.
+template <int D>
+__host__ __device__ constexpr int64_t part_floats(int rows) { return static_cast<int64_t>(rows) * (D + 2); }
+
+}  // namespace fmha_tree
+}  // namespace ob
