@@ -8,7 +8,7 @@
 // q is the distribution that the children of n were drawn from (draft_probs[n]), or 1 at x where drafts are taken as chosen.  A
 // temperature of zero puts all of p on the first maximum.  Whoever drafted, the tokens are distributed as the target alone would give them.
 //
-// The answer is whole numbers, so what decides is computed in 64 bits: weights e^(l / temperature) to some 1e-13, their sums in a fixed order.
+// The answer is whole numbers, so what decides is computed in 64 bits: weights e^(l / temperature) to some 2^-31, their sums in a fixed order.
 // They come out of a table of 2^(i / 256) and a polynomial of degree 3 for the rest (the method of Tang, "Table-driven implementation of the exponential
 // function in IEEE floating-point arithmetic", 1989).  Weights are taken relative to logits of 0: 64 bits reach 2^250 above and 2^500 below; rows
 // that lie elsewhere are taken again relative to their maximum.
@@ -30,7 +30,7 @@ namespace ob {
 namespace verify {
 namespace {
 
-constexpr int kWarps = 16, kMaxCluster = 8, kTable = 256, kMaxNodes = 1024;
+constexpr int kWarps = 16, kMaxCluster = 8, kSlots = kWarps * kMaxCluster, kTable = 256, kCopies = 16, kMaxNodes = 1024, kVec = 8;
 
 struct Args {
   int32_t *tokens, *path, *counts;
@@ -41,74 +41,187 @@ struct Args {
   int64_t ls_b, ls_n, ps_b, ps_n, parents_b;   // strides: logits, draft probabilities, parents of a sequence (0: one tree for all)
   int B, T, V;
   float temperature;
+  uint32_t two12, two21;   // 2^12 and 2^21 as numbers that the compiler does not know: products with them are no shifts (see near_zero)
 };
 
-struct Kid {
-  int node, token;
-  float logit, u, q;
+// 2^((i - 1/2) / 256) less i 2^12 in its upper word, so that k 2^12 added there gives table[k mod 256] 2^(k div 256)
+struct Table {
+  uint64_t e[kTable];
+  constexpr Table() : e() {
+    for (int i = 0; i < kTable; ++i) {
+      const double x = (i - 0.5) * (0.69314718055994530942 / kTable);
+      double sum = 1., term = 1.;
+      for (int n = 1; n < 24; ++n) term = term * x / n, sum += term;
+      // the bits of a number of [1/2, 2)
+      const bool low = sum < 1.;
+      e[i] = (static_cast<uint64_t>(low ? 1022 : 1023) << 52) + static_cast<uint64_t>((low ? 2. * sum : sum) * 4503599627370496. - 4503599627370496.) - (static_cast<uint64_t>(i) << 44);
+    }
+  }
 };
+__device__ constexpr Table g_table{};
 
-// What the blocks of a cluster tell one another about a row, a number and a whole number of each warp, and the children of the node.
-// Two of each in turn: a barrier lies between a use and the next writing of the same one.
+// The table lies there 16 times: half a warp reads 16 entries of 8 bytes at a time, each lane from banks of its own.  What the warps of a cluster
+// tell one another about a row (a number and a whole number each) is held twice, in turn: a barrier lies between a use and the next
+// writing of the same one.  Behind it: parents, drafts, uniforms, first child and next sibling of T nodes.
 struct Shared {
-  double table[kTable];
-  double sum[2][kMaxCluster * kWarps];
-  int id[2][kMaxCluster * kWarps];
-  int kid_count[2];
+  double table[kTable][kCopies];
+  double sum[2][kSlots];
+  int id[2][kSlots];
 };
 
+// e^((l - ref) / temperature).  A row that lies around zero has ref 0; then the multiple of 2^(1 / 256) and the rest f come from fp32 operations
+// (a product is exact inside its sum, and the rest is small), and 2^(f / 256) is the 64-bit number 1 + G 2^-31 with G out of the low bits of an fp32
+// sum: one 64-bit multiply-add a weight.  Both 64-bit numbers are put together by integer multiply-adds: logic and shifts, half as fast, were 0.94
+// busy (65537 logits by four blocks: 6.3k clocks).  Any other row takes it in 64 bits throughout.
 struct Weigher {
-  const double* table;
-  double rate, ref;   // 256 log2(e) / temperature; weights are relative to e^(ref / temperature)
-  float lo, hi;       // logits below are weights of zero, logits above are out of range
+  const double* table;   // the lane's copy
+  double rate, ref;      // 256 log2(e) / temperature
+  float rate_hi, rate_lo, lo, hi;   // logits below lo have no weight, logits above hi are out of range
+  uint32_t two12, two21;
+  bool centered;
 
-  __device__ __forceinline__ void relative_to(float r) {
+  __device__ __forceinline__ void relative_to(float r, bool centered_) {
     ref = r;
+    centered = centered_;
+    rate_hi = static_cast<float>(rate), rate_lo = static_cast<float>(rate - static_cast<double>(rate_hi));
     lo = static_cast<float>(fmax(ref - 500. * kTable / rate, static_cast<double>(-FLT_MAX)));   // rounded away from ref by at most as much again
     hi = static_cast<float>(fmin(ref + 250. * kTable / rate, static_cast<double>(FLT_MAX)));
   }
-  // e^((l - ref) / temperature)
-  __device__ __forceinline__ double operator()(float l) const {
-    constexpr double kMagic = 6755399441055744.;   // 1.5 * 2^52: the sum's low word is the rounded number
-    constexpr double c1 = 0.6931471805599453 / kTable, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;
-    if (!(l >= lo)) return 0.;
-    const double d = static_cast<double>(fminf(l, hi)) - ref;
-    const double t = fma(d, rate, kMagic);
-    const int k = __double2loint(t);
-    const double f = fma(d, rate, -(t - kMagic));   // in [-1/2, 1/2]
-    const double v = table[k & (kTable - 1)], g = fma(fma(f, c3, c2), f, c1);
-    const double w = fma(v * f, g, v);
-    return __hiloint2double(__double2hiint(w) + ((k >> 8) << 20), __double2loint(w));
+  // the weight of lo <= l <= hi, ref 0, in two factors: table[k mod 256] 2^(k div 256), entries for half a step less, and 2^((f + 1/2) / 256)
+  __device__ __forceinline__ void near_zero(float l, double& v, double& d) const {
+    constexpr float kMagic = 12582912.f, kUnit = 1.f / 256.f;   // 1.5 * 2^23 and 2^-8: low bits of a sum with them are whole numbers
+    constexpr double kStep = 0.6931471805599453 / kTable, kHalf = kStep / 2, kRoot = 1 + kHalf * (1 + kHalf / 2 * (1 + kHalf / 3 * (1 + kHalf / 4)));   // 2^(1 / 512)
+    constexpr float c0 = static_cast<float>(kUnit + (kRoot - 1)), c1 = static_cast<float>(kRoot * kStep), c2 = static_cast<float>(kRoot * kStep * kStep / 2),
+                    c3 = static_cast<float>(kRoot * kStep * kStep * kStep / 6);
+    const float t = fmaf(l, rate_hi, kMagic);
+    const float f = fmaf(l, rate_lo, fmaf(l, rate_hi, kMagic - t));   // in [-1/2, 1/2]
+    const uint32_t k = __float_as_uint(t), g = __float_as_uint(fmaf(fmaf(fmaf(f, c3, c2), f, c1), f, c0));
+    v = scaled(k);
+    constexpr uint64_t kOne = (uint64_t(0x3ff00000) << 32) - (uint64_t(0x3b800000) << 21);
+    uint64_t r;
+    asm("mad.wide.u32 %0, %1, %2, %3;" : "=l"(r) : "r"(g), "r"(two21), "l"(kOne));
+    d = __longlong_as_double(r);
   }
+  __device__ __forceinline__ double scaled(uint32_t k) const {   // (of k only the low 20 bits matter: 1.5 2^23 has none there)
+    const double e = table[(k & (kTable - 1)) * kCopies];
+    uint32_t hi_word;
+    asm("mad.lo.u32 %0, %1, %2, %3;" : "=r"(hi_word) : "r"(k), "r"(two12), "r"(__double2hiint(e)));
+    return __hiloint2double(hi_word, __double2loint(e));
+  }
+  __device__ __forceinline__ double near_zero(float l) const {
+    double v, d;
+    near_zero(l, v, d);
+    return v * d;
+  }
+  __device__ __forceinline__ double far(float l) const {
+    constexpr double kMagic = 6755399441055744.;   // 1.5 * 2^52
+    constexpr double c1 = 0.6931471805599453 / kTable, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;
+    const double x = static_cast<double>(fminf(l, hi)) - ref;
+    const double t = fma(x, rate, kMagic);
+    const double f = fma(x, rate, -(t - kMagic)) + 0.5;
+    return scaled(__double2loint(t)) * fma(fma(fma(f, c3, c2), f, c1), f, 1.);
+  }
+  __device__ __forceinline__ double operator()(float l) const;
 };
 static_assert(kTable == 256, "the exponent is what is above 8 bits");
+// Out of line (instructions that a block runs once come from memory, and there are enough of them), by value (a struct whose address is taken
+// lives there too).
+__device__ __noinline__ double far_weight(const double* table, double rate, double ref, float hi, uint32_t two12, float l) {
+  return Weigher{table, rate, ref, 0.f, 0.f, 0.f, hi, two12, 0, false}.far(l);
+}
+__device__ __forceinline__ double Weigher::operator()(float l) const {
+  if (!(l >= lo)) return 0.;
+  return centered ? near_zero(fminf(l, hi)) : far_weight(table, rate, ref, hi, two12, l);
+}
 
 __device__ __forceinline__ double warp_sum64(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ double warp_scan64(double v) {   // sums of the lanes up to this one
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double w = __shfl_up_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) >= o) v += w;
+  }
+  return v;
+}
 
-// A row of logits in vectors of 16 bytes that start at their own boundary: vector j has tokens first(j) .. first(j) + kVec - 1, those
-// outside [0, V) at -inf.
+// A row of logits in vectors of eight that start on a boundary of 16 bytes: vector j has tokens first(j) .. first(j) + 7, those outside
+// [0, V) at -inf.
+template <typename T>
+struct Vec {
+  Pack<T> p[kVec / Elem<T>::kVec];
+  __device__ __forceinline__ T& operator[](int i) { return p[i / Elem<T>::kVec].v[i % Elem<T>::kVec]; }
+  __device__ __forceinline__ const T& operator[](int i) const { return p[i / Elem<T>::kVec].v[i % Elem<T>::kVec]; }
+  __device__ __forceinline__ float operator()(int i) const { return Elem<T>::to_f((*this)[i]); }
+};
+// The largest of many logits (NaN where there is one) and logits raised to a least one, two 16-bit ones an instruction.
+template <typename T>
+struct Range;
+template <>
+struct Range<float> {
+  static constexpr float kLeast = -FLT_MAX;
+  float lo, top = -INFINITY;
+  __device__ __forceinline__ explicit Range(float l) : lo(l) {}
+  __device__ __forceinline__ void take(Vec<float>& x) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(x[i]));
+      x[i] = fmaxf(x[i], lo);
+    }
+  }
+  __device__ __forceinline__ float largest() const { return top; }
+};
+template <typename T, typename T2>
+struct Range16 {
+  T2 lo, top;
+  __device__ __forceinline__ explicit Range16(float l) {
+    lo.x = lo.y = Elem<T>::from_f(l);
+    top.x = top.y = Elem<T>::from_f(-INFINITY);
+  }
+  __device__ __forceinline__ void take(Vec<T>& x) {
+#pragma unroll
+    for (int i = 0; i < kVec; i += 2) {
+      T2& v = *reinterpret_cast<T2*>(&x[i]);
+      top = __hmax2_nan(top, v);
+      v = __hmax2(v, lo);
+    }
+  }
+  __device__ __forceinline__ float largest() const {
+    const float a = Elem<T>::to_f(top.x), b = Elem<T>::to_f(top.y);
+    return a != a ? a : b != b ? b : fmaxf(a, b);
+  }
+};
+template <>
+struct Range<__half> : Range16<__half, __half2> {
+  using Range16::Range16;
+  static constexpr float kLeast = -65504.f;
+};
+template <>
+struct Range<__nv_bfloat16> : Range16<__nv_bfloat16, __nv_bfloat162> {
+  using Range16::Range16;
+  static constexpr float kLeast = -3.3895314e38f;
+};
 template <typename T>
 struct Row {
-  static constexpr int kVec = Elem<T>::kVec;
   const T* p;
   int V, skew;
   __device__ __forceinline__ Row(const T* p_, int V_) : p(p_), V(V_), skew(static_cast<int>(reinterpret_cast<uintptr_t>(p_) % 16 / sizeof(T))) {}
   __device__ __forceinline__ int vectors() const { return (V + skew + kVec - 1) / kVec; }
   __device__ __forceinline__ int first(int j) const { return j * kVec - skew; }
-  __device__ __forceinline__ void load(int j, float (&x)[kVec]) const {
+  __device__ __forceinline__ Vec<T> load(int j) const {
     const int v0 = first(j);
+    Vec<T> v;
     if (v0 >= 0 && v0 + kVec <= V) {
-      const Pack<T> v = ld128(p + v0);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) x[i] = Elem<T>::to_f(v.v[i]);
+      for (int i = 0; i < kVec / Elem<T>::kVec; ++i) v.p[i] = ld128(p + v0 + i * Elem<T>::kVec);
     } else {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) x[i] = v0 + i >= 0 && v0 + i < V ? Elem<T>::to_f(p[v0 + i]) : -INFINITY;
+      for (int i = 0; i < kVec; ++i) v[i] = v0 + i >= 0 && v0 + i < V ? p[v0 + i] : Elem<T>::from_f(-INFINITY);
     }
+    return v;
   }
   // the draft's probabilities of the same tokens
   __device__ __forceinline__ void load_probs(const float* q, int j, float (&x)[kVec]) const {
@@ -124,31 +237,162 @@ struct Row {
       for (int i = 0; i < kVec; ++i) x[i] = v0 + i >= 0 && v0 + i < V ? q[v0 + i] : 0.f;
     }
   }
+  // f(j, logits) for this lane's vectors j0 + lane, j0 + lane + 32, ... below j1, two loads ahead
+  template <typename F>
+  __device__ __forceinline__ void each(int j0, int j1, F&& f) const {
+    int j = j0 + static_cast<int>(threadIdx.x & 31);
+    Vec<T> now{}, next{};
+    if (j < j1) now = load(j);
+    if (j + 32 < j1) next = load(j + 32);
+#pragma unroll 1
+    for (; j < j1; j += 32) {
+      Vec<T> after = next;
+      if (j + 64 < j1) after = load(j + 64);
+      f(j, now);
+      now = next, next = after;
+    }
+  }
 };
+
+// The passes over a warp's run [j0, j1) of a row.  Each is a function of its own, with the registers to itself: inlined into the walk through the
+// tree the constants of the first were made anew for every logit (37 instructions each in the place of 17).
+
+// this lane's sum of weights around zero, NaN where a logit lies outside.  Logits below the range count as ones at its end: 2^-500 or
+// less each, against a total of 2^-200 or more
+template <typename T>
+__device__ __noinline__ double sum_near(const Row<T> row, const Weigher weigh, const int j0, const int j1) {
+  double s0 = 0., s1 = 0.;
+  Range<T> range(weigh.lo);
+  row.each(j0, j1, [&](int, Vec<T>& x) {
+    range.take(x);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      double v, d;
+      weigh.near_zero(x(i), v, d);
+      if (i & 1) s1 = fma(v, d, s1);
+      else s0 = fma(v, d, s0);
+    }
+  });
+  return range.largest() <= weigh.hi ? s0 + s1 : NAN;
+}
+
+// the largest logit (NaN: there is one) and its first token
+struct Largest {
+  float l;
+  int token;
+  __device__ __forceinline__ void take(float v, int w) {
+    if (v != v || v > l || (v == l && w < token)) l = l != l ? l : v, token = w;
+  }
+  __device__ __forceinline__ void of_warp() {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) take(__shfl_xor_sync(0xffffffffu, l, o), __shfl_xor_sync(0xffffffffu, token, o));
+  }
+};
+template <typename T>
+__device__ __noinline__ Largest largest_of(const Row<T> row, const int j0, const int j1) {
+  Largest best{-INFINITY, 0x7fffffff};
+  row.each(j0, j1, [&](int j, const Vec<T>& x) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) best.take(x(i), row.first(j) + i);
+  });
+  best.of_warp();
+  return best;
+}
+
+// What is left of eight tokens' weights: max(w inv - beta q, 0), with beta 0 w.
+template <typename T>
+__device__ __forceinline__ void remaining(const Row<T>& row, const Weigher& weigh, const int j, const Vec<T>& x, const float* q, double inv, double beta,
+                                          double (&w)[kVec]) {
+  if (weigh.centered) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) w[i] = weigh.near_zero(fmaxf(x(i), weigh.lo));
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) w[i] = weigh(x(i));
+  }
+  if (beta > 0.) {
+    float y[kVec];
+    row.load_probs(q, j, y);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) w[i] = fma(w[i], inv, -beta * static_cast<double>(y[i]));
+  }
+#pragma unroll
+  for (int i = 0; i < kVec; ++i)
+    if (!(x(i) >= weigh.lo && w[i] > 0.)) w[i] = 0.;
+}
+// this lane's sum of it
+template <typename T>
+__device__ __noinline__ double sum_remaining(const Row<T> row, const Weigher weigh, const int j0, const int j1, const float* q, const double inv, const double beta) {
+  double s = 0.;
+  row.each(j0, j1, [&](int j, const Vec<T>& x) {
+    double w[kVec];
+    remaining(row, weigh, j, x, q, inv, beta, w);
+    s += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+  });
+  return s;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, const int C) {
-  constexpr int kVec = Elem<T>::kVec;
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& sh = *reinterpret_cast<Shared*>(smem);
   int* const parents = reinterpret_cast<int*>(smem + sizeof(Shared));
-  Kid* const all_kids = reinterpret_cast<Kid*>(parents + a.T);   // two lists of up to T
+  int* const drafts = parents + a.T;
+  float* const u = reinterpret_cast<float*>(drafts + a.T);
+  int* const first_kid = reinterpret_cast<int*>(u + a.T);   // a.T: none
+  int* const sibling = first_kid + a.T;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = C > 1 ? static_cast<int>(ptx::cluster_ctarank()) : 0, b = static_cast<int>(blockIdx.x) / C;
-  for (int i = threadIdx.x; i < kTable; i += kWarps * 32) sh.table[i] = exp2(i * (1. / kTable));
+  if (threadIdx.x < kTable) {
+    const double v = __longlong_as_double(g_table.e[threadIdx.x]);
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) sh.table[threadIdx.x][(threadIdx.x + i) % kCopies] = v;
+  }
+  if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // waited for before the first word to another block
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
-  for (int i = threadIdx.x; i < a.T; i += kWarps * 32) parents[i] = a.parents[b * a.parents_b + i];
+  const int slots = C * kWarps, mine = warp * C + rank;   // in the order of the vocabulary: few runs are dealt to all blocks
+  auto row_of = [&](int n) { return Row<T>(static_cast<const T*>(a.logits) + b * a.ls_b + n * a.ls_n, a.V); };
+  auto run_of = [&](const Row<T>& row, int& per, int& j0, int& j1) {
+    per = max((row.vectors() + slots - 1) / slots, 32), j0 = min(mine * per, row.vectors()), j1 = min(j0 + per, row.vectors());
+  };
+  // elements [e0, e1) of a row of V, towards the L2 cache
+  auto ahead = [&](const auto* p, int e0, int e1) {
+    const char *at = reinterpret_cast<const char*>(p + max(e0, 0)) + lane * 128, *end = reinterpret_cast<const char*>(p + min(e1, a.V));
+#pragma unroll 1
+    for (; at < end; at += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+  };
+  {
+    const Row<T> row = row_of(0);
+    int per, j0, j1;
+    run_of(row, per, j0, j1);
+    ahead(row.p, row.first(j0), row.first(j1));
+  }
+  for (int i = threadIdx.x; i < a.T; i += kWarps * 32) {
+    parents[i] = a.parents[b * a.parents_b + i];
+    drafts[i] = a.drafts[static_cast<int64_t>(b) * a.T + i];
+    u[i] = a.uniforms[static_cast<int64_t>(b) * a.T + i];
+  }
   const float temperature = a.temperatures ? a.temperatures[b] : a.temperature;
   const bool greedy = !(temperature > 0.f);
-  const int slots = C * kWarps, mine = rank * kWarps + warp;
-  const float* const u = a.uniforms + static_cast<int64_t>(b) * a.T;
-  const int32_t* const drafts = a.drafts + static_cast<int64_t>(b) * a.T;
   int32_t* const tokens = a.tokens + static_cast<int64_t>(b) * a.T;
   int32_t* const path = a.path + static_cast<int64_t>(b) * a.T;
   const bool writer = rank == 0 && threadIdx.x == 0;
   __syncthreads();
-  if (C > 1) ptx::cluster_sync();   // every block of the cluster runs: its shared memory may be written
+  for (int i = warp; i < a.T; i += kWarps) {   // a warp per node: its children, from the last one on
+    int next = a.T;
+#pragma unroll 1
+    for (int base = (a.T - 1) & ~31; base + 31 > i; base -= 32) {
+      const int k = base + lane;
+      const bool is = k > i && k < a.T && parents[k] == i;
+      const uint32_t m = __ballot_sync(0xffffffffu, is), above = m & ~((2u << lane) - 1);
+      if (is) sibling[k] = above ? base + __ffs(above) - 1 : next;
+      if (m) next = base + __ffs(m) - 1;
+    }
+    if (lane == 0) first_kid[i] = next;
+  }
+  __syncthreads();
+  if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every block of the cluster runs: its shared memory may be written
 
   int turn = 0;
   auto meet = [&](double sum, int id) {   // all warps' numbers in sum[turn ^ 1], id[turn ^ 1] of every block
@@ -166,275 +410,221 @@ __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, co
     turn ^= 1;
   };
   auto sum_all = [&]() {   // of all warps, in an order that is the same everywhere
-    double s = 0.;
-    for (int i = lane; i < slots; i += 32) s += sh.sum[turn ^ 1][i];
-    return warp_sum64(s);
-  };
-  auto any_flag = [&]() {
-    int f = 0;
-    for (int i = lane; i < slots; i += 32) f |= sh.id[turn ^ 1][i];
-    return __any_sync(0xffffffffu, f != 0);
+    double s[kSlots / 32];
+#pragma unroll
+    for (int i = 0; i < kSlots / 32; ++i) s[i] = i * 32 + lane < slots ? sh.sum[turn ^ 1][i * 32 + lane] : 0.;
+    static_assert(kSlots / 32 == 4, "four a lane");
+    return warp_sum64((s[0] + s[1]) + (s[2] + s[3]));
   };
 
-  int n = 0, count = 0, token = -1, kid_turn = 0;
+  int n = 0, count = 0;
   if (writer) path[0] = 0;
-  Weigher weigh{sh.table, kTable * 1.4426950408889634 / static_cast<double>(temperature), 0., 0.f, 0.f};
+  Weigher weigh{&sh.table[0][lane % kCopies], kTable * 1.4426950408889634 / static_cast<double>(temperature), 0., 0.f, 0.f, 0.f, 0.f, a.two12, a.two21, true};
+#pragma unroll 1
   for (;;) {
-    const Row<T> row(static_cast<const T*>(a.logits) + b * a.ls_b + n * a.ls_n, a.V);
+    const Row<T> row = row_of(n);
     const float* const q = a.probs ? a.probs + b * a.ps_b + n * a.ps_n : nullptr;
-    const int per = (row.vectors() + slots - 1) / slots, j0 = min(mine * per, row.vectors()), j1 = min(j0 + per, row.vectors());
-    Kid* const kids = all_kids + kid_turn * a.T;
-    if (warp == 0) {   // the node's children that are tokens
-      int found = 0;
-      for (int i0 = (n + 1) & ~31; i0 < a.T; i0 += 32) {
-        const int i = i0 + lane;
-        int x = -1;
-        if (i > n && i < a.T && parents[i] == n) x = drafts[i];
-        const bool is = x >= 0 && x < a.V;
-        const uint32_t m = __ballot_sync(0xffffffffu, is);
-        if (is) kids[found + __popc(m & ((1u << lane) - 1))] = Kid{i, x, Elem<T>::to_f(row.p[x]), u[i], q ? q[x] : 1.f};
-        found += __popc(m);
+    int per, j0, j1;
+    run_of(row, per, j0, j1);
+    // Children of the node, one a lane, up to 32 at a time.  A lane without one, or whose draft is no token, has token -1.
+    const int kid0 = first_kid[n];
+    int kid = a.T, kid_token = -1;
+    T kid_logit = Elem<T>::from_f(0.f);
+    float kid_q = 1.f;
+    auto take_kids = [&](int from) {   // -> the first one that is left
+      kid = a.T;
+      int i = 0;
+#pragma unroll 1
+      for (; i < 32 && from < a.T; ++i, from = sibling[from])
+        if (lane == i) kid = from;
+      kid_token = kid < a.T ? drafts[kid] : -1;
+      if (kid_token >= a.V || kid_token < 0) kid_token = -1;
+      if (kid_token >= 0) {
+        kid_logit = row.p[kid_token];
+        if (q) kid_q = q[kid_token];
       }
-      if (lane == 0) sh.kid_count[kid_turn] = found;
+      return from;
+    };
+    int more = take_kids(kid0);
+    bool several = false;   // more than 32 of them
+    if (kid0 < a.T) {   // the row of the child that is tried first, and the draft's, towards the L2 cache while this row is walked through
+      ahead(row_of(kid0).p, row.first(j0), row.first(j1));
+      if (q) ahead(q, row.first(j0), row.first(j1));
     }
 
-    // the row's largest logit, its first token, and whether there is a NaN
-    auto largest = [&](float& best, int& at) {
-      best = -INFINITY, at = 0x7fffffff;
-      bool bad = false;
-      for (int j = j0 + lane; j < j1; j += 32) {
-        float x[kVec];
-        row.load(j, x);
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          bad |= x[i] != x[i];
-          if (x[i] > best) best = x[i], at = row.first(j) + i;
-        }
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const float v = __shfl_xor_sync(0xffffffffu, best, o);
-        const int w = __shfl_xor_sync(0xffffffffu, at, o);
-        if (v > best || (v == best && w < at)) best = v, at = w;
-      }
-      bad = __any_sync(0xffffffffu, bad);
-      meet(static_cast<double>(bad ? NAN : best), at);
-      best = -INFINITY, at = 0x7fffffff, bad = false;
-      for (int i = lane; i < slots; i += 32) {
-        const float v = static_cast<float>(sh.sum[turn ^ 1][i]);
-        const int w = sh.id[turn ^ 1][i];
-        bad |= v != v;
-        if (v > best || (v == best && w < at)) best = v, at = w;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const float v = __shfl_xor_sync(0xffffffffu, best, o);
-        const int w = __shfl_xor_sync(0xffffffffu, at, o);
-        if (v > best || (v == best && w < at)) best = v, at = w;
-      }
-      return !__any_sync(0xffffffffu, bad) && fabsf(best) < INFINITY;   // there is a distribution
+    auto tell_sum = [&](double s) {
+      s = warp_sum64(s);
+      meet(s < 0x1p-400 ? 0. : s, 0);
+      return sum_all();
     };
 
-    int accepted = -1, accepted_token = 0;
-    if (greedy) {
-      float best;
-      int at;
-      const bool fine = largest(best, at);
-      const int kid_count = sh.kid_count[kid_turn];
-      double beta = 0.;   // q = draft probabilities: p is 1 at `at`, what is left of it after k rejections max(1 - beta q(at), 0)
-      double left = 1.;   // (of Pi_k; the other tokens have nothing at any time)
-      const float q_at = fine && q ? q[at] : 1.f;
-      for (int k = 0; fine && k < kid_count && accepted < 0; ++k) {
-        const Kid kid = kids[k];
-        if (kid.token == at && static_cast<double>(kid.u) * kid.q * (beta > 0. ? left : 1.) < left) {
-          accepted = kid.node, accepted_token = kid.token;
-        } else if (q) {
-          beta = beta > 0. ? beta + left : 1.;
-          left = fmax(1. - beta * q_at, 0.);
-        } else if (kid.token == at) {
-          left = 0.;
-        }
-      }
-      if (accepted < 0) {
-        token = fine && left > 0. ? at : -1;
-        if (writer) tokens[count] = token;
-        break;
-      }
-    } else {
-      // ---- weights of the row
-      auto weigh_all = [&](bool& over) {
-        double s0 = 0., s1 = 0.;
-        bool out = false;
-        for (int j = j0 + lane; j < j1; j += 32) {
-          float x[kVec];
-          row.load(j, x);
-#pragma unroll
-          for (int i = 0; i < kVec; i += 2) {
-            out |= !(x[i] <= weigh.hi) || !(x[i + 1] <= weigh.hi);
-            s0 += weigh(x[i]);
-            s1 += weigh(x[i + 1]);
-          }
-        }
-        out = __any_sync(0xffffffffu, out);
-        meet(warp_sum64(s0 + s1), out);
-        over = any_flag();
-        return sum_all();
-      };
-      bool over, fine = true;
-      weigh.relative_to(0.f);
-      double total = weigh_all(over);
-      if (over || !(total >= 0x1p-200)) {   // the row does not lie around zero
-        float best;
-        int at;
-        fine = largest(best, at);
-        if (fine) {
-          weigh.relative_to(best);
-          total = weigh_all(over);
-        }
-      }
-      const int kid_count = sh.kid_count[kid_turn];
-      double rest = total, beta = 0., inv = 1.;
-      // (q) sum of max(p - beta q, 0) over the vocabulary
-      auto residue = [&]() {
-        double s = 0.;
-        for (int j = j0 + lane; j < j1; j += 32) {
-          float x[kVec], y[kVec];
-          row.load(j, x);
-          row.load_probs(q, j, y);
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) s += fmax(fma(weigh(x[i]), inv, -beta * static_cast<double>(y[i])), 0.);
-        }
-        meet(warp_sum64(s), 0);
-        return sum_all();
-      };
-      auto repeated = [&](int k) {   // an earlier child had the same token
-        bool same = false;
-        for (int i = lane; i < k; i += 32) same |= kids[i].token == kids[k].token;
-        return __any_sync(0xffffffffu, same);
-      };
-      for (int k = 0; fine && k < kid_count && accepted < 0; ++k) {
-        const Kid kid = kids[k];
-        double w = weigh(kid.logit);
-        if (q) {
-          if (beta > 0.) w = fmax(fma(w, inv, -beta * static_cast<double>(kid.q)), 0.);
-        } else if (repeated(k)) {
-          continue;
-        }
-        if (static_cast<double>(kid.u) * static_cast<double>(kid.q) * rest < w) {
-          accepted = kid.node, accepted_token = kid.token;
-        } else if (q) {
-          inv = 1. / total;
-          beta = beta > 0. ? beta + rest : 1.;
-          rest = residue();
-        } else {
-          rest = fmax(rest - w, 0.);
-        }
-      }
-      if (accepted < 0) {
-        // ---- the token behind the path
-        const int turn_read = turn ^ 1, span = (slots + 31) / 32;   // a lane's warps: their order is the vocabulary's
-        const bool without = !q && fine;
-        double part[kMaxCluster * kWarps / 32];
-        double lane_sum = 0.;
-#pragma unroll
-        for (int i = 0; i < kMaxCluster * kWarps / 32; ++i) part[i] = i < span && lane * span + i < slots ? sh.sum[turn_read][lane * span + i] : 0.;
-        for (int k = 0; without && k < kid_count; ++k) {
-          if (repeated(k)) continue;
-          const int owner = (kids[k].token + row.skew) / kVec / per;
-          const double w = weigh(kids[k].logit);
-#pragma unroll
-          for (int i = 0; i < kMaxCluster * kWarps / 32; ++i)
-            if (owner == lane * span + i && i < span) part[i] = fmax(part[i] - w, 0.);
-        }
-#pragma unroll
-        for (int i = 0; i < kMaxCluster * kWarps / 32; ++i) lane_sum += part[i];
-        double upto = lane_sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double v = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += v;
-        }
-        const double all = __shfl_sync(0xffffffffu, upto, 31), target = static_cast<double>(u[0]) * all;
-        // the first warp whose cumulative sum passes the target, else the last one with something in it
-        const uint32_t past = __ballot_sync(0xffffffffu, lane_sum > 0. && upto > target), some = __ballot_sync(0xffffffffu, lane_sum > 0.);
-        const int lane_of = past ? __ffs(past) - 1 : 31 - __clz(some | 1u);
-        double before = upto - lane_sum, prefix = 0.;
-        int owner = -1, last_owner = -1;
-        double last_prefix = 0.;
-#pragma unroll
-        for (int i = 0; i < kMaxCluster * kWarps / 32; ++i) {
-          if (part[i] > 0.) {
-            last_owner = lane * span + i, last_prefix = before;
-            if (owner < 0 && before + part[i] > target) owner = lane * span + i, prefix = before;
-          }
-          before += part[i];
-        }
-        if (owner < 0) owner = last_owner, prefix = last_prefix;
-        owner = __shfl_sync(0xffffffffu, owner, lane_of);
-        prefix = __shfl_sync(0xffffffffu, prefix, lane_of);
-        if (!fine || !some) {
-          if (writer) tokens[count] = -1;
-        } else if (owner == mine) {
-          const double goal = target - prefix;
-          double passed = 0.;
-          int last_positive = -1;
-          token = -1;
-          for (int j = j0; j < j1 && token < 0; j += 32) {
-            float x[kVec], y[kVec];
-            double w[kVec], s = 0.;
-            int last = -1;
-            const bool in = j + lane < j1;
-            if (in) row.load(j + lane, x);
-            if (in && beta > 0.) row.load_probs(q, j + lane, y);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) {
-              w[i] = in ? weigh(x[i]) : 0.;
-              if (in && beta > 0.) w[i] = fmax(fma(w[i], inv, -beta * static_cast<double>(y[i])), 0.);
-            }
-            if (without) {
-              for (int k = 0; k < kid_count; ++k) {
-                const int off = kids[k].token - row.first(j + lane);
-#pragma unroll
-                for (int i = 0; i < kVec; ++i)
-                  if (off == i) w[i] = 0.;
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) {
-              s += w[i];
-              if (w[i] > 0.) last = row.first(j + lane) + i;
-            }
-            double upto_here = s;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const double v = __shfl_up_sync(0xffffffffu, upto_here, o);
-              if (lane >= o) upto_here += v;
-            }
-            const uint32_t over_goal = __ballot_sync(0xffffffffu, last >= 0 && passed + upto_here > goal);
-            if (over_goal) {
-              double run = passed + (upto_here - s);
-              int mine_token = last;   // (sums in another order may fall short of the goal by a rounding)
-              bool done = false;
-#pragma unroll
-              for (int i = 0; i < kVec; ++i) {
-                run += w[i];
-                if (!done && w[i] > 0. && run > goal) mine_token = row.first(j + lane) + i, done = true;
-              }
-              token = __shfl_sync(0xffffffffu, mine_token, __ffs(over_goal) - 1);
-            }
-            const uint32_t positive = __ballot_sync(0xffffffffu, last >= 0);
-            if (positive) last_positive = __shfl_sync(0xffffffffu, last, 31 - __clz(positive));
-            passed += __shfl_sync(0xffffffffu, upto_here, 31);
-          }
-          if (lane == 0) tokens[count] = token >= 0 ? token : last_positive;
-        }
-        break;
+    int accepted = -1, accepted_token = -1, at = 0;
+    double total = 0.;
+    bool fine = true;
+    weigh.relative_to(0.f, true);
+    if (!greedy && weigh.lo > Range<T>::kLeast) total = tell_sum(sum_near(row, weigh, j0, j1));
+    if (!(total >= 0x1p-200)) {   // greedy, or the row does not lie around zero (or all of a type's numbers do)
+      Largest best = largest_of(row, j0, j1);
+      meet(best.l, best.token);
+      best = {-INFINITY, 0x7fffffff};
+      for (int i = lane; i < slots; i += 32) best.take(static_cast<float>(sh.sum[turn ^ 1][i]), sh.id[turn ^ 1][i]);
+      best.of_warp();
+      fine = fabsf(best.l) < INFINITY;   // there is a distribution
+      at = best.token;
+      if (fine && !greedy) {
+        weigh.relative_to(best.l, false);
+        total = tell_sum(sum_remaining<T>(row, weigh, j0, j1, nullptr, 1., 0.));
       }
     }
-    if (writer) tokens[count] = accepted_token, path[count + 1] = accepted;
-    ++count;
-    n = accepted;
-    kid_turn ^= 1;
+    // ---- the children in turn.  `rest` is Pi (of p unnormalised while nothing is rejected): p = max(weight inv - beta q, 0) / rest.
+    double beta = 0., inv = 1., rest = greedy ? 1. : total;
+    const float q_at = greedy && fine && q ? q[at] : 0.f;
+    auto own_weight = [&]() { return kid_token < 0 ? 0. : greedy ? (kid_token == at ? 1. : 0.) : weigh(Elem<T>::to_f(kid_logit)); };
+    // whether an earlier child had this lane's token
+    auto repeated = [&]() {
+      bool same = (__match_any_sync(0xffffffffu, kid_token) & ((1u << lane) - 1)) != 0;
+      if (several && kid_token >= 0)
+        for (int k = kid0; !same && k < kid; k = sibling[k]) same = drafts[k] == kid_token;
+      return same;
+    };
+    double kid_w = 0.;
+    bool kid_again = false;
+#pragma unroll 1
+    while (fine && kid0 < a.T) {
+      kid_w = own_weight();
+      kid_again = repeated();
+      const float kid_u = kid < a.T ? u[kid] : 0.f;
+      uint32_t todo = __ballot_sync(0xffffffffu, kid_token >= 0);
+#pragma unroll 1
+      for (; todo && accepted < 0; todo &= todo - 1) {
+        const int k = __ffs(todo) - 1;
+        if (q) {
+          const double w = beta > 0. ? fmax(fma(kid_w, inv, -beta * static_cast<double>(kid_q)), 0.) : kid_w;
+          const bool good = static_cast<double>(kid_u) * static_cast<double>(kid_q) * rest < w;
+          if (__shfl_sync(0xffffffffu, good, k)) {
+            accepted = __shfl_sync(0xffffffffu, kid, k), accepted_token = __shfl_sync(0xffffffffu, kid_token, k);
+            break;
+          }
+          inv = greedy ? 1. : 1. / total;
+          beta = beta > 0. ? beta + rest : 1.;
+          if (greedy) {
+            rest = fmax(1. - beta * q_at, 0.);
+          } else {
+            meet(warp_sum64(sum_remaining(row, weigh, j0, j1, q, inv, beta)), 0);
+            rest = sum_all();
+          }
+        } else {
+          const double w = kid_again ? 0. : kid_w;
+          const bool good = static_cast<double>(kid_u) * rest < w;
+          if (__shfl_sync(0xffffffffu, good, k)) {
+            accepted = __shfl_sync(0xffffffffu, kid, k), accepted_token = __shfl_sync(0xffffffffu, kid_token, k);
+            break;
+          }
+          rest = fmax(rest - __shfl_sync(0xffffffffu, w, k), 0.);
+        }
+      }
+      if (accepted >= 0 || more >= a.T) break;
+      several = true;
+      more = take_kids(more);
+    }
+    if (accepted >= 0) {
+      if (writer) tokens[count] = accepted_token, path[count + 1] = accepted;
+      ++count;
+      n = accepted;
+      continue;
+    }
+    // ---- the token behind the path
+    if (!fine || greedy) {
+      if (writer) tokens[count] = fine && rest > 0. ? at : -1;
+      break;
+    }
+    // The warps' sums in the order of the vocabulary, `span` to a lane, without the children's weights where those are out.
+    const int span = (slots + 31) / 32;
+    double part[kSlots / 32];
+#pragma unroll
+    for (int i = 0; i < kSlots / 32; ++i) part[i] = i < span && lane * span + i < slots ? sh.sum[turn ^ 1][lane * span + i] : 0.;
+    const bool without = q == nullptr && kid0 < a.T;
+    auto each_kid = [&](auto&& f) {   // f(token, weight) for every rejected child's token, once
+      int left = several ? take_kids(kid0) : a.T;
+#pragma unroll 1
+      for (;;) {
+        if (several) kid_w = own_weight(), kid_again = repeated();
+#pragma unroll 1
+        for (uint32_t todo = __ballot_sync(0xffffffffu, kid_token >= 0 && !kid_again); todo; todo &= todo - 1) {
+          const int k = __ffs(todo) - 1;
+          f(__shfl_sync(0xffffffffu, kid_token, k), __shfl_sync(0xffffffffu, kid_w, k));
+        }
+        if (left >= a.T) break;
+        left = take_kids(left);
+      }
+    };
+    bool touched = false;   // a child's token lies in this warp's run
+    if (without)
+      each_kid([&](int token, double w) {
+        const int owner = (token + row.skew) / kVec / per;
+        touched |= owner == mine;
+#pragma unroll
+        for (int i = 0; i < kSlots / 32; ++i)
+          if (owner == lane * span + i && i < span) part[i] = fmax(part[i] - w, 0.);
+      });
+    const double lane_sum = (part[0] + part[1]) + (part[2] + part[3]), upto = warp_scan64(lane_sum);
+    const double all = __shfl_sync(0xffffffffu, upto, 31), target = static_cast<double>(u[0]) * all;
+    // the first warp whose cumulative sum passes the target, else the last one with something in it
+    const uint32_t past = __ballot_sync(0xffffffffu, lane_sum > 0. && upto > target), some = __ballot_sync(0xffffffffu, lane_sum > 0.);
+    const int lane_of = past ? __ffs(past) - 1 : 31 - __clz(some | 1u);
+    double before = upto - lane_sum, prefix = 0., last_prefix = 0.;
+    int owner = -1, last_owner = -1;
+#pragma unroll
+    for (int i = 0; i < kSlots / 32; ++i) {
+      if (part[i] > 0.) {
+        last_owner = lane * span + i, last_prefix = before;
+        if (owner < 0 && before + part[i] > target) owner = lane * span + i, prefix = before;
+      }
+      before += part[i];
+    }
+    if (owner < 0) owner = last_owner, prefix = last_prefix;
+    owner = __shfl_sync(0xffffffffu, owner, lane_of);
+    const double goal = target - __shfl_sync(0xffffffffu, prefix, lane_of);
+    if (!some) {
+      if (writer) tokens[count] = -1;
+    } else if (owner == mine) {   // its run once more: 256 logits at a time until the goal is passed
+      double passed = 0.;
+      int last_positive = -1, token = -1;
+#pragma unroll 1
+      for (int base = j0; base < j1 && token < 0; base += 32) {
+        const int j = base + lane;
+        double w[kVec] = {};
+        if (j < j1) remaining(row, weigh, j, row.load(j), q, inv, beta, w);
+        if (touched)
+          each_kid([&](int out, double) {
+            const int off = out - row.first(j);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i)
+              if (off == i) w[i] = 0.;
+          });
+        int last = -1;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i)
+          if (w[i] > 0.) last = row.first(j) + i;
+        const double sum = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])), through = warp_scan64(sum);
+        const uint32_t there = __ballot_sync(0xffffffffu, last >= 0 && passed + through > goal), positive = __ballot_sync(0xffffffffu, last >= 0);
+        if (there) {
+          double run = passed + (through - sum);
+          int found = last;   // (sums in another order may fall short of the goal by a rounding)
+          bool done = false;
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) {
+            run += w[i];
+            if (!done && w[i] > 0. && run > goal) found = row.first(j) + i, done = true;
+          }
+          token = __shfl_sync(0xffffffffu, found, __ffs(there) - 1);
+        }
+        if (positive) last_positive = __shfl_sync(0xffffffffu, last, 31 - __clz(positive));
+        passed += __shfl_sync(0xffffffffu, through, 31);
+      }
+      if (lane == 0) tokens[count] = token >= 0 ? token : last_positive;
+    }
+    break;
   }
   if (writer) a.counts[b] = count + 1;
   if (rank == 0)
@@ -443,10 +633,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, co
 
 template <typename T>
 int launch(const Args& a, cudaStream_t s) {
-  // Blocks of a cluster: as many as there are SMs for, as long as each warp has two vectors a lane.
+  // Blocks of a cluster: as many as there are SMs for, as long as each has work for eight warps.
   int C = 1;
-  while (C < kMaxCluster && a.B * C * 2 <= sm_count() && a.V > C * kWarps * 64 * Elem<T>::kVec) C *= 2;
-  auto bytes = [](int nodes) { return static_cast<int>(sizeof(Shared) + nodes * (4 + 2 * sizeof(Kid))); };
+  while (C < kMaxCluster && a.B * C * 2 <= sm_count() && a.V > C * 8 * 32 * kVec) C *= 2;
+  auto bytes = [](int nodes) { return static_cast<int>(sizeof(Shared) + nodes * 20); };
   static SmemLimit limit;
   const cudaError_t e = limit.raise(verify_kernel<T>, bytes(kMaxNodes));
   if (e != cudaSuccess) return set_error(OASR_ERR_CUDA, "verify_drafts: shared memory limit: %s", cudaGetErrorString(e));
@@ -486,7 +676,7 @@ extern "C" int oasr_b200_verify_drafts(int32_t* tokens, int32_t* path, int32_t* 
                  is_aligned(parents, 4) && is_aligned(uniforms, 4) && is_aligned(draft_probs, 4) && is_aligned(temperatures, 4),
              OASR_ERR_ALIGN, "verify_drafts: operands must be aligned to their elements");
   const verify::Args a{tokens, path, counts, logits, draft_probs, drafts, parents, uniforms, temperatures, logits_stride_b, logits_stride_n, probs_stride_b,
-                       probs_stride_n, parents_stride, static_cast<int>(B), static_cast<int>(T), static_cast<int>(V), static_cast<float>(temperature)};
+                       probs_stride_n, parents_stride, static_cast<int>(B), static_cast<int>(T), static_cast<int>(V), static_cast<float>(temperature), 1u << 12, 1u << 21};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   return OB_DISPATCH_FLOAT(dtype, T_, [&]() -> int { return verify::launch<T_>(a, st); });
 }
