@@ -795,7 +795,7 @@ OASR_API int oasr_b200_draft_tree(uint32_t* mask, int32_t* depth, const int32_t*
  * rounded to the element type before the second product.  The workspace (16-byte aligned; its size from the function below, which may be 0) is
  * this call's alone until it has run.  The work is split by blocks_per_seq: a table much wider than the sequences costs time. */
 OASR_API int64_t oasr_b200_fmha_tree_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t D,
-                                                     int64_t blocks_per_seq, int64_t block_size);
+                                                     int64_t blocks_per_seq, int64_t block_size, int64_t num_blocks);
 OASR_API int oasr_b200_fmha_tree(void* out, const int64_t* out_strides, const void* q, const int64_t* q_strides,
                                  const void* k_pool, const void* v_pool, const int32_t* block_table, const int32_t* seqlens,
                                  const int32_t* seqstarts, const int32_t* q_lens, const uint32_t* mask, int64_t mask_stride,

@@ -210,7 +210,7 @@ def load() -> ctypes.CDLL:
     lib.oasr_b200_fmha_relpos_plan_bytes.restype = c_int64
     lib.oasr_b200_fmha_relpos_plan_bytes.argtypes = [I, I, I]
     lib.oasr_b200_fmha_tree_workspace_bytes.restype = c_int64
-    lib.oasr_b200_fmha_tree_workspace_bytes.argtypes = [I] * 7
+    lib.oasr_b200_fmha_tree_workspace_bytes.argtypes = [I] * 8
     lib.oasr_b200_fastconformer_workspace_bytes.restype = c_int64
     lib.oasr_b200_fastconformer_workspace_bytes.argtypes = [POINTER(FastConformerModel), I, I, I]
     lib.oasr_b200_fastconformer_chunk_workspace_bytes.restype = c_int64

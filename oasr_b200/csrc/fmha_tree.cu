@@ -21,6 +21,9 @@
 
 namespace ob {
 namespace fmha_tree {
+
+int g_path = 0;   // tunable "fmha_tree_path": 0 by size, 1 the few-row form, 2 the form for many rows
+
 namespace {
 
 template <typename T>
@@ -423,13 +426,25 @@ __global__ void __launch_bounds__(256) fmha_tree_join_kernel(const Args a, const
 struct Plan {
   int rows, row_blocks, splits;   // rows of a block; blocks of rows of a (sequence, key head); blocks that share a cache
   int64_t groups;
+  bool wide;
 };
 
 // How a call is cut.  Blocks that share a cache: until the SMs are full, as long as each of a block's warps has four tiles.  The block table's width
 // stands for the lengths, which are on the GPU.
-Plan plan(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t D, int64_t keys) {
+Plan plan(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t D, int64_t keys, int64_t pool_rows) {
   Plan p;
   const int64_t rows = H / Hkv * Tq;
+  p.wide = pool_rows <= 0x7fffffff - 128 && (g_path ? g_path == 2 : rows > 32);
+  if (p.wide) {
+    p.rows = rows <= 128 ? 128 : 256;
+    p.row_blocks = static_cast<int>((rows + p.rows - 1) / p.rows);
+    p.groups = B * Hkv * p.row_blocks;
+    const int64_t most = keys / 512;
+    int64_t s = p.groups > 0 ? sm_count() / p.groups : 1;
+    s = s < most ? s : most;
+    p.splits = static_cast<int>(s < 1 ? 1 : s > 256 ? 256 : s);
+    return p;
+  }
   p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
   p.row_blocks = static_cast<int>((rows + p.rows - 1) / p.rows);
   p.groups = B * Hkv * p.row_blocks;
@@ -451,8 +466,8 @@ int launch(const Args& a, const Plan& p, cudaStream_t s) {
 }
 
 template <typename T, int D>
-int run(const Args& a, const Plan& p, cudaStream_t s) {
-  const int rc = p.rows == 8 ? launch<T, D, 1>(a, p, s) : p.rows == 16 ? launch<T, D, 2>(a, p, s) : launch<T, D, 4>(a, p, s);
+int run(const Args& a, const Plan& p, int dtype, cudaStream_t s) {
+  const int rc = p.wide ? run_wide(a, D, dtype, p.rows, p.groups, p.row_blocks, s) : p.rows == 8 ? launch<T, D, 1>(a, p, s) : p.rows == 16 ? launch<T, D, 2>(a, p, s) : launch<T, D, 4>(a, p, s);
   if (rc != OASR_OK || p.splits == 1) return rc;
   launch_pdl(fmha_tree_join_kernel<T, D>, dim3(static_cast<unsigned>((p.groups * p.rows + 7) / 8)), dim3(256), 0, s, a, p.row_blocks, p.rows,
              static_cast<int>(p.groups));
@@ -464,10 +479,10 @@ int run(const Args& a, const Plan& p, cudaStream_t s) {
 }  // namespace ob
 
 extern "C" int64_t oasr_b200_fmha_tree_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t D, int64_t blocks_per_seq,
-                                                       int64_t block_size) {
+                                                       int64_t block_size, int64_t num_blocks) {
   using namespace ob::fmha_tree;
   if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || Tq <= 0 || (D != 64 && D != 128) || blocks_per_seq < 0 || block_size <= 0) return 0;
-  const Plan p = plan(B, H, Hkv, Tq, D, blocks_per_seq * block_size);
+  const Plan p = plan(B, H, Hkv, Tq, D, blocks_per_seq * block_size, num_blocks * block_size);
   return p.splits > 1 ? p.splits * p.groups * (D == 64 ? part_floats<64>(p.rows) : part_floats<128>(p.rows)) * 4 : 0;
 }
 
@@ -498,9 +513,9 @@ extern "C" int oasr_b200_fmha_tree(void* out, const int64_t* out_strides, const 
     OB_REQUIRE(out_strides[i] % 8 == 0 && q_strides[i] % 8 == 0, OASR_ERR_ALIGN, "fmha_tree: strides must be multiples of 8 elements");
   OB_REQUIRE(is_aligned(out, 16) && is_aligned(q, 16) && is_aligned(k_pool, 16) && is_aligned(v_pool, 16) && is_aligned(mask, 4) && is_aligned(workspace, 16),
              OASR_ERR_ALIGN, "fmha_tree: operands must be 16-byte aligned");
-  const Plan p = plan(B, H, Hkv, Tq, D, blocks_per_seq * block_size);
+  const Plan p = plan(B, H, Hkv, Tq, D, blocks_per_seq * block_size, num_blocks * block_size);
   OB_REQUIRE(p.groups * p.splits <= 0x7fffffff && p.groups * p.rows <= 0x7fffffff, OASR_ERR_INVALID, "fmha_tree: too many rows for one call");
-  const int64_t need = oasr_b200_fmha_tree_workspace_bytes(B, H, Hkv, Tq, D, blocks_per_seq, block_size);
+  const int64_t need = oasr_b200_fmha_tree_workspace_bytes(B, H, Hkv, Tq, D, blocks_per_seq, block_size, num_blocks);
   OB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), OASR_ERR_INVALID, "fmha_tree: %lld bytes of workspace needed, %lld given", (long long)need,
              (long long)workspace_bytes);
   const Args a{out, q, k_pool, v_pool, block_table, seqlens, seqstarts, q_lens, mask, need ? static_cast<float*>(workspace) : nullptr, q_strides[0], q_strides[1],
@@ -508,5 +523,5 @@ extern "C" int oasr_b200_fmha_tree(void* out, const int64_t* out_strides, const 
                static_cast<int>(H), static_cast<int>(Hkv), static_cast<int>(Tq), static_cast<int>(mask_words), p.splits,
                static_cast<float>(scale * 1.4426950408889634)};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return OB_DISPATCH_HALF(dtype, T_, [&]() -> int { return D == 64 ? run<T_, 64>(a, p, st) : run<T_, 128>(a, p, st); });
+  return OB_DISPATCH_HALF(dtype, T_, [&]() -> int { return D == 64 ? run<T_, 64>(a, p, dtype, st) : run<T_, 128>(a, p, dtype, st); });
 }

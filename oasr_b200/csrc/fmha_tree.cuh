@@ -53,5 +53,8 @@ __device__ __forceinline__ const uint32_t* mask_row(const Args& a, int b, int t)
 template <int D>
 __host__ __device__ constexpr int64_t part_floats(int rows) { return static_cast<int64_t>(rows) * (D + 2); }
 
+// The form for many rows (fmha_tree_wide.cu): tensor memory, 128 or 256 rows a block.
+int run_wide(const Args& a, int head_dim, int dtype, int block_rows, int64_t groups, int row_blocks, cudaStream_t s);
+
 }  // namespace fmha_tree
 }  // namespace ob

@@ -1,0 +1,499 @@
+// Attention of a tree of drafted tokens over 16-bit pages when many rows share a key head (fmha_tree.cu has the formula, and the form for few
+// rows): tcgen05 products, keys and values by TMA straight out of the pages.
+//
+// A block has 128 or 256 rows of one (sequence, key head) and walks its share of the keys 128 at a time.  Ten warps:
+//   0-3, 4-7  softmax of two streams: a thread owns a row, reads its scores from tensor memory and writes its weights there;
+//   8         issues the products: S = Q K^T into 128 columns of tensor memory per stream, O += P V into D columns per stream;
+//   9         fetches tiles of keys and values: pieces of 16 to 128 rows (whatever power of two divides a page), 128-byte swizzle.
+// The streams are the two halves of 256 rows over the same keys, or the same 128 rows over the even and the odd tiles (kKeys2), put together at
+// the end.  They run half a step apart: while one's softmax works, the tensor cores have the other's products.  Weights take the place of the scores
+// they were made of (16 bits for 32) and are the A operand of the second product from there.  The maximum moves only when a score passes it by 2^8.
+// A piece without a page is fetched from behind the pool, which gives zeros.  In tiles at the ends of the sequence, and among the drafted keys, the
+// values are looked through before their product: those that no row sees become zeros, and so do those that are not finite and that some
+// rows may not see; the rows that do see one get it by hand at the end.
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "device_status.cuh"
+#include "fmha_tree.cuh"
+#include "sm100_ptx.cuh"
+#include "smem_limit.cuh"
+#include "tma_host.cuh"
+
+namespace ob {
+namespace fmha_tree {
+namespace {
+
+constexpr int kMmaWarp = 8, kProducer = 9, kThreads = 320;
+constexpr int kAtom = 128 * 128;   // 128 rows of 128 bytes
+constexpr int kKeys = 128;
+
+// two fp32 operations in one instruction
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <typename T>
+__device__ __forceinline__ bool odd_word(uint32_t w) {   // one of two 16-bit values is not finite
+  constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return (w & kExponent) == kExponent || (w >> 16 & kExponent) == kExponent;
+}
+
+template <int D, bool kKeys2>
+struct Smem {
+  static constexpr int kAtoms = D / 64, kTiles = kKeys2 ? 1 : 2, kSlots = D == 64 ? 8 : kKeys2 ? 6 : 5;
+  static constexpr int kQ = 0, kRing = kQ + kTiles * kAtoms * kAtom, kBars = kRing + kSlots * kAtoms * kAtom;
+  static constexpr int kNumBars = 2 * kSlots + 6;
+  static constexpr int kTotal = kBars + kNumBars * 8 + 32, kDynamic = kTotal + 1024;
+};
+
+template <typename T, int D, bool kKeys2>
+__global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                                                                     const int row_blocks, const int piece_rows, uint32_t* status) {
+  using S = Smem<D, kKeys2>;
+  constexpr int NR = kKeys2 ? 128 : 256;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t kIdescQK = ptx::umma_idesc_f16(kBf16, 128, kKeys, false, false);
+  constexpr uint32_t kIdescPV = ptx::umma_idesc_f16(kBf16, 128, D, false, true);   // V: keys are its rows
+  constexpr uint32_t kColS = 0, kColO = 256, kCols = 512;
+
+  ptx::grid_dep_wait();
+  const int split = static_cast<int>(blockIdx.x) % a.splits, group = static_cast<int>(blockIdx.x) / a.splits, groups = static_cast<int>(gridDim.x) / a.splits;
+  int at = group;
+  const int rb = at % row_blocks;
+  at /= row_blocks;
+  const int hk = at % a.Hkv, b = at / a.Hkv;
+  const int share = a.H / a.Hkv, rows = share * a.Tq, row0 = rb * NR;
+  const Sequence seq(a, b);
+  const int all0 = seq.start / kKeys, all1 = row0 < seq.live * share ? max((seq.end + kKeys - 1) / kKeys, all0) : all0;
+  const int per = (all1 - all0 + a.splits - 1) / a.splits;
+  const int tile0 = min(all0 + split * per, all1), tiles = min(tile0 + per, all1) - tile0;
+  float* const part = a.parts ? a.parts + (static_cast<int64_t>(split) * groups + group) * part_floats<D>(NR) : nullptr;
+  auto out_row = [&](int r) { return static_cast<T*>(a.out) + b * a.os_b + (hk * share + r % share) * a.os_h + static_cast<int64_t>(r / share) * a.os_t; };
+  if (tiles == 0) {   // nothing to see: zero rows
+    for (int i = threadIdx.x; i < min(NR, rows - row0) * (D / 8); i += kThreads) {
+      const int r = i / (D / 8), d = i % (D / 8) * 8;
+      if (part) {
+        if (d == 0) part[2 * r] = kEmpty, part[2 * r + 1] = 0.f;
+        float4* dst = reinterpret_cast<float4*>(part + 2 * NR + r * D + d);
+        dst[0] = dst[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+      } else {
+        *reinterpret_cast<uint4*>(out_row(row0 + r) + d) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    return;
+  }
+  // streams with something in them, and their steps
+  const int streams = kKeys2 ? min(tiles, 2) : (min(rows, seq.live * share) > row0 + 128 ? 2 : 1);
+  auto steps_of = [&](int x) { return kKeys2 ? (tiles - x + 1) / 2 : tiles; };
+  auto tile_of = [&](int x, int j) { return kKeys2 ? 2 * j + x : j; };
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars);
+  uint64_t* empty = full + S::kSlots;
+  uint64_t* s_full = empty + S::kSlots;   // [2]  scores are there (and the output has all weights before)
+  uint64_t* p_full = s_full + 2;          // [2]  weights are there, output is scaled
+  uint64_t* o_done = s_full + 4;          // [2]  output has the weights
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 6);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+  volatile uint32_t* odd_values = tmem_slot + 2;   // a drafted key has a value that is not finite
+  volatile uint32_t* drain_flag = tmem_slot + 3;
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kSlots; ++i) {
+      ptx::mbar_init(&full[i], 1);
+      ptx::mbar_init(&empty[i], 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      ptx::mbar_init(&s_full[x], 1);
+      ptx::mbar_init(&p_full[x], 128);
+      ptx::mbar_init(&o_done[x], 1);
+    }
+    *abort_flag = 0;
+    *odd_values = 0;
+    *drain_flag = 0;
+    ptx::fence_barrier_init();
+  }
+  if (warp == kMmaWarp) {
+    ptx::tmem_alloc(tmem_slot, kCols);
+    ptx::tmem_relinquish();
+  }
+  // queries, with the sign of the scale
+  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+  for (int i = threadIdx.x; i < (kKeys2 ? 1 : streams) * 128 * (D / 8); i += kThreads) {
+    const int r = i / (D / 8), o = i % (D / 8), rr = row0 + r;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (rr < rows)
+      v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.qs_b + (hk * share + rr % share) * a.qs_h +
+                                          static_cast<int64_t>(rr / share) * a.qs_t + o * 8);
+    *reinterpret_cast<uint4*>(smem + S::kQ + ((r >> 7) * S::kAtoms + o / 8) * kAtom + (r & 127) * 128 + ((o & 7) ^ (r & 7)) * 16) =
+        make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+  }
+  ptx::fence_proxy_async_smem();
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  ptx::grid_dep_launch();   // only now: see sm100_ptx.cuh
+
+  const int table_len = static_cast<int>(a.blocks_per_seq), block_size = static_cast<int>(a.block_size);
+  const int32_t* table = a.block_table + b * a.blocks_per_seq;
+  auto page_at = [&](int key) {   // -1: none
+    const int blk = key / block_size;
+    const int page = blk < table_len ? table[blk] : -1;
+    return page < a.num_blocks ? page : -1;
+  };
+  bool ok = true;
+  float m = kEmpty, l = 0.f;
+
+  if (warp == kMmaWarp) {
+    const bool issuer = ptx::elect_one();
+    const uint32_t base = ptx::smem_u32(smem);
+    auto slot_of = [&](int h) { return base + S::kRing + (h % S::kSlots) * S::kAtoms * kAtom; };
+    auto wait = [&](uint64_t* bar, int parity) { return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity & 1, abort_flag)) != 0; };   // the warp stays together
+    auto wait_full = [&](int h) { return wait(&full[h % S::kSlots], h / S::kSlots); };
+    auto scores = [&](int x, int j) {
+      if (!issuer) return;
+      const int h = 2 * tile_of(x, j);
+      const uint64_t ad = ptx::smem_desc_kmajor_sw128(base + S::kQ + (kKeys2 ? 0 : x) * S::kAtoms * kAtom), bd = ptx::smem_desc_kmajor_sw128(slot_of(h));
+#pragma unroll
+      for (int kk = 0; kk < S::kAtoms * 4; ++kk) {
+        const uint32_t off = ((kk / 4) * kAtom + (kk % 4) * 32) >> 4;
+        ptx::umma_f16(tmem + kColS + x * 128, ad + off, bd + off, kIdescQK, kk > 0);
+      }
+      ptx::umma_commit(&s_full[x]);
+      if (kKeys2 || x == streams - 1) ptx::umma_commit(&empty[h % S::kSlots]);
+    };
+    auto output = [&](int x, int j) {
+      if (!issuer) return;
+      const int h = 2 * tile_of(x, j) + 1;
+      const uint64_t bd = ptx::smem_desc_mnmajor_sw128(slot_of(h), kAtom, 1024);
+#pragma unroll
+      for (int kk = 0; kk < kKeys / 16; ++kk)
+        ptx::umma_f16_ts(tmem + kColO + x * 128, tmem + kColS + x * 128 + kk * 8, bd + ((kk * 2048) >> 4), kIdescPV, j > 0 || kk > 0);
+      ptx::umma_commit(&o_done[x]);
+      if (kKeys2 || x == streams - 1) ptx::umma_commit(&empty[h % S::kSlots]);
+    };
+    // the values of a tile that some row may not see as they are
+    auto look_through = [&](int i) {
+      const int key0 = (tile0 + i) * kKeys;
+      if (key0 >= seq.start && key0 + kKeys <= min(seq.prefix, seq.end)) return;
+      uint8_t* slot = smem + S::kRing + ((2 * i + 1) % S::kSlots) * S::kAtoms * kAtom;
+      bool odd = false;
+      for (int p = lane; p < kKeys * S::kAtoms * 8; p += 32) {
+        const int row = p / 8 % kKeys, key = key0 + row;
+        uint4* v = reinterpret_cast<uint4*>(slot + p / 8 * 128 + (p % 8) * 16);   // (the order within a row does not matter here)
+        if (key < seq.start || key >= seq.end) {
+          *v = make_uint4(0, 0, 0, 0);
+        } else if (key >= seq.prefix) {
+          uint32_t w[4] = {v->x, v->y, v->z, v->w};
+          if (odd_word<T>(w[0]) || odd_word<T>(w[1]) || odd_word<T>(w[2]) || odd_word<T>(w[3])) {
+            odd = true;
+            T* e = reinterpret_cast<T*>(v);
+            for (int y = 0; y < 8; ++y)
+              if (!(fabsf(Elem<T>::to_f(e[y])) < INFINITY)) e[y] = Elem<T>::from_f(0.f);
+          }
+        }
+      }
+      if (odd) *odd_values = 1;
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+    };
+    for (int x = 0; ok && x < streams; ++x) {
+      if (kKeys2 || x == 0) ok = wait_full(2 * tile_of(x, 0));
+      if (!ok) break;
+      ptx::tc_fence_after_sync();
+      scores(x, 0);
+    }
+    for (int j = 0; ok && j < steps_of(0); ++j) {
+      for (int x = 0; ok && x < streams; ++x) {
+        if (j >= steps_of(x)) continue;
+        if (kKeys2 || x == 0) {
+          ok = wait_full(2 * tile_of(x, j) + 1);
+          if (!ok) break;
+          look_through(tile_of(x, j));
+        }
+        ok = wait(&p_full[x], j);
+        if (!ok) break;
+        ptx::tc_fence_after_sync();
+        output(x, j);
+        if (j + 1 < steps_of(x)) {
+          if (kKeys2 || x == 0) ok = wait_full(2 * tile_of(x, j + 1));
+          // products into other columns are not bound to stay in order: the weights go only once they are used
+          ok = ok && wait(&o_done[x], j);
+          if (!ok) break;
+          ptx::tc_fence_after_sync();
+          scores(x, j + 1);
+        }
+      }
+    }
+    if (!ok && issuer && status) atomicOr(status, kStatusFmhaMma);
+    __syncwarp();
+  } else if (warp == kProducer) {
+    // lane i fetches piece i / kAtoms of a tile, dims 64 (i % kAtoms) .. of it; pages are asked for a tile ahead
+    const int pieces = kKeys / piece_rows * S::kAtoms, atom = lane % S::kAtoms, first = lane / S::kAtoms * piece_rows;
+    const int no_row = static_cast<int>(a.num_blocks * a.block_size);
+    auto row_at = [&](int i) {
+      const int key = (tile0 + i) * kKeys + first, page = lane < pieces ? page_at(key) : -1;
+      return page >= 0 ? page * block_size + key % block_size : no_row;
+    };
+    const uint32_t dst = atom * kAtom + first * 128;
+    int h = 0, row = row_at(0);
+    for (int i = 0; ok && i < tiles; ++i) {
+      const int here = row;
+      if (i + 1 < tiles) row = row_at(i + 1);
+      for (int v = 0; ok && v < 2; ++v, ++h) {
+        const int s = h % S::kSlots;
+        if (h >= S::kSlots) ok = ptx::mbar_wait(&empty[s], (h / S::kSlots - 1) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) ptx::mbar_expect_tx(&full[s], S::kAtoms * kAtom);
+        __syncwarp();
+        if (lane < pieces) ptx::tma_load_3d(smem + S::kRing + s * S::kAtoms * kAtom + dst, v ? &v_map : &k_map, atom * 64, hk, here, &full[s]);
+      }
+    }
+    // nothing may be on its way when the block ends
+    if (!ok)
+      for (int x = max(h - S::kSlots, 0); x < h; ++x) ptx::mbar_wait(&full[x % S::kSlots], (x / S::kSlots) & 1, drain_flag);
+    if (!ok && lane == 0 && status) atomicOr(status, kStatusFmhaLoad);
+    __syncwarp();
+  } else if (warp / 4 < streams) {
+    // ---- softmax of stream x
+    const int x = warp / 4, r = (warp & 3) * 32 + lane, rr = row0 + (kKeys2 ? 0 : x * 128) + r;
+    const int tq = min(rr / share, a.Tq - 1);
+    const uint32_t* const words = mask_row(a, b, tq);
+    const float unit = fmaxf(fabsf(a.scale_log2), 1.2e-38f);   // a scale of zero leaves masked scores at -inf
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lanes + kColS + x * 128, t_o = tmem + lanes + kColO + x * 128;
+    const int steps = steps_of(x);
+    // bits of the 32 keys from `key` on that the row sees, pages aside
+    auto sees32 = [&](int key) {
+      auto below = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; };   // the first n bits
+      uint32_t bits = below(seq.prefix - key);
+      const int u = key - seq.prefix;   // the first one's node
+      if (u + 32 > 0) {
+        uint32_t tree;
+        if (words == nullptr) {
+          tree = below(tq + 1 - u);
+        } else {
+          const int w = u >> 5, off = u & 31;
+          const uint32_t lo = w >= 0 && w < a.mask_words ? words[w] : 0u, hi = off && w + 1 >= 0 && w + 1 < a.mask_words ? words[w + 1] : 0u;
+          tree = __funnelshift_r(lo, hi, off);
+        }
+        bits |= tree & below(seq.live - u) & ~below(-u);
+      }
+      return bits & below(seq.end - key) & ~below(seq.start - key);
+    };
+    for (int j = 0; j < steps; ++j) {
+      const int key0 = (tile0 + tile_of(x, j)) * kKeys;
+      // 16 keys a bit: those with a page.  (A piece without one has keys of zero, whose scores are no less than others.)
+      const uint32_t pages = __ballot_sync(0xffffffffu, lane < 8 && page_at(key0 + lane * 16) >= 0);
+      const bool whole = pages == 0xffu && key0 >= seq.start && key0 + kKeys <= min(seq.prefix, seq.end);
+      uint32_t seen[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+      if (!whole) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          seen[w] = sees32(key0 + 32 * w) & ((pages >> (2 * w) & 1u ? 0xffffu : 0u) | (pages >> (2 * w + 1) & 1u ? 0xffff0000u : 0u));
+      }
+      ok = ptx::mbar_wait(&s_full[x], j & 1, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      ptx::tc_fence_after_sync();
+      uint32_t v[2][64];
+      ptx::tmem_ld_32x64(t_s, v[0]);
+      ptx::tmem_ld_32x64(t_s + 64, v[1]);
+      ptx::tmem_ld_wait();
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < 128; ++i)
+          if (!(seen[i / 32] >> (i % 32) & 1u)) v[i / 64][i % 64] = 0xff800000u;
+      }
+      float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < 128; ++i) t[i & 3] = fmaxf(t[i & 3], __uint_as_float(v[i / 64][i % 64]));
+      const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * unit;
+      const bool raise = top > m + 8.f;
+      if (__any_sync(0xffffffffu, raise)) {
+        const float f = raise ? ex2(m - top) : 1.f;
+        m = raise ? top : m;
+        l *= f;
+        if (j > 0) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += 16) {
+            uint32_t o[16];
+            ptx::tmem_ld_32x16(t_o + c0, o);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            ptx::tmem_st_32x16(t_o + c0, o);
+          }
+        }
+      }
+      const uint64_t unit2 = pair(unit, unit), minus_m = pair(-m, -m);
+      uint64_t s0 = 0, s1 = 0;   // sums of two at a time
+#pragma unroll
+      for (int c0 = 0; c0 < kKeys; c0 += 32) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float2 e = unpair(fma2(pair(__uint_as_float(v[(c0 + i) / 64][(c0 + i) % 64]), __uint_as_float(v[(c0 + i) / 64][(c0 + i + 1) % 64])), unit2, minus_m));
+          const float p0 = ex2(e.x), p1 = ex2(e.y);
+          (i & 2 ? s1 : s0) = add2(i & 2 ? s1 : s0, pair(p0, p1));
+          packed[i / 2] = pack2<T>(p0, p1);
+        }
+        ptx::tmem_st_32x16(t_s + c0 / 2, packed);   // all of the row's scores are read
+      }
+      const float2 both = unpair(add2(s0, s1));
+      l += both.x + both.y;
+      ptx::tmem_st_wait();
+      ptx::tc_fence_before_sync();
+      ptx::mbar_arrive(&p_full[x]);
+    }
+    if (ok) ok = ptx::mbar_wait(&o_done[x], (steps - 1) & 1, abort_flag);
+    ok = __all_sync(0xffffffffu, ok);
+    ptx::tc_fence_after_sync();
+    if (!ok && lane == 0 && status) atomicOr(status, kStatusFmhaSoftmax);
+  }
+  __syncthreads();
+  const bool done = *abort_flag == 0;
+  float* const other = reinterpret_cast<float*>(smem + S::kRing);   // kKeys2: the second stream's output, dims outside, then maxima and sums
+  if (kKeys2 && streams == 2) {
+    if (warp >= 4 && warp < 8) {
+      const int r = (warp & 3) * 32 + lane;
+      const uint32_t t_o = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + kColO + 128;
+#pragma unroll 1
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t v[32];
+        ptx::tmem_ld_32x32(t_o + c0, v);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) other[(c0 + i) * 128 + r] = __uint_as_float(v[i]);
+      }
+      other[D * 128 + r] = m;
+      other[D * 128 + 128 + r] = l;
+    }
+    __syncthreads();
+  }
+  if (warp < (kKeys2 ? 4 : 8) && row0 + (kKeys2 ? 0 : (warp / 4) * 128) < rows) {
+    const int x = warp / 4, r = x * 128 + (warp & 3) * 32 + lane, rr = row0 + r;
+    const bool there = rr < rows, valid = there && rr / share < seq.live && x < streams && done;
+    float f0 = 1.f, f1 = 0.f;
+    if (kKeys2 && streams == 2) {
+      const float m1 = other[D * 128 + r], top = fmaxf(m, m1);
+      f0 = ex2(m - top), f1 = ex2(m1 - top);
+      m = top;
+      l = fmaf(f0, l, f1 * other[D * 128 + 128 + r]);
+    }
+    const uint32_t t_o = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + kColO + x * 128;
+    const float inv = !valid ? 0.f : part ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;   // NaN stays
+    if (part && there) part[2 * r] = valid ? m : kEmpty, part[2 * r + 1] = valid ? l : 0.f;
+    const bool by_hand = *odd_values && valid;
+    T* out = out_row(there ? rr : 0);
+#pragma unroll 1
+    for (int c0 = 0; c0 < D; c0 += 32) {
+      uint32_t v[32];
+      float y[32];
+      if (x < streams && done) {   // uniform in the warp
+        ptx::tmem_ld_32x32(t_o + c0, v);
+        ptx::tmem_ld_wait();
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        y[i] = __uint_as_float(v[i]);
+        if (kKeys2 && streams == 2) y[i] = fmaf(f0, y[i], f1 * other[(c0 + i) * 128 + r]);
+        y[i] = valid ? y[i] * inv : 0.f;
+      }
+      if (by_hand) {
+        const int tq = rr / share;
+        const uint32_t* const words = mask_row(a, b, tq);
+        const int k0 = max(max(seq.prefix, seq.start), tile0 * kKeys), k1 = min(seq.end, (tile0 + tiles) * kKeys);
+        for (int key = k0; key < k1; ++key) {
+          const int page = page_at(key);
+          if (page < 0 || !sees(a, words, tq, key - seq.prefix, seq.live)) continue;
+          const T* vs = static_cast<const T*>(a.v) + ((static_cast<int64_t>(page) * block_size + key % block_size) * a.Hkv + hk) * D + c0;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float e = Elem<T>::to_f(vs[i]);
+            if (!(fabsf(e) < INFINITY)) y[i] += e;
+          }
+        }
+      }
+      if (!there) continue;
+      if (part) {
+        float4* dst = reinterpret_cast<float4*>(part + 2 * NR + r * D + c0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dst[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint4*>(out + c0 + 8 * i) = make_uint4(pack2<T>(y[8 * i], y[8 * i + 1]), pack2<T>(y[8 * i + 2], y[8 * i + 3]),
+                                                                   pack2<T>(y[8 * i + 4], y[8 * i + 5]), pack2<T>(y[8 * i + 6], y[8 * i + 7]));
+      }
+    }
+    ptx::tc_fence_before_sync();
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) ptx::tmem_dealloc(tmem, kCols);
+}
+
+template <typename T, int D, bool kKeys2>
+int launch(const Args& a, int dtype, int64_t groups, int row_blocks, cudaStream_t s) {
+  using S = Smem<D, kKeys2>;
+  static SmemLimit limit;
+  const cudaError_t e = limit.raise(fmha_tree_wide_kernel<T, D, kKeys2>, S::kDynamic);
+  if (e != cudaSuccess) return set_error(OASR_ERR_CUDA, "fmha_tree: shared memory limit: %s", cudaGetErrorString(e));
+  int piece = 16;
+  while (piece < 128 && a.block_size % (2 * piece) == 0) piece *= 2;
+  // (64 dims of a head, head, row of the pool)
+  const uint64_t dims[3] = {static_cast<uint64_t>(D), static_cast<uint64_t>(a.Hkv), static_cast<uint64_t>(a.num_blocks * a.block_size)};
+  const uint64_t strides[3] = {2, static_cast<uint64_t>(D) * 2, static_cast<uint64_t>(a.Hkv) * D * 2};
+  const uint32_t box[3] = {64, 1, static_cast<uint32_t>(piece)};
+  CUtensorMap k_map, v_map;
+  int rc = make_tensor_map(&k_map, tma_dtype(dtype), 3, a.k, dims, strides, box);
+  if (rc == OASR_OK) rc = make_tensor_map(&v_map, tma_dtype(dtype), 3, a.v, dims, strides, box);
+  if (rc != OASR_OK) return rc;
+  launch_pdl(fmha_tree_wide_kernel<T, D, kKeys2>, dim3(static_cast<unsigned>(groups * a.splits)), dim3(kThreads), S::kDynamic, s, a, k_map, v_map, row_blocks, piece,
+             device_status_ptr());
+  return check_launch("fmha_tree launch");
+}
+
+}  // namespace
+
+int run_wide(const Args& a, int head_dim, int dtype, int block_rows, int64_t groups, int row_blocks, cudaStream_t s) {
+  return OB_DISPATCH_HALF(dtype, T_, [&]() -> int {
+    if (head_dim == 64) return block_rows == 128 ? launch<T_, 64, true>(a, dtype, groups, row_blocks, s) : launch<T_, 64, false>(a, dtype, groups, row_blocks, s);
+    return block_rows == 128 ? launch<T_, 128, true>(a, dtype, groups, row_blocks, s) : launch<T_, 128, false>(a, dtype, groups, row_blocks, s);
+  });
+}
+
+}  // namespace fmha_tree
+}  // namespace ob

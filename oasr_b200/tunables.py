@@ -12,6 +12,8 @@ per (stream, head), or inside the Conformer's step of few streams a block that a
 128-row tcgen05 kernel behind a page write (fp8 pages: the warp-per-(stream, head) form behind one).
 ``fmha_q4_path``: attention over 4-bit pages - 0 (default) chooses by size, 1 always the few-row kernel, 2 always the tcgen05
 kernel of long chunks.
+``fmha_tree_path``: attention of drafted tokens over 16-bit pages - 0 (default) chooses by size, 1 always the few-row kernel, 2 always
+the tcgen05 kernel of many rows.
 ``fmha_relpos_path``: 1 (default) runs packed relative-position attention on the two-CTAs-per-SM kernel, 0 on the general one.
 ``conv1_mma``: 1 (default) runs the first subsampling convolution (parity-split output, 256 / 512 channels) as a K = 32
 split-bf16 GEMM on the tensor cores, 0 as the fp32 stencil kernel.

@@ -41,10 +41,11 @@ def test_fmha_tree(how, code):
 
 def test_fmha_tree_workspace():
     need = _lib.load().oasr_b200_fmha_tree_workspace_bytes
-    assert need(1, 8, 8, 1, 64, 4, 16) == 0                       # a short cache is not split
-    assert need(1, 8, 2, 5, 128, 4096, 16) > 0
+    assert need(1, 8, 8, 1, 64, 4, 16, 4) == 0                       # a short cache is not split
+    assert need(1, 8, 2, 5, 128, 4096, 16, 4096) > 0
     for bad in [(0, 8, 8, 1, 64, 4096, 16), (1, 8, 3, 1, 64, 4096, 16), (1, 8, 8, 1, 96, 4096, 16), (1, 8, 8, 0, 64, 4096, 16), (1, 8, 0, 1, 64, 4096, 16), (1, 8, 8, 1, 64, 4096, 0)]:
-        assert need(*bad) == 0
+        assert need(*bad, 4096) == 0
+    refused("set_tunable", (b"fmha_tree_path", 3), -1)
 
 
 def verify(**how):

@@ -61,6 +61,14 @@ def test_draft_tree_of_nothing():
 
 
 # ---- attention ----------------------------------------------------------------------------------------------------------
+@pytest.fixture(params=[0, 1, 2], ids=["by_size", "few_rows", "many_rows"])
+def tree_form(request):
+    """Both kernels of fmha_tree, and the choice between them."""
+    ob.tunables.set("fmha_tree_path", request.param)
+    yield request.param
+    ob.tunables.set("fmha_tree_path", 0)
+
+
 def pool16(seed, n, block, Hkv, D, dt):
     return [rand(seed + i, n, block, Hkv, D).to(dt).cuda() for i in range(2)]
 
@@ -120,7 +128,7 @@ CASES = [  # B, H, Hkv, T, D, block, lens, starts, q_lens, width
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("B,H,Hkv,T,D,block,lens,starts,q_lens,width", CASES)
-def test_fmha_tree(dtype, B, H, Hkv, T, D, block, lens, starts, q_lens, width):
+def test_fmha_tree(tree_form, dtype, B, H, Hkv, T, D, block, lens, starts, q_lens, width):
     dt = DTYPES[dtype]
     bt, n = pages(3, B, -(-max(max(lens), 1) // block) + 1)
     pools = pool16(10, n, block, Hkv, D, dt)
@@ -151,7 +159,7 @@ def test_fmha_tree(dtype, B, H, Hkv, T, D, block, lens, starts, q_lens, width):
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("T,D,share", [(1, 64, 2), (6, 128, 4), (20, 64, 2), (70, 128, 4)])
-def test_fmha_tree_unseen_keys_say_nothing(dtype, T, D, share):
+def test_fmha_tree_unseen_keys_say_nothing(tree_form, dtype, T, D, share):
     """NaN and infinities behind the length and before the start, pages outside the pool, a table wider than the length, rows that see nothing."""
     dt, block = DTYPES[dtype], 16
     lens, starts = [100 + T, 77 + T, T], [5, 2, 0]
@@ -177,7 +185,7 @@ def test_fmha_tree_unseen_keys_say_nothing(dtype, T, D, share):
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("T,D,share", [(3, 64, 1), (12, 128, 4), (40, 64, 2), (70, 128, 4)])
-def test_fmha_tree_nan_reaches_the_rows_that_see_it_and_no_other(dtype, T, D, share):
+def test_fmha_tree_nan_reaches_the_rows_that_see_it_and_no_other(tree_form, dtype, T, D, share):
     dt, block, N = DTYPES[dtype], 16, T + 90
     bt, n = pages(3, 1, -(-N // block))
     pools = pool16(10, n, block, 2, D, dt)
@@ -210,7 +218,7 @@ def test_fmha_tree_nan_reaches_the_rows_that_see_it_and_no_other(dtype, T, D, sh
 
 @pytest.mark.parametrize("T", [1, 5, 40, 70])
 @pytest.mark.parametrize("D", [64, 128])
-def test_fmha_tree_of_scores_of_any_size(T, D):
+def test_fmha_tree_of_scores_of_any_size(tree_form, T, D):
     """One key with all the weight, equal weights, a scale of zero and one below it."""
     N = 200 + T
     bt, n = pages(3, 1, 20)
@@ -225,7 +233,7 @@ def test_fmha_tree_of_scores_of_any_size(T, D):
         check(got, want, bound(x, k, scale, size, want, torch.bfloat16) + size_of * 1e-3 * (size_of > 1) * v.abs().max())
 
 
-def test_fmha_tree_lengths_outside_the_table():
+def test_fmha_tree_lengths_outside_the_table(tree_form):
     """Lengths below zero, below the tree's, and of more than the table has; 64-bit tables and lengths."""
     T, D = 4, 64
     bt, n = pages(3, 4, 3)
@@ -255,7 +263,7 @@ def test_fmha_tree_lengths_outside_the_table():
     assert torch.equal(got64[same.cuda()], got[same.cuda()])
 
 
-def test_fmha_tree_takes_any_query_view():
+def test_fmha_tree_takes_any_query_view(tree_form):
     T, D = 6, 64
     bt, n = pages(3, 2, 8)
     pools = pool16(10, n, 16, 2, D, torch.bfloat16)
@@ -272,7 +280,7 @@ def test_fmha_tree_takes_any_query_view():
                        ob.fmha_tree(one.contiguous(), *pools, softmax_scale=0.125, block_table=bt[:1].cuda(), cache_seqlens=i32([50])))
 
 
-def test_fmha_tree_far_pages():
+def test_fmha_tree_far_pages(tree_form):
     """Rows behind 2^31 elements of a pool."""
     Hkv, D, block, n = 8, 128, 128, 16500                      # 2.16e9 elements a pool
     pools = [torch.zeros(n, block, Hkv, D, dtype=torch.float16, device="cuda") for _ in range(2)]
