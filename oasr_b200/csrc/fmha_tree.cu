@@ -385,37 +385,58 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? (NT == 4 ? 3 : 4) : 2) 
   }
 }
 
-// Joins the partial results of a group's blocks: a warp per row, 32 rows of `NR` to a group.
-template <typename T, int D>
+// Joins the partial results of a group's blocks: `kWays` warps a row, each with its share of the parts (one warp alone took 20 us for 74 of them).
+template <typename T, int D, int kWays>
 __global__ void __launch_bounds__(256) fmha_tree_join_kernel(const Args a, const int row_blocks, const int NR, const int groups) {
+  constexpr int kRows = 8 / kWays, kV = D / 32;
+  __shared__ float tops[8], sums[8], outs[8][D];
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int64_t group = item / NR;
-  if (group >= groups) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, way = warp % kWays;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * kRows + warp / kWays, group = item / NR;
   const int n = static_cast<int>(item - group * NR), rb = static_cast<int>(group % row_blocks), at = static_cast<int>(group / row_blocks);
   const int hk = at % a.Hkv, b = at / a.Hkv, share = a.H / a.Hkv, r = rb * NR + n;
-  if (r >= share * a.Tq) return;
+  const bool there = group < groups && r < share * a.Tq;
   const int64_t part = part_floats<D>(NR), step = part * groups;
   const float* src = a.parts + group * part;
-  float top = kEmpty;
-  for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, src[s * step + 2 * n]);
-  top = warp_max(top);
-  constexpr int kV = D / 32;
-  float sum = 0.f, acc[kV] = {};
+  float top = kEmpty, sum = 0.f, acc[kV] = {};
+  if (there) {
+    for (int s = way + lane * kWays; s < a.splits; s += 32 * kWays) top = fmaxf(top, src[s * step + 2 * n]);
+    top = warp_max(top);
 #pragma unroll 4
-  for (int s = 0; s < a.splits; ++s) {
-    const float* p = src + s * step;
-    const float2 ml = *reinterpret_cast<const float2*>(p + 2 * n);
-    const float f = ex2(ml.x - top);
-    float v[kV];
+    for (int s = way; s < a.splits; s += kWays) {
+      const float* p = src + s * step;
+      const float2 ml = *reinterpret_cast<const float2*>(p + 2 * n);
+      const float f = ex2(ml.x - top);
+      float v[kV];
 #pragma unroll
-    for (int x = 0; x < kV; ++x) v[x] = p[2 * NR + n * D + lane * kV + x];
-    sum = fmaf(f, ml.y, sum);
+      for (int x = 0; x < kV; ++x) v[x] = p[2 * NR + n * D + lane * kV + x];
+      sum = fmaf(f, ml.y, sum);
 #pragma unroll
-    for (int x = 0; x < kV; ++x) acc[x] = fmaf(f, v[x], acc[x]);
+      for (int x = 0; x < kV; ++x) acc[x] = fmaf(f, v[x], acc[x]);
+    }
   }
+  if constexpr (kWays > 1) {
+    if (lane == 0) tops[warp] = top, sums[warp] = sum;
+#pragma unroll
+    for (int x = 0; x < kV; ++x) outs[warp][lane * kV + x] = acc[x];
+    __syncthreads();
+    if (way) return;
+#pragma unroll
+    for (int w = 1; w < kWays; ++w) top = fmaxf(top, tops[warp + w]);
+    const float own = ex2(tops[warp] - top);
+    sum *= own;
+#pragma unroll
+    for (int x = 0; x < kV; ++x) acc[x] *= own;
+#pragma unroll
+    for (int w = 1; w < kWays; ++w) {
+      const float f = ex2(tops[warp + w] - top);
+      sum = fmaf(f, sums[warp + w], sum);
+#pragma unroll
+      for (int x = 0; x < kV; ++x) acc[x] = fmaf(f, outs[warp + w][lane * kV + x], acc[x]);
+    }
+  }
+  if (!there) return;
   const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;   // NaN stays
   const int tq = r / share, live = a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq;
   T* out = static_cast<T*>(a.out) + b * a.os_b + (hk * share + r - tq * share) * a.os_h + static_cast<int64_t>(tq) * a.os_t + lane * kV;
@@ -469,8 +490,12 @@ template <typename T, int D>
 int run(const Args& a, const Plan& p, int dtype, cudaStream_t s) {
   const int rc = p.wide ? run_wide(a, D, dtype, p.rows, p.groups, p.row_blocks, s) : p.rows == 8 ? launch<T, D, 1>(a, p, s) : p.rows == 16 ? launch<T, D, 2>(a, p, s) : launch<T, D, 4>(a, p, s);
   if (rc != OASR_OK || p.splits == 1) return rc;
-  launch_pdl(fmha_tree_join_kernel<T, D>, dim3(static_cast<unsigned>((p.groups * p.rows + 7) / 8)), dim3(256), 0, s, a, p.row_blocks, p.rows,
-             static_cast<int>(p.groups));
+  const int64_t rows = p.groups * p.rows;
+  const auto join = [&](auto kern, int ways) {
+    launch_pdl(kern, dim3(static_cast<unsigned>((rows * ways + 7) / 8)), dim3(256), 0, s, a, p.row_blocks, p.rows, static_cast<int>(p.groups));
+  };
+  if (p.splits <= 4) join(fmha_tree_join_kernel<T, D, 1>, 1);
+  else join(fmha_tree_join_kernel<T, D, 8>, 8);
   return check_launch("fmha_tree join launch");
 }
 

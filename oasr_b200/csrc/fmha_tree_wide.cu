@@ -1,10 +1,11 @@
 // Attention of a tree of drafted tokens over 16-bit pages when many rows share a key head (fmha_tree.cu has the formula, and the form for few
 // rows): tcgen05 products, keys and values by TMA straight out of the pages.
 //
-// A block has 128 or 256 rows of one (sequence, key head) and walks its share of the keys 128 at a time.  Ten warps:
-//   0-3, 4-7  softmax of two streams: a thread owns a row, reads its scores from tensor memory and writes its weights there;
-//   8         issues the products: S = Q K^T into 128 columns of tensor memory per stream, O += P V into D columns per stream;
-//   9         fetches tiles of keys and values: pieces of 16 to 128 rows (whatever power of two divides a page), 128-byte swizzle.
+// A block has 128 or 256 rows of one (sequence, key head) and walks its share of the keys 128 at a time.  18 warps:
+//   0-7, 8-15 softmax of two streams: two threads to a row, each with 64 of a step's keys: they read their scores from tensor memory and write
+//             weights there;
+//   16        issues the products: S = Q K^T into 128 columns of tensor memory per stream, O += P V into D columns per stream;
+//   17        fetches tiles of keys and values: pieces of 16 to 128 rows (whatever power of two divides a page), 128-byte swizzle.
 // The streams are the two halves of 256 rows over the same keys, or the same 128 rows over the even and the odd tiles (kKeys2), put together at
 // the end.  They run half a step apart: while one's softmax works, the tensor cores have the other's products.  Weights take the place of the scores
 // they were made of (16 bits for 32) and are the A operand of the second product from there.  The maximum moves only when a score passes it by 2^8.
@@ -26,7 +27,7 @@ namespace ob {
 namespace fmha_tree {
 namespace {
 
-constexpr int kMmaWarp = 8, kProducer = 9, kThreads = 320;
+constexpr int kMmaWarp = 16, kProducer = 17, kThreads = 576;
 constexpr int kAtom = 128 * 128;   // 128 rows of 128 bytes
 constexpr int kKeys = 128;
 
@@ -67,12 +68,29 @@ __device__ __forceinline__ bool odd_word(uint32_t w) {   // one of two 16-bit va
   return (w & kExponent) == kExponent || (w >> 16 & kExponent) == kExponent;
 }
 
+// Barrier of a stream's 256 threads: whether any of them says yes.
+__device__ __forceinline__ bool any_of_stream(int x, bool yes) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %1, 0;\n\t"
+      "bar.red.or.pred p, %2, 256, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(any)
+      : "r"(yes ? 1u : 0u), "r"(x + 1)
+      : "memory");
+  return any != 0;
+}
+
 template <int D, bool kKeys2>
 struct Smem {
   static constexpr int kAtoms = D / 64, kTiles = kKeys2 ? 1 : 2, kSlots = D == 64 ? 8 : kKeys2 ? 6 : 5;
   static constexpr int kQ = 0, kRing = kQ + kTiles * kAtoms * kAtom, kBars = kRing + kSlots * kAtoms * kAtom;
   static constexpr int kNumBars = 2 * kSlots + 6;
-  static constexpr int kTotal = kBars + kNumBars * 8 + 32, kDynamic = kTotal + 1024;
+  static constexpr int kTops = kBars + kNumBars * 8 + 32, kTotal = kTops + 2 * 128 * 4, kDynamic = kTotal + 1024;
+  static_assert(kDynamic <= 232448, "what a block may have");
 };
 
 template <typename T, int D, bool kKeys2>
@@ -136,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
     }
     for (int x = 0; x < 2; ++x) {
       ptx::mbar_init(&s_full[x], 1);
-      ptx::mbar_init(&p_full[x], 128);
+      ptx::mbar_init(&p_full[x], 256);
       ptx::mbar_init(&o_done[x], 1);
     }
     *abort_flag = 0;
@@ -287,14 +305,15 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
       for (int x = max(h - S::kSlots, 0); x < h; ++x) ptx::mbar_wait(&full[x % S::kSlots], (x / S::kSlots) & 1, drain_flag);
     if (!ok && lane == 0 && status) atomicOr(status, kStatusFmhaLoad);
     __syncwarp();
-  } else if (warp / 4 < streams) {
-    // ---- softmax of stream x
-    const int x = warp / 4, r = (warp & 3) * 32 + lane, rr = row0 + (kKeys2 ? 0 : x * 128) + r;
+  } else if (warp / 8 < streams) {
+    // ---- softmax of stream x, keys 64 half .. of each step
+    const int x = warp / 8, half = warp >> 2 & 1, r = (warp & 3) * 32 + lane, rr = row0 + (kKeys2 ? 0 : x * 128) + r;
     const int tq = min(rr / share, a.Tq - 1);
     const uint32_t* const words = mask_row(a, b, tq);
     const float unit = fmaxf(fabsf(a.scale_log2), 1.2e-38f);   // a scale of zero leaves masked scores at -inf
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lanes + kColS + x * 128, t_o = tmem + lanes + kColO + x * 128;
+    const uint32_t t_s = tmem + lanes + kColS + x * 128, t_o = tmem + lanes + kColO + x * 128 + half * (D / 2);
+    float* const row_top = reinterpret_cast<float*>(smem + S::kTops) + x * 128 + r;
     const int steps = steps_of(x);
     // bits of the 32 keys from `key` on that the row sees, pages aside
     auto sees32 = [&](int key) {
@@ -314,41 +333,48 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
       }
       return bits & below(seq.end - key) & ~below(seq.start - key);
     };
+    // (Where a wait is given up the walk goes on with whatever is there: all warps of a stream meet at every barrier.)
     for (int j = 0; j < steps; ++j) {
-      const int key0 = (tile0 + tile_of(x, j)) * kKeys;
+      const int key0 = (tile0 + tile_of(x, j)) * kKeys + half * 64;
       // 16 keys a bit: those with a page.  (A piece without one has keys of zero, whose scores are no less than others.)
-      const uint32_t pages = __ballot_sync(0xffffffffu, lane < 8 && page_at(key0 + lane * 16) >= 0);
-      const bool whole = pages == 0xffu && key0 >= seq.start && key0 + kKeys <= min(seq.prefix, seq.end);
-      uint32_t seen[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+      const uint32_t pages = __ballot_sync(0xffffffffu, lane < 4 && page_at(key0 + lane * 16) >= 0);
+      const bool whole = pages == 0xfu && key0 >= seq.start && key0 + 64 <= min(seq.prefix, seq.end);
+      uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
       if (!whole) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int w = 0; w < 2; ++w)
           seen[w] = sees32(key0 + 32 * w) & ((pages >> (2 * w) & 1u ? 0xffffu : 0u) | (pages >> (2 * w + 1) & 1u ? 0xffff0000u : 0u));
       }
-      ok = ptx::mbar_wait(&s_full[x], j & 1, abort_flag);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      ok &= __all_sync(0xffffffffu, ptx::mbar_wait(&s_full[x], j & 1, abort_flag)) != 0;
       ptx::tc_fence_after_sync();
-      uint32_t v[2][64];
-      ptx::tmem_ld_32x64(t_s, v[0]);
-      ptx::tmem_ld_32x64(t_s + 64, v[1]);
+      uint32_t v[64];
+      ptx::tmem_ld_32x64(t_s + half * 64, v);
       ptx::tmem_ld_wait();
       if (!whole) {
 #pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (!(seen[i / 32] >> (i % 32) & 1u)) v[i / 64][i % 64] = 0xff800000u;
+        for (int i = 0; i < 64; ++i)
+          if (!(seen[i / 32] >> (i % 32) & 1u)) v[i] = 0xff800000u;
       }
       float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 128; ++i) t[i & 3] = fmaxf(t[i & 3], __uint_as_float(v[i / 64][i % 64]));
+      for (int i = 0; i < 64; ++i) t[i & 3] = fmaxf(t[i & 3], __uint_as_float(v[i]));
       const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * unit;
-      const bool raise = top > m + 8.f;
-      if (__any_sync(0xffffffffu, raise)) {
-        const float f = raise ? ex2(m - top) : 1.f;
-        m = raise ? top : m;
+      ptx::tc_fence_before_sync();
+      if (any_of_stream(x, top > m + 8.f)) {   // (also: all scores are read, and weights may take their place)
+        float both = top;   // of the row: there and back between its two threads
+        if (half) *row_top = top;
+        ptx::named_barrier_sync(x + 1, 256);
+        if (!half) *row_top = both = fmaxf(top, *row_top);
+        ptx::named_barrier_sync(x + 1, 256);
+        if (half) both = *row_top;
+        const bool raise = both > m + 8.f;
+        const float f = raise ? ex2(m - both) : 1.f;
+        m = raise ? both : m;
         l *= f;
         if (j > 0) {
+          ptx::tc_fence_after_sync();
 #pragma unroll 1
-          for (int c0 = 0; c0 < D; c0 += 16) {
+          for (int c0 = 0; c0 < D / 2; c0 += 16) {
             uint32_t o[16];
             ptx::tmem_ld_32x16(t_o + c0, o);
             ptx::tmem_ld_wait();
@@ -358,19 +384,20 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
           }
         }
       }
+      ptx::tc_fence_after_sync();
       const uint64_t unit2 = pair(unit, unit), minus_m = pair(-m, -m);
       uint64_t s0 = 0, s1 = 0;   // sums of two at a time
 #pragma unroll
-      for (int c0 = 0; c0 < kKeys; c0 += 32) {
+      for (int c0 = 0; c0 < 64; c0 += 32) {
         uint32_t packed[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          const float2 e = unpair(fma2(pair(__uint_as_float(v[(c0 + i) / 64][(c0 + i) % 64]), __uint_as_float(v[(c0 + i) / 64][(c0 + i + 1) % 64])), unit2, minus_m));
+          const float2 e = unpair(fma2(pair(__uint_as_float(v[c0 + i]), __uint_as_float(v[c0 + i + 1])), unit2, minus_m));
           const float p0 = ex2(e.x), p1 = ex2(e.y);
           (i & 2 ? s1 : s0) = add2(i & 2 ? s1 : s0, pair(p0, p1));
           packed[i / 2] = pack2<T>(p0, p1);
         }
-        ptx::tmem_st_32x16(t_s + c0 / 2, packed);   // all of the row's scores are read
+        ptx::tmem_st_32x16(t_s + half * 32 + c0 / 2, packed);
       }
       const float2 both = unpair(add2(s0, s1));
       l += both.x + both.y;
@@ -378,48 +405,51 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
       ptx::tc_fence_before_sync();
       ptx::mbar_arrive(&p_full[x]);
     }
-    if (ok) ok = ptx::mbar_wait(&o_done[x], (steps - 1) & 1, abort_flag);
-    ok = __all_sync(0xffffffffu, ok);
+    ok &= __all_sync(0xffffffffu, ptx::mbar_wait(&o_done[x], (steps - 1) & 1, abort_flag)) != 0;
     ptx::tc_fence_after_sync();
     if (!ok && lane == 0 && status) atomicOr(status, kStatusFmhaSoftmax);
   }
   __syncthreads();
   const bool done = *abort_flag == 0;
-  float* const other = reinterpret_cast<float*>(smem + S::kRing);   // kKeys2: the second stream's output, dims outside, then maxima and sums
-  if (kKeys2 && streams == 2) {
-    if (warp >= 4 && warp < 8) {
-      const int r = (warp & 3) * 32 + lane;
-      const uint32_t t_o = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + kColO + 128;
+  // the ring is free: sums of both halves of a row; kKeys2: the second stream's maxima and output, dims outside
+  float* const sums = reinterpret_cast<float*>(smem + S::kRing);
+  float* const other_m = sums + 512;
+  float* const other = other_m + 128;
+  if (warp < 16) {
+    const int x = warp / 8, half = warp >> 2 & 1, r = (warp & 3) * 32 + lane;
+    sums[(x * 2 + half) * 128 + r] = l;
+    if (kKeys2 && x == 1 && streams == 2) {
+      const uint32_t t_o = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + kColO + 128 + half * (D / 2);
 #pragma unroll 1
-      for (int c0 = 0; c0 < D; c0 += 32) {
+      for (int c0 = 0; c0 < D / 2; c0 += 32) {
         uint32_t v[32];
         ptx::tmem_ld_32x32(t_o + c0, v);
         ptx::tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) other[(c0 + i) * 128 + r] = __uint_as_float(v[i]);
+        for (int i = 0; i < 32; ++i) other[(half * (D / 2) + c0 + i) * 128 + r] = __uint_as_float(v[i]);
       }
-      other[D * 128 + r] = m;
-      other[D * 128 + 128 + r] = l;
+      if (half == 0) other_m[r] = m;
     }
-    __syncthreads();
   }
-  if (warp < (kKeys2 ? 4 : 8) && row0 + (kKeys2 ? 0 : (warp / 4) * 128) < rows) {
-    const int x = warp / 4, r = x * 128 + (warp & 3) * 32 + lane, rr = row0 + r;
+  __syncthreads();
+  if (warp < (kKeys2 ? 8 : 16) && row0 + (kKeys2 ? 0 : (warp / 8) * 128) < rows) {
+    const int x = warp / 8, half = warp >> 2 & 1, rs = (warp & 3) * 32 + lane, r = x * 128 + rs, rr = row0 + r;
     const bool there = rr < rows, valid = there && rr / share < seq.live && x < streams && done;
+    l = sums[x * 256 + rs] + sums[x * 256 + 128 + rs];
     float f0 = 1.f, f1 = 0.f;
     if (kKeys2 && streams == 2) {
-      const float m1 = other[D * 128 + r], top = fmaxf(m, m1);
-      f0 = ex2(m - top), f1 = ex2(m1 - top);
+      const float top = fmaxf(m, other_m[rs]);
+      f0 = ex2(m - top), f1 = ex2(other_m[rs] - top);
       m = top;
-      l = fmaf(f0, l, f1 * other[D * 128 + 128 + r]);
+      l = fmaf(f0, l, f1 * (sums[256 + rs] + sums[384 + rs]));
     }
     const uint32_t t_o = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + kColO + x * 128;
     const float inv = !valid ? 0.f : part ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;   // NaN stays
-    if (part && there) part[2 * r] = valid ? m : kEmpty, part[2 * r + 1] = valid ? l : 0.f;
+    if (part && there && half == 0) part[2 * r] = valid ? m : kEmpty, part[2 * r + 1] = valid ? l : 0.f;
     const bool by_hand = *odd_values && valid;
     T* out = out_row(there ? rr : 0);
 #pragma unroll 1
-    for (int c0 = 0; c0 < D; c0 += 32) {
+    for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
       uint32_t v[32];
       float y[32];
       if (x < streams && done) {   // uniform in the warp
@@ -429,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         y[i] = __uint_as_float(v[i]);
-        if (kKeys2 && streams == 2) y[i] = fmaf(f0, y[i], f1 * other[(c0 + i) * 128 + r]);
+        if (kKeys2 && streams == 2) y[i] = fmaf(f0, y[i], f1 * other[(c0 + i) * 128 + rs]);
         y[i] = valid ? y[i] * inv : 0.f;
       }
       if (by_hand) {
