@@ -1,17 +1,18 @@
 // Attention of a tree of drafted tokens over 16-bit pages when many rows share a key head (fmha_tree.cu has the formula, and the form for few
 // rows): tcgen05 products, keys and values by TMA straight out of the pages.
 //
-// A block has 128 or 256 rows of one (sequence, key head) and walks its share of the keys 128 at a time.  18 warps:
+// A block has 128 or 256 rows of one (sequence, key head) and walks its share of the keys 128 at a time.  19 warps:
 //   0-7, 8-15 softmax of two streams: two threads to a row, each with 64 of a step's keys: they read their scores from tensor memory and write
 //             weights there;
-//   16        issues the products: S = Q K^T into 128 columns of tensor memory per stream, O += P V into D columns per stream;
+//   16        one thread issues the products: S = Q K^T into 128 columns of tensor memory per stream, O += P V into D columns per stream
+//             (a whole warp that waits and votes together took 5.1k clocks a step for 2.7k of products);
+//   18        looks through the values of tiles at the ends of the sequence and among the drafted keys before their product;
 //   17        fetches tiles of keys and values: pieces of 16 to 128 rows (whatever power of two divides a page), 128-byte swizzle.
 // The streams are the two halves of 256 rows over the same keys, or the same 128 rows over the even and the odd tiles (kKeys2), put together at
 // the end.  They run half a step apart: while one's softmax works, the tensor cores have the other's products.  Weights take the place of the scores
 // they were made of (16 bits for 32) and are the A operand of the second product from there.  The maximum moves only when a score passes it by 2^8.
-// A piece without a page is fetched from behind the pool, which gives zeros.  In tiles at the ends of the sequence, and among the drafted keys, the
-// values are looked through before their product: those that no row sees become zeros, and so do those that are not finite and that some
-// rows may not see; the rows that do see one get it by hand at the end.
+// A piece without a page is fetched from behind the pool, which gives zeros.  Values that no row sees become zeros as they are looked through, and
+// so do those that are not finite and that some rows may not see; the rows that do see one get it by hand at the end.
 #include <cuda.h>
 
 #include <type_traits>
@@ -27,7 +28,7 @@ namespace ob {
 namespace fmha_tree {
 namespace {
 
-constexpr int kMmaWarp = 16, kProducer = 17, kThreads = 576;
+constexpr int kMmaWarp = 16, kProducer = 17, kReader = 18, kThreads = 608;
 constexpr int kAtom = 128 * 128;   // 128 rows of 128 bytes
 constexpr int kKeys = 128;
 
@@ -68,18 +69,18 @@ __device__ __forceinline__ bool odd_word(uint32_t w) {   // one of two 16-bit va
   return (w & kExponent) == kExponent || (w >> 16 & kExponent) == kExponent;
 }
 
-// Barrier of a stream's 256 threads: whether any of them says yes.
-__device__ __forceinline__ bool any_of_stream(int x, bool yes) {
+// Barrier of the two warps that share 32 rows: whether any of them says yes.
+__device__ __forceinline__ bool any_of_rows(int id, bool yes) {
   uint32_t any;
   asm volatile(
       "{\n\t"
       ".reg .pred p, q;\n\t"
       "setp.ne.u32 q, %1, 0;\n\t"
-      "bar.red.or.pred p, %2, 256, q;\n\t"
+      "bar.red.or.pred p, %2, 64, q;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t"
       "}\n"
       : "=r"(any)
-      : "r"(yes ? 1u : 0u), "r"(x + 1)
+      : "r"(yes ? 1u : 0u), "r"(id)
       : "memory");
   return any != 0;
 }
@@ -88,7 +89,7 @@ template <int D, bool kKeys2>
 struct Smem {
   static constexpr int kAtoms = D / 64, kTiles = kKeys2 ? 1 : 2, kSlots = D == 64 ? 8 : kKeys2 ? 6 : 5;
   static constexpr int kQ = 0, kRing = kQ + kTiles * kAtoms * kAtom, kBars = kRing + kSlots * kAtoms * kAtom;
-  static constexpr int kNumBars = 2 * kSlots + 6;
+  static constexpr int kNumBars = 3 * kSlots + 6;
   static constexpr int kTops = kBars + kNumBars * 8 + 32, kTotal = kTops + 2 * 128 * 4, kDynamic = kTotal + 1024;
   static_assert(kDynamic <= 232448, "what a block may have");
 };
@@ -141,7 +142,8 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
   uint64_t* s_full = empty + S::kSlots;   // [2]  scores are there (and the output has all weights before)
   uint64_t* p_full = s_full + 2;          // [2]  weights are there, output is scaled
   uint64_t* o_done = s_full + 4;          // [2]  output has the weights
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 6);
+  uint64_t* looked = s_full + 6;          // [kSlots]  values are there and looked through
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(looked + S::kSlots);
   volatile uint32_t* abort_flag = tmem_slot + 1;
   volatile uint32_t* odd_values = tmem_slot + 2;   // a drafted key has a value that is not finite
   volatile uint32_t* drain_flag = tmem_slot + 3;
@@ -151,6 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
     for (int i = 0; i < S::kSlots; ++i) {
       ptx::mbar_init(&full[i], 1);
       ptx::mbar_init(&empty[i], 1);
+      ptx::mbar_init(&looked[i], 1);
     }
     for (int x = 0; x < 2; ++x) {
       ptx::mbar_init(&s_full[x], 1);
@@ -194,48 +197,86 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
   bool ok = true;
   float m = kEmpty, l = 0.f;
 
+  // which use of its slot for values item h is
+  auto value_use = [](int h) { return S::kSlots % 2 ? h / S::kSlots / 2 : h / S::kSlots; };
+  // whether tile i has values that some row may not see as they are
+  auto partial = [&](int i) {
+    const int key0 = (tile0 + i) * kKeys;
+    return key0 < seq.start || key0 + kKeys > min(seq.prefix, seq.end);
+  };
   if (warp == kMmaWarp) {
-    const bool issuer = ptx::elect_one();
-    const uint32_t base = ptx::smem_u32(smem);
-    auto slot_of = [&](int h) { return base + S::kRing + (h % S::kSlots) * S::kAtoms * kAtom; };
-    auto wait = [&](uint64_t* bar, int parity) { return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity & 1, abort_flag)) != 0; };   // the warp stays together
-    auto wait_full = [&](int h) { return wait(&full[h % S::kSlots], h / S::kSlots); };
-    auto scores = [&](int x, int j) {
-      if (!issuer) return;
-      const int h = 2 * tile_of(x, j);
-      const uint64_t ad = ptx::smem_desc_kmajor_sw128(base + S::kQ + (kKeys2 ? 0 : x) * S::kAtoms * kAtom), bd = ptx::smem_desc_kmajor_sw128(slot_of(h));
+    if (ptx::elect_one()) {
+      const uint32_t base = ptx::smem_u32(smem);
+      auto slot_of = [&](int h) { return base + S::kRing + (h % S::kSlots) * S::kAtoms * kAtom; };
+      auto wait_full = [&](int h) { return ptx::mbar_wait(&full[h % S::kSlots], (h / S::kSlots) & 1, abort_flag); };
+      // (a slot has keys and values in turn where their number is odd, and one kind where it is even)
+      auto wait_looked = [&](int h) { return ptx::mbar_wait(&looked[h % S::kSlots], value_use(h) & 1, abort_flag); };
+      auto scores = [&](int x, int h) {
+        const uint64_t ad = ptx::smem_desc_kmajor_sw128(base + S::kQ + (kKeys2 ? 0 : x) * S::kAtoms * kAtom), bd = ptx::smem_desc_kmajor_sw128(slot_of(h));
 #pragma unroll
-      for (int kk = 0; kk < S::kAtoms * 4; ++kk) {
-        const uint32_t off = ((kk / 4) * kAtom + (kk % 4) * 32) >> 4;
-        ptx::umma_f16(tmem + kColS + x * 128, ad + off, bd + off, kIdescQK, kk > 0);
+        for (int kk = 0; kk < S::kAtoms * 4; ++kk) {
+          const uint32_t off = ((kk / 4) * kAtom + (kk % 4) * 32) >> 4;
+          ptx::umma_f16(tmem + kColS + x * 128, ad + off, bd + off, kIdescQK, kk > 0);
+        }
+        ptx::umma_commit(&s_full[x]);
+        if (kKeys2 || x == streams - 1) ptx::umma_commit(&empty[h % S::kSlots]);
+      };
+      auto output = [&](int x, int h, bool more) {
+        const uint64_t bd = ptx::smem_desc_mnmajor_sw128(slot_of(h), kAtom, 1024);
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+          ptx::umma_f16_ts(tmem + kColO + x * 128, tmem + kColS + x * 128 + kk * 8, bd + ((kk * 2048) >> 4), kIdescPV, more || kk > 0);
+        ptx::umma_commit(&o_done[x]);
+        if (kKeys2 || x == streams - 1) ptx::umma_commit(&empty[h % S::kSlots]);
+      };
+      for (int x = 0; ok && x < streams; ++x) {
+        const int h = 2 * tile_of(x, 0);
+        if (kKeys2 || x == 0) ok = wait_full(h);
+        if (!ok) break;
+        ptx::tc_fence_after_sync();
+        scores(x, h);
       }
-      ptx::umma_commit(&s_full[x]);
-      if (kKeys2 || x == streams - 1) ptx::umma_commit(&empty[h % S::kSlots]);
-    };
-    auto output = [&](int x, int j) {
-      if (!issuer) return;
-      const int h = 2 * tile_of(x, j) + 1;
-      const uint64_t bd = ptx::smem_desc_mnmajor_sw128(slot_of(h), kAtom, 1024);
-#pragma unroll
-      for (int kk = 0; kk < kKeys / 16; ++kk)
-        ptx::umma_f16_ts(tmem + kColO + x * 128, tmem + kColS + x * 128 + kk * 8, bd + ((kk * 2048) >> 4), kIdescPV, j > 0 || kk > 0);
-      ptx::umma_commit(&o_done[x]);
-      if (kKeys2 || x == streams - 1) ptx::umma_commit(&empty[h % S::kSlots]);
-    };
-    // the values of a tile that some row may not see as they are
-    auto look_through = [&](int i) {
-      const int key0 = (tile0 + i) * kKeys;
-      if (key0 >= seq.start && key0 + kKeys <= min(seq.prefix, seq.end)) return;
-      uint8_t* slot = smem + S::kRing + ((2 * i + 1) % S::kSlots) * S::kAtoms * kAtom;
+      const int steps = steps_of(0);
+      for (int j = 0; ok && j < steps; ++j) {
+        for (int x = 0; ok && x < streams; ++x) {
+          const int i = tile_of(x, j), next = tile_of(x, j + 1);
+          if (i >= tiles) continue;
+          if (kKeys2 || x == 0) ok = wait_looked(2 * i + 1);
+          ok = ok && ptx::mbar_wait(&p_full[x], j & 1, abort_flag);
+          if (!ok) break;
+          ptx::tc_fence_after_sync();
+          output(x, 2 * i + 1, j > 0);
+          if (next >= tiles) continue;
+          if (kKeys2 || x == 0) ok = wait_full(2 * next);
+          // products into other columns are not bound to stay in order: the weights go only once they are used
+          ok = ok && ptx::mbar_wait(&o_done[x], j & 1, abort_flag);
+          if (!ok) break;
+          ptx::tc_fence_after_sync();
+          scores(x, 2 * next);
+        }
+      }
+      if (!ok && status) atomicOr(status, kStatusFmhaMma);
+    }
+    __syncwarp();
+  } else if (warp == kReader) {
+    for (int i = 0; ok && i < tiles; ++i) {
+      const int h = 2 * i + 1, key0 = (tile0 + i) * kKeys;
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(&full[h % S::kSlots], (h / S::kSlots) & 1, abort_flag)) != 0;
+      if (!ok) break;
+      if (!partial(i)) {
+        if (lane == 0) ptx::mbar_arrive(&looked[h % S::kSlots]);
+        continue;
+      }
+      uint8_t* slot = smem + S::kRing + (h % S::kSlots) * S::kAtoms * kAtom;
       bool odd = false;
       for (int p = lane; p < kKeys * S::kAtoms * 8; p += 32) {
-        const int row = p / 8 % kKeys, key = key0 + row;
-        uint4* v = reinterpret_cast<uint4*>(slot + p / 8 * 128 + (p % 8) * 16);   // (the order within a row does not matter here)
+        const int key = key0 + p / 8 % kKeys;
+        uint4* v = reinterpret_cast<uint4*>(slot + p * 16);   // (the order within a row does not matter here)
         if (key < seq.start || key >= seq.end) {
           *v = make_uint4(0, 0, 0, 0);
         } else if (key >= seq.prefix) {
-          uint32_t w[4] = {v->x, v->y, v->z, v->w};
-          if (odd_word<T>(w[0]) || odd_word<T>(w[1]) || odd_word<T>(w[2]) || odd_word<T>(w[3])) {
+          const uint4 w = *v;
+          if (odd_word<T>(w.x) || odd_word<T>(w.y) || odd_word<T>(w.z) || odd_word<T>(w.w)) {
             odd = true;
             T* e = reinterpret_cast<T*>(v);
             for (int y = 0; y < 8; ++y)
@@ -246,36 +287,9 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
       if (odd) *odd_values = 1;
       ptx::fence_proxy_async_smem();
       __syncwarp();
-    };
-    for (int x = 0; ok && x < streams; ++x) {
-      if (kKeys2 || x == 0) ok = wait_full(2 * tile_of(x, 0));
-      if (!ok) break;
-      ptx::tc_fence_after_sync();
-      scores(x, 0);
+      if (lane == 0) ptx::mbar_arrive(&looked[h % S::kSlots]);
     }
-    for (int j = 0; ok && j < steps_of(0); ++j) {
-      for (int x = 0; ok && x < streams; ++x) {
-        if (j >= steps_of(x)) continue;
-        if (kKeys2 || x == 0) {
-          ok = wait_full(2 * tile_of(x, j) + 1);
-          if (!ok) break;
-          look_through(tile_of(x, j));
-        }
-        ok = wait(&p_full[x], j);
-        if (!ok) break;
-        ptx::tc_fence_after_sync();
-        output(x, j);
-        if (j + 1 < steps_of(x)) {
-          if (kKeys2 || x == 0) ok = wait_full(2 * tile_of(x, j + 1));
-          // products into other columns are not bound to stay in order: the weights go only once they are used
-          ok = ok && wait(&o_done[x], j);
-          if (!ok) break;
-          ptx::tc_fence_after_sync();
-          scores(x, j + 1);
-        }
-      }
-    }
-    if (!ok && issuer && status) atomicOr(status, kStatusFmhaMma);
+    if (!ok && lane == 0 && status) atomicOr(status, kStatusFmhaLoad);
     __syncwarp();
   } else if (warp == kProducer) {
     // lane i fetches piece i / kAtoms of a tile, dims 64 (i % kAtoms) .. of it; pages are asked for a tile ahead
@@ -314,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + lanes + kColS + x * 128, t_o = tmem + lanes + kColO + x * 128 + half * (D / 2);
     float* const row_top = reinterpret_cast<float*>(smem + S::kTops) + x * 128 + r;
-    const int steps = steps_of(x);
+    const int steps = steps_of(x), rows_id = 1 + x * 4 + (warp & 3);
     // bits of the 32 keys from `key` on that the row sees, pages aside
     auto sees32 = [&](int key) {
       auto below = [](int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; };   // the first n bits
@@ -333,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
       }
       return bits & below(seq.end - key) & ~below(seq.start - key);
     };
-    // (Where a wait is given up the walk goes on with whatever is there: all warps of a stream meet at every barrier.)
+    // (Where a wait is given up the walk goes on with whatever is there: both warps of the rows meet at every barrier.)
     for (int j = 0; j < steps; ++j) {
       const int key0 = (tile0 + tile_of(x, j)) * kKeys + half * 64;
       // 16 keys a bit: those with a page.  (A piece without one has keys of zero, whose scores are no less than others.)
@@ -360,12 +374,12 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
       for (int i = 0; i < 64; ++i) t[i & 3] = fmaxf(t[i & 3], __uint_as_float(v[i]));
       const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * unit;
       ptx::tc_fence_before_sync();
-      if (any_of_stream(x, top > m + 8.f)) {   // (also: all scores are read, and weights may take their place)
+      if (any_of_rows(rows_id, top > m + 8.f)) {   // (also: all scores of these rows are read, and weights may take their place)
         float both = top;   // of the row: there and back between its two threads
         if (half) *row_top = top;
-        ptx::named_barrier_sync(x + 1, 256);
+        ptx::named_barrier_sync(rows_id, 64);
         if (!half) *row_top = both = fmaxf(top, *row_top);
-        ptx::named_barrier_sync(x + 1, 256);
+        ptx::named_barrier_sync(rows_id, 64);
         if (half) both = *row_top;
         const bool raise = both > m + 8.f;
         const float f = raise ? ex2(m - both) : 1.f;
@@ -393,9 +407,9 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           const float2 e = unpair(fma2(pair(__uint_as_float(v[c0 + i]), __uint_as_float(v[c0 + i + 1])), unit2, minus_m));
-          const float p0 = ex2(e.x), p1 = ex2(e.y);
-          (i & 2 ? s1 : s0) = add2(i & 2 ? s1 : s0, pair(p0, p1));
-          packed[i / 2] = pack2<T>(p0, p1);
+          const float2 w = make_float2(ex2(e.x), ex2(e.y));
+          (i & 2 ? s1 : s0) = add2(i & 2 ? s1 : s0, pair(w.x, w.y));
+          packed[i / 2] = pack2<T>(w.x, w.y);
         }
         ptx::tmem_st_32x16(t_s + half * 32 + c0 / 2, packed);
       }
