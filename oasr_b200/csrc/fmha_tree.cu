@@ -75,32 +75,33 @@ __device__ __forceinline__ void copies_but() {   // all but the last N groups of
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-constexpr int kWarps = 4, kKeys = 16;
+constexpr int kKeys = 16;
 
 // A tile of 16 keys in the ring, K then V; the 16-byte pieces of row r lie at piece ^ (r & 7).
-template <int D>
+template <int D, int kWarps>
 struct Ring {
-  static constexpr int kRow = 2 * D, kHalf = kKeys * kRow, kBytes = 2 * kHalf, kStages = D == 64 ? 4 : 3;
+  static constexpr int kRow = 2 * D, kHalf = kKeys * kRow, kBytes = 2 * kHalf, kStages = D == 64 && kWarps == 4 ? 4 : 3;
   static __device__ __forceinline__ int at(int row, int piece) { return row * kRow + ((piece ^ (row & 7)) << 4); }
 };
 
-template <int D, int NT>
+template <int D, int NT, int kWarps>
 struct Merge {   // the warps' maxima, sums and outputs
   float m[kWarps][8 * NT], l[kWarps][8 * NT];
   float o[kWarps][8 * NT][D + 4];
 };
 
-template <int D, int NT>
+template <int D, int NT, int kWarps>
 struct Smem {
-  static constexpr int kRings = kWarps * Ring<D>::kStages * Ring<D>::kBytes;
+  static constexpr int kRings = kWarps * Ring<D, kWarps>::kStages * Ring<D, kWarps>::kBytes;
   static constexpr int kQ = NT == 4 ? 8 * NT * 2 * D : 0;   // 32 rows of queries are too many for registers
-  static constexpr int kMerge = sizeof(Merge<D, NT>);
+  static constexpr int kMerge = sizeof(Merge<D, NT, kWarps>);
   static constexpr int kBytes = (kRings > kMerge ? kRings : kMerge) + kQ;
 };
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, D == 64 ? (NT == 4 ? 3 : 4) : 2) fmha_tree_kernel(const Args a, const int row_blocks) {
-  using R = Ring<D>;
+template <typename T, int D, int NT, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, D == 128 ? 8 / kWarps : kWarps == 8 ? 2 : NT == 4 ? 3 : 4) fmha_tree_kernel(const Args a, const int row_blocks) {
+  using R = Ring<D, kWarps>;
+  using S = Smem<D, NT, kWarps>;
   constexpr int NR = 8 * NT, KD = D / 16;   // rows; steps of 16 dims
   extern __shared__ __align__(128) uint8_t smem[];
   ptx::grid_dep_launch();
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? (NT == 4 ? 3 : 4) : 2) 
   const float unit = fmaxf(fabsf(a.scale_log2), 1.2e-38f);   // a scale of zero leaves masked scores at -inf
   auto q_row = [&](int r) { return static_cast<const T*>(a.q) + b * a.qs_b + (hk * share + r % share) * a.qs_h + static_cast<int64_t>(r / share) * a.qs_t; };
   uint32_t qf[NT == 4 ? 1 : NT][NT == 4 ? 1 : KD][2];
-  const uint32_t q_smem = ptx::smem_u32(smem) + (Smem<D, NT>::kBytes - Smem<D, NT>::kQ);
+  const uint32_t q_smem = ptx::smem_u32(smem) + (S::kBytes - S::kQ);
   if constexpr (NT < 4) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? (NT == 4 ? 3 : 4) : 2) 
       const int r = i / kPieces, p = i % kPieces;
       uint4 v = make_uint4(0, 0, 0, 0);
       if (row0 + r < rows) v = reinterpret_cast<const uint4*>(q_row(row0 + r))[p];
-      *reinterpret_cast<uint4*>(smem + (Smem<D, NT>::kBytes - Smem<D, NT>::kQ) + R::at(r, p)) = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+      *reinterpret_cast<uint4*>(smem + (S::kBytes - S::kQ) + R::at(r, p)) = make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
     }
     __syncthreads();
   }
@@ -229,18 +230,28 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? (NT == 4 ? 3 : 4) : 2) 
     }
     bool odd = false;
     if (!whole) {
+      // the rows' bits of the tile's 16 keys; all words are asked for before the first is looked at
+      const int u = j0 - seq.prefix, w = u >> 5, off = u & 31;
+      auto first = [](int n) { return n >= 16 ? 0xffffu : n <= 0 ? 0u : (1u << n) - 1; };
+      const uint32_t in = known ? first(seq.end - j0) & ~first(seq.start - j0) : 0u, before = first(-u), live = first(seq.live - u) & ~before;
+      uint32_t lo[NT][2], hi[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int r = row0 + n * 8 + 2 * t + c, tq = min(r / share, a.Tq - 1);
+          const int tq = min((row0 + n * 8 + 2 * t + c) / share, a.Tq - 1);
           const uint32_t* words = mask_row(a, b, tq);
+          lo[n][c] = words ? (w >= 0 && w < a.mask_words ? words[w] : 0u) : first(tq + 1 - u);
+          hi[n][c] = words && w + 1 >= 0 && w + 1 < a.mask_words ? words[w + 1] : 0u;
+        }
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int j = j0 + g + 8 * x;
-            const bool seen = known && j >= seq.start && j < seq.end && (j < seq.prefix || sees(a, words, tq, j - seq.prefix, seq.live));
-            if (!seen) s[n][2 * x + c] = -INFINITY;
-          }
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t tree = a.mask ? __funnelshift_r(lo[n][c], hi[n][c], off) : lo[n][c], seen = ((tree & live) | before) & in;
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            if (!(seen >> (g + 8 * x) & 1u)) s[n][2 * x + c] = -INFINITY;
         }
       // Values that no row sees are zeros, as a weight of zero does not undo a NaN.
 #pragma unroll 1
@@ -338,7 +349,8 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? (NT == 4 ? 3 : 4) : 2) 
   copies_but<0>();
 
   // ---- the warps meet
-  Merge<D, NT>& sh = *reinterpret_cast<Merge<D, NT>*>(smem);
+  using M = Merge<D, NT, kWarps>;
+  M& sh = *reinterpret_cast<M*>(smem);
   __syncthreads();   // the rings are done with
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -448,10 +460,13 @@ struct Plan {
   int rows, row_blocks, splits;   // rows of a block; blocks of rows of a (sequence, key head); blocks that share a cache
   int64_t groups;
   bool wide;
+  int warps;   // of a block of the few-row form
 };
 
-// How a call is cut.  Blocks that share a cache: until the SMs are full, as long as each of a block's warps has four tiles.  The block table's width
-// stands for the lengths, which are on the GPU.
+// How a call is cut.  An SM holds 16 warps of the few-row form at 64 dims and 8 at 128: eight to a block as long as all blocks fit, else four
+// (37 trees of 21 over up to 1001 keys, 8 heads of 64: 18.7 us with four).  Blocks that share a cache: until the SMs are full, as long as each warp has
+// four tiles, and if that saves more than the second kernel costs, some 6 us, at 0.4 us a tile (the same trees in two parts: 24 us).  The
+// block table's width stands for the lengths, which are on the GPU.
 Plan plan(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t D, int64_t keys, int64_t pool_rows) {
   Plan p;
   const int64_t rows = H / Hkv * Tq;
@@ -469,21 +484,28 @@ Plan plan(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t D, int64_t keys
   p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
   p.row_blocks = static_cast<int>((rows + p.rows - 1) / p.rows);
   p.groups = B * Hkv * p.row_blocks;
-  const int64_t slots = sm_count() * (D == 64 ? 4 : 2), most = keys / (kWarps * kKeys * 4);
-  int64_t s = (slots + p.groups - 1) / (p.groups > 0 ? p.groups : 1);
-  if (p.groups > slots / 2) s = 1;
+  const int64_t warps = sm_count() * (D == 64 ? 16 : 8);
+  p.warps = p.groups * 8 <= warps ? 8 : 4;
+  const int64_t slots = warps / p.warps, most = keys / (p.warps * kKeys * 4);
+  int64_t s = p.groups > 0 ? slots / p.groups : 1;
   s = s < most ? s : most;
+  if (keys * (s - 1) < 16 * p.warps * 16 * s) s = 1;
   p.splits = static_cast<int>(s < 1 ? 1 : s > 256 ? 256 : s);
   return p;
 }
 
+template <typename T, int D, int NT, int kWarps>
+int launch(const Args& a, const Plan& p, cudaStream_t s) {
+  using S = Smem<D, NT, kWarps>;
+  static SmemLimit limit;
+  const cudaError_t e = limit.raise(fmha_tree_kernel<T, D, NT, kWarps>, S::kBytes);
+  if (e != cudaSuccess) return set_error(OASR_ERR_CUDA, "fmha_tree: shared memory limit: %s", cudaGetErrorString(e));
+  launch_pdl(fmha_tree_kernel<T, D, NT, kWarps>, dim3(static_cast<unsigned>(p.groups * p.splits)), dim3(kWarps * 32), S::kBytes, s, a, p.row_blocks);
+  return check_launch("fmha_tree launch");
+}
 template <typename T, int D, int NT>
 int launch(const Args& a, const Plan& p, cudaStream_t s) {
-  static SmemLimit limit;
-  const cudaError_t e = limit.raise(fmha_tree_kernel<T, D, NT>, Smem<D, NT>::kBytes);
-  if (e != cudaSuccess) return set_error(OASR_ERR_CUDA, "fmha_tree: shared memory limit: %s", cudaGetErrorString(e));
-  launch_pdl(fmha_tree_kernel<T, D, NT>, dim3(static_cast<unsigned>(p.groups * p.splits)), dim3(kWarps * 32), Smem<D, NT>::kBytes, s, a, p.row_blocks);
-  return check_launch("fmha_tree launch");
+  return p.warps == 8 ? launch<T, D, NT, 8>(a, p, s) : launch<T, D, NT, 4>(a, p, s);
 }
 
 template <typename T, int D>
