@@ -165,12 +165,14 @@ struct Range<float> {
   static constexpr float kLeast = -FLT_MAX;
   float lo, top = -INFINITY;
   __device__ __forceinline__ explicit Range(float l) : lo(l) {}
-  __device__ __forceinline__ void take(Vec<float>& x) {
+  __device__ __forceinline__ void note(const Vec<float>& x) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(x[i]));
-      x[i] = fmaxf(x[i], lo);
-    }
+    for (int i = 0; i < kVec; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(x[i]));
+  }
+  __device__ __forceinline__ void take(Vec<float>& x) {
+    note(x);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) x[i] = fmaxf(x[i], lo);
   }
   __device__ __forceinline__ float largest() const { return top; }
 };
@@ -181,11 +183,15 @@ struct Range16 {
     lo.x = lo.y = Elem<T>::from_f(l);
     top.x = top.y = Elem<T>::from_f(-INFINITY);
   }
+  __device__ __forceinline__ void note(const Vec<T>& x) {
+#pragma unroll
+    for (int i = 0; i < kVec; i += 2) top = __hmax2_nan(top, *reinterpret_cast<const T2*>(&x[i]));
+  }
   __device__ __forceinline__ void take(Vec<T>& x) {
+    note(x);
 #pragma unroll
     for (int i = 0; i < kVec; i += 2) {
       T2& v = *reinterpret_cast<T2*>(&x[i]);
-      top = __hmax2_nan(top, v);
       v = __hmax2(v, lo);
     }
   }
@@ -237,19 +243,24 @@ struct Row {
       for (int i = 0; i < kVec; ++i) x[i] = v0 + i >= 0 && v0 + i < V ? q[v0 + i] : 0.f;
     }
   }
-  // f(j, logits) for this lane's vectors j0 + lane, j0 + lane + 32, ... below j1, two loads ahead
-  template <typename F>
+  // f(j, logits) for this lane's vectors j0 + lane, j0 + lane + 32, ... below j1, kBatch loads at a time
+  template <int kBatch, typename F>
   __device__ __forceinline__ void each(int j0, int j1, F&& f) const {
     int j = j0 + static_cast<int>(threadIdx.x & 31);
-    Vec<T> now{}, next{};
-    if (j < j1) now = load(j);
-    if (j + 32 < j1) next = load(j + 32);
 #pragma unroll 1
-    for (; j < j1; j += 32) {
-      Vec<T> after = next;
-      if (j + 64 < j1) after = load(j + 64);
-      f(j, now);
-      now = next, next = after;
+    for (; j + 32 * (kBatch - 1) < j1; j += 32 * kBatch) {
+      Vec<T> x[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) x[i] = load(j + 32 * i);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) f(j + 32 * i, x[i]);
+    }
+    if constexpr (kBatch > 1) {
+#pragma unroll 1
+      for (; j < j1; j += 32) {
+        Vec<T> x = load(j);
+        f(j, x);
+      }
     }
   }
 };
@@ -263,7 +274,7 @@ template <typename T>
 __device__ __noinline__ double sum_near(const Row<T> row, const Weigher weigh, const int j0, const int j1) {
   double s0 = 0., s1 = 0.;
   Range<T> range(weigh.lo);
-  row.each(j0, j1, [&](int, Vec<T>& x) {
+  row.template each<2>(j0, j1, [&](int, Vec<T>& x) {
     range.take(x);
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
@@ -274,6 +285,25 @@ __device__ __noinline__ double sum_near(const Row<T> row, const Weigher weigh, c
     }
   });
   return range.largest() <= weigh.hi ? s0 + s1 : NAN;
+}
+
+// The same in fp32, 4 instructions a logit in the place of 20.  |log2(weight)| stays below 127, so its product and its factor are off by 2^-17.4 and
+// 2^-17.4 at most, the exponential by 2^-22, sums of 16 in a row by 2^-20: kSlack holds them all.
+constexpr double kSlack = 0x1p-15;
+template <typename T>
+__device__ __noinline__ float sum_fast(const Row<T> row, const float rate, const float hi, const int j0, const int j1) {
+  float s[4] = {};
+  Range<T> range(-INFINITY);
+  row.template each<2>(j0, j1, [&](int, const Vec<T>& x) {
+    range.note(x);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      float e;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x(i) * rate));
+      s[i & 3] += e;
+    }
+  });
+  return range.largest() <= hi ? (s[0] + s[1]) + (s[2] + s[3]) : NAN;
 }
 
 // the largest logit (NaN: there is one) and its first token
@@ -291,7 +321,7 @@ struct Largest {
 template <typename T>
 __device__ __noinline__ Largest largest_of(const Row<T> row, const int j0, const int j1) {
   Largest best{-INFINITY, 0x7fffffff};
-  row.each(j0, j1, [&](int j, const Vec<T>& x) {
+  row.template each<1>(j0, j1, [&](int j, const Vec<T>& x) {
 #pragma unroll
     for (int i = 0; i < kVec; ++i) best.take(x(i), row.first(j) + i);
   });
@@ -299,10 +329,9 @@ __device__ __noinline__ Largest largest_of(const Row<T> row, const int j0, const
   return best;
 }
 
-// What is left of eight tokens' weights: max(w inv - beta q, 0), with beta 0 w.
+// What is left of eight tokens' weights: max(w inv - beta y, 0) with y the draft's probabilities, with beta 0 w.
 template <typename T>
-__device__ __forceinline__ void remaining(const Row<T>& row, const Weigher& weigh, const int j, const Vec<T>& x, const float* q, double inv, double beta,
-                                          double (&w)[kVec]) {
+__device__ __forceinline__ void remaining(const Weigher& weigh, const Vec<T>& x, const float (&y)[kVec], double inv, double beta, double (&w)[kVec]) {
   if (weigh.centered) {
 #pragma unroll
     for (int i = 0; i < kVec; ++i) w[i] = weigh.near_zero(fmaxf(x(i), weigh.lo));
@@ -311,8 +340,6 @@ __device__ __forceinline__ void remaining(const Row<T>& row, const Weigher& weig
     for (int i = 0; i < kVec; ++i) w[i] = weigh(x(i));
   }
   if (beta > 0.) {
-    float y[kVec];
-    row.load_probs(q, j, y);
 #pragma unroll
     for (int i = 0; i < kVec; ++i) w[i] = fma(w[i], inv, -beta * static_cast<double>(y[i]));
   }
@@ -324,11 +351,15 @@ __device__ __forceinline__ void remaining(const Row<T>& row, const Weigher& weig
 template <typename T>
 __device__ __noinline__ double sum_remaining(const Row<T> row, const Weigher weigh, const int j0, const int j1, const float* q, const double inv, const double beta) {
   double s = 0.;
-  row.each(j0, j1, [&](int j, const Vec<T>& x) {
+#pragma unroll 1
+  for (int j = j0 + static_cast<int>(threadIdx.x & 31); j < j1; j += 32) {
+    const Vec<T> x = row.load(j);
+    float y[kVec] = {};
+    if (beta > 0.) row.load_probs(q, j, y);
     double w[kVec];
-    remaining(row, weigh, j, x, q, inv, beta, w);
+    remaining(weigh, x, y, inv, beta, w);
     s += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-  });
+  }
   return s;
 }
 
@@ -343,18 +374,17 @@ __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, co
   int* const sibling = first_kid + a.T;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = C > 1 ? static_cast<int>(ptx::cluster_ctarank()) : 0, b = static_cast<int>(blockIdx.x) / C;
-  if (threadIdx.x < kTable) {
-    const double v = __longlong_as_double(g_table.e[threadIdx.x]);
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i) sh.table[threadIdx.x][(threadIdx.x + i) % kCopies] = v;
-  }
+  const uint64_t entry = g_table.e[threadIdx.x % kTable];   // (stored once the tree's loads are on their way)
   if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // waited for before the first word to another block
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
-  const int slots = C * kWarps, mine = warp * C + rank;   // in the order of the vocabulary: few runs are dealt to all blocks
+  const int slots = C * kWarps, slot_bits = __ffs(slots) - 1, mine = warp * C + rank;   // in the order of the vocabulary: few runs are dealt to all blocks
   auto row_of = [&](int n) { return Row<T>(static_cast<const T*>(a.logits) + b * a.ls_b + n * a.ls_n, a.V); };
-  auto run_of = [&](const Row<T>& row, int& per, int& j0, int& j1) {
-    per = max((row.vectors() + slots - 1) / slots, 32), j0 = min(mine * per, row.vectors()), j1 = min(j0 + per, row.vectors());
+  // A row's vectors in units of 32, as evenly over the warps as units go: the first `more` have one above `each`.
+  auto run_of = [&](const Row<T>& row, int& each, int& more, int& j0, int& j1) {
+    const int units = (row.vectors() + 31) >> 5;
+    each = units >> slot_bits, more = units & (slots - 1);
+    j0 = min((mine * each + min(mine, more)) * 32, row.vectors()), j1 = min(j0 + (each + (mine < more)) * 32, row.vectors());
   };
   // elements [e0, e1) of a row of V, towards the L2 cache
   auto ahead = [&](const auto* p, int e0, int e1) {
@@ -364,8 +394,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, co
   };
   {
     const Row<T> row = row_of(0);
-    int per, j0, j1;
-    run_of(row, per, j0, j1);
+    int each, more, j0, j1;
+    run_of(row, each, more, j0, j1);
     ahead(row.p, row.first(j0), row.first(j1));
   }
   for (int i = threadIdx.x; i < a.T; i += kWarps * 32) {
@@ -374,6 +404,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, co
     u[i] = a.uniforms[static_cast<int64_t>(b) * a.T + i];
   }
   const float temperature = a.temperatures ? a.temperatures[b] : a.temperature;
+#pragma unroll
+  for (int i = 0; i < kCopies / 2; ++i)
+    sh.table[threadIdx.x % kTable][(threadIdx.x + i) % (kCopies / 2) + threadIdx.x / kTable * (kCopies / 2)] = __longlong_as_double(entry);
+  static_assert(kWarps * 32 == 2 * kTable, "half of the copies a thread");
   const bool greedy = !(temperature > 0.f);
   int32_t* const tokens = a.tokens + static_cast<int64_t>(b) * a.T;
   int32_t* const path = a.path + static_cast<int64_t>(b) * a.T;
@@ -424,8 +458,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, co
   for (;;) {
     const Row<T> row = row_of(n);
     const float* const q = a.probs ? a.probs + b * a.ps_b + n * a.ps_n : nullptr;
-    int per, j0, j1;
-    run_of(row, per, j0, j1);
+    int each, longer, j0, j1;
+    run_of(row, each, longer, j0, j1);
     // Children of the node, one a lane, up to 32 at a time.  A lane without one, or whose draft is no token, has token -1.
     const int kid0 = first_kid[n];
     int kid = a.T, kid_token = -1;
@@ -461,25 +495,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, co
     int accepted = -1, accepted_token = -1, at = 0;
     double total = 0.;
     bool fine = true;
-    weigh.relative_to(0.f, true);
-    if (!greedy && weigh.lo > Range<T>::kLeast) total = tell_sum(sum_near(row, weigh, j0, j1));
-    if (!(total >= 0x1p-200)) {   // greedy, or the row does not lie around zero (or all of a type's numbers do)
-      Largest best = largest_of(row, j0, j1);
-      meet(best.l, best.token);
-      best = {-INFINITY, 0x7fffffff};
-      for (int i = lane; i < slots; i += 32) best.take(static_cast<float>(sh.sum[turn ^ 1][i]), sh.id[turn ^ 1][i]);
-      best.of_warp();
-      fine = fabsf(best.l) < INFINITY;   // there is a distribution
-      at = best.token;
-      if (fine && !greedy) {
-        weigh.relative_to(best.l, false);
-        total = tell_sum(sum_remaining<T>(row, weigh, j0, j1, nullptr, 1., 0.));
-      }
-    }
-    // ---- the children in turn.  `rest` is Pi (of p unnormalised while nothing is rejected): p = max(weight inv - beta q, 0) / rest.
-    double beta = 0., inv = 1., rest = greedy ? 1. : total;
-    const float q_at = greedy && fine && q ? q[at] : 0.f;
-    auto own_weight = [&]() { return kid_token < 0 ? 0. : greedy ? (kid_token == at ? 1. : 0.) : weigh(Elem<T>::to_f(kid_logit)); };
+    double kid_w = 0.;
+    bool kid_again = false;
     // whether an earlier child had this lane's token
     auto repeated = [&]() {
       bool same = (__match_any_sync(0xffffffffu, kid_token) & ((1u << lane) - 1)) != 0;
@@ -487,10 +504,53 @@ __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, co
         for (int k = kid0; !same && k < kid; k = sibling[k]) same = drafts[k] == kid_token;
       return same;
     };
-    double kid_w = 0.;
-    bool kid_again = false;
+    weigh.relative_to(0.f, true);
+    const bool in_range = !greedy && weigh.lo > Range<T>::kLeast;
+    if (in_range && kid0 < a.T && more >= a.T && each >= 2) {
+      // ---- a child that is accepted, or refused, by more than what fp32 may be off needs no more than that (runs of less are as fast in 64 bits)
+      const float rate = weigh.rate_hi * (1.f / kTable);
+      total = tell_sum(sum_fast(row, rate, 120.f / rate, j0, j1));
+      if (total >= 0x1p-60) {
+        kid_w = kid_token >= 0 ? weigh(Elem<T>::to_f(kid_logit)) : 0.;
+        kid_again = repeated();
+        const double draw = (kid < a.T ? static_cast<double>(u[kid]) : 0.) * static_cast<double>(kid_q), slack = total * kSlack;
+        double rest = total;
 #pragma unroll 1
-    while (fine && kid0 < a.T) {
+        for (uint32_t todo = __ballot_sync(0xffffffffu, kid_token >= 0); todo; todo &= todo - 1) {
+          const int k = __ffs(todo) - 1;
+          const double w = q == nullptr && kid_again ? 0. : kid_w;
+          if (__shfl_sync(0xffffffffu, draw * (rest + slack) < w, k)) {
+            accepted = __shfl_sync(0xffffffffu, kid, k), accepted_token = __shfl_sync(0xffffffffu, kid_token, k);
+            break;
+          }
+          if (q || __shfl_sync(0xffffffffu, draw * (rest - slack) < w, k)) break;
+          rest = fmax(rest - __shfl_sync(0xffffffffu, w, k), 0.);
+        }
+      }
+      total = 0.;
+    }
+    if (accepted < 0) {
+      if (in_range) total = tell_sum(sum_near(row, weigh, j0, j1));
+      if (!(total >= 0x1p-200)) {   // greedy, or the row does not lie around zero (or all of a type's numbers do)
+        Largest best = largest_of(row, j0, j1);
+        meet(best.l, best.token);
+        best = {-INFINITY, 0x7fffffff};
+        for (int i = lane; i < slots; i += 32) best.take(static_cast<float>(sh.sum[turn ^ 1][i]), sh.id[turn ^ 1][i]);
+        best.of_warp();
+        fine = fabsf(best.l) < INFINITY;   // there is a distribution
+        at = best.token;
+        if (fine && !greedy) {
+          weigh.relative_to(best.l, false);
+          total = tell_sum(sum_remaining<T>(row, weigh, j0, j1, nullptr, 1., 0.));
+        }
+      }
+    }
+    // ---- the children in turn.  `rest` is Pi (of p unnormalised while nothing is rejected): p = max(weight inv - beta q, 0) / rest.
+    double beta = 0., inv = 1., rest = greedy ? 1. : total;
+    const float q_at = greedy && fine && q ? q[at] : 0.f;
+    auto own_weight = [&]() { return kid_token < 0 ? 0. : greedy ? (kid_token == at ? 1. : 0.) : weigh(Elem<T>::to_f(kid_logit)); };
+#pragma unroll 1
+    while (accepted < 0 && fine && kid0 < a.T) {
       kid_w = own_weight();
       kid_again = repeated();
       const float kid_u = kid < a.T ? u[kid] : 0.f;
@@ -561,7 +621,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, co
     bool touched = false;   // a child's token lies in this warp's run
     if (without)
       each_kid([&](int token, double w) {
-        const int owner = (token + row.skew) / kVec / per;
+        const int unit = (token + row.skew) / (kVec * 32), split = longer * (each + 1);
+        const int owner = unit < split ? unit / (each + 1) : longer + (unit - split) / each;   // (`each` 0: all units lie below the split)
         touched |= owner == mine;
 #pragma unroll
         for (int i = 0; i < kSlots / 32; ++i)
@@ -594,7 +655,12 @@ __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, co
       for (int base = j0; base < j1 && token < 0; base += 32) {
         const int j = base + lane;
         double w[kVec] = {};
-        if (j < j1) remaining(row, weigh, j, row.load(j), q, inv, beta, w);
+        if (j < j1) {
+          const Vec<T> x = row.load(j);
+          float y[kVec] = {};
+          if (beta > 0.) row.load_probs(q, j, y);
+          remaining(weigh, x, y, inv, beta, w);
+        }
         if (touched)
           each_kid([&](int out, double) {
             const int off = out - row.first(j);
