@@ -81,7 +81,7 @@ struct Pool {
   uint8_t* p;
   int64_t layer_bytes;
   uint32_t layers, outer, row_bytes, unit;   // unit: bytes that a thread moves of a row (1 to 16)
-  uint32_t blocks;                           // that move its columns
+  uint32_t wide_bits, of_block, blocks;      // a strip has up to 2^wide_bits units; strips of a block; blocks
 };
 constexpr int kMaxPools = 64;
 struct Move {
@@ -91,54 +91,68 @@ struct Move {
   int pools, T;
 };
 
-// A column is `unit` bytes of a row of one head of one layer.  A block moves 32 columns (the lanes) of one sequence, 64 rows at a time, eight to a
-// warp: all are loaded, and when the whole block has them, stored.  The path ascends, so a row's place lies below all rows that are loaded later.
-// (A thread with its column's rows all to itself, eight at a time, left 96 paths of 24 rows in 16 layers of 4-bit pages at 51 us.)
-constexpr int kMoveThreads = 256, kMoveRows = 64, kOfThread = kMoveRows * 32 / kMoveThreads;
+// A block moves some strips of one pool (up to 32 units of the rows of one head of one layer), for one sequence, 64 rows at a time: all rows are
+// loaded, and when the whole block has them, stored.  The path ascends, so a row's place lies below all rows that are loaded later.
+// A warp's lanes are 2^wide_bits units of each of 32 >> wide_bits rows: rows of 4-bit codes and scales are 64 and 8 bytes, and lie together by
+// head.  A thread has eight rows (or two or four of each of four or two strips, where a row is one unit or two).
+// (96 paths of 24 rows in 16 layers of 4-bit pages: 27 us; 51 with a thread to a column of all rows, 36 with heads on neighbouring lanes.)
+constexpr int kMoveThreads = 256, kMoveRows = 64, kOfThread = 8;
 
-template <typename U>
-__device__ __forceinline__ void move_rows(uint8_t* base, const int64_t* from, const int64_t* to, const int n, const int64_t stride) {
-  U v[kOfThread];
-  const int warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int x = 0; x < kOfThread; ++x) {
-    const int i = x * (kMoveThreads / 32) + warp;
-    if (base && i < n && from[i] >= 0) v[x] = *reinterpret_cast<const U*>(base + from[i] * stride);
+__device__ __forceinline__ uint4 load_unit(const uint8_t* p, uint32_t unit) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  switch (unit) {
+    case 16: v = *reinterpret_cast<const uint4*>(p); break;
+    case 8: {
+      const uint2 w = *reinterpret_cast<const uint2*>(p);
+      v.x = w.x, v.y = w.y;
+      break;
+    }
+    case 4: v.x = *reinterpret_cast<const uint32_t*>(p); break;
+    case 2: v.x = *reinterpret_cast<const uint16_t*>(p); break;
+    default: v.x = *p; break;
   }
-  __syncthreads();
-#pragma unroll
-  for (int x = 0; x < kOfThread; ++x) {
-    const int i = x * (kMoveThreads / 32) + warp;
-    if (base && i < n && from[i] >= 0) *reinterpret_cast<U*>(base + to[i] * stride) = v[x];
+  return v;
+}
+__device__ __forceinline__ void store_unit(uint8_t* p, const uint4& v, uint32_t unit) {
+  switch (unit) {
+    case 16: *reinterpret_cast<uint4*>(p) = v; break;
+    case 8: *reinterpret_cast<uint2*>(p) = make_uint2(v.x, v.y); break;
+    case 4: *reinterpret_cast<uint32_t*>(p) = v.x; break;
+    case 2: *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(v.x); break;
+    default: *p = static_cast<uint8_t>(v.x); break;
   }
 }
 
 __global__ void __launch_bounds__(kMoveThreads) commit_drafts_kernel(const __grid_constant__ Move a) {
-  __shared__ int64_t from[kMoveRows], to[kMoveRows];   // in rows of one head; -1: nothing to move
+  __shared__ int64_t from[kMoveRows], to[kMoveRows];   // page * block_size and slot in the low half, the page in the high one; -1: nothing to move
   __shared__ int end;
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
-  const int b = blockIdx.y, lane = threadIdx.x & 31;
+  const int b = blockIdx.y;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int32_t* table = a.block_table + b * a.blocks_per_seq;
   const int32_t* path = a.path + static_cast<int64_t>(b) * a.T;
   const int64_t offset = a.offset[b];
   const int count = min(max(a.counts[b], 0), a.T);
-  // a block's columns are of one pool
-  uint32_t block = blockIdx.x;
-  int k = 0;
-  for (; k + 1 < a.pools && block >= a.pool[k].blocks; ++k) block -= a.pool[k].blocks;
-  const Pool& pool = a.pool[k];
-  const uint32_t of_row = pool.row_bytes / pool.unit, column = block * 32 + lane, rest = column / of_row;
-  const uint32_t o = rest % pool.outer, layer = rest / pool.outer;
-  uint8_t* const base = layer < pool.layers
-                            ? pool.p + layer * pool.layer_bytes + (static_cast<int64_t>(o) * a.block_size * pool.row_bytes + (column - rest * of_row) * pool.unit)
-                            : nullptr;
   // page (or -1) and slot of a position below 2^32
   auto place = [&](int64_t pos, int64_t& page, int& slot) {
     const uint32_t at = static_cast<uint32_t>(pos), blk = at / static_cast<uint32_t>(a.block_size);
     page = pos >= 0 && blk < a.blocks_per_seq ? table[blk] : -1;
     if (page >= a.num_blocks) page = -1;
     slot = static_cast<int>(at - blk * static_cast<uint32_t>(a.block_size));
+  };
+  uint32_t block = blockIdx.x;
+  int k = 0;
+  for (; k + 1 < a.pools && block >= a.pool[k].blocks; ++k) block -= a.pool[k].blocks;
+  const Pool& pool = a.pool[k];
+  const uint32_t of_row = pool.row_bytes / pool.unit, of_head = (of_row + 31) / 32;   // units of a row; strips of a head
+  const uint32_t all_strips = pool.layers * pool.outer * of_head, bits = pool.wide_bits, more = bits > 2 ? bits - 2 : 0;   // 2^more warps share a strip
+  const uint32_t strip0 = block * pool.of_block + (bits >= 2 ? warp >> more : warp * (4u >> bits));
+  const uint32_t passes = bits >= 2 ? 8u : 2u << bits, row0 = lane >> bits, rows = 32u >> bits;
+  const int64_t head_bytes = a.block_size * pool.row_bytes, page_bytes = pool.outer * head_bytes;
+  auto strip_at = [&](uint32_t strip) -> uint8_t* {   // the lane's unit of its row 0; null: none
+    const uint32_t head = strip / of_head, unit = (strip - head * of_head) * 32 + (lane & ((1u << bits) - 1)), layer = head / pool.outer;
+    return strip < all_strips && unit < of_row ? pool.p + layer * pool.layer_bytes + (head - layer * pool.outer) * head_bytes + unit * pool.unit : nullptr;
   };
   for (int i0 = 0; i0 < count; i0 += kMoveRows) {
     if (threadIdx.x == 0) end = count;
@@ -149,18 +163,27 @@ __global__ void __launch_bounds__(kMoveThreads) commit_drafts_kernel(const __gri
       int64_t f = -1, t = -1;
       int sf = 0, st = 0;
       if (p >= 0 && p != i) place(offset + p, f, sf), place(offset + i, t, st);
-      const int64_t page_rows = pool.outer * a.block_size;
-      from[threadIdx.x] = f >= 0 && t >= 0 ? f * page_rows + sf : -1;
-      to[threadIdx.x] = t * page_rows + st;
+      from[threadIdx.x] = f >= 0 && t >= 0 ? f << 32 | sf : -1;
+      to[threadIdx.x] = t << 32 | st;
     }
     __syncthreads();
     const int n = min(end - i0, kMoveRows);
-    switch (pool.unit) {
-      case 16: move_rows<uint4>(base, from, to, n, pool.row_bytes); break;
-      case 8: move_rows<uint2>(base, from, to, n, pool.row_bytes); break;
-      case 4: move_rows<uint32_t>(base, from, to, n, pool.row_bytes); break;
-      case 2: move_rows<uint16_t>(base, from, to, n, pool.row_bytes); break;
-      default: move_rows<uint8_t>(base, from, to, n, pool.row_bytes); break;
+    uint4 v[kOfThread];
+    uint32_t moved = 0;
+    uint8_t* p = nullptr;   // row 0 of the strip
+    auto row_of = [&](int x) { return (((x & (passes - 1)) << more) + (warp & ((1u << more) - 1))) * rows + row0; };
+    auto at = [&](int64_t place) { return p + (place >> 32) * page_bytes + static_cast<uint32_t>(place) * static_cast<int64_t>(pool.row_bytes); };
+#pragma unroll
+    for (int x = 0; x < kOfThread; ++x) {
+      if ((x & (passes - 1)) == 0) p = strip_at(strip0 + x / passes);
+      const int i = row_of(x);
+      if (p && i < n && from[i] >= 0) v[x] = load_unit(at(from[i]), pool.unit), moved |= 1u << x;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < kOfThread; ++x) {
+      if (passes < kOfThread && (x & (passes - 1)) == 0) p = strip_at(strip0 + x / passes);
+      if (moved >> x & 1u) store_unit(at(to[row_of(x)]), v[x], pool.unit);
     }
     if (n < kMoveRows) break;
   }
@@ -211,9 +234,13 @@ extern "C" int oasr_b200_commit_drafts(const oasr_b200_draft_pool* pools, int64_
       const oasr_b200_draft_pool& p = pools[done + a.pools];
       const uint64_t bits = reinterpret_cast<uintptr_t>(p.data) | static_cast<uint64_t>(p.row_bytes) | 16u;
       const int64_t unit = static_cast<int64_t>(bits & (~bits + 1));   // (a layer is a whole number of rows)
-      const int64_t blocks = (p.layers * p.outer * (p.row_bytes / unit) + 31) / 32;
+      const int64_t of_row = p.row_bytes / unit, strips = p.layers * p.outer * ((of_row + 31) / 32);
+      uint32_t wide_bits = 0;
+      while (wide_bits < 5 && (1 << wide_bits) < of_row) ++wide_bits;
+      const int64_t of_block = 32 >> wide_bits, blocks = (strips + of_block - 1) / of_block;
       a.pool[a.pools] = drafts::Pool{static_cast<uint8_t*>(p.data), num_blocks * p.outer * block_size * p.row_bytes, static_cast<uint32_t>(p.layers),
-                                     static_cast<uint32_t>(p.outer), static_cast<uint32_t>(p.row_bytes), static_cast<uint32_t>(unit), static_cast<uint32_t>(blocks)};
+                                     static_cast<uint32_t>(p.outer), static_cast<uint32_t>(p.row_bytes), static_cast<uint32_t>(unit), wide_bits,
+                                     static_cast<uint32_t>(of_block), static_cast<uint32_t>(blocks)};
       all += blocks;
     }
     launch_pdl(drafts::commit_drafts_kernel, dim3(static_cast<unsigned>(all), static_cast<unsigned>(B)), dim3(drafts::kMoveThreads), 0,
