@@ -470,7 +470,11 @@ struct Plan {
 Plan plan(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t D, int64_t keys, int64_t pool_rows) {
   Plan p;
   const int64_t rows = H / Hkv * Tq;
-  p.wide = pool_rows <= 0x7fffffff - 128 && (g_path ? g_path == 2 : rows > 32);
+  // Which form: measured in us, few rows against many, rows of 4 heads a key head.  128 dims, 64 groups of 6000 keys: 32 rows 42 / 47, 48 rows 60 / 48, 256
+  // rows 206 / 77; 512 groups of 3000: 132 / 169, 217 / 173, 775 / 259.  64 dims, 64 of 6000: 30 / 36, 45 / 36, 146 / 66.  Few blocks over short caches are
+  // the few-row form's whatever their rows: 128 dims, 8 groups of 1000: 48 rows 15 / 18, 256 rows 16 / 28.
+  const bool short_and_few = keys <= 2048 && (rows + 31) / 32 * B * Hkv <= sm_count();
+  p.wide = pool_rows <= 0x7fffffff - 128 && (g_path ? g_path == 2 : rows > 32 && !short_and_few);
   if (p.wide) {
     p.rows = rows <= 128 ? 128 : 256;
     p.row_blocks = static_cast<int>((rows + p.rows - 1) / p.rows);
