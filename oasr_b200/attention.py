@@ -339,12 +339,17 @@ def fmha_q4(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_co
 
 def _tree_mask(mask: torch.Tensor, B: int, T: int):
     """``(mask, stride from sequence to sequence in words, words of a row)``."""
-    words = (T + 31) // 32
-    if mask.dtype != torch.int32 or mask.dim() not in (2, 3) or tuple(mask.shape) != ((B, T, words) if mask.dim() == 3 else (T, words)):
-        raise ValueError(f"tree_mask must be int32 ({B}, {T}, {words}) or ({T}, {words}) (draft_tree), got {tuple(mask.shape)} {mask.dtype}")
-    if not mask.is_contiguous():
-        mask = mask.contiguous()
-    return mask, T * words if mask.dim() == 3 else 0, words
+    words, shape = (T + 31) // 32, mask.shape
+    each = len(shape) == 3
+    if mask.dtype is not torch.int32 or shape != ((B, T, words) if each else (T, words)):
+        raise ValueError(f"tree_mask must be int32 ({B}, {T}, {words}) or ({T}, {words}) (draft_tree), got {tuple(shape)} {mask.dtype}")
+    return mask if mask.is_contiguous() else mask.contiguous(), T * words if each else 0, words
+
+
+@functools.lru_cache(maxsize=4096)
+def _tree_workspace(device: int, *sizes: int) -> int:
+    """Bytes of workspace of a call of these sizes on this device (``tunables.set`` forgets them)."""
+    return _lib.load().oasr_b200_fmha_tree_workspace_bytes(*sizes)
 
 
 def fmha_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *, softmax_scale: float, block_table: torch.Tensor,
@@ -362,14 +367,15 @@ def fmha_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *, 
     Scores, their maximum and sum and the output are fp32; the weights are rounded to ``q``'s type before they meet the values (``fmha``
     does the same), and the result once more.  How the work is split goes by the width of ``block_table``, as lengths are on the GPU: over a
     table many times wider than the longest sequence pass ``block_table[:, :blocks]`` of what is in use."""
-    if q.dim() != 4:
-        raise ValueError(f"q must be (B, H, T_q, D); got {tuple(q.shape)}")
-    B, H, T, D = q.shape
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+    shape, pool, dtype = q.shape, k_cache.shape, q.dtype      # (calls of few rows are as long as their checks)
+    if len(shape) != 4:
+        raise ValueError(f"q must be (B, H, T_q, D); got {tuple(shape)}")
+    B, H, T, D = shape
+    if len(pool) != 4 or v_cache.shape != pool:
         raise ValueError("pools must be (num_blocks, block_size, H_kv, D) and match")
-    num_blocks, block_size, Hkv, pool_dim = k_cache.shape
-    if q.dtype not in _HALF or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
-        raise ValueError(f"fmha_tree supports fp16/bf16 with one dtype for q and pools, got {q.dtype}, {k_cache.dtype}, {v_cache.dtype}")
+    num_blocks, block_size, Hkv, pool_dim = pool
+    if dtype not in _HALF or k_cache.dtype is not dtype or v_cache.dtype is not dtype:
+        raise ValueError(f"fmha_tree supports fp16/bf16 with one dtype for q and pools, got {dtype}, {k_cache.dtype}, {v_cache.dtype}")
     if pool_dim != D:
         raise ValueError("q and k head_dim must match")
     if Hkv == 0 or H % Hkv:
@@ -377,35 +383,45 @@ def fmha_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *, 
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("pools must be contiguous")
     block_table = _table32(block_table, B)
-    lens, starts = _index32("cache_seqlens", cache_seqlens, B), _index32("cache_seqstarts", cache_seqstarts, B)
-    q_lens = _index32("q_lens", q_lens, B)
+    lens = _index32("cache_seqlens", cache_seqlens, B)
+    starts = None if cache_seqstarts is None else _index32("cache_seqstarts", cache_seqstarts, B)
+    if q_lens is not None:
+        q_lens = _index32("q_lens", q_lens, B)
     mask_stride = words = 0
+    mask = None
     if tree_mask is not None:
         tree_mask, mask_stride, words = _tree_mask(tree_mask, B, T)
+        mask = tree_mask.data_ptr()
     _one_device(q, k_cache, v_cache, block_table, lens, starts, q_lens, tree_mask, out)
-    qs = q.stride()
-    sb, sh, st = _used_strides(B, H, T, *qs[:3])
-    if qs[3] != 1 or sb % 8 or sh % 8 or st % 8 or q.data_ptr() % 16:
-        q = q.clone(memory_format=torch.contiguous_format)
-        sb, sh, st = H * T * D, T * D, D
+    sb, sh, st, unit = q.stride()
+    if B == 1:
+        sb = 0                            # the stride of a dimension of size 1 may be any number
+    if H == 1:
+        sh = 0
+    if T == 1:
+        st = 0
+    src = q.data_ptr()
+    if unit != 1 or (sb | sh | st) % 8 or src % 16:
+        q = q.clone(memory_format=torch.contiguous_format)   # (contiguous() would keep one that is merely misaligned)
+        src, sb, sh, st = q.data_ptr(), H * T * D, T * D, D
     if out is None:
         if token_major:
-            out = torch.empty(B, T, H, D, dtype=q.dtype, device=q.device)
+            out = torch.empty((B, T, H, D), dtype=dtype, device=q.device)
             os = _stride_array(T * H * D, D, H * D)
         else:
-            out = torch.empty(B, H, T, D, dtype=q.dtype, device=q.device)
+            out = torch.empty((B, H, T, D), dtype=dtype, device=q.device)
             os = _stride_array(H * T * D, T * D, D)
     else:
         want = (B, T, H, D) if token_major else (B, H, T, D)
-        if tuple(out.shape) != want or out.dtype != q.dtype or out.stride(3) != 1:
+        if tuple(out.shape) != want or out.dtype != dtype or out.stride(3) != 1:
             raise ValueError(f"out must be {want} in q's dtype, with unit stride along D")
         _check_distinct_rows(out=out)
         ob, oh, ot = (out.stride(0), out.stride(2), out.stride(1)) if token_major else out.stride()[:3]
         os = _stride_array(*_used_strides(B, H, T, ob, oh, ot))
     per = block_table.shape[1]
-    need = _lib.load().oasr_b200_fmha_tree_workspace_bytes(B, H, Hkv, T, D, per, block_size, num_blocks)
+    need = _tree_workspace(q.get_device(), B, H, Hkv, T, D, per, block_size, num_blocks)
     work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _lib.call("oasr_b200_fmha_tree", out.data_ptr(), os, q.data_ptr(), _stride_array(sb, sh, st), k_cache.data_ptr(), v_cache.data_ptr(),
-              block_table.data_ptr(), lens.data_ptr(), _p(starts), _p(q_lens), _p(tree_mask), mask_stride, words, _p(work), need, per, block_size,
-              num_blocks, B, H, Hkv, T, D, softmax_scale, _DTYPE_ID[q.dtype], _stream(q))
+    _lib.call("oasr_b200_fmha_tree", out.data_ptr(), os, src, _stride_array(sb, sh, st), k_cache.data_ptr(), v_cache.data_ptr(),
+              block_table.data_ptr(), lens.data_ptr(), _p(starts), _p(q_lens), mask, mask_stride, words, _p(work), need, per, block_size,
+              num_blocks, B, H, Hkv, T, D, softmax_scale, _DTYPE_ID[dtype], _stream(q))
     return out

@@ -81,36 +81,40 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, parents: torch.Ten
     random numbers of 1 or more where nothing of ``p`` is left.  -inf logits are impossible tokens; a draft outside ``[0, V)`` is not accepted.
 
     Decisions are taken in 64 bits (weights to 1e-12, those below 2^-300 of the largest may be zeros; sums in a fixed order); only rows on the accepted path are read."""
-    if logits.dim() != 3 or logits.shape[2] < 1:
-        raise RuntimeError(f"logits must be (B, T, V), got {tuple(logits.shape)}")
-    B, T, V = logits.shape
-    if drafts.shape != (B, T) or (parents.shape != (B, T) and parents.shape != (T,)):
+    shape = logits.shape
+    if len(shape) != 3 or shape[2] < 1:
+        raise RuntimeError(f"logits must be (B, T, V), got {tuple(shape)}")
+    B, T, V = shape
+    tree, one = (B, T), parents.dim() == 1
+    if drafts.shape != tree or parents.shape != ((T,) if one else tree):
         raise RuntimeError(f"drafts must be ({B}, {T}) and parents ({B}, {T}) or ({T},), got {tuple(drafts.shape)} and {tuple(parents.shape)}")
-    if uniforms.shape != (B, T) or uniforms.dtype != torch.float32:
+    if uniforms.shape != tree or uniforms.dtype is not torch.float32:
         raise RuntimeError(f"uniforms must be fp32 ({B}, {T}), got {tuple(uniforms.shape)} {uniforms.dtype}")
     temperatures = None
     if isinstance(temperature, torch.Tensor):
         if temperature.shape != (B,) or temperature.dtype != torch.float32:
             raise RuntimeError(f"temperature must be a number or fp32 ({B},), got {tuple(temperature.shape)} {temperature.dtype}")
         temperatures, temperature = temperature if temperature.is_contiguous() else temperature.contiguous(), 1.0
-    if draft_probs is not None and (draft_probs.shape != logits.shape or draft_probs.dtype != torch.float32):
-        raise RuntimeError(f"draft_probs must be fp32 {tuple(logits.shape)}, got {tuple(draft_probs.shape)} {draft_probs.dtype}")
+    if draft_probs is not None and (draft_probs.shape != shape or draft_probs.dtype != torch.float32):
+        raise RuntimeError(f"draft_probs must be fp32 {tuple(shape)}, got {tuple(draft_probs.shape)} {draft_probs.dtype}")
     drafts, parents = _whole32("drafts", drafts), _whole32("parents", parents)
     if not uniforms.is_contiguous():
         uniforms = uniforms.contiguous()
     _one_device(logits, drafts, parents, uniforms, temperatures, draft_probs)
-    if logits.stride(2) != 1 and V > 1:
+    ls_b, ls_n, unit = logits.stride()
+    if unit != 1 and V > 1:
         logits = logits.contiguous()
-    ls_b, ls_n, _ = logits.stride()
+        ls_b, ls_n, _ = logits.stride()
     ps_b = ps_n = 0
     if draft_probs is not None:
         if draft_probs.stride(2) != 1 and V > 1:
             draft_probs = draft_probs.contiguous()
         ps_b, ps_n, _ = draft_probs.stride()
-    tokens = torch.empty(B, T, dtype=torch.int32, device=logits.device)
+    device = logits.device
+    tokens = torch.empty(tree, dtype=torch.int32, device=device)
     path = torch.empty_like(tokens)
-    counts = torch.empty(B, dtype=torch.int32, device=logits.device)
+    counts = torch.empty(B, dtype=torch.int32, device=device)
     _lib.call("oasr_b200_verify_drafts", tokens.data_ptr(), path.data_ptr(), counts.data_ptr(), logits.data_ptr(), ls_b, ls_n, drafts.data_ptr(),
-              parents.data_ptr(), T if parents.dim() == 2 else 0, uniforms.data_ptr(), _p(draft_probs), ps_b, ps_n, _p(temperatures), temperature,
+              parents.data_ptr(), 0 if one else T, uniforms.data_ptr(), _p(draft_probs), ps_b, ps_n, _p(temperatures), temperature,
               B, T, V, _dt(logits), _stream(logits))
     return VerifiedDrafts(tokens, path, counts)

@@ -32,4 +32,7 @@ from . import _lib
 
 
 def set(name: str, value: int) -> None:  # noqa: A001 - mirrors the C entry point's name
+    from . import attention
+
     _lib.call("oasr_b200_set_tunable", name.encode(), int(value))
+    attention._tree_workspace.cache_clear()
