@@ -288,8 +288,9 @@ __device__ __noinline__ double sum_near(const Row<T> row, const Weigher weigh, c
 }
 
 // The same in fp32, 4 instructions a logit in the place of 20.  |log2(weight)| stays below 127, so its product and its factor are off by 2^-17.4 and
-// 2^-17.4 at most, the exponential by 2^-22, sums of 16 in a row by 2^-20: kSlack holds them all.
+// 2^-17.4 at most, the exponential by 2^-22, sums of up to 128 in a row (kMostUnits) by 2^-17: kSlack holds them all.
 constexpr double kSlack = 0x1p-15;
+constexpr int kMostUnits = 64;   // of a warp: 512 logits a lane, in four sums
 template <typename T>
 __device__ __noinline__ float sum_fast(const Row<T> row, const float rate, const float hi, const int j0, const int j1) {
   float s[4] = {};
@@ -506,7 +507,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, co
     };
     weigh.relative_to(0.f, true);
     const bool in_range = !greedy && weigh.lo > Range<T>::kLeast;
-    if (in_range && kid0 < a.T && more >= a.T && each >= 2) {
+    if (in_range && kid0 < a.T && more >= a.T && each >= 2 && each < kMostUnits) {
       // ---- a child that is accepted, or refused, by more than what fp32 may be off needs no more than that (runs of less are as fast in 64 bits)
       const float rate = weigh.rate_hi * (1.f / kTable);
       total = tell_sum(sum_fast(row, rate, 120.f / rate, j0, j1));

@@ -113,7 +113,7 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, parents: torch.Ten
     device = logits.device
     tokens = torch.empty(tree, dtype=torch.int32, device=device)
     path = torch.empty_like(tokens)
-    counts = torch.empty(B, dtype=torch.int32, device=device)
+    counts = torch.empty(B, dtype=torch.int32, device=device) if T else torch.zeros(B, dtype=torch.int32, device=device)
     _lib.call("oasr_b200_verify_drafts", tokens.data_ptr(), path.data_ptr(), counts.data_ptr(), logits.data_ptr(), ls_b, ls_n, drafts.data_ptr(),
               parents.data_ptr(), 0 if one else T, uniforms.data_ptr(), _p(draft_probs), ps_b, ps_n, _p(temperatures), temperature,
               B, T, V, _dt(logits), _stream(logits))

@@ -469,6 +469,59 @@ def test_verify_drafts_of_odd_rows(dtype, V):
     assert (got.counts == 1).all() and ((got.tokens[:, 0] >= -1) & (got.tokens[:, 0] < V)).all()
 
 
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("T,V", [(33, 40), (34, 3000), (100, 60), (1024, 200), (1024, 20000)])
+def test_verify_drafts_of_many_children(drawn, T, V):
+    """All drafts continue node 0, or every second one does and the others its first child: many of the same token, more than a warp's lanes."""
+    g, rng = torch.Generator().manual_seed(T + V), np.random.RandomState(T)
+    B = 3
+    parents = np.zeros((B, T), np.int64)
+    parents[1, 2:] = np.arange(T - 2) % 2
+    x = 2 * torch.randn(B, 1, V, generator=g).expand(B, T, V).clone()
+    x[:, 1] = 2 * torch.randn(B, V, generator=g)
+    drafts = rng.randint(0, V, (B, T))
+    u = (0.5 + 0.5 * rng.rand(B, T)).astype(np.float32)       # most are refused
+    u[:, 0] = rng.rand(B)
+    if T > 40:
+        u[0, T - 3], x[0, 0, drafts[0, T - 3]] = 1e-4, 6.0       # one of the last stands
+    probs = None
+    if drawn:
+        probs = torch.softmax(x[:, :1].double() + torch.randn(B, 1, V, generator=g).double(), -1).float().expand(B, T, V).contiguous().cuda()
+    for temps in ([1.0, 0.8, 1.3], [0.0] * 3):
+        check_verify(x.cuda(), drafts, parents, u, temps, probs)
+
+
+def test_verify_drafts_of_long_rows():
+    """A run of more logits than the shorter sums are for, and a vocabulary of one block's."""
+    V = 2 ** 20 + 3
+    x = (2 * torch.randn(1, 3, V, generator=torch.Generator().manual_seed(1))).half()
+    x[0, 0, 77] = x[0, 1, 99] = 14.0
+    many = x.expand(150, 3, V)
+    u = np.random.RandomState(1).rand(150, 3).astype(np.float32)
+    drafts, parents = np.tile([[0, 77, 99]], (150, 1)), np.tile([[0, 0, 1]], (150, 1))
+    x = x.cuda()
+    one = check_verify(x, drafts[:1], parents[:1], u[:1], [1.0])
+    got = ob.verify_drafts(x.expand(150, 3, V), torch.from_numpy(drafts).cuda(), torch.from_numpy(parents).cuda(), torch.from_numpy(u).cuda())
+    assert torch.equal(got.tokens[0], one.tokens[0])
+    for b in (1, 2, 3, 149):
+        assert torch.equal(got.tokens[b], ob.verify_drafts(x, torch.from_numpy(drafts[:1]).cuda(), torch.from_numpy(parents[:1]).cuda(), torch.from_numpy(u[b:b + 1]).cuda()).tokens[0])
+    assert many.shape == got.tokens.shape + (V,)
+
+
+def test_verify_drafts_shapes_and_numbers():
+    x = torch.randn(2, 3, 20, device="cuda")
+    i, u = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), torch.full((2, 3), 0.5, device="cuda")
+    for temperature, tensor in ((0.7, 0.7), (0, 0.0), (-1.0, 0.0), (2, 2.0)):
+        a, b = ob.verify_drafts(x, i, i, u, temperature=temperature), ob.verify_drafts(x, i, i[0], u, temperature=torch.full((2,), tensor, device="cuda"))
+        assert all(torch.equal(s, t) for s, t in zip(a, b))
+    for none in (ob.verify_drafts(x[:0], i[:0], i[:0], u[:0]), ob.verify_drafts(x[:, :0], i[:, :0], i[:, :0], u[:, :0])):
+        assert none.tokens.numel() == none.path.numel() == 0 and not none.counts.any()
+    with pytest.raises(RuntimeError):
+        ob.verify_drafts(x, i, i, u, temperature=math.nan)
+    with pytest.raises(RuntimeError):
+        ob.verify_drafts(x.double(), i, i, u)
+
+
 def test_verify_drafts_outside_the_vocabulary_and_the_tree():
     V, T = 50, 6
     x = torch.zeros(1, T, V, device="cuda")
