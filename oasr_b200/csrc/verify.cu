@@ -30,7 +30,7 @@ namespace ob {
 namespace verify {
 namespace {
 
-constexpr int kWarps = 16, kMaxCluster = 8, kSlots = kWarps * kMaxCluster, kTable = 256, kCopies = 16, kMaxNodes = 1024, kVec = 8;
+constexpr int kMaxWarps = 16, kMaxCluster = 8, kSlots = kMaxWarps * kMaxCluster, kTable = 256, kCopies = 16, kMaxNodes = 1024, kVec = 8;
 
 struct Args {
   int32_t *tokens, *path, *counts;
@@ -364,8 +364,8 @@ __device__ __noinline__ double sum_remaining(const Row<T> row, const Weigher wei
   return s;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, const int C) {
+template <typename T, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel(const Args a, const int C) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& sh = *reinterpret_cast<Shared*>(smem);
   int* const parents = reinterpret_cast<int*>(smem + sizeof(Shared));
@@ -373,9 +373,14 @@ __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, co
   float* const u = reinterpret_cast<float*>(drafts + a.T);
   int* const first_kid = reinterpret_cast<int*>(u + a.T);   // a.T: none
   int* const sibling = first_kid + a.T;
+  int* const token_of = sibling + a.T;                       // what the walk has found so far: stored at the end, as a barrier waits for stores
+  int* const node_of = token_of + a.T;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = C > 1 ? static_cast<int>(ptx::cluster_ctarank()) : 0, b = static_cast<int>(blockIdx.x) / C;
-  const uint64_t entry = g_table.e[threadIdx.x % kTable];   // (stored once the tree's loads are on their way)
+  constexpr int kThreads = kWarps * 32, kFills = 2 * kTable / kThreads;   // a thread fills half of the copies of so many entries
+  uint64_t entry[kFills];                                                 // (stored once the tree's loads are on their way)
+#pragma unroll
+  for (int i = 0; i < kFills; ++i) entry[i] = g_table.e[(threadIdx.x + i * kThreads) % kTable];
   if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // waited for before the first word to another block
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
@@ -399,16 +404,18 @@ __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, co
     run_of(row, each, more, j0, j1);
     ahead(row.p, row.first(j0), row.first(j1));
   }
-  for (int i = threadIdx.x; i < a.T; i += kWarps * 32) {
+  for (int i = threadIdx.x; i < a.T; i += kThreads) {
     parents[i] = a.parents[b * a.parents_b + i];
     drafts[i] = a.drafts[static_cast<int64_t>(b) * a.T + i];
     u[i] = a.uniforms[static_cast<int64_t>(b) * a.T + i];
   }
   const float temperature = a.temperatures ? a.temperatures[b] : a.temperature;
 #pragma unroll
-  for (int i = 0; i < kCopies / 2; ++i)
-    sh.table[threadIdx.x % kTable][(threadIdx.x + i) % (kCopies / 2) + threadIdx.x / kTable * (kCopies / 2)] = __longlong_as_double(entry);
-  static_assert(kWarps * 32 == 2 * kTable, "half of the copies a thread");
+  for (int f = 0; f < kFills; ++f) {
+    const int item = threadIdx.x + f * kThreads, at = item % kTable;
+#pragma unroll
+    for (int i = 0; i < kCopies / 2; ++i) sh.table[at][(at + i) % (kCopies / 2) + item / kTable * (kCopies / 2)] = __longlong_as_double(entry[f]);
+  }
   const bool greedy = !(temperature > 0.f);
   int32_t* const tokens = a.tokens + static_cast<int64_t>(b) * a.T;
   int32_t* const path = a.path + static_cast<int64_t>(b) * a.T;
@@ -453,7 +460,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, co
   };
 
   int n = 0, count = 0;
-  if (writer) path[0] = 0;
+  if (writer) node_of[0] = 0;
   Weigher weigh{&sh.table[0][lane % kCopies], kTable * 1.4426950408889634 / static_cast<double>(temperature), 0., 0.f, 0.f, 0.f, 0.f, a.two12, a.two21, true};
 #pragma unroll 1
   for (;;) {
@@ -589,7 +596,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, co
       more = take_kids(more);
     }
     if (accepted >= 0) {
-      if (writer) tokens[count] = accepted_token, path[count + 1] = accepted;
+      if (writer) token_of[count] = accepted_token, node_of[count + 1] = accepted;
       ++count;
       n = accepted;
       continue;
@@ -693,19 +700,21 @@ __global__ void __launch_bounds__(kWarps * 32, 1) verify_kernel(const Args a, co
     }
     break;
   }
-  if (writer) a.counts[b] = count + 1;
-  if (rank == 0)
-    for (int i = count + 1 + threadIdx.x; i < a.T; i += kWarps * 32) tokens[i] = -1, path[i] = -1;
+  if (rank == 0) {
+    if (writer) a.counts[b] = count + 1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.T; i += kThreads) {
+      if (i != count) tokens[i] = i < count ? token_of[i] : -1;   // (the new token is stored by who found it)
+      path[i] = i <= count ? node_of[i] : -1;
+    }
+  }
 }
 
-template <typename T>
-int launch(const Args& a, cudaStream_t s) {
-  // Blocks of a cluster: as many as there are SMs for, as long as each has work for eight warps.
-  int C = 1;
-  while (C < kMaxCluster && a.B * C * 2 <= sm_count() && a.V > C * 8 * 32 * kVec) C *= 2;
-  auto bytes = [](int nodes) { return static_cast<int>(sizeof(Shared) + nodes * 20); };
+template <typename T, int kWarps>
+int launch(const Args& a, const int C, cudaStream_t s) {
+  auto bytes = [](int nodes) { return static_cast<int>(sizeof(Shared) + nodes * 28); };
   static SmemLimit limit;
-  const cudaError_t e = limit.raise(verify_kernel<T>, bytes(kMaxNodes));
+  const cudaError_t e = limit.raise(verify_kernel<T, kWarps>, bytes(kMaxNodes));
   if (e != cudaSuccess) return set_error(OASR_ERR_CUDA, "verify_drafts: shared memory limit: %s", cudaGetErrorString(e));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(a.B * C));
@@ -719,8 +728,21 @@ int launch(const Args& a, cudaStream_t s) {
   at[1].val.clusterDim = {static_cast<unsigned>(C), 1, 1};
   cfg.attrs = at;
   cfg.numAttrs = C > 1 ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, verify_kernel<T>, a, C);
+  cudaLaunchKernelEx(&cfg, verify_kernel<T, kWarps>, a, C);
   return check_launch("verify_drafts launch");
+}
+
+template <typename T>
+int launch(const Args& a, cudaStream_t s) {
+  // Blocks of eight warps, two to an SM, and of a cluster as many as fit, as long as each has work for four of its warps.  Long rows of few sequences
+  // take blocks of sixteen: every warp decides for itself, and more warps take longer for that (3 chains of 5 over 5002 tokens: 12.6 us with eight, 14.2
+  // with sixteen; 32 drawn chains of 8 over 65537: 34.6, 36.7), but a row is walked through in fewer steps (16 trees of 48 over 131071: 21, 16).
+  // Clusters of sixteen were no faster.
+  const int sms = sm_count(), units = a.V / (32 * kVec);
+  int C = 1;
+  while (C < kMaxCluster && a.B * C <= sms && units > C * 4) C *= 2;
+  if (units > 192 && a.B * kMaxCluster <= sms) return launch<T, 16>(a, C, s);
+  return launch<T, 8>(a, C, s);
 }
 
 }  // namespace
