@@ -514,7 +514,8 @@ int launch(const Args& a, const Plan& p, cudaStream_t s) {
 
 template <typename T, int D>
 int run(const Args& a, const Plan& p, int dtype, cudaStream_t s) {
-  const int rc = p.wide ? run_wide(a, D, dtype, p.rows, p.groups, p.row_blocks, s) : p.rows == 8 ? launch<T, D, 1>(a, p, s) : p.rows == 16 ? launch<T, D, 2>(a, p, s) : launch<T, D, 4>(a, p, s);
+  if (p.wide) return run_wide(a, D, dtype, p.rows, p.groups, p.row_blocks, s);
+  const int rc = p.rows == 8 ? launch<T, D, 1>(a, p, s) : p.rows == 16 ? launch<T, D, 2>(a, p, s) : launch<T, D, 4>(a, p, s);
   if (rc != OASR_OK || p.splits == 1) return rc;
   const int64_t rows = p.groups * p.rows;
   const auto join = [&](auto kern, int ways) {

@@ -49,7 +49,8 @@ __device__ __forceinline__ const uint32_t* mask_row(const Args& a, int b, int t)
   return a.mask ? a.mask + b * a.mask_b + static_cast<int64_t>(t) * a.mask_words : nullptr;
 }
 
-// Partial results of one (split, group, row block of `rows` rows): rows x (maximum, sum), then rows x D of output.
+// Partial results of one (split, group, row block of `rows` rows): maxima, sums and outputs; rows x (maximum, sum), then rows x D of output, or in the
+// form for many rows the maxima, the sums, then D x rows of output.
 template <int D>
 __host__ __device__ constexpr int64_t part_floats(int rows) { return static_cast<int64_t>(rows) * (D + 2); }
 

@@ -118,16 +118,12 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
   float* const part = a.parts ? a.parts + (static_cast<int64_t>(split) * groups + group) * part_floats<D>(NR) : nullptr;
   auto out_row = [&](int r) { return static_cast<T*>(a.out) + b * a.os_b + (hk * share + r % share) * a.os_h + static_cast<int64_t>(r / share) * a.os_t; };
   if (tiles == 0) {   // nothing to see: zero rows
-    for (int i = threadIdx.x; i < min(NR, rows - row0) * (D / 8); i += kThreads) {
-      const int r = i / (D / 8), d = i % (D / 8) * 8;
-      if (part) {
-        if (d == 0) part[2 * r] = kEmpty, part[2 * r + 1] = 0.f;
-        float4* dst = reinterpret_cast<float4*>(part + 2 * NR + r * D + d);
-        dst[0] = dst[1] = make_float4(0.f, 0.f, 0.f, 0.f);
-      } else {
-        *reinterpret_cast<uint4*>(out_row(row0 + r) + d) = make_uint4(0, 0, 0, 0);
-      }
+    if (part) {
+      for (int i = threadIdx.x; i < NR * (D + 2); i += kThreads) part[i] = i < NR ? kEmpty : 0.f;
+      return;
     }
+    for (int i = threadIdx.x; i < min(NR, rows - row0) * (D / 8); i += kThreads)
+      *reinterpret_cast<uint4*>(out_row(row0 + i / (D / 8)) + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
     return;
   }
   // streams with something in them, and their steps
@@ -459,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
     }
     const uint32_t t_o = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + kColO + x * 128;
     const float inv = !valid ? 0.f : part ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;   // NaN stays
-    if (part && there && half == 0) part[2 * r] = valid ? m : kEmpty, part[2 * r + 1] = valid ? l : 0.f;
+    if (part && half == 0) part[r] = valid ? m : kEmpty, part[NR + r] = valid ? l : 0.f;
     const bool by_hand = *odd_values && valid;
     T* out = out_row(there ? rr : 0);
 #pragma unroll 1
@@ -491,12 +487,10 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
           }
         }
       }
-      if (!there) continue;
-      if (part) {
-        float4* dst = reinterpret_cast<float4*>(part + 2 * NR + r * D + c0);
+      if (part) {   // dims outside: the lanes' rows lie together
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dst[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-      } else {
+        for (int i = 0; i < 32; ++i) part[(2 + c0 + i) * NR + r] = y[i];
+      } else if (there) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           *reinterpret_cast<uint4*>(out + c0 + 8 * i) = make_uint4(pack2<T>(y[8 * i], y[8 * i + 1]), pack2<T>(y[8 * i + 2], y[8 * i + 3]),
@@ -507,6 +501,64 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
   }
   __syncthreads();
   if (warp == kMmaWarp) ptx::tmem_dealloc(tmem, kCols);
+}
+
+// Joins the partial results of a group's blocks.  A lane has a row; with kWays 1 a warp has D / 8 dims of 32 rows, with kWays 8 an eighth of the parts of 16
+// dims of 32 rows.  Output rows go through shared memory.
+template <typename T, int D, int kWays>
+__global__ void __launch_bounds__(256) fmha_tree_wide_join_kernel(const Args a, const int row_blocks, const int NR, const int groups) {
+  constexpr int kDims = kWays == 1 ? D / 8 : 16, kOfBlock = kWays == 1 ? D : 16;   // of a warp, of a block
+  __shared__ float outs[8][32][kDims + 1];
+  __shared__ float tops[8][32], sums[8][32];
+  ptx::grid_dep_launch();
+  ptx::grid_dep_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int at = blockIdx.x;
+  const int dims0 = at % (D / kOfBlock) * kOfBlock;
+  at /= D / kOfBlock;
+  const int n0 = at % (NR / 32) * 32, group = at / (NR / 32), rb = group % row_blocks, hk = group / row_blocks % a.Hkv, b = group / row_blocks / a.Hkv;
+  const int share = a.H / a.Hkv, rows = share * a.Tq, r0 = rb * NR + n0;
+  if (r0 >= rows) return;
+  const int64_t part = part_floats<D>(NR), step = part * groups;
+  const float* src = a.parts + group * part + n0 + lane;
+  const int first = kWays == 1 ? 0 : warp, d0 = dims0 + (kWays == 1 ? warp * kDims : 0);
+  float top = kEmpty, sum = 0.f, acc[kDims] = {};
+  for (int s = first; s < a.splits; s += kWays) top = fmaxf(top, src[s * step]);
+#pragma unroll 2
+  for (int s = first; s < a.splits; s += kWays) {
+    const float* p = src + s * step;
+    float v[kDims];
+#pragma unroll
+    for (int i = 0; i < kDims; ++i) v[i] = p[(2 + d0 + i) * NR];
+    const float f = ex2(p[0] - top);
+    sum = fmaf(f, p[NR], sum);
+#pragma unroll
+    for (int i = 0; i < kDims; ++i) acc[i] = fmaf(f, v[i], acc[i]);
+  }
+  tops[warp][lane] = top, sums[warp][lane] = sum;
+#pragma unroll
+  for (int i = 0; i < kDims; ++i) outs[warp][lane][i] = acc[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * kOfBlock; i += 256) {
+    const int n = i / kOfBlock, d = i % kOfBlock, r = r0 + n;
+    if (r >= rows) break;
+    float y = 0.f, all = 0.f;
+    if constexpr (kWays == 1) {
+      y = outs[d / kDims][n][d % kDims], all = sums[0][n];
+    } else {
+      float most = kEmpty;
+#pragma unroll
+      for (int w = 0; w < kWays; ++w) most = fmaxf(most, tops[w][n]);
+#pragma unroll
+      for (int w = 0; w < kWays; ++w) {
+        const float f = ex2(tops[w][n] - most);
+        y = fmaf(f, outs[w][n][d], y), all = fmaf(f, sums[w][n], all);
+      }
+    }
+    const int tq = r / share, live = a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq;
+    const float inv = all > 0.f ? 1.f / all : all == 0.f ? 0.f : all;   // NaN stays
+    static_cast<T*>(a.out)[b * a.os_b + (hk * share + r - tq * share) * a.os_h + static_cast<int64_t>(tq) * a.os_t + dims0 + d] = Elem<T>::from_f(tq < live ? y * inv : 0.f);
+  }
 }
 
 template <typename T, int D, bool kKeys2>
@@ -527,7 +579,15 @@ int launch(const Args& a, int dtype, int64_t groups, int row_blocks, cudaStream_
   if (rc != OASR_OK) return rc;
   launch_pdl(fmha_tree_wide_kernel<T, D, kKeys2>, dim3(static_cast<unsigned>(groups * a.splits)), dim3(kThreads), S::kDynamic, s, a, k_map, v_map, row_blocks, piece,
              device_status_ptr());
-  return check_launch("fmha_tree launch");
+  rc = check_launch("fmha_tree launch");
+  if (rc != OASR_OK || a.splits == 1) return rc;
+  constexpr int NR = kKeys2 ? 128 : 256;
+  const int64_t blocks = groups * (NR / 32);
+  if (a.splits <= 8)
+    launch_pdl(fmha_tree_wide_join_kernel<T, D, 1>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a, row_blocks, NR, static_cast<int>(groups));
+  else
+    launch_pdl(fmha_tree_wide_join_kernel<T, D, 8>, dim3(static_cast<unsigned>(blocks * (D / 16))), dim3(256), 0, s, a, row_blocks, NR, static_cast<int>(groups));
+  return check_launch("fmha_tree join launch");
 }
 
 }  // namespace
