@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(256) fmha_tree_join_kernel(const Args a, const
 struct Plan {
   int rows, row_blocks, splits;   // rows of a block; blocks of rows of a (sequence, key head); blocks that share a cache
   int64_t groups;
-  bool wide;
+  bool wide, parts;   // the form for many rows; blocks that share a cache leave partial results
   int warps;   // of a block of the few-row form
 };
 
@@ -470,19 +470,27 @@ struct Plan {
 Plan plan(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t D, int64_t keys, int64_t pool_rows) {
   Plan p;
   const int64_t rows = H / Hkv * Tq;
-  // Which form: measured in us, few rows against many, rows of 4 heads a key head.  128 dims, 64 groups of 6000 keys: 32 rows 42 / 47, 48 rows 60 / 48, 256
-  // rows 206 / 77; 512 groups of 3000: 132 / 169, 217 / 173, 775 / 259.  64 dims, 64 of 6000: 30 / 36, 45 / 36, 146 / 66.  Few blocks over short caches are
-  // the few-row form's whatever their rows: 128 dims, 8 groups of 1000: 48 rows 15 / 18, 256 rows 16 / 28.
+  // Which form: measured in us, few rows against many, rows of 4 heads a key head.  128 dims, 64 groups of 6000 keys: 32 rows 42 / 45, 48 rows 60 / 45, 256
+  // rows 206 / 63; 512 groups of 3000: 131 / 170, 217 / 172, 789 / 250.  64 dims, 64 of 6000: 29 / 34, 45 / 35, 146 / 57.  Few blocks over short caches are
+  // the few-row form's whatever their rows: 128 dims, 8 groups of 1000: 48 rows 15 / 19, 256 rows 16 / 25 (where the rule is wrong it costs little: 64 dims,
+  // 64 groups of 1000, 64 rows 17 / 15).
   const bool short_and_few = keys <= 2048 && (rows + 31) / 32 * B * Hkv <= sm_count();
   p.wide = pool_rows <= 0x7fffffff - 128 && (g_path ? g_path == 2 : rows > 32 && !short_and_few);
   if (p.wide) {
     p.rows = rows <= 128 ? 128 : 256;
     p.row_blocks = static_cast<int>((rows + p.rows - 1) / p.rows);
     p.groups = B * Hkv * p.row_blocks;
-    const int64_t most = keys / 512;
+    // Blocks that share a cache: until each SM has one, as long as each has four steps.  Up to eight are a cluster (as many as its size allows in groups of
+    // 18 SMs), which saves the partial results and the kernel that joins them: 64 groups of 256 rows of 128 dims over 6000 keys, two blocks each: 63 us, 77
+    // through partial results (some of it from tiles asked for ahead of the queries).  More than eight only where that shortens the walk by more than two
+    // steps: two groups of 112 rows of 128 dims over 100003 keys, 74 blocks each: 32 us.
+    const int64_t most = keys / 512, steps = keys / 128;
     int64_t s = p.groups > 0 ? sm_count() / p.groups : 1;
     s = s < most ? s : most;
+    if (s > kMostOfCluster && steps / kMostOfCluster - steps / s <= 2) s = kMostOfCluster;
+    while (s > 1 && s <= kMostOfCluster && p.groups > sm_count() / 18 * (18 / s)) --s;
     p.splits = static_cast<int>(s < 1 ? 1 : s > 256 ? 256 : s);
+    p.parts = p.splits > kMostOfCluster;
     return p;
   }
   p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
@@ -495,6 +503,7 @@ Plan plan(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t D, int64_t keys
   s = s < most ? s : most;
   if (keys * (s - 1) < 16 * p.warps * 16 * s) s = 1;
   p.splits = static_cast<int>(s < 1 ? 1 : s > 256 ? 256 : s);
+  p.parts = p.splits > 1;
   return p;
 }
 
@@ -535,7 +544,7 @@ extern "C" int64_t oasr_b200_fmha_tree_workspace_bytes(int64_t B, int64_t H, int
   using namespace ob::fmha_tree;
   if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || Tq <= 0 || (D != 64 && D != 128) || blocks_per_seq < 0 || block_size <= 0) return 0;
   const Plan p = plan(B, H, Hkv, Tq, D, blocks_per_seq * block_size, num_blocks * block_size);
-  return p.splits > 1 ? p.splits * p.groups * (D == 64 ? part_floats<64>(p.rows) : part_floats<128>(p.rows)) * 4 : 0;
+  return p.parts ? p.splits * p.groups * (D == 64 ? part_floats<64>(p.rows) : part_floats<128>(p.rows)) * 4 : 0;
 }
 
 extern "C" int oasr_b200_fmha_tree(void* out, const int64_t* out_strides, const void* q, const int64_t* q_strides, const void* k_pool,

@@ -18,6 +18,8 @@ struct Args {
   float scale_log2;
 };
 
+constexpr int kMostOfCluster = 8;   // blocks of the form for many rows that share a cache as a cluster; more leave partial results
+
 constexpr float kEmpty = -3e38f;   // a maximum below every score: differences to it overflow to -inf or are zero, never NaN
 
 __device__ __forceinline__ float ex2(float x) {

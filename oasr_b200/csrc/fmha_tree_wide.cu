@@ -31,6 +31,7 @@ namespace {
 constexpr int kMmaWarp = 16, kProducer = 17, kReader = 18, kThreads = 608;
 constexpr int kAtom = 128 * 128;   // 128 rows of 128 bytes
 constexpr int kKeys = 128;
+constexpr int kMaxCluster = kMostOfCluster;
 
 // two fp32 operations in one instruction
 __device__ __forceinline__ uint64_t pair(float a, float b) {
@@ -104,33 +105,6 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
   constexpr uint32_t kIdescPV = ptx::umma_idesc_f16(kBf16, 128, D, false, true);   // V: keys are its rows
   constexpr uint32_t kColS = 0, kColO = 256, kCols = 512;
 
-  ptx::grid_dep_wait();
-  const int split = static_cast<int>(blockIdx.x) % a.splits, group = static_cast<int>(blockIdx.x) / a.splits, groups = static_cast<int>(gridDim.x) / a.splits;
-  int at = group;
-  const int rb = at % row_blocks;
-  at /= row_blocks;
-  const int hk = at % a.Hkv, b = at / a.Hkv;
-  const int share = a.H / a.Hkv, rows = share * a.Tq, row0 = rb * NR;
-  const Sequence seq(a, b);
-  const int all0 = seq.start / kKeys, all1 = row0 < seq.live * share ? max((seq.end + kKeys - 1) / kKeys, all0) : all0;
-  const int per = (all1 - all0 + a.splits - 1) / a.splits;
-  const int tile0 = min(all0 + split * per, all1), tiles = min(tile0 + per, all1) - tile0;
-  float* const part = a.parts ? a.parts + (static_cast<int64_t>(split) * groups + group) * part_floats<D>(NR) : nullptr;
-  auto out_row = [&](int r) { return static_cast<T*>(a.out) + b * a.os_b + (hk * share + r % share) * a.os_h + static_cast<int64_t>(r / share) * a.os_t; };
-  if (tiles == 0) {   // nothing to see: zero rows
-    if (part) {
-      for (int i = threadIdx.x; i < NR * (D + 2); i += kThreads) part[i] = i < NR ? kEmpty : 0.f;
-      return;
-    }
-    for (int i = threadIdx.x; i < min(NR, rows - row0) * (D / 8); i += kThreads)
-      *reinterpret_cast<uint4*>(out_row(row0 + i / (D / 8)) + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  // streams with something in them, and their steps
-  const int streams = kKeys2 ? min(tiles, 2) : (min(rows, seq.live * share) > row0 + 128 ? 2 : 1);
-  auto steps_of = [&](int x) { return kKeys2 ? (tiles - x + 1) / 2 : tiles; };
-  auto tile_of = [&](int x, int j) { return kKeys2 ? 2 * j + x : j; };
-
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars);
@@ -144,44 +118,110 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
   volatile uint32_t* odd_values = tmem_slot + 2;   // a drafted key has a value that is not finite
   volatile uint32_t* drain_flag = tmem_slot + 3;
 
+  // what needs nothing of the kernels before
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < S::kSlots; ++i) {
-      ptx::mbar_init(&full[i], 1);
-      ptx::mbar_init(&empty[i], 1);
-      ptx::mbar_init(&looked[i], 1);
+  if (warp == kProducer) {
+    if (lane == 0) {
+      ptx::prefetch_tensormap(&k_map);
+      ptx::prefetch_tensormap(&v_map);
+      for (int i = 0; i < S::kSlots; ++i) {
+        ptx::mbar_init(&full[i], 1);
+        ptx::mbar_init(&empty[i], 1);
+        ptx::mbar_init(&looked[i], 1);
+      }
+      for (int x = 0; x < 2; ++x) {
+        ptx::mbar_init(&s_full[x], 1);
+        ptx::mbar_init(&p_full[x], 256);
+        ptx::mbar_init(&o_done[x], 1);
+      }
+      *abort_flag = 0;
+      *odd_values = 0;
+      *drain_flag = 0;
+      ptx::fence_barrier_init();
     }
-    for (int x = 0; x < 2; ++x) {
-      ptx::mbar_init(&s_full[x], 1);
-      ptx::mbar_init(&p_full[x], 256);
-      ptx::mbar_init(&o_done[x], 1);
-    }
-    *abort_flag = 0;
-    *odd_values = 0;
-    *drain_flag = 0;
-    ptx::fence_barrier_init();
+    __syncwarp();
   }
   if (warp == kMmaWarp) {
     ptx::tmem_alloc(tmem_slot, kCols);
     ptx::tmem_relinquish();
   }
-  // queries, with the sign of the scale
-  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-  for (int i = threadIdx.x; i < (kKeys2 ? 1 : streams) * 128 * (D / 8); i += kThreads) {
-    const int r = i / (D / 8), o = i % (D / 8), rr = row0 + r;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (rr < rows)
-      v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.qs_b + (hk * share + rr % share) * a.qs_h +
-                                          static_cast<int64_t>(rr / share) * a.qs_t + o * 8);
-    *reinterpret_cast<uint4*>(smem + S::kQ + ((r >> 7) * S::kAtoms + o / 8) * kAtom + (r & 127) * 128 + ((o & 7) ^ (r & 7)) * 16) =
-        make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip);
+
+  ptx::grid_dep_wait();
+  const int split = static_cast<int>(blockIdx.x) % a.splits, group = static_cast<int>(blockIdx.x) / a.splits, groups = static_cast<int>(gridDim.x) / a.splits;
+  int at = group;
+  const int rb = at % row_blocks;
+  at /= row_blocks;
+  const int hk = at % a.Hkv, b = at / a.Hkv;
+  const int share = a.H / a.Hkv, rows = share * a.Tq, row0 = rb * NR;
+  const Sequence seq(a, b);
+  const int all0 = seq.start / kKeys, all1 = row0 < seq.live * share ? max((seq.end + kKeys - 1) / kKeys, all0) : all0;
+  const int per = (all1 - all0 + a.splits - 1) / a.splits;
+  const int tile0 = min(all0 + split * per, all1), tiles = min(tile0 + per, all1) - tile0;
+  float* const part = a.parts ? a.parts + (static_cast<int64_t>(split) * groups + group) * part_floats<D>(NR) : nullptr;
+  const bool cluster = a.splits > 1 && part == nullptr;   // the blocks that share the keys are a cluster, whose rank is `split`
+  auto out_row = [&](int r) { return static_cast<T*>(a.out) + b * a.os_b + (hk * share + r % share) * a.os_h + static_cast<int64_t>(r / share) * a.os_t; };
+
+  // After the walk, in the ring's place: sums of both halves of a row; kKeys2: the second stream's maxima and output, dims outside; in a cluster the
+  // block's maxima, sums and output, dims outside.
+  float* const sums = reinterpret_cast<float*>(smem + S::kRing);
+  float* const other_m = sums + 512;
+  float* const other = other_m + 128;
+  float* const my_m = other + (kKeys2 ? D * 128 : 0);
+  float* const my_l = my_m + NR;
+  float* const my_o = my_l + NR;
+  static_assert((640 + (kKeys2 ? D * 128 : 0) + NR * (D + 2)) * 4 <= S::kSlots * S::kAtoms * kAtom, "fits the ring");
+  auto meet = [&] {   // the blocks of a cluster put their results together, each eight dims in turn
+    ptx::cluster_sync();
+    const int r = threadIdx.x % NR, ways = 512 / NR, rr = row0 + r;
+    if (threadIdx.x < 512 && rr < rows) {
+      auto of = [&](const float* p, int rank) {
+        float v;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ptx::map_to_cta(p, rank)));
+        return v;
+      };
+      float f[kMaxCluster], top = kEmpty, sum = 0.f;
+#pragma unroll
+      for (int x = 0; x < kMaxCluster; ++x) f[x] = x < a.splits ? of(my_m + r, x) : kEmpty, top = fmaxf(top, f[x]);
+#pragma unroll
+      for (int x = 0; x < kMaxCluster; ++x) {
+        const bool some = f[x] > kEmpty;
+        f[x] = some ? ex2(f[x] - top) : 0.f;
+        if (some) sum = fmaf(f[x], of(my_l + r, x), sum);
+      }
+      const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;   // NaN stays
+      T* const out = out_row(rr);
+      for (int c = split + a.splits * static_cast<int>(threadIdx.x / NR); c < D / 8; c += a.splits * ways) {
+        float y[8] = {};
+#pragma unroll
+        for (int x = 0; x < kMaxCluster; ++x)
+          if (f[x] != 0.f)   // (a block without keys has nothing there)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = fmaf(f[x], of(my_o + (8 * c + i) * NR + r, x), y[i]);
+        *reinterpret_cast<uint4*>(out + 8 * c) = make_uint4(pack2<T>(y[0] * inv, y[1] * inv), pack2<T>(y[2] * inv, y[3] * inv), pack2<T>(y[4] * inv, y[5] * inv),
+                                                            pack2<T>(y[6] * inv, y[7] * inv));
+      }
+    }
+    __syncwarp();
+    ptx::cluster_sync();   // nobody leaves while its results are read
+  };
+  if (tiles == 0) {   // nothing to see: zero rows
+    if (cluster) {
+      for (int i = threadIdx.x; i < NR; i += kThreads) my_m[i] = kEmpty;
+    } else if (part) {
+      for (int i = threadIdx.x; i < NR * (D + 2); i += kThreads) part[i] = i < NR ? kEmpty : 0.f;
+    } else {
+      for (int i = threadIdx.x; i < min(NR, rows - row0) * (D / 8); i += kThreads)
+        *reinterpret_cast<uint4*>(out_row(row0 + i / (D / 8)) + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    if (warp == kMmaWarp) ptx::tmem_dealloc(*tmem_slot, kCols);
+    if (cluster) meet();
+    return;
   }
-  ptx::fence_proxy_async_smem();
-  ptx::tc_fence_before_sync();
-  __syncthreads();
-  ptx::tc_fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
-  ptx::grid_dep_launch();   // only now: see sm100_ptx.cuh
+  // streams with something in them, and their steps
+  const int streams = kKeys2 ? min(tiles, 2) : (min(rows, seq.live * share) > row0 + 128 ? 2 : 1);
+  auto steps_of = [&](int x) { return kKeys2 ? (tiles - x + 1) / 2 : tiles; };
+  auto tile_of = [&](int x, int j) { return kKeys2 ? 2 * j + x : j; };
 
   const int table_len = static_cast<int>(a.blocks_per_seq), block_size = static_cast<int>(a.block_size);
   const int32_t* table = a.block_table + b * a.blocks_per_seq;
@@ -190,6 +230,52 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
     const int page = blk < table_len ? table[blk] : -1;
     return page < a.num_blocks ? page : -1;
   };
+  // The producer's lane i fetches piece i / kAtoms of a tile, dims 64 (i % kAtoms) .. of it.  Pages are asked for a tile ahead; what the ring holds is on its
+  // way before the queries are.
+  const int pieces = kKeys / piece_rows * S::kAtoms, atom = lane % S::kAtoms, first = lane / S::kAtoms * piece_rows;
+  int row_now = 0, row_next = 0;
+  auto row_at = [&](int i) {
+    const int key = (tile0 + i) * kKeys + first, page = lane < pieces && i < tiles ? page_at(key) : -1;
+    return page >= 0 ? page * block_size + key % block_size : static_cast<int>(a.num_blocks * a.block_size);   // (behind the pool)
+  };
+  auto fetch = [&](int h) {
+    const int slot = h % S::kSlots;
+    if (h % 2 == 0) row_now = row_next, row_next = row_at(h / 2 + 1);
+    if (lane == 0) ptx::mbar_expect_tx(&full[slot], S::kAtoms * kAtom);
+    __syncwarp();
+    if (lane < pieces)
+      ptx::tma_load_3d(smem + S::kRing + slot * S::kAtoms * kAtom + atom * kAtom + first * 128, h % 2 ? &v_map : &k_map, atom * 64, hk, row_now, &full[slot]);
+  };
+  if (warp == kProducer) {
+    row_next = row_at(0);
+    for (int h = 0; h < min(S::kSlots, 2 * tiles); ++h) fetch(h);
+  }
+  // queries, with the sign of the scale
+  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+  if (warp < 16) {
+    constexpr int kLoads = S::kTiles * 128 * (D / 8) / 512;   // of a thread, all on their way at once
+    uint4 v[kLoads];
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      const int i = k * 512 + static_cast<int>(threadIdx.x), rr = row0 + i / (D / 8), tq = rr / share;
+      v[k] = make_uint4(0, 0, 0, 0);
+      if (rr < rows)
+        v[k] = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.qs_b + (hk * share + rr - tq * share) * a.qs_h + static_cast<int64_t>(tq) * a.qs_t)[i % (D / 8)];
+    }
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      const int i = k * 512 + static_cast<int>(threadIdx.x), r = i / (D / 8), o = i % (D / 8);
+      *reinterpret_cast<uint4*>(smem + S::kQ + ((r >> 7) * S::kAtoms + o / 8) * kAtom + (r & 127) * 128 + ((o & 7) ^ (r & 7)) * 16) =
+          make_uint4(v[k].x ^ flip, v[k].y ^ flip, v[k].z ^ flip, v[k].w ^ flip);
+    }
+  }
+  ptx::fence_proxy_async_smem();
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  ptx::grid_dep_launch();   // only now: see sm100_ptx.cuh
+
   bool ok = true;
   float m = kEmpty, l = 0.f;
 
@@ -288,27 +374,12 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
     if (!ok && lane == 0 && status) atomicOr(status, kStatusFmhaLoad);
     __syncwarp();
   } else if (warp == kProducer) {
-    // lane i fetches piece i / kAtoms of a tile, dims 64 (i % kAtoms) .. of it; pages are asked for a tile ahead
-    const int pieces = kKeys / piece_rows * S::kAtoms, atom = lane % S::kAtoms, first = lane / S::kAtoms * piece_rows;
-    const int no_row = static_cast<int>(a.num_blocks * a.block_size);
-    auto row_at = [&](int i) {
-      const int key = (tile0 + i) * kKeys + first, page = lane < pieces ? page_at(key) : -1;
-      return page >= 0 ? page * block_size + key % block_size : no_row;
-    };
-    const uint32_t dst = atom * kAtom + first * 128;
-    int h = 0, row = row_at(0);
-    for (int i = 0; ok && i < tiles; ++i) {
-      const int here = row;
-      if (i + 1 < tiles) row = row_at(i + 1);
-      for (int v = 0; ok && v < 2; ++v, ++h) {
-        const int s = h % S::kSlots;
-        if (h >= S::kSlots) ok = ptx::mbar_wait(&empty[s], (h / S::kSlots - 1) & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (lane == 0) ptx::mbar_expect_tx(&full[s], S::kAtoms * kAtom);
-        __syncwarp();
-        if (lane < pieces) ptx::tma_load_3d(smem + S::kRing + s * S::kAtoms * kAtom + dst, v ? &v_map : &k_map, atom * 64, hk, here, &full[s]);
-      }
+    int h = min(S::kSlots, 2 * tiles);
+    for (; ok && h < 2 * tiles; ++h) {
+      const int slot = h % S::kSlots;
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(&empty[slot], (h / S::kSlots - 1) & 1, abort_flag)) != 0;
+      if (!ok) break;
+      fetch(h);
     }
     // nothing may be on its way when the block ends
     if (!ok)
@@ -421,10 +492,6 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
   }
   __syncthreads();
   const bool done = *abort_flag == 0;
-  // the ring is free: sums of both halves of a row; kKeys2: the second stream's maxima and output, dims outside
-  float* const sums = reinterpret_cast<float*>(smem + S::kRing);
-  float* const other_m = sums + 512;
-  float* const other = other_m + 128;
   if (warp < 16) {
     const int x = warp / 8, half = warp >> 2 & 1, r = (warp & 3) * 32 + lane;
     sums[(x * 2 + half) * 128 + r] = l;
@@ -442,7 +509,8 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
     }
   }
   __syncthreads();
-  if (warp < (kKeys2 ? 8 : 16) && row0 + (kKeys2 ? 0 : (warp / 8) * 128) < rows) {
+  const bool join = part || cluster;
+  if (warp < (kKeys2 ? 8 : 16) && (join || row0 + (kKeys2 ? 0 : (warp / 8) * 128) < rows)) {
     const int x = warp / 8, half = warp >> 2 & 1, rs = (warp & 3) * 32 + lane, r = x * 128 + rs, rr = row0 + r;
     const bool there = rr < rows, valid = there && rr / share < seq.live && x < streams && done;
     l = sums[x * 256 + rs] + sums[x * 256 + 128 + rs];
@@ -454,8 +522,9 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
       l = fmaf(f0, l, f1 * (sums[256 + rs] + sums[384 + rs]));
     }
     const uint32_t t_o = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + kColO + x * 128;
-    const float inv = !valid ? 0.f : part ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;   // NaN stays
-    if (part && half == 0) part[r] = valid ? m : kEmpty, part[NR + r] = valid ? l : 0.f;
+    const float inv = !valid ? 0.f : join ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;   // NaN stays
+    float *const to_m = part ? part : my_m, *const to_o = part ? part + 2 * NR : my_o;
+    if (join && half == 0) to_m[r] = valid ? m : kEmpty, to_m[NR + r] = valid ? l : 0.f;
     const bool by_hand = *odd_values && valid;
     T* out = out_row(there ? rr : 0);
 #pragma unroll 1
@@ -487,9 +556,9 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
           }
         }
       }
-      if (part) {   // dims outside: the lanes' rows lie together
+      if (join) {   // dims outside: the lanes' rows lie together
 #pragma unroll
-        for (int i = 0; i < 32; ++i) part[(2 + c0 + i) * NR + r] = y[i];
+        for (int i = 0; i < 32; ++i) to_o[(c0 + i) * NR + r] = y[i];
       } else if (there) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -501,31 +570,32 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
   }
   __syncthreads();
   if (warp == kMmaWarp) ptx::tmem_dealloc(tmem, kCols);
+  if (cluster) meet();
 }
 
-// Joins the partial results of a group's blocks.  A lane has a row; with kWays 1 a warp has D / 8 dims of 32 rows, with kWays 8 an eighth of the parts of 16
-// dims of 32 rows.  Output rows go through shared memory.
-template <typename T, int D, int kWays>
+// Joins the partial results of a group's blocks, more than a cluster has: a block has 4 dims of 32 rows (the lanes), its warps an eighth of the
+// parts each (16 dims: a part's loads fill the registers, and 74 parts take 8 us longer).
+template <typename T, int D>
 __global__ void __launch_bounds__(256) fmha_tree_wide_join_kernel(const Args a, const int row_blocks, const int NR, const int groups) {
-  constexpr int kDims = kWays == 1 ? D / 8 : 16, kOfBlock = kWays == 1 ? D : 16;   // of a warp, of a block
-  __shared__ float outs[8][32][kDims + 1];
-  __shared__ float tops[8][32], sums[8][32];
+  constexpr int kDims = 4, kWays = 8;
+  __shared__ float outs[kWays][32][kDims + 1];
+  __shared__ float tops[kWays][32], sums[kWays][32];
   ptx::grid_dep_launch();
   ptx::grid_dep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int at = blockIdx.x;
-  const int dims0 = at % (D / kOfBlock) * kOfBlock;
-  at /= D / kOfBlock;
+  const int d0 = at % (D / kDims) * kDims;
+  at /= D / kDims;
   const int n0 = at % (NR / 32) * 32, group = at / (NR / 32), rb = group % row_blocks, hk = group / row_blocks % a.Hkv, b = group / row_blocks / a.Hkv;
   const int share = a.H / a.Hkv, rows = share * a.Tq, r0 = rb * NR + n0;
   if (r0 >= rows) return;
   const int64_t part = part_floats<D>(NR), step = part * groups;
   const float* src = a.parts + group * part + n0 + lane;
-  const int first = kWays == 1 ? 0 : warp, d0 = dims0 + (kWays == 1 ? warp * kDims : 0);
   float top = kEmpty, sum = 0.f, acc[kDims] = {};
-  for (int s = first; s < a.splits; s += kWays) top = fmaxf(top, src[s * step]);
-#pragma unroll 2
-  for (int s = first; s < a.splits; s += kWays) {
+#pragma unroll 8
+  for (int s = warp; s < a.splits; s += kWays) top = fmaxf(top, src[s * step]);
+#pragma unroll 8
+  for (int s = warp; s < a.splits; s += kWays) {
     const float* p = src + s * step;
     float v[kDims];
 #pragma unroll
@@ -539,25 +609,20 @@ __global__ void __launch_bounds__(256) fmha_tree_wide_join_kernel(const Args a, 
 #pragma unroll
   for (int i = 0; i < kDims; ++i) outs[warp][lane][i] = acc[i];
   __syncthreads();
-  for (int i = threadIdx.x; i < 32 * kOfBlock; i += 256) {
-    const int n = i / kOfBlock, d = i % kOfBlock, r = r0 + n;
-    if (r >= rows) break;
-    float y = 0.f, all = 0.f;
-    if constexpr (kWays == 1) {
-      y = outs[d / kDims][n][d % kDims], all = sums[0][n];
-    } else {
-      float most = kEmpty;
+  if (threadIdx.x < 32 * kDims) {
+    const int n = threadIdx.x / kDims, d = threadIdx.x % kDims, r = r0 + n;
+    if (r >= rows) return;
+    float y = 0.f, all = 0.f, most = kEmpty;
 #pragma unroll
-      for (int w = 0; w < kWays; ++w) most = fmaxf(most, tops[w][n]);
+    for (int w = 0; w < kWays; ++w) most = fmaxf(most, tops[w][n]);
 #pragma unroll
-      for (int w = 0; w < kWays; ++w) {
-        const float f = ex2(tops[w][n] - most);
-        y = fmaf(f, outs[w][n][d], y), all = fmaf(f, sums[w][n], all);
-      }
+    for (int w = 0; w < kWays; ++w) {
+      const float f = ex2(tops[w][n] - most);
+      y = fmaf(f, outs[w][n][d], y), all = fmaf(f, sums[w][n], all);
     }
     const int tq = r / share, live = a.q_lens ? min(max(a.q_lens[b], 0), a.Tq) : a.Tq;
     const float inv = all > 0.f ? 1.f / all : all == 0.f ? 0.f : all;   // NaN stays
-    static_cast<T*>(a.out)[b * a.os_b + (hk * share + r - tq * share) * a.os_h + static_cast<int64_t>(tq) * a.os_t + dims0 + d] = Elem<T>::from_f(tq < live ? y * inv : 0.f);
+    static_cast<T*>(a.out)[b * a.os_b + (hk * share + r - tq * share) * a.os_h + static_cast<int64_t>(tq) * a.os_t + d0 + d] = Elem<T>::from_f(tq < live ? y * inv : 0.f);
   }
 }
 
@@ -577,16 +642,23 @@ int launch(const Args& a, int dtype, int64_t groups, int row_blocks, cudaStream_
   int rc = make_tensor_map(&k_map, tma_dtype(dtype), 3, a.k, dims, strides, box);
   if (rc == OASR_OK) rc = make_tensor_map(&v_map, tma_dtype(dtype), 3, a.v, dims, strides, box);
   if (rc != OASR_OK) return rc;
-  launch_pdl(fmha_tree_wide_kernel<T, D, kKeys2>, dim3(static_cast<unsigned>(groups * a.splits)), dim3(kThreads), S::kDynamic, s, a, k_map, v_map, row_blocks, piece,
-             device_status_ptr());
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(groups * a.splits));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kDynamic;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = g_pdl ? 1 : 0;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim = {static_cast<unsigned>(a.splits), 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = a.parts == nullptr && a.splits > 1 ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, fmha_tree_wide_kernel<T, D, kKeys2>, a, k_map, v_map, row_blocks, piece, device_status_ptr());
   rc = check_launch("fmha_tree launch");
-  if (rc != OASR_OK || a.splits == 1) return rc;
+  if (rc != OASR_OK || a.parts == nullptr) return rc;
   constexpr int NR = kKeys2 ? 128 : 256;
-  const int64_t blocks = groups * (NR / 32);
-  if (a.splits <= 8)
-    launch_pdl(fmha_tree_wide_join_kernel<T, D, 1>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, a, row_blocks, NR, static_cast<int>(groups));
-  else
-    launch_pdl(fmha_tree_wide_join_kernel<T, D, 8>, dim3(static_cast<unsigned>(blocks * (D / 16))), dim3(256), 0, s, a, row_blocks, NR, static_cast<int>(groups));
+  launch_pdl(fmha_tree_wide_join_kernel<T, D>, dim3(static_cast<unsigned>(groups * (NR / 32) * (D / 4))), dim3(256), 0, s, a, row_blocks, NR, static_cast<int>(groups));
   return check_launch("fmha_tree join launch");
 }
 
