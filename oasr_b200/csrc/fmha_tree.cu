@@ -98,6 +98,31 @@ struct Smem {
   static constexpr int kBytes = (kRings > kMerge ? kRings : kMerge) + kQ;
 };
 
+// The n-th longest sequence, where blocks outnumber their places: a long one that starts last would end alone.  `lens` has room for B + 1.
+constexpr int kMostInOrder = 64;
+template <int kThreads>
+__device__ __forceinline__ int nth_longest(const Args& a, int n, int32_t* lens) {
+  for (int i = threadIdx.x; i < a.B; i += kThreads) {
+    const Sequence s(a, i);
+    lens[i] = s.live > 0 ? max(s.end - s.start, 0) : 0;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.B; i += kThreads) {
+    const int mine = lens[i];
+    int before = 0;
+#pragma unroll 8
+    for (int j = 0; j < a.B; ++j) {
+      const int other = lens[j];
+      before += other > mine || (other == mine && j < i);
+    }
+    if (before == n) lens[a.B] = i;
+  }
+  __syncthreads();
+  const int b = lens[a.B];
+  __syncthreads();   // the room is used for other things
+  return b;
+}
+
 template <typename T, int D, int NT, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, D == 128 ? 8 / kWarps : kWarps == 8 ? 2 : NT == 4 ? 3 : 4) fmha_tree_kernel(const Args a, const int row_blocks) {
   using R = Ring<D, kWarps>;
@@ -111,7 +136,11 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? 8 / kWarps : kWarps ==
   int at = group;
   const int rb = at % row_blocks;
   at /= row_blocks;
-  const int hk = at % a.Hkv, b = at / a.Hkv;
+  const int hk = at % a.Hkv;
+  int b = at / a.Hkv;
+  if constexpr (kWarps == 4) {   // (eight: all blocks have a place)
+    if (a.longest_first) b = nth_longest<kWarps * 32>(a, b, reinterpret_cast<int32_t*>(smem));
+  }
   const int share = a.H / a.Hkv, rows = share * a.Tq, row0 = rb * NR;
   const Sequence seq(a, b);
 
@@ -460,6 +489,7 @@ struct Plan {
   int rows, row_blocks, splits;   // rows of a block; blocks of rows of a (sequence, key head); blocks that share a cache
   int64_t groups;
   bool wide, parts;   // the form for many rows; blocks that share a cache leave partial results
+  bool longest_first;
   int warps;   // of a block of the few-row form
 };
 
@@ -491,6 +521,7 @@ Plan plan(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t D, int64_t keys
     while (s > 1 && s <= kMostOfCluster && p.groups > sm_count() / 18 * (18 / s)) --s;
     p.splits = static_cast<int>(s < 1 ? 1 : s > 256 ? 256 : s);
     p.parts = p.splits > kMostOfCluster;
+    p.longest_first = false;
     return p;
   }
   p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
@@ -504,6 +535,9 @@ Plan plan(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t D, int64_t keys
   if (keys * (s - 1) < 16 * p.warps * 16 * s) s = 1;
   p.splits = static_cast<int>(s < 1 ? 1 : s > 256 ? 256 : s);
   p.parts = p.splits > 1;
+  // (64 sequences of 500 to 6000 keys, 8 heads of 128, 20 rows: 127 us, 159 in their own order; of 300 keys each: 26 and 25.  With 64 dims more blocks have a
+  // place at once, and there is nothing to gain: 113 and 112.)
+  p.longest_first = D == 128 && B > 1 && B <= kMostInOrder && p.groups > slots && keys >= 2048;
   return p;
 }
 
@@ -581,7 +615,7 @@ extern "C" int oasr_b200_fmha_tree(void* out, const int64_t* out_strides, const 
              (long long)workspace_bytes);
   const Args a{out, q, k_pool, v_pool, block_table, seqlens, seqstarts, q_lens, mask, need ? static_cast<float*>(workspace) : nullptr, q_strides[0], q_strides[1],
                q_strides[2], out_strides[0], out_strides[1], out_strides[2], mask_stride, blocks_per_seq, block_size, num_blocks, static_cast<int>(B),
-               static_cast<int>(H), static_cast<int>(Hkv), static_cast<int>(Tq), static_cast<int>(mask_words), p.splits,
+               static_cast<int>(H), static_cast<int>(Hkv), static_cast<int>(Tq), static_cast<int>(mask_words), p.splits, p.longest_first,
                static_cast<float>(scale * 1.4426950408889634)};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   return OB_DISPATCH_HALF(dtype, T_, [&]() -> int { return D == 64 ? run<T_, 64>(a, p, dtype, st) : run<T_, 128>(a, p, dtype, st); });

@@ -15,6 +15,7 @@ struct Args {
   int64_t mask_b;                // words from one sequence's mask to the next one's; 0: one for all
   int64_t blocks_per_seq, block_size, num_blocks;
   int B, H, Hkv, Tq, mask_words, splits;
+  int longest_first;             // sequences in the order of their lengths
   float scale_log2;
 };
 

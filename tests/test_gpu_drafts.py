@@ -124,7 +124,8 @@ CASES = [  # B, H, Hkv, T, D, block, lens, starts, q_lens, width
     (1, 3, 1, 70, 64, 16, [40], None, None, 6), (2, 32, 8, 3, 128, 16, [1000, 7], None, [3, 0], 2), (1, 1, 1, 300, 128, 16, [333], None, [257], 30),
     (3, 16, 2, 16, 64, 16, [5000, 16, 777], None, None, 4), (1, 14, 2, 16, 128, 128, [9001], None, None, 4), (2, 32, 8, 61, 128, 16, [700, 3001], None, [61, 40], 8),
     (1, 4, 4, 40, 64, 16, [2500], [2470], None, 7), (5, 8, 2, 2, 128, 16, [1, 0, 2, 3, 100], None, [1, 2, 2, 2, 2], 1), (2, 16, 1, 9, 64, 32, [4097, 30], None, None, 3),
-    (1, 4, 1, 40, 64, 64, [40000], None, None, 4), (5, 16, 8, 20, 64, 16, [2000, 1500, 20, 700, 1999], None, [20, 7, 20, 0, 19], 3), (3, 16, 8, 9, 128, 32, [3300, 2000, 100], [0, 1990, 99], None, 2)]
+    (1, 4, 1, 40, 64, 64, [40000], None, None, 4), (5, 16, 8, 20, 64, 16, [2000, 1500, 20, 700, 1999], None, [20, 7, 20, 0, 19], 3), (3, 16, 8, 9, 128, 32, [3300, 2000, 100], [0, 1990, 99], None, 2),
+    (40, 8, 8, 3, 128, 16, [(i * 997) % 2100 // (i % 3 + 1) + 3 for i in range(40)], [i % 5 for i in range(40)], [i % 4 for i in range(40)], 1)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
