@@ -80,7 +80,7 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, parents: torch.Ten
     of the cache stay (``commit_drafts``).  A row of logits with a NaN, or whose maximum is not finite, ends the walk with token -1, and so do
     random numbers of 1 or more where nothing of ``p`` is left.  -inf logits are impossible tokens; a draft outside ``[0, V)`` is not accepted.
 
-    Decisions are taken in 64 bits (weights to 1e-12, those below 2^-300 of the largest may be zeros; sums in a fixed order); only rows on the accepted path are read."""
+    Decisions are taken in 64 bits (weights to 2^-31, those below 2^-300 of the largest may be zeros; sums in a fixed order); only rows on the accepted path are read."""
     shape = logits.shape
     if len(shape) != 3 or shape[2] < 1:
         raise RuntimeError(f"logits must be (B, T, V), got {tuple(shape)}")
