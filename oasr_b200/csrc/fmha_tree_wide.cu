@@ -13,6 +13,9 @@
 // they were made of (16 bits for 32) and are the A operand of the second product from there.  The maximum moves only when a score passes it by 2^8.
 // A piece without a page is fetched from behind the pool, which gives zeros.  Values that no row sees become zeros as they are looked through, and
 // so do those that are not finite and that some rows may not see; the rows that do see one get it by hand at the end.
+// Bound by the steps: 256 rows x 128 keys of 128 dims take 4.0k clocks, 2.0k of them products at the tensor cores' rate; the rest is what softmax and products
+// hand over to one another.  8 trees of 61 over 4000 to 8191 keys, 32 heads over 8: 83 us, floor 32 (products and cache alike); the longest sequence's blocks
+// have 32 steps, the mean is 21.
 #include <cuda.h>
 
 #include <type_traits>
@@ -574,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
 }
 
 // Joins the partial results of a group's blocks, more than a cluster has: a block has 4 dims of 32 rows (the lanes), its warps an eighth of the
-// parts each (16 dims: a part's loads fill the registers, and 74 parts take 8 us longer).
+// parts each (16 dims: a part's loads fill the registers, and 74 parts take 7 us longer).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) fmha_tree_wide_join_kernel(const Args a, const int row_blocks, const int NR, const int groups) {
   constexpr int kDims = 4, kWays = 8;
