@@ -12,7 +12,7 @@
 // They come out of a table of 2^(i / 256) and a polynomial of degree 3 for the rest (the method of Tang, "Table-driven implementation of the exponential
 // function in IEEE floating-point arithmetic", 1989).  Weights are taken relative to logits of 0: 64 bits reach 2^250 above and 2^500 below; rows
 // that lie elsewhere are taken again relative to their maximum.
-// Bound by the chain: a node's rows are read, summed and decided before the next one's address is known, 3 to 5 us a node (16 trees of 48 over 131071 bf16 logits: 16.0 us,
+// Bound by the chain: a node's rows are read, summed and decided before the next one's address is known (16 trees of 48 over 131071 bf16 logits: 16.0 us,
 // floor 1.3; 32 chains of 8 with their own probabilities over 65537 fp32 logits: 34.6 us, floor 3.8).
 // p and q unnormalised: with k children rejected  p_k = max(p - beta_k q, 0) / Pi_k,  Pi_k the sum of the numerators, beta_1 = 1 and
 // beta_{k+1} = beta_k + Pi_k.  With q = 1 at x a rejection takes x's weight out of the sum.
