@@ -159,12 +159,13 @@ struct Vec {
   __device__ __forceinline__ const T& operator[](int i) const { return p[i / Elem<T>::kVec].v[i % Elem<T>::kVec]; }
   __device__ __forceinline__ float operator()(int i) const { return Elem<T>::to_f((*this)[i]); }
 };
-// The largest of many logits (NaN where there is one) and logits raised to a least one, two 16-bit ones an instruction.
+// The largest of many logits (NaN where there is one) and logits raised to a least one, two 16-bit ones an instruction.  That one lies between kLeast
+// and -kFinest (see verify_kernel): the type has it to its full precision there (fp16: above its subnormal numbers), and the rates, 1.3e5 over it, fit fp32.
 template <typename T>
 struct Range;
 template <>
 struct Range<float> {
-  static constexpr float kLeast = -FLT_MAX;
+  static constexpr float kLeast = -FLT_MAX, kFinest = 1e-32f;
   float lo, top = -INFINITY;
   __device__ __forceinline__ explicit Range(float l) : lo(l) {}
   __device__ __forceinline__ void note(const Vec<float>& x) {
@@ -205,12 +206,12 @@ struct Range16 {
 template <>
 struct Range<__half> : Range16<__half, __half2> {
   using Range16::Range16;
-  static constexpr float kLeast = -65504.f;
+  static constexpr float kLeast = -65504.f, kFinest = 6.103515625e-5f;
 };
 template <>
 struct Range<__nv_bfloat16> : Range16<__nv_bfloat16, __nv_bfloat162> {
   using Range16::Range16;
-  static constexpr float kLeast = -3.3895314e38f;
+  static constexpr float kLeast = -3.3895314e38f, kFinest = 1e-32f;
 };
 template <typename T>
 struct Row {
@@ -515,7 +516,8 @@ __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel
       return same;
     };
     weigh.relative_to(0.f, true);
-    const bool in_range = !greedy && weigh.lo > Range<T>::kLeast;
+    // (Temperatures of up to 3e-35, fp16 2e-7, or from 1e36, fp16 200, on: weights relative to the row's largest logit, in 64 bits throughout.)
+    const bool in_range = !greedy && weigh.lo > Range<T>::kLeast && weigh.lo <= -Range<T>::kFinest;
     if (in_range && kid0 < a.T && more >= a.T && each >= 2 && each < kMostUnits) {
       // ---- a child that is accepted, or refused, by more than what fp32 may be off needs no more than that (runs of less are as fast in 64 bits)
       const float rate = weigh.rate_hi * (1.f / kTable);
