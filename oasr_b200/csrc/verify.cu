@@ -613,8 +613,11 @@ __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel
     // The warps' sums in the order of the vocabulary, `span` to a lane, without the children's weights where those are out.
     const int span = (slots + 31) / 32;
     double part[kSlots / 32];
+    auto take_sums = [&]() {
 #pragma unroll
-    for (int i = 0; i < kSlots / 32; ++i) part[i] = i < span && lane * span + i < slots ? sh.sum[turn ^ 1][lane * span + i] : 0.;
+      for (int i = 0; i < kSlots / 32; ++i) part[i] = i < span && lane * span + i < slots ? sh.sum[turn ^ 1][lane * span + i] : 0.;
+    };
+    take_sums();
     const bool without = q == nullptr && kid0 < a.T;
     auto each_kid = [&](auto&& f) {   // f(token, weight) for every rejected child's token, once
       int left = several ? take_kids(kid0) : a.T;
@@ -630,8 +633,10 @@ __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel
         left = take_kids(left);
       }
     };
-    bool touched = false;   // a child's token lies in this warp's run
-    if (without)
+    // A run that has little but its children's weights (2^-32 of its sum; the differences are off by 2^-35 at most) is summed again without them: a
+    // difference of roundings would be a run that has no token to give, or hide one that has.
+    bool touched = false, again = false;   // a child's token lies in this warp's run; there are such runs
+    if (without) {
       each_kid([&](int token, double w) {
         const int unit = (token + row.skew) / (kVec * 32), split = longer * (each + 1);
         const int owner = unit < split ? unit / (each + 1) : longer + (unit - split) / each;   // (`each` 0: all units lie below the split)
@@ -640,67 +645,84 @@ __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel
         for (int i = 0; i < kSlots / 32; ++i)
           if (owner == lane * span + i && i < span) part[i] = fmax(part[i] - w, 0.);
       });
-    const double lane_sum = (part[0] + part[1]) + (part[2] + part[3]), upto = warp_scan64(lane_sum);
-    const double all = __shfl_sync(0xffffffffu, upto, 31), target = static_cast<double>(u[0]) * all;
-    // the first warp whose cumulative sum passes the target, else the last one with something in it
-    const uint32_t past = __ballot_sync(0xffffffffu, lane_sum > 0. && upto > target), some = __ballot_sync(0xffffffffu, lane_sum > 0.);
-    const int lane_of = past ? __ffs(past) - 1 : 31 - __clz(some | 1u);
-    double before = upto - lane_sum, prefix = 0., last_prefix = 0.;
-    int owner = -1, last_owner = -1;
 #pragma unroll
-    for (int i = 0; i < kSlots / 32; ++i) {
-      if (part[i] > 0.) {
-        last_owner = lane * span + i, last_prefix = before;
-        if (owner < 0 && before + part[i] > target) owner = lane * span + i, prefix = before;
+      for (int i = 0; i < kSlots / 32; ++i) {
+        const double with = i < span && lane * span + i < slots ? sh.sum[turn ^ 1][lane * span + i] : 0.;
+        again |= with > 0. && part[i] <= with * 0x1p-32;
       }
-      before += part[i];
+      again = __any_sync(0xffffffffu, again);
     }
-    if (owner < 0) owner = last_owner, prefix = last_prefix;
-    owner = __shfl_sync(0xffffffffu, owner, lane_of);
-    const double goal = target - __shfl_sync(0xffffffffu, prefix, lane_of);
-    if (!some) {
-      if (writer) tokens[count] = -1;
-    } else if (owner == mine) {   // its run once more: 256 logits at a time until the goal is passed
-      double passed = 0.;
-      int last_positive = -1, token = -1;
 #pragma unroll 1
-      for (int base = j0; base < j1 && token < 0; base += 32) {
-        const int j = base + lane;
-        double w[kVec] = {};
-        if (j < j1) {
-          const Vec<T> x = row.load(j);
-          float y[kVec] = {};
-          if (beta > 0.) row.load_probs(q, j, y);
-          remaining(weigh, x, y, inv, beta, w);
-        }
-        if (touched)
-          each_kid([&](int out, double) {
-            const int off = out - row.first(j);
+    for (;; again = false) {
+      double goal = INFINITY;
+      bool here = touched;   // whether this warp walks through its run
+      if (!again) {
+        const double lane_sum = (part[0] + part[1]) + (part[2] + part[3]), upto = warp_scan64(lane_sum);
+        const double all = __shfl_sync(0xffffffffu, upto, 31), target = static_cast<double>(u[0]) * all;
+        // the first warp whose cumulative sum passes the target, else the last one with something in it
+        const uint32_t past = __ballot_sync(0xffffffffu, lane_sum > 0. && upto > target), some = __ballot_sync(0xffffffffu, lane_sum > 0.);
+        const int lane_of = past ? __ffs(past) - 1 : 31 - __clz(some | 1u);
+        double before = upto - lane_sum, prefix = 0., last_prefix = 0.;
+        int owner = -1, last_owner = -1;
 #pragma unroll
-            for (int i = 0; i < kVec; ++i)
-              if (off == i) w[i] = 0.;
-          });
-        int last = -1;
-#pragma unroll
-        for (int i = 0; i < kVec; ++i)
-          if (w[i] > 0.) last = row.first(j) + i;
-        const double sum = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])), through = warp_scan64(sum);
-        const uint32_t there = __ballot_sync(0xffffffffu, last >= 0 && passed + through > goal), positive = __ballot_sync(0xffffffffu, last >= 0);
-        if (there) {
-          double run = passed + (through - sum);
-          int found = last;   // (sums in another order may fall short of the goal by a rounding)
-          bool done = false;
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            run += w[i];
-            if (!done && w[i] > 0. && run > goal) found = row.first(j) + i, done = true;
+        for (int i = 0; i < kSlots / 32; ++i) {
+          if (part[i] > 0.) {
+            last_owner = lane * span + i, last_prefix = before;
+            if (owner < 0 && before + part[i] > target) owner = lane * span + i, prefix = before;
           }
-          token = __shfl_sync(0xffffffffu, found, __ffs(there) - 1);
+          before += part[i];
         }
-        if (positive) last_positive = __shfl_sync(0xffffffffu, last, 31 - __clz(positive));
-        passed += __shfl_sync(0xffffffffu, through, 31);
+        if (owner < 0) owner = last_owner, prefix = last_prefix;
+        owner = __shfl_sync(0xffffffffu, owner, lane_of);
+        goal = target - __shfl_sync(0xffffffffu, prefix, lane_of);
+        here = some && owner == mine;
+        if (!some && writer) tokens[count] = -1;
       }
-      if (lane == 0) tokens[count] = token >= 0 ? token : last_positive;
+      double passed = 0.;
+      if (here) {   // its run once more: 256 logits at a time until the goal is passed
+        int last_positive = -1, token = -1;
+#pragma unroll 1
+        for (int base = j0; base < j1 && token < 0; base += 32) {
+          const int j = base + lane;
+          double w[kVec] = {};
+          if (j < j1) {
+            const Vec<T> x = row.load(j);
+            float y[kVec] = {};
+            if (beta > 0.) row.load_probs(q, j, y);
+            remaining(weigh, x, y, inv, beta, w);
+          }
+          if (touched)
+            each_kid([&](int out, double) {
+              const int off = out - row.first(j);
+#pragma unroll
+              for (int i = 0; i < kVec; ++i)
+                if (off == i) w[i] = 0.;
+            });
+          int last = -1;
+#pragma unroll
+          for (int i = 0; i < kVec; ++i)
+            if (w[i] > 0.) last = row.first(j) + i;
+          const double sum = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])), through = warp_scan64(sum);
+          const uint32_t there = __ballot_sync(0xffffffffu, last >= 0 && passed + through > goal), positive = __ballot_sync(0xffffffffu, last >= 0);
+          if (there) {
+            double run = passed + (through - sum);
+            int found = last;   // (sums in another order may fall short of the goal by a rounding)
+            bool done = false;
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+              run += w[i];
+              if (!done && w[i] > 0. && run > goal) found = row.first(j) + i, done = true;
+            }
+            token = __shfl_sync(0xffffffffu, found, __ffs(there) - 1);
+          }
+          if (positive) last_positive = __shfl_sync(0xffffffffu, last, 31 - __clz(positive));
+          passed += __shfl_sync(0xffffffffu, through, 31);
+        }
+        if (!again && lane == 0) tokens[count] = token >= 0 ? token : last_positive;
+      }
+      if (!again) break;
+      meet(touched ? passed : sh.sum[turn ^ 1][mine], 0);
+      take_sums();
     }
     break;
   }

@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 
+import oasr_b200 as ob
 from tests.test_gpu_decoding import DTYPES
 from tests.test_gpu_drafts import check_verify
 
@@ -32,3 +33,67 @@ def test_small_temperatures(dtype, V):
         drafts[::2, 1] = best[::2]                         # the largest, which stands, or one that hardly ever does
         check_verify(x, drafts, np.array([[-1, 0, 1]] * B), rng.rand(B, 3).astype(np.float32), [temp] * B)
         check_verify(x, drafts, np.array([[-1, 0, 0]] * B), rng.rand(B, 3).astype(np.float32), [temp] * B)
+
+
+def refused_children(x, drafts, parents, B, T):
+    """Children that are refused: whatever the kernel makes of it, then the token at the very start of what is left."""
+    u = np.full((B, T), 0.999, np.float32)
+    u[:, 0] = np.random.RandomState(T).rand(B)
+    got = check_verify(x, drafts, parents, u, [1.0] * B)
+    assert (got.counts == 1).all()
+    u[:, 0] = 0.0
+    check_verify(x, drafts, parents, u, [1.0] * B, margin=-1)       # (decisions about children are those that were checked with a margin)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shift", [0.0, -900.0])
+@pytest.mark.parametrize("V,kids", [(12, 2), (300, 2), (5002, 3), (5002, 40), (60001, 5)])
+def test_nothing_is_left_beside_the_refused_children(dtype, shift, V, kids):
+    """All that is possible is a few tokens that lie together, all of them refused children, and one far behind them: that one is next."""
+    rng = np.random.RandomState(V + kids)
+    B, T = 60, kids + 1
+    x = torch.full((B, T, V), -math.inf)
+    drafts = np.zeros((B, T), np.int64)
+    for b in range(B):
+        at = rng.choice(min(V - 1, 2 * kids + 3), kids, replace=False)
+        x[b, 0, at] = torch.from_numpy(rng.randn(kids)).float()
+        x[b, 0, V - 1] = 2.0
+        drafts[b, 1:] = at
+    refused_children((x + shift).to(DTYPES[dtype]).cuda(), drafts, np.zeros((B, T), np.int64), B, T)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shift", [0.0, -900.0])
+@pytest.mark.parametrize("V", [12, 300, 5002, 60001])
+def test_little_is_left_beside_the_refused_children(dtype, shift, V):
+    """A refused child and, next to it, tokens of e^-20 to e^-100 of its weight; a likely token far behind them."""
+    gaps = [20.0, 24.0, 30.0, 36.0, 40.0, 60.0, 100.0]
+    B, T = len(gaps), 3
+    x = torch.full((B, T, V), -math.inf)
+    for b, gap in enumerate(gaps):
+        x[b, 0, 1:V // 2] = 1.0 - gap
+        x[b, 0, [5, V - 1]] = 1.0
+    drafts = np.array([[0, 5, 0]] * B)
+    refused_children((x + shift).to(DTYPES[dtype]).cuda(), drafts, np.zeros((B, T), np.int64), B, T)
+
+
+def test_shortened_rows_captured():
+    """The second look at the runs of refused children inside a graph: the same answers."""
+    V, B, T = 5002, 8, 4
+    x = torch.full((B, T, V), -math.inf)
+    x[:, 0, 3:6] = torch.randn(B, 3, generator=torch.Generator().manual_seed(2))
+    x[:, 0, 4000] = 2.0
+    x, drafts = x.cuda(), torch.tensor([[0, 3, 4, 5]] * B, device="cuda", dtype=torch.int32)
+    parents, u = torch.zeros(B, T, device="cuda", dtype=torch.int32), torch.full((B, T), 0.999, device="cuda")
+    u[:, 0] = 0.0
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    want = ob.verify_drafts(x, drafts, parents, u)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        got = ob.verify_drafts(x, drafts, parents, u)
+    for _ in range(3):
+        got.tokens.fill_(-7)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and (got.tokens[:, 0] == 4000).all()
