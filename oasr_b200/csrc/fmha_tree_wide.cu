@@ -183,13 +183,15 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
         return v;
       };
       float f[kMaxCluster], top = kEmpty, sum = 0.f;
+      uint32_t blocks = 0;   // those with keys; the others have left nothing but a maximum of -inf
 #pragma unroll
-      for (int x = 0; x < kMaxCluster; ++x) f[x] = x < a.splits ? of(my_m + r, x) : kEmpty, top = fmaxf(top, f[x]);
+      for (int x = 0; x < kMaxCluster; ++x) f[x] = x < a.splits ? of(my_m + r, x) : -INFINITY, top = fmaxf(top, f[x]);
 #pragma unroll
       for (int x = 0; x < kMaxCluster; ++x) {
-        const bool some = f[x] > kEmpty;
-        f[x] = some ? ex2(f[x] - top) : 0.f;
-        if (some) sum = fmaf(f[x], of(my_l + r, x), sum);
+        if (!(f[x] > -INFINITY)) continue;
+        blocks |= 1u << x;
+        f[x] = ex2(f[x] - top);
+        sum = fmaf(f[x], of(my_l + r, x), sum);   // (a sum that is NaN, of a query or keys that are, counts whatever its maximum)
       }
       const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;   // NaN stays
       T* const out = out_row(rr);
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
         float y[8] = {};
 #pragma unroll
         for (int x = 0; x < kMaxCluster; ++x)
-          if (f[x] != 0.f)   // (a block without keys has nothing there)
+          if (blocks >> x & 1u)   // (a weight of zero too: it makes NaN of values that are not finite)
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = fmaf(f[x], of(my_o + (8 * c + i) * NR + r, x), y[i]);
         *reinterpret_cast<uint4*>(out + 8 * c) = make_uint4(pack2<T>(y[0] * inv, y[1] * inv), pack2<T>(y[2] * inv, y[3] * inv), pack2<T>(y[4] * inv, y[5] * inv),
@@ -209,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
   };
   if (tiles == 0) {   // nothing to see: zero rows
     if (cluster) {
-      for (int i = threadIdx.x; i < NR; i += kThreads) my_m[i] = kEmpty;
+      for (int i = threadIdx.x; i < NR; i += kThreads) my_m[i] = -INFINITY;
     } else if (part) {
       for (int i = threadIdx.x; i < NR * (D + 2); i += kThreads) part[i] = i < NR ? kEmpty : 0.f;
     } else {

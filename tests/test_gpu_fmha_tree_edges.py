@@ -1,0 +1,91 @@
+"""Attention of trees of drafts where blocks share a cache: what is not finite, against plain implementations in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import oasr_b200 as ob
+from tests.test_gpu_decoding import DTYPES, pages, rand
+from tests.test_gpu_drafts import bound, check, dense16, i32, pool16, tree_form, words_of  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+# rows that share a key head, and keys of a sequence: one block, blocks as a cluster or with partial results, many partial results
+SPLITS = [(2, 64, 1, 700), (5, 128, 4, 3000), (40, 64, 2, 3000), (70, 128, 4, 3000), (5, 64, 4, 40000), (40, 128, 2, 40000)]
+
+
+def attend(q, pools, bt, N, rows, scale, start=0):
+    return ob.fmha_tree(q, *pools, softmax_scale=scale, block_table=bt.cuda(), cache_seqlens=i32([N]), cache_seqstarts=i32([start]), tree_mask=words_of(rows, q.shape[2]).cuda()).cpu().double()
+
+
+def plain(q, k, v, scale, N, rows, start=0):
+    """One sequence in 64 bits: the result, and for each row the sum of weights times |v|."""
+    T, share = q.shape[2], q.shape[1] // k.shape[1]
+    seen = torch.arange(k.shape[2])[None].repeat(T, 1) < N - T
+    for t, row in enumerate(rows):
+        seen[t, torch.tensor(row) + N - T] = True
+    seen[:, :start] = False
+    k, v = k[0].repeat_interleave(share, 0), v[0].repeat_interleave(share, 0)
+    p = torch.softmax((q[0] @ k.transpose(1, 2) * scale).masked_fill(~seen, -math.inf), -1).nan_to_num(0)
+    return (p @ v)[None], (p @ v.abs())[None]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("far", [False, True], ids=["", "no_weight"])
+@pytest.mark.parametrize("T,D,share,N", SPLITS)
+def test_values_that_are_not_finite_in_split_caches(tree_form, dtype, far, T, D, share, N):
+    """A row that sees such a value has it, however little the weight (infinity, or NaN where the weight is zero in fp32); no other row does."""
+    dt, block = DTYPES[dtype], 16
+    bt, n = pages(3, 1, -(-N // block))
+    pools = pool16(10, n, block, 2, D, dt)
+    way = torch.sign(rand(20, D))
+    q = (way + 0.01 * rand(12, 1, 2 * share, T, D)).to(dt).cuda()
+    if far:                                                # the first keys have scores of more than 170 above all others
+        for j in range(40):
+            pools[0][bt[0, j // block], j % block] = (2048.0 / D * way).to(dt).cuda()
+    k, v, _ = dense16(pools, bt)
+    rows = [sorted({t, t // 2, 0}) for t in range(T)]
+    def put(u, head, dim, value):
+        pools[1][bt[0, (N - T + u) // block], (N - T + u) % block, head, dim] = value
+    put(1, 1, 5, math.nan)
+    put(1, 1, D - 1, math.inf)
+    got = attend(q, pools, bt, N, rows, 0.125)
+    x = q.cpu().double()
+    want, size = plain(x, k, v, 0.125, N, rows)
+    tol = bound(x, k, 0.125, size, want, dt)
+    for t in range(T):
+        if 1 in rows[t]:
+            want[0, share:, t, 5], want[0, share:, t, D - 1] = math.nan, math.inf
+    assert torch.equal(torch.isfinite(got), torch.isfinite(want))
+    assert torch.isnan(got[torch.isnan(want)]).all()
+    if not far:
+        assert (got[torch.isinf(want)] == math.inf).all()
+    fine = torch.isfinite(want)
+    check(got[fine], want[fine], tol[fine])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,D,share,N", SPLITS)
+def test_queries_and_keys_that_are_nan_in_split_caches(tree_form, dtype, T, D, share, N):
+    """A query that is NaN gives a row of it.  So does a seen key, alone in its tile, in a block of its own: a start leaves few tiles for many blocks."""
+    dt, block = DTYPES[dtype], 16
+    N = N // 128 * 128 + 1                                 # the last key is the only one of its tile
+    bt, n = pages(3, 1, -(-N // block))
+    pools = pool16(10, n, block, 2, D, dt)
+    k, v, _ = dense16(pools, bt)
+    rows = [sorted({t, t // 2, 0}) for t in range(T)]
+    q = rand(12, 1, 2 * share, T, D).to(dt).cuda()
+    q[0, 0, T - 1] = math.nan
+    pools[0][bt[0, (N - 1) // block], (N - 1) % block, 1, 3] = math.nan
+    x = q.nan_to_num(0).cpu().double()
+    for start in (0, N - 300):
+        got = attend(q, pools, bt, N, rows, 0.125, start)
+        want, size = plain(x, k, v, 0.125, N, rows, start)
+        tol = bound(x, k, 0.125, size, want, dt)
+        want[0, 0, T - 1] = math.nan
+        for t in range(T):
+            if T - 1 in rows[t]:
+                want[0, share:, t] = math.nan
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.isfinite(got[~torch.isnan(want)]).all()
+        fine = torch.isfinite(want)
+        check(got[fine], want[fine], tol[fine])
