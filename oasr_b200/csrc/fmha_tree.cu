@@ -8,7 +8,7 @@
 // Keys are the M side of both products (mma.m16n8k16: S^T = K Q^T, O^T = V^T P^T), the rows of all query heads that share a key
 // head the N side, so that a single token wastes 7 of 8 columns and not 15 of 16 rows.  P takes one transpose in registers
 // (movmatrix) between the two.  Weights are rounded to the type before they meet the values, as in the package's other attention; their
-// sum, the maximum and the output are fp32.  The maximum moves only when a score passes it by 2^8.
+// sum, the maximum and the output are fp32.  What weights are relative to (m) moves only when a score passes it by far (kLag).
 // Every warp walks its own tiles of 16 keys (always of one page) with its own maximum, sum and output, behind its own ring of tiles in
 // shared memory that asynchronous copies fill; the warps of a block meet in shared memory at the end, and the blocks that share a long
 // cache through partial results that a second, small kernel joins.
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? 8 / kWarps : kWarps ==
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) raise |= fmaxf(s[n][c], s[n][2 + c]) * unit > m[n][c] + 8.f;
+      for (int c = 0; c < 2; ++c) raise |= fmaxf(s[n][c], s[n][2 + c]) * unit > m[n][c] + (kBelow<T> + kLag);
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? 8 / kWarps : kWarps ==
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-          v = fmaxf(v, m[n][c]);
+          v = fmaxf(v - kBelow<T>, m[n][c]);
           const float f = ex2(m[n][c] - v);
           m[n][c] = v;
           l[n][c] *= f;

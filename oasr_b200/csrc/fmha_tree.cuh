@@ -1,5 +1,7 @@
 // What the kernels of attention over 16-bit pages with a tree of drafted tokens share.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace ob {
@@ -22,6 +24,13 @@ struct Args {
 constexpr int kMostOfCluster = 8;   // blocks of the form for many rows that share a cache as a cluster; more leave partial results
 
 constexpr float kEmpty = -3e38f;   // a maximum below every score: differences to it overflow to -inf or are zero, never NaN
+
+// Weights are taken relative to a reference, kBelow (in powers of two) below the row's maximum when it is set; it moves when a score passes it by
+// kBelow + kLag.  So fp16 weights lie up to 2^15, are rounded by half a step down to 2^-21 of the maximum, and vanish below 2^-32 of it.  (Relative to
+// the maximum itself, 2^-14 and 2^-25: many keys of little weight behind one of much were lost.)  bf16 has the exponents of fp32.
+template <typename T>
+constexpr float kBelow = std::is_same<T, __half>::value ? 7.f : 0.f;
+constexpr float kLag = 8.f;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

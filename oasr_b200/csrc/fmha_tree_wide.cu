@@ -10,7 +10,8 @@
 //   17        fetches tiles of keys and values: pieces of 16 to 128 rows (whatever power of two divides a page), 128-byte swizzle.
 // The streams are the two halves of 256 rows over the same keys, or the same 128 rows over the even and the odd tiles (kKeys2), put together at
 // the end.  They run half a step apart: while one's softmax works, the tensor cores have the other's products.  Weights take the place of the scores
-// they were made of (16 bits for 32) and are the A operand of the second product from there.  The maximum moves only when a score passes it by 2^8.
+// they were made of (16 bits for 32) and are the A operand of the second product from there.  What they are relative to (m) moves only when
+// a score passes it by far (kLag).
 // A piece without a page is fetched from behind the pool, which gives zeros.  Values that no row sees become zeros as they are looked through, and
 // so do those that are not finite and that some rows may not see; the rows that do see one get it by hand at the end.
 // Bound by the steps: 256 rows x 128 keys of 128 dims take 4.0k clocks, 2.0k of them products at the tensor cores' rate; the rest is what softmax and products
@@ -446,14 +447,15 @@ __global__ void __launch_bounds__(kThreads, 1) fmha_tree_wide_kernel(const Args 
       for (int i = 0; i < 64; ++i) t[i & 3] = fmaxf(t[i & 3], __uint_as_float(v[i]));
       const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * unit;
       ptx::tc_fence_before_sync();
-      if (any_of_rows(rows_id, top > m + 8.f)) {   // (also: all scores of these rows are read, and weights may take their place)
+      if (any_of_rows(rows_id, top > m + (kBelow<T> + kLag))) {   // (also: all scores of these rows are read, and weights may take their place)
         float both = top;   // of the row: there and back between its two threads
         if (half) *row_top = top;
         ptx::named_barrier_sync(rows_id, 64);
         if (!half) *row_top = both = fmaxf(top, *row_top);
         ptx::named_barrier_sync(rows_id, 64);
         if (half) both = *row_top;
-        const bool raise = both > m + 8.f;
+        const bool raise = both > m + (kBelow<T> + kLag);
+        both -= kBelow<T>;
         const float f = raise ? ex2(m - both) : 1.f;
         m = raise ? both : m;
         l *= f;

@@ -1,4 +1,4 @@
-"""Attention of trees of drafts where blocks share a cache: what is not finite, against plain implementations in 64 bits."""
+"""Attention of trees of drafts where blocks share a cache: what is not finite, and many keys of little weight, against plain implementations in 64 bits."""
 import math
 
 import pytest
@@ -89,3 +89,28 @@ def test_queries_and_keys_that_are_nan_in_split_caches(tree_form, dtype, T, D, s
         assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.isfinite(got[~torch.isnan(want)]).all()
         fine = torch.isfinite(want)
         check(got[fine], want[fine], tol[fine])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,D,share,N", SPLITS)
+def test_many_keys_of_little_weight(tree_form, dtype, T, D, share, N):
+    """The first key has nearly all the weight and values of zero; the others, 2^-14 to 2^-25 of it each, are what comes out.  A weight is off by half a
+    step, and in fp16 by half a step of its subnormal numbers when it is taken relative to 2^-7 of the largest: 2^-32 of that."""
+    dt, block = DTYPES[dtype], 16
+    bt, n = pages(3, 1, -(-N // block))
+    pools = [torch.zeros(n, block, 1, D, dtype=dt, device="cuda") for _ in range(2)]
+    pools[1].copy_((1 + rand(5, n, block, 1, D).abs().clamp(max=6)).to(dt))
+    pools[0][bt[0, 0], 0, 0, 0] = 1.0
+    pools[1][bt[0, 0], 0] = 0.0
+    k, v, _ = dense16(pools, bt)
+    q = torch.zeros(1, share, T, D)
+    q[0, :, :, 0] = torch.linspace(14.1, 24.9, share * T).view(share, T) * math.log(2)
+    q = q.to(dt).cuda()
+    rows = [list(range(t + 1)) for t in range(T)]
+    got = attend(q, pools, bt, N, rows, 1.0)
+    x = q.cpu().double()
+    want, size = plain(x, k, v, 1.0, N, rows)
+    tol = bound(x, k, 1.0, size, want, dt)
+    if dt == torch.float16:
+        tol -= (2.0 ** -25 - 2.0 ** -32) * 8 * (1 + k.shape[2])
+    check(got, want, tol)
