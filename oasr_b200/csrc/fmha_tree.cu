@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? 8 / kWarps : kWarps ==
 
   // ---- queries as the second operand (column g), with the sign of the scale
   const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-  const float unit = fmaxf(fabsf(a.scale_log2), 1.2e-38f);   // a scale of zero leaves masked scores at -inf
+  const float unit = unit_of(a);
   auto q_row = [&](int r) { return static_cast<const T*>(a.q) + b * a.qs_b + (hk * share + r % share) * a.qs_h + static_cast<int64_t>(r / share) * a.qs_t; };
   uint32_t qf[NT == 4 ? 1 : NT][NT == 4 ? 1 : KD][2];
   const uint32_t q_smem = ptx::smem_u32(smem) + (S::kBytes - S::kQ);
@@ -308,18 +308,18 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? 8 / kWarps : kWarps ==
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) raise |= fmaxf(s[n][c], s[n][2 + c]) * unit > m[n][c] + (kBelow<T> + kLag);
+      for (int c = 0; c < 2; ++c) raise |= (fmaxf(s[n][c], s[n][2 + c]) - m[n][c]) * unit > kLag;
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float v = fmaxf(s[n][c], s[n][2 + c]) * unit;
+          float v = fmaxf(s[n][c], s[n][2 + c]);
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
           v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-          v = fmaxf(v - kBelow<T>, m[n][c]);
-          const float f = ex2(m[n][c] - v);
+          v = fmaxf(v, m[n][c]);
+          const float f = ex2((m[n][c] - v) * unit);
           m[n][c] = v;
           l[n][c] *= f;
 #pragma unroll
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? 8 / kWarps : kWarps ==
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const float e0 = ex2(fmaf(s[n][2 * x], unit, -m[n][0])), e1 = ex2(fmaf(s[n][2 * x + 1], unit, -m[n][1]));
+        const float e0 = ex2(fmaf(s[n][2 * x] - m[n][0], unit, kBelow<T>)), e1 = ex2(fmaf(s[n][2 * x + 1] - m[n][1], unit, kBelow<T>));
         l[n][0] += e0;
         l[n][1] += e1;
         pf[n][x] = transpose8x8(Op<T>::pack(e0, e1));
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 128 ? 8 / kWarps : kWarps ==
     for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sh.m[w][n]);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = ex2(sh.m[w][n] - top);
+      const float f = ex2((sh.m[w][n] - top) * unit);
       const float4 a0 = *reinterpret_cast<const float4*>(&sh.o[w][n][d]), a1 = *reinterpret_cast<const float4*>(&sh.o[w][n][d + 4]);
       sum = fmaf(f, sh.l[w][n], sum);
       acc[0] = fmaf(f, a0.x, acc[0]), acc[1] = fmaf(f, a0.y, acc[1]), acc[2] = fmaf(f, a0.z, acc[2]), acc[3] = fmaf(f, a0.w, acc[3]);
@@ -442,6 +442,7 @@ __global__ void __launch_bounds__(256) fmha_tree_join_kernel(const Args a, const
   const bool there = group < groups && r < share * a.Tq;
   const int64_t part = part_floats<D>(NR), step = part * groups;
   const float* src = a.parts + group * part;
+  const float unit = unit_of(a);
   float top = kEmpty, sum = 0.f, acc[kV] = {};
   if (there) {
     for (int s = way + lane * kWays; s < a.splits; s += 32 * kWays) top = fmaxf(top, src[s * step + 2 * n]);
@@ -450,7 +451,7 @@ __global__ void __launch_bounds__(256) fmha_tree_join_kernel(const Args a, const
     for (int s = way; s < a.splits; s += kWays) {
       const float* p = src + s * step;
       const float2 ml = *reinterpret_cast<const float2*>(p + 2 * n);
-      const float f = ex2(ml.x - top);
+      const float f = ex2((ml.x - top) * unit);
       float v[kV];
 #pragma unroll
       for (int x = 0; x < kV; ++x) v[x] = p[2 * NR + n * D + lane * kV + x];
@@ -467,13 +468,13 @@ __global__ void __launch_bounds__(256) fmha_tree_join_kernel(const Args a, const
     if (way) return;
 #pragma unroll
     for (int w = 1; w < kWays; ++w) top = fmaxf(top, tops[warp + w]);
-    const float own = ex2(tops[warp] - top);
+    const float own = ex2((tops[warp] - top) * unit);
     sum *= own;
 #pragma unroll
     for (int x = 0; x < kV; ++x) acc[x] *= own;
 #pragma unroll
     for (int w = 1; w < kWays; ++w) {
-      const float f = ex2(tops[warp + w] - top);
+      const float f = ex2((tops[warp + w] - top) * unit);
       sum = fmaf(f, sums[warp + w], sum);
 #pragma unroll
       for (int x = 0; x < kV; ++x) acc[x] = fmaf(f, outs[warp + w][lane * kV + x], acc[x]);

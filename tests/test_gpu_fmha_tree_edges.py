@@ -1,11 +1,11 @@
-"""Attention of trees of drafts where blocks share a cache: what is not finite, and many keys of little weight, against plain implementations in 64 bits."""
+"""Attention of trees of drafts where blocks share a cache: what is not finite, many keys of little weight, and scores of any size, against plain implementations in 64 bits."""
 import math
 
 import pytest
 import torch
 
 import oasr_b200 as ob
-from tests.test_gpu_decoding import DTYPES, pages, rand
+from tests.test_gpu_decoding import DTYPES, HALF, pages, rand
 from tests.test_gpu_drafts import bound, check, dense16, i32, pool16, tree_form, words_of  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -114,3 +114,36 @@ def test_many_keys_of_little_weight(tree_form, dtype, T, D, share, N):
     if dt == torch.float16:
         tol -= (2.0 ** -25 - 2.0 ** -32) * 8 * (1 + k.shape[2])
     check(got, want, tol)
+
+
+LARGE = {"bf16": (2.0 ** 22, 2.0 ** 26, 2.0 ** 30, 2.0 ** 40, 2.0 ** 80, 2.0 ** 126), "fp16": (2.0 ** 22, 2.0 ** 26, 2.0 ** 29)}
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,D,share,N", SPLITS)
+def test_scores_of_any_finite_size(tree_form, dtype, T, D, share, N):
+    """Scores far from zero, above and below it, that are exact in fp32: all weight to the largest, equal ones in equal parts, and next to them scores that
+    differ by small whole numbers."""
+    dt, block = DTYPES[dtype], 16
+    bt, n = pages(3, 1, -(-N // block))
+    rows = [list(range(t + 1)) for t in range(T)]
+    g = torch.Generator().manual_seed(N)
+    for level in LARGE[dtype]:
+        for sign, scale in ((1, 1.0), (-1, 1.0), (-1, 0.7), (1, -1.3)):
+            if dtype == "fp16" and level == 2.0 ** 29:
+                scale *= 2.0 ** 60
+            pools = pool16(10, n, block, 1, D, dt)
+            side = 2.0 ** (math.log2(level) // 2)           # a score: level times 1, 1 + 1/8, ..., 1 + 7/8, plus 0 to 3
+            pools[0].zero_()
+            steps = torch.randint(0, 8, (n, block), generator=g) if level > 2.0 ** 22 else torch.zeros(n, block)
+            pools[0][:, :, 0, 0] = (sign * level / side * (1 + steps / 8)).to(dt).cuda()
+            pools[0][:, :, 0, D - 1] = torch.randint(0, 4, (n, block), generator=g).to(dt).cuda()
+            k, v, _ = dense16(pools, bt)
+            q = torch.zeros(1, share, T, D)
+            q[..., 0] = side
+            q[..., D - 1] = 1.0 if level <= 2.0 ** 22 else 0.0
+            got = attend(q.to(dt).cuda(), pools, bt, N, rows, scale)
+            want, size = plain(q.double(), k, v, scale, N, rows)
+            # (weights are rounded, and off by 2^-16 for their exponents, as in `bound`; the scores are exact)
+            least = 2.0 ** -32 if dt == torch.float16 else 2.0 ** -118
+            check(got, want, HALF[dt] * want.abs() + (HALF[dt] + 2.0 ** -16) * size + least * 8 * (1 + k.shape[2]))
