@@ -222,6 +222,9 @@ class PagedKVCacheQ4:
         return gather_paged_kv_q4(*self.pools, self.block_table, None, max_total_kv)
 
 
+_WHOLE = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+
+
 def _commit(pools, geometry, block_table, offset, path, counts):
     """``geometry(shape)``: (num_blocks, block_size, outer) of one layer's pages, and which of its dimensions a row has."""
     if path.dim() != 2:
@@ -241,9 +244,12 @@ def _commit(pools, geometry, block_table, offset, path, counts):
         entry.data, entry.layers, entry.outer, entry.row_bytes = pool.data_ptr(), layers, outer, row * pool.element_size()
     if shape is None:
         raise ValueError("no pools")
-    block_table = _table32(block_table, B)
     if isinstance(offset, int):
         offset = torch.full((B,), offset, dtype=torch.int32, device=path.device)
+    for name, index in (("block_table", block_table), ("offset", offset), ("path", path), ("counts", counts)):
+        if index.dtype not in _WHOLE:      # (rows are moved in place by them: no rounding of something else)
+            raise ValueError(f"{name} must be whole numbers, got {index.dtype}")
+    block_table = _table32(block_table, B)
     offset, counts = _index32("offset", offset, B), _index32("counts", counts, B)
     path = _narrow(path) if path.dtype != torch.int32 else path
     if not path.is_contiguous():
