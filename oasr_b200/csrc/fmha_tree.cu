@@ -79,10 +79,12 @@ __device__ __forceinline__ void copies_but() {   // all but the last N groups of
 
 constexpr int kKeys = 16;
 
-// A tile of 16 keys in the ring, K then V; the 16-byte pieces of row r lie at piece ^ (r & 7).
-template <int D, int kWarps>
+// A tile of 16 keys in the ring, K then V; the 16-byte pieces of row r lie at piece ^ (r & 7).  With four stages only three blocks of four warps of 64 dims
+// have a place on an SM, with three stages four: 64 sequences of 4000 keys, 8 heads, 4 rows 99.6 and 81.7 us, 16 rows 110 and 87 (200 sequences of 2000
+// keys, 4 heads: 65 and 68, 68 and 76).
+template <int D>
 struct Ring {
-  static constexpr int kRow = 2 * D, kHalf = kKeys * kRow, kBytes = 2 * kHalf, kStages = D == 64 && kWarps == 4 ? 4 : 3;
+  static constexpr int kRow = 2 * D, kHalf = kKeys * kRow, kBytes = 2 * kHalf, kStages = 3;
   static __device__ __forceinline__ int at(int row, int piece) { return row * kRow + ((piece ^ (row & 7)) << 4); }
 };
 
@@ -94,7 +96,7 @@ struct Merge {   // the warps' maxima, sums and outputs
 
 template <int D, int NT, int kWarps>
 struct Smem {
-  static constexpr int kRings = kWarps * Ring<D, kWarps>::kStages * Ring<D, kWarps>::kBytes;
+  static constexpr int kRings = kWarps * Ring<D>::kStages * Ring<D>::kBytes;
   static constexpr int kQ = NT == 4 ? 8 * NT * 2 * D : 0;   // 32 rows of queries are too many for registers
   static constexpr int kMerge = sizeof(Merge<D, NT, kWarps>);
   static constexpr int kBytes = (kRings > kMerge ? kRings : kMerge) + kQ;
@@ -127,7 +129,7 @@ __device__ __forceinline__ int nth_longest(const Args& a, int n, int32_t* lens) 
 
 template <typename T, int D, int NT, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, D == 128 ? 8 / kWarps : kWarps == 8 ? 2 : NT == 4 ? 3 : 4) fmha_tree_kernel(const Args a, const int row_blocks) {
-  using R = Ring<D, kWarps>;
+  using R = Ring<D>;
   using S = Smem<D, NT, kWarps>;
   constexpr int NR = 8 * NT, KD = D / 16;   // rows; steps of 16 dims
   extern __shared__ __align__(128) uint8_t smem[];
@@ -496,7 +498,8 @@ struct Plan {
   int warps;   // of a block of the few-row form
 };
 
-// How a call is cut.  An SM holds 16 warps of the few-row form at 64 dims and 8 at 128: eight to a block as long as all blocks fit, else four
+// How a call is cut.  An SM holds 16 warps of the few-row form at 64 dims (12 in blocks of four with 32 rows, for their registers) and 8 at 128: eight to a
+// block as long as all blocks fit, else four
 // (37 trees of 21 over up to 1001 keys, 8 heads of 64: 18.7 us with four).  Blocks that share a cache: until the SMs are full, as long as each warp has
 // four tiles, and if that saves more than the second kernel costs, some 6 us, at 0.4 us a tile (the same trees in two parts: 24 us).  The
 // block table's width stands for the lengths, which are on the GPU.

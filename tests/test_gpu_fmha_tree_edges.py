@@ -1,4 +1,4 @@
-"""Attention of trees of drafts where blocks share a cache: what is not finite, many keys of little weight, and scores of any size, against plain implementations in 64 bits."""
+"""Attention of trees of drafts where blocks share a cache, or wait for a place: what is not finite, many keys of little weight, and scores of any size, against plain implementations in 64 bits."""
 import math
 
 import pytest
@@ -6,7 +6,7 @@ import torch
 
 import oasr_b200 as ob
 from tests.test_gpu_decoding import DTYPES, HALF, pages, rand
-from tests.test_gpu_drafts import bound, check, dense16, i32, pool16, tree_form, words_of  # noqa: F401
+from tests.test_gpu_drafts import bound, check, dense16, i32, pool16, tree64, tree_form, words_of  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -147,3 +147,22 @@ def test_scores_of_any_finite_size(tree_form, dtype, T, D, share, N):
             # (weights are rounded, and off by 2^-16 for their exponents, as in `bound`; the scores are exact)
             least = 2.0 ** -32 if dt == torch.float16 else 2.0 ** -118
             check(got, want, HALF[dt] * want.abs() + (HALF[dt] + 2.0 ** -16) * size + least * 8 * (1 + k.shape[2]))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D,Hkv", [(64, 8), (128, 4)])
+@pytest.mark.parametrize("T,share", [(1, 3), (3, 4), (5, 4), (20, 2)])
+def test_more_sequences_than_places(tree_form, dtype, D, Hkv, T, share):
+    """Blocks that wait for their turn: 360 groups of 64 dims, 180 of 128, of up to 200 keys, with starts, padding and empty sequences among them."""
+    dt, B, block = DTYPES[dtype], 45, 16
+    lens = [(i * 67) % 200 + 1 for i in range(B)]
+    starts, q_lens = [(i * 13) % 40 for i in range(B)], [(i * 7) % (T + 1) for i in range(B)]
+    bt, n = pages(3, B, 13)
+    pools = pool16(10, n, block, Hkv, D, dt)
+    k, v, known = dense16(pools, bt)
+    q = rand(12, B, Hkv * share, T, D).to(dt).cuda()
+    rows = [sorted({t, t // 2, 0}) for t in range(T)]
+    got = ob.fmha_tree(q, *pools, softmax_scale=0.125, block_table=bt.cuda(), cache_seqlens=i32(lens), cache_seqstarts=i32(starts), q_lens=i32(q_lens), tree_mask=words_of(rows, T).cuda())
+    x = q.cpu().double()
+    want, size = tree64(x, k, v, 0.125, lens, starts, q_lens, [rows] * B, known)
+    check(got, want, bound(x, k, 0.125, size, want, dt))
