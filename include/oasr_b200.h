@@ -787,12 +787,13 @@ OASR_API int oasr_b200_token_log_probs(float* log_probs, float* entropy, float* 
 OASR_API int oasr_b200_draft_tree(uint32_t* mask, int32_t* depth, const int32_t* parents, int64_t B, int64_t T, int64_t words,
                                   void* stream);
 /* Attention of q (B, H, Tq, D) over 16-bit pages (num_blocks, block_size, Hkv, D) whose last q_lens[b] positions are the rows' own
- * (q_lens NULL: Tq): row t sees the keys seqstarts[b] <= j < P = seqlens[b] - q_lens[b] (seqstarts NULL: 0) and the key P + u where
- * bit u of its mask is set (mask NULL: u <= t), if its page lies in the pool.  Rows t >= q_lens[b] and rows that see nothing are
+ * (q_lens NULL: Tq): row t sees the keys j < P = seqlens[b] - q_lens[b] and the key P + u where bit u of its mask is set (mask NULL:
+ * u <= t), of those the ones at seqstarts[b] (NULL: 0) or behind whose page lies in the pool.  Rows t >= q_lens[b] and rows that see nothing are
  * zeros; a length below zero is zero.  mask: sequence b's rows of mask_words words each, mask_stride words further for the next
  * sequence (0: one mask for all).  Strides are host int64[3] (batch, head, row) in elements, multiples of 8.  D 64 or 128, H a multiple
- * of Hkv, block_size of 16, blocks_per_seq * block_size up to 2^31 - 2^16, a finite scale.  fp32 scores, sums and output; the weights are
- * rounded to the element type before the second product.  The workspace (16-byte aligned; its size from the function below, which may be 0) is
+ * of Hkv, block_size of 16, blocks_per_seq * block_size up to 2^31 - 2^16, B up to 65535, Tq up to 32767, a finite scale.  fp32 scores, sums
+ * and output; the weights are rounded to the element type before the second product (in fp16 those below 2^-32 of the row's largest may
+ * be zeros there).  The workspace (16-byte aligned; its size from the function below, which may be 0) is
  * this call's alone until it has run.  The work is split by blocks_per_seq: a table much wider than the sequences costs time. */
 OASR_API int64_t oasr_b200_fmha_tree_workspace_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Tq, int64_t D,
                                                      int64_t blocks_per_seq, int64_t block_size, int64_t num_blocks);
@@ -825,7 +826,8 @@ typedef struct oasr_b200_draft_pool {
 } oasr_b200_draft_pool;
 /* In every pool (a host array), the row of position offset[b] + path[b, i] moves to offset[b] + i for i < counts[b].  A path (B, T) ascends from
  * 0 on or more; it ends at the first entry that does not.  A position without a page moves nothing.  The sequences
- * of a call share no page that is written.  Any number of pools; one launch for each 64. */
+ * of a call share no page that is written.  Any number of pools; one launch for each 64.  B up to 65535; a row up to 16 MB, a position's
+ * rows over all layers of a pool up to 32 MB. */
 OASR_API int oasr_b200_commit_drafts(const oasr_b200_draft_pool* pools, int64_t num_pools, const int32_t* block_table,
                                      const int32_t* offset, const int32_t* path, const int32_t* counts, int64_t B, int64_t T,
                                      int64_t blocks_per_seq, int64_t block_size, int64_t num_blocks, void* stream);

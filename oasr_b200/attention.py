@@ -359,14 +359,16 @@ def fmha_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *, 
     (``PagedKVCache``), D 64 or 128, pages of a multiple of 16 rows.
 
     The rows' own keys have been written: they are the last ``q_lens[b]`` positions of the ``cache_seqlens[b]`` (``q_lens`` None: T).
-    Row ``t`` sees all keys before those, from ``cache_seqstarts[b]`` on (None: 0), and of its tree the nodes ``u`` whose bit is set in row
-    ``t`` of ``tree_mask``: int32 words ``(B, T, ceil(T / 32))`` or, for one tree of all sequences, ``(T, ceil(T / 32))``, as ``draft_tree``
-    makes them.  Without a mask row ``t`` sees the nodes ``0 .. t``: a chunk, or a single token.  Rows ``t >= q_lens[b]`` are padding; those
-    and rows that see nothing are zeros.  Keys whose page lies outside the pool are not seen.  ``token_major=True`` returns ``(B, T, H, D)``.
+    Row ``t`` sees all keys before those, and of its tree the nodes ``u`` whose bit is set in row ``t`` of ``tree_mask``, but nothing before
+    ``cache_seqstarts[b]`` (None: 0).  ``tree_mask`` has int32 words ``(B, T, ceil(T / 32))`` or, for one tree of all sequences,
+    ``(T, ceil(T / 32))``, as ``draft_tree`` makes them.  Without a mask row ``t`` sees the nodes ``0 .. t``: a chunk, or a single token.
+    Rows ``t >= q_lens[b]`` are padding; those and rows that see nothing are zeros.  Keys whose page lies outside the pool are not seen.
+    ``token_major=True`` returns ``(B, T, H, D)``.  Up to 65535 sequences and 32767 rows.
 
     Scores, their maximum and sum and the output are fp32; the weights are rounded to ``q``'s type before they meet the values (``fmha``
-    does the same), and the result once more.  How the work is split goes by the width of ``block_table``, as lengths are on the GPU: over a
-    table many times wider than the longest sequence pass ``block_table[:, :blocks]`` of what is in use."""
+    does the same; in fp16 those below 2^-32 of the largest may be zeros there), and the result once more.  How the work is split goes by
+    the width of ``block_table``, as lengths are on the GPU: over a table many times wider than the longest sequence pass
+    ``block_table[:, :blocks]`` of what is in use (a captured call keeps the width that it was captured with)."""
     shape, pool, dtype = q.shape, k_cache.shape, q.dtype      # (calls of few rows are as long as their checks)
     if len(shape) != 4:
         raise ValueError(f"q must be (B, H, T_q, D); got {tuple(shape)}")

@@ -267,14 +267,15 @@ def commit_drafts(pools: Sequence[torch.Tensor], block_table: torch.Tensor, offs
     ``pools`` are the keys and values, of any element type, of one layer ``(num_blocks, block_size, H_kv, D)`` or of several
     ``(layers, num_blocks, block_size, H_kv, D)``; all of them are done in one launch (for each 64).  A path ascends; it ends at the first
     entry that does not.  Positions without a page move nothing.  Rows behind the path stay as they are.  The
-    sequences of a call must not share pages that are written."""
+    sequences of a call (up to 65535) must not share pages that are written."""
     _commit(pools, lambda s: (s[0], s[1], 1, s[2] * s[3]), block_table, offset, path, counts)
 
 
 def commit_drafts_q4(pools: Sequence[torch.Tensor], block_table: torch.Tensor, offset: Union[int, torch.Tensor], path: torch.Tensor,
                      counts: torch.Tensor) -> None:
     """``commit_drafts`` in 4-bit pages: codes and scales of ``PagedKVCacheQ4``, ``(num_blocks, H_kv, block_size, ...)`` or with the layers
-    before them."""
+    before them.  (``fmha_q4`` attends chains, whose accepted rows lie together already; paths of branching trees come from an attention over
+    these pages that the caller brings, ``fmha_tree`` reads 16-bit pages.)"""
     _commit(pools, lambda s: (s[0], s[2], s[1], s[3]), block_table, offset, path, counts)
 
 

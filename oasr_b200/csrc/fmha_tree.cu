@@ -1,6 +1,6 @@
 // Attention of a tree of drafted tokens over 16-bit pages:
 //
-//   out[t] = sum_j softmax_j(scale q_t . k_j) v_j      over the keys  start <= j < P  and  j = P + u  with bit u of mask[t],
+//   out[t] = sum_j softmax_j(scale q_t . k_j) v_j      over the keys  j < P  and  j = P + u  with bit u of mask[t],  start <= j < the table's end,
 //
 // P = len - q_len: the drafted rows' own keys are the last ones of the cache.  A single token is a tree of one node, a chunk a chain
 // (no mask: bits 0 .. t).  A row that sees nothing, and rows t >= q_len, are zeros.
@@ -13,7 +13,7 @@
 // shared memory that asynchronous copies fill; the warps of a block meet in shared memory at the end, and the blocks that share a long
 // cache through partial results that a second, small kernel joins.
 // Bound by memory where caches are long (64 chains of 5 over 500 to 6000 keys, 32 heads over 8 of 128: 140 us, 0.94 of the measured copy rate), by the start and end of
-// blocks where they are short (37 trees of 21 over up to 1001 keys, 8 heads of 64: 17.6 us, floor 6.6; one token over 300 keys 4.3 us).
+// blocks where they are short (37 trees of 21 over up to 1001 keys, 8 heads of 64: 18.1 us, floor 6.6; one token over 300 keys 4.4 us).  21 rows run as 32.
 #include <cmath>
 
 #include "common.cuh"
@@ -102,7 +102,8 @@ struct Smem {
   static constexpr int kBytes = (kRings > kMerge ? kRings : kMerge) + kQ;
 };
 
-// The n-th longest sequence, where blocks outnumber their places: a long one that starts last would end alone.  `lens` has room for B + 1.
+// The n-th longest sequence, where blocks outnumber their places: a long one that starts last would end alone.  `lens` has room for B + 1.  Every block
+// ranks all sequences against all: of 256 that takes 15 to 20 us, more than it gives, and beyond 64 they stay in their own order.
 constexpr int kMostInOrder = 64;
 template <int kThreads>
 __device__ __forceinline__ int nth_longest(const Args& a, int n, int32_t* lens) {

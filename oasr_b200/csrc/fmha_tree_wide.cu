@@ -15,7 +15,7 @@
 // A piece without a page is fetched from behind the pool, which gives zeros.  Values that no row sees become zeros as they are looked through, and
 // so do those that are not finite and that some rows may not see; the rows that do see one get it by hand at the end.
 // Bound by the steps: 256 rows x 128 keys of 128 dims take 4.0k clocks, 2.0k of them products at the tensor cores' rate; the rest is what softmax and products
-// hand over to one another.  8 trees of 61 over 4000 to 8191 keys, 32 heads over 8: 83 us, floor 32 (products and cache alike); the longest sequence's blocks
+// hand over to one another.  8 trees of 61 over 4000 to 8191 keys, 32 heads over 8: 85 us, floor 32 (products and cache alike); the longest sequence's blocks
 // have 32 steps, the mean is 21.
 #include <cuda.h>
 

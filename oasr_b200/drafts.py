@@ -73,14 +73,16 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, parents: torch.Ten
     ``p`` becomes ``max(p - q, 0)``, normalised.  ``q`` is ``draft_probs[b, n]`` (fp32 ``(B, T, V)``: the distribution that all children of ``n``
     were drawn from, independently), or without it 1 at ``x``.  Where no child is accepted, the next token is the first whose cumulative ``p``
     passes ``uniforms[b, 0]``.  So the tokens are distributed as the target alone would draw them.  ``temperature`` is a number or ``(B,)``
-    fp32; 0 or less is greedy: all of ``p`` on the first maximum.
+    fp32; 0 or less (or NaN) is greedy: all of ``p`` on the first maximum.
 
     Returns int32 ``path (B, T)``, the nodes from node 0 on that stand, ``tokens (B, T)``, the token behind each of them (the last is the new
     one), both -1 behind the ``counts (B,)`` entries that they have: ``counts`` is how many tokens the step has brought and how many rows
     of the cache stay (``commit_drafts``).  A row of logits with a NaN, or whose maximum is not finite, ends the walk with token -1, and so do
     random numbers of 1 or more where nothing of ``p`` is left.  -inf logits are impossible tokens; a draft outside ``[0, V)`` is not accepted.
 
-    Decisions are taken in 64 bits (weights to 2^-31, those below 2^-300 of the largest may be zeros; sums in a fixed order); only rows on the accepted path are read."""
+    Decisions are taken in 64 bits: weights to 2^-31, those below 2^-300 of the largest may be zeros.  The order of sums follows from the sizes of the call,
+    so that the same call gives the same answer; a random number within some 2^-50 of a border may fall to either side of it in a batch of another size.
+    Only rows on the accepted path are read."""
     shape = logits.shape
     if len(shape) != 3 or shape[2] < 1:
         raise RuntimeError(f"logits must be (B, T, V), got {tuple(shape)}")
