@@ -826,7 +826,7 @@ typedef struct oasr_b200_draft_pool {
 } oasr_b200_draft_pool;
 /* In every pool (a host array), the row of position offset[b] + path[b, i] moves to offset[b] + i for i < counts[b].  A path (B, T) ascends from
  * 0 on or more; it ends at the first entry that does not.  A position without a page moves nothing.  The sequences
- * of a call share no page that is written.  Any number of pools; one launch for each 64.  B up to 65535; a row up to 16 MB, a position's
+ * of a call share no page that is written, and the pools no memory.  Any number of pools; one launch for each 64.  B up to 65535; a row up to 16 MB, a position's
  * rows over all layers of a pool up to 32 MB. */
 OASR_API int oasr_b200_commit_drafts(const oasr_b200_draft_pool* pools, int64_t num_pools, const int32_t* block_table,
                                      const int32_t* offset, const int32_t* path, const int32_t* counts, int64_t B, int64_t T,

@@ -230,6 +230,8 @@ def _commit(pools, geometry, block_table, offset, path, counts):
     if path.dim() != 2:
         raise ValueError(f"path must be (B, T), got {tuple(path.shape)}")
     B, T = path.shape
+    if len(pools) == 2 and pools[0] is pools[1]:
+        pools = pools[:1]                  # keys that are the values too
     table = (_lib.DraftPool * len(pools))()
     shape = None
     for entry, pool in zip(table, pools):
@@ -265,9 +267,9 @@ def commit_drafts(pools: Sequence[torch.Tensor], block_table: torch.Tensor, offs
     i`` for ``i < counts[b]`` (``verify_drafts`` gives ``path (B, T)`` and ``counts (B,)``; ``offset`` is where the tree's node 0 lies).
 
     ``pools`` are the keys and values, of any element type, of one layer ``(num_blocks, block_size, H_kv, D)`` or of several
-    ``(layers, num_blocks, block_size, H_kv, D)``; all of them are done in one launch (for each 64).  A path ascends; it ends at the first
-    entry that does not.  Positions without a page move nothing.  Rows behind the path stay as they are.  The
-    sequences of a call (up to 65535) must not share pages that are written."""
+    ``(layers, num_blocks, block_size, H_kv, D)``; all of them are done in one launch (for each 64).  Pools share no memory (one tensor
+    as keys and values is one pool).  A path ascends; it ends at the first entry that does not.  Positions without a page move nothing.
+    Rows behind the path stay as they are.  The sequences of a call (up to 65535) must not share pages that are written."""
     _commit(pools, lambda s: (s[0], s[1], 1, s[2] * s[3]), block_table, offset, path, counts)
 
 

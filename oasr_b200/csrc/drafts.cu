@@ -225,6 +225,19 @@ extern "C" int oasr_b200_commit_drafts(const oasr_b200_draft_pool* pools, int64_
     OB_REQUIRE(pools[i].data && pools[i].layers > 0 && pools[i].outer > 0 && pools[i].row_bytes > 0 && pools[i].layers <= 0x7fff &&
                    pools[i].outer <= 0xffff && pools[i].row_bytes <= 0xffffff && pools[i].layers * pools[i].outer * pools[i].row_bytes <= 0x1ffffff,
                OASR_ERR_INVALID, "commit_drafts: bad pool, or rows too large");
+  // A row that lies in two pools would be moved twice.  (Pools mostly ascend or descend: then each lies beside all before it.)
+  const auto begin = [](const oasr_b200_draft_pool& p) { return static_cast<unsigned __int128>(reinterpret_cast<uintptr_t>(p.data)); };
+  const auto end = [&](const oasr_b200_draft_pool& p) {
+    return begin(p) + static_cast<unsigned __int128>(p.layers * p.outer * p.row_bytes) * static_cast<uint64_t>(num_blocks * block_size);
+  };
+  unsigned __int128 lowest = begin(pools[0]), highest = end(pools[0]);
+  for (int64_t i = 1; i < num_pools; ++i) {
+    const unsigned __int128 b0 = begin(pools[i]), b1 = end(pools[i]);
+    if (b0 < highest && lowest < b1)
+      for (int64_t k = 0; k < i; ++k)
+        OB_REQUIRE(b0 >= end(pools[k]) || begin(pools[k]) >= b1, OASR_ERR_INVALID, "commit_drafts: pools %lld and %lld share memory", (long long)k, (long long)i);
+    lowest = b0 < lowest ? b0 : lowest, highest = b1 > highest ? b1 : highest;
+  }
   for (int64_t done = 0; done < num_pools; done += drafts::kMaxPools) {
     drafts::Move a{};
     a.block_table = block_table, a.offset = offset, a.path = path, a.counts = counts;
