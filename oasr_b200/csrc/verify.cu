@@ -274,8 +274,11 @@ struct Row {
 // The passes over a warp's run [j0, j1) of a row.  Each is a function of its own, with the registers to itself: inlined into the walk through the
 // tree the constants of the first were made anew for every logit (37 instructions each in the place of 17).
 
-// this lane's sum of weights around zero, NaN where a logit lies outside.  Logits below the range count as ones at its end: 2^-500 or
-// less each, against a total of 2^-200 or more
+// What a total of weights around zero has to reach, and a warp's sum to be one: a row's weights down to 2^-300 of its largest count.
+constexpr double kLeastTotal = 0x1p-160, kLeastSum = 0x1p-465;
+
+// this lane's sum of weights around zero, NaN where a logit lies outside.  Logits below the range count as ones at its end: 2^-499 or
+// less each, of up to 2^27 together less than kLeastSum
 template <typename T>
 __device__ __noinline__ double sum_near(const Row<T> row, const Weigher weigh, const int j0, const int j1) {
   double s0 = 0., s1 = 0.;
@@ -502,7 +505,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel
 
     auto tell_sum = [&](double s) {
       s = warp_sum64(s);
-      meet(s < 0x1p-400 ? 0. : s, 0);
+      meet(s < kLeastSum ? 0. : s, 0);
       return sum_all();
     };
 
@@ -546,7 +549,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel
     }
     if (accepted < 0) {
       if (in_range) total = tell_sum(sum_near(row, weigh, j0, j1));
-      if (!(total >= 0x1p-200)) {   // greedy, or the row does not lie around zero (or all of a type's numbers do)
+      if (!(total >= kLeastTotal)) {   // greedy, or the row does not lie around zero (or all of a type's numbers do)
         Largest best = largest_of(row, j0, j1);
         meet(best.l, best.token);
         best = {-INFINITY, 0x7fffffff};

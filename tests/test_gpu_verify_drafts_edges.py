@@ -77,6 +77,25 @@ def test_little_is_left_beside_the_refused_children(dtype, shift, V):
     refused_children((x + shift).to(DTYPES[dtype]).cuda(), drafts, np.zeros((B, T), np.int64), B, T)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [12, 300, 5002, 60001])
+def test_weights_down_to_2_to_the_minus_300_count(dtype, V):
+    """The first possible token has e^-200 of the weight of one far behind it, wherever the row lies; nothing is drafted, or a token without weight."""
+    tops = [0.0, 50.0, 160.0, -60.0, -104.0, -110.0, -126.0, -138.0, -139.0, -200.0]      # (around zero from -110 on)
+    B, T = len(tops), 2
+    x = torch.full((B, T, V), -math.inf)
+    for b, top in enumerate(tops):
+        x[b, 0, 1], x[b, 0, V - 1] = top - 200, top
+    x = x.to(DTYPES[dtype]).cuda()
+    u = np.full((B, T), 0.5, np.float32)
+    parents = np.zeros((B, T), np.int64)
+    for drafts in (np.full((B, T), -1), np.full((B, T), 2)):
+        u[:, 0] = 0.5
+        assert check_verify(x, drafts, parents, u, [1.0] * B).tokens[:, 0].tolist() == [V - 1] * B
+        u[:, 0] = 0.0
+        assert check_verify(x, drafts, parents, u, [1.0] * B, margin=-1).tokens[:, 0].tolist() == [1] * B
+
+
 def test_shortened_rows_captured():
     """The second look at the runs of refused children inside a graph: the same answers."""
     V, B, T = 5002, 8, 4
