@@ -13,12 +13,13 @@
 // They come out of a table of 2^(i / 256) and a polynomial of degree 3 for the rest (the method of Tang, "Table-driven implementation of the exponential
 // function in IEEE floating-point arithmetic", 1989).  Weights are taken relative to logits of 0: 64 bits reach 2^250 above and 2^500 below; rows
 // that lie elsewhere are taken again relative to their maximum.
-// Bound by the walk: a node's rows are read, summed and decided before the next one's address is known (16 trees of 48 over 131071 bf16 logits: 16.0 us,
-// floor 1.3; 32 chains of 8 with their own probabilities over 65537 fp32 logits: 34.8 us, floor 3.8).  That is this kernel's choice: only which row comes
+// Bound by the walk: a node's rows are read, summed and decided before the next one's address is known (16 trees of 48 over 131071 bf16 logits: 15.0 us,
+// floor 1.3; 32 chains of 8 with their own probabilities over 65537 fp32 logits: 34.2 us, floor 3.8).  That is this kernel's choice: only which row comes
 // next depends on the decisions.  All rows of all nodes would take 31 us at the first of these, but 10 at the second and 0.02 at 3 chains of 5 over 5002
-// (12.9 us).
+// (12.1 us).
 // p and q unnormalised: with k children rejected  p_k = max(p - beta_k q, 0) / Pi_k,  Pi_k the sum of the numerators, beta_1 = 1 and
-// beta_{k+1} = beta_k + Pi_k.  With q = 1 at x a rejection takes x's weight out of the sum.
+// beta_{k+1} = beta_k + Pi_k.  Where Pi_k has become so small that the next difference would be one of roundings, p_k takes p's place and it begins anew.
+// With q = 1 at x a rejection takes x's weight out of the sum.
 //
 // A cluster of blocks walks one sequence's tree and reads the rows on the accepted path only; every warp owns a run of the vocabulary.  Per
 // node: a pass over the row, the warps' sums to every block of the cluster, and every warp takes the same decision from them.  The warp whose
@@ -67,11 +68,12 @@ __device__ constexpr Table g_table{};
 
 // The table lies there 16 times: half a warp reads 16 entries of 8 bytes at a time, each lane from banks of its own.  What the warps of a cluster
 // tell one another about a row (a number and a whole number each) is held twice, in turn: a barrier lies between a use and the next
-// writing of the same one.  Behind it: parents, drafts, uniforms, first child and next sibling of T nodes.
+// writing of the same one.  Behind it: stages of rejections, parents, drafts, uniforms, first child and next sibling of T nodes.
 struct Shared {
   double table[kTable][kCopies];
   double sum[2][kSlots];
   int id[2][kSlots];
+  int stages[kMaxWarps];   // each warp's count of them
 };
 
 // e^((l - ref) / temperature).  A row that lies around zero has ref 0; then the multiple of 2^(1 / 256) and the rest f come from fp32 operations
@@ -339,9 +341,23 @@ __device__ __noinline__ Largest largest_of(const Row<T> row, const int j0, const
   return best;
 }
 
-// What is left of eight tokens' weights: max(w inv - beta y, 0) with y the draft's probabilities, with beta 0 w.
+// What rejections have made of p: p = weight inv, then n times p <- max(p - beta q, 0) scale, of each stage's numbers, and at last max(p - beta q, 0) (not
+// divided by its sum).  With beta 0 nothing was rejected, and it is the weight as it stands.  The stages lie in shared memory behind what Shared has.
+struct Stage {
+  double beta, scale;
+};
+__device__ __forceinline__ double left_in_stages(double p, const double y, const double beta, const int n) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const Stage* const stages = reinterpret_cast<const Stage*>(smem + sizeof(Shared));
+#pragma unroll 1
+  for (int i = 0; i < n; ++i) p = fmax(fma(-stages[i].beta, y, p), 0.) * stages[i].scale;
+  return fmax(fma(-beta, y, p), 0.);
+}
+constexpr double kLeastRest = 0x1p-16;   // a difference of numbers of 53 bits keeps 37 of them: more than weights have
+
+// What is left of eight tokens' weights, with y the draft's probabilities.
 template <typename T>
-__device__ __forceinline__ void remaining(const Weigher& weigh, const Vec<T>& x, const float (&y)[kVec], double inv, double beta, double (&w)[kVec]) {
+__device__ __forceinline__ void remaining(const Weigher& weigh, const Vec<T>& x, const float (&y)[kVec], double inv, double beta, int stages, double (&w)[kVec]) {
   if (weigh.centered) {
 #pragma unroll
     for (int i = 0; i < kVec; ++i) w[i] = weigh.near_zero(fmaxf(x(i), weigh.lo));
@@ -350,8 +366,13 @@ __device__ __forceinline__ void remaining(const Weigher& weigh, const Vec<T>& x,
     for (int i = 0; i < kVec; ++i) w[i] = weigh(x(i));
   }
   if (beta > 0.) {
+    if (stages > 0) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) w[i] = fma(w[i], inv, -beta * static_cast<double>(y[i]));
+      for (int i = 0; i < kVec; ++i) w[i] = left_in_stages(w[i] * inv, static_cast<double>(y[i]), beta, stages);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) w[i] = fma(w[i], inv, -beta * static_cast<double>(y[i]));
+    }
   }
 #pragma unroll
   for (int i = 0; i < kVec; ++i)
@@ -359,7 +380,8 @@ __device__ __forceinline__ void remaining(const Weigher& weigh, const Vec<T>& x,
 }
 // this lane's sum of it
 template <typename T>
-__device__ __noinline__ double sum_remaining(const Row<T> row, const Weigher weigh, const int j0, const int j1, const float* q, const double inv, const double beta) {
+__device__ __noinline__ double sum_remaining(const Row<T> row, const Weigher weigh, const int j0, const int j1, const float* q, const double inv, const double beta,
+                                              const int stages) {
   double s = 0.;
 #pragma unroll 1
   for (int j = j0 + static_cast<int>(threadIdx.x & 31); j < j1; j += 32) {
@@ -367,17 +389,20 @@ __device__ __noinline__ double sum_remaining(const Row<T> row, const Weigher wei
     float y[kVec] = {};
     if (beta > 0.) row.load_probs(q, j, y);
     double w[kVec];
-    remaining(weigh, x, y, inv, beta, w);
+    remaining(weigh, x, y, inv, beta, stages, w);
     s += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
   }
   return s;
 }
 
-template <typename T, int kWarps>
+// kDrawn: with the draft's probabilities.  (One kernel for both fetches the instructions of either around the other's: 3 chains of 5 over 5002 logits 13.1 us,
+// 12.1 so; 32 drawn chains of 8 over 65537 36.9, 34.2.)
+template <typename T, int kWarps, bool kDrawn>
 __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel(const Args a, const int C) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& sh = *reinterpret_cast<Shared*>(smem);
-  int* const parents = reinterpret_cast<int*>(smem + sizeof(Shared));
+  Stage* const stages = reinterpret_cast<Stage*>(smem + sizeof(Shared));   // (see left_in_stages)
+  int* const parents = reinterpret_cast<int*>(stages + a.T);
   int* const drafts = parents + a.T;
   float* const u = reinterpret_cast<float*>(drafts + a.T);
   int* const first_kid = reinterpret_cast<int*>(u + a.T);   // a.T: none
@@ -474,7 +499,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel
 #pragma unroll 1
   for (;;) {
     const Row<T> row = row_of(n);
-    const float* const q = a.probs ? a.probs + b * a.ps_b + n * a.ps_n : nullptr;
+    const float* const q = kDrawn ? a.probs + b * a.ps_b + n * a.ps_n : nullptr;
     int each, longer, j0, j1;
     run_of(row, each, longer, j0, j1);
     // Children of the node, one a lane, up to 32 at a time.  A lane without one, or whose draft is no token, has token -1.
@@ -492,7 +517,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel
       if (kid_token >= a.V || kid_token < 0) kid_token = -1;
       if (kid_token >= 0) {
         kid_logit = row.p[kid_token];
-        if (q) kid_q = q[kid_token];
+        if (kDrawn) kid_q = q[kid_token];
       }
       return from;
     };
@@ -500,7 +525,7 @@ __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel
     bool several = false;   // more than 32 of them
     if (kid0 < a.T) {   // the row of the child that is tried first, and the draft's, towards the L2 cache while this row is walked through
       ahead(row_of(kid0).p, row.first(j0), row.first(j1));
-      if (q) ahead(q, row.first(j0), row.first(j1));
+      if (kDrawn) ahead(q, row.first(j0), row.first(j1));
     }
 
     auto tell_sum = [&](double s) {
@@ -536,12 +561,12 @@ __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel
 #pragma unroll 1
         for (uint32_t todo = __ballot_sync(0xffffffffu, kid_token >= 0); todo; todo &= todo - 1) {
           const int k = __ffs(todo) - 1;
-          const double w = q == nullptr && kid_again ? 0. : kid_w;
+          const double w = !kDrawn && kid_again ? 0. : kid_w;
           if (__shfl_sync(0xffffffffu, draw * (rest + slack) < w, k)) {
             accepted = __shfl_sync(0xffffffffu, kid, k), accepted_token = __shfl_sync(0xffffffffu, kid_token, k);
             break;
           }
-          if (q || __shfl_sync(0xffffffffu, draw * (rest - slack) < w, k)) break;
+          if (kDrawn || __shfl_sync(0xffffffffu, draw * (rest - slack) < w, k)) break;
           rest = fmax(rest - __shfl_sync(0xffffffffu, w, k), 0.);
         }
       }
@@ -559,13 +584,16 @@ __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel
         at = best.token;
         if (fine && !greedy) {
           weigh.relative_to(best.l, false);
-          total = tell_sum(sum_remaining<T>(row, weigh, j0, j1, nullptr, 1., 0.));
+          total = tell_sum(sum_remaining<T>(row, weigh, j0, j1, nullptr, 1., 0., 0));
         }
       }
     }
-    // ---- the children in turn.  `rest` is Pi (of p unnormalised while nothing is rejected): p = max(weight inv - beta q, 0) / rest.
+    // ---- the children in turn.  `rest` is Pi (of p unnormalised while nothing is rejected): p is what is left of a weight (max(weight inv - beta q, 0), or
+    // that in stages) divided by it.
     double beta = 0., inv = 1., rest = greedy ? 1. : total;
-    const float q_at = greedy && fine && q ? q[at] : 0.f;
+    if (kDrawn && lane == 0) sh.stages[warp] = 0;
+    __syncwarp();
+    const float q_at = greedy && fine && kDrawn ? q[at] : 0.f;
     auto own_weight = [&]() { return kid_token < 0 ? 0. : greedy ? (kid_token == at ? 1. : 0.) : weigh(Elem<T>::to_f(kid_logit)); };
 #pragma unroll 1
     while (accepted < 0 && fine && kid0 < a.T) {
@@ -576,19 +604,27 @@ __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel
 #pragma unroll 1
       for (; todo && accepted < 0; todo &= todo - 1) {
         const int k = __ffs(todo) - 1;
-        if (q) {
-          const double w = beta > 0. ? fmax(fma(kid_w, inv, -beta * static_cast<double>(kid_q)), 0.) : kid_w;
+        if (kDrawn) {
+          const double w = beta > 0. ? left_in_stages(kid_w * inv, static_cast<double>(kid_q), beta, sh.stages[warp]) : kid_w;
           const bool good = static_cast<double>(kid_u) * static_cast<double>(kid_q) * rest < w;
           if (__shfl_sync(0xffffffffu, good, k)) {
             accepted = __shfl_sync(0xffffffffu, kid, k), accepted_token = __shfl_sync(0xffffffffu, kid_token, k);
             break;
           }
           inv = greedy ? 1. : 1. / total;
+          if (beta > 0. && rest > 0. && rest < kLeastRest) {   // (every warp writes the same, and reads what it has written)
+            const int s = sh.stages[warp];
+            __syncwarp();
+            stages[s] = Stage{beta, 1. / rest};
+            if (lane == 0) sh.stages[warp] = s + 1;
+            __syncwarp();
+            beta = 0.;
+          }
           beta = beta > 0. ? beta + rest : 1.;
           if (greedy) {
-            rest = fmax(1. - beta * q_at, 0.);
+            rest = left_in_stages(1., static_cast<double>(q_at), beta, sh.stages[warp]);
           } else {
-            meet(warp_sum64(sum_remaining(row, weigh, j0, j1, q, inv, beta)), 0);
+            meet(warp_sum64(sum_remaining(row, weigh, j0, j1, q, inv, beta, sh.stages[warp])), 0);
             rest = sum_all();
           }
         } else {
@@ -624,9 +660,9 @@ __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel
       for (int i = 0; i < kSlots / 32; ++i) part[i] = i < span && lane * span + i < slots ? sh.sum[turn ^ 1][lane * span + i] : 0.;
     };
     take_sums();
-    const bool without = q == nullptr && kid0 < a.T;
+    const bool without = !kDrawn && kid0 < a.T;
     auto each_kid = [&](auto&& f) {   // f(token, weight) for every rejected child's token, once
-      int left = several ? take_kids(kid0) : a.T;
+      int further = several ? take_kids(kid0) : a.T;
 #pragma unroll 1
       for (;;) {
         if (several) kid_w = own_weight(), kid_again = repeated();
@@ -635,8 +671,8 @@ __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel
           const int k = __ffs(todo) - 1;
           f(__shfl_sync(0xffffffffu, kid_token, k), __shfl_sync(0xffffffffu, kid_w, k));
         }
-        if (left >= a.T) break;
-        left = take_kids(left);
+        if (further >= a.T) break;
+        further = take_kids(further);
       }
     };
     // A run that has little but its children's weights (2^-32 of its sum; the differences are off by 2^-35 at most) is summed again without them: a
@@ -694,8 +730,8 @@ __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel
           if (j < j1) {
             const Vec<T> x = row.load(j);
             float y[kVec] = {};
-            if (beta > 0.) row.load_probs(q, j, y);
-            remaining(weigh, x, y, inv, beta, w);
+            if (kDrawn && beta > 0.) row.load_probs(q, j, y);
+            remaining(weigh, x, y, inv, kDrawn ? beta : 0., kDrawn && beta > 0. ? sh.stages[warp] : 0, w);
           }
           if (touched)
             each_kid([&](int out, double) {
@@ -742,11 +778,11 @@ __global__ void __launch_bounds__(kWarps * 32, kMaxWarps / kWarps) verify_kernel
   }
 }
 
-template <typename T, int kWarps>
+template <typename T, int kWarps, bool kDrawn>
 int launch(const Args& a, const int C, cudaStream_t s) {
-  auto bytes = [](int nodes) { return static_cast<int>(sizeof(Shared) + nodes * 28); };
+  auto bytes = [](int nodes) { return static_cast<int>(sizeof(Shared) + nodes * 44); };
   static SmemLimit limit;
-  const cudaError_t e = limit.raise(verify_kernel<T, kWarps>, bytes(kMaxNodes));
+  const cudaError_t e = limit.raise(verify_kernel<T, kWarps, kDrawn>, bytes(kMaxNodes));
   if (e != cudaSuccess) return set_error(OASR_ERR_CUDA, "verify_drafts: shared memory limit: %s", cudaGetErrorString(e));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(a.B * C));
@@ -760,11 +796,11 @@ int launch(const Args& a, const int C, cudaStream_t s) {
   at[1].val.clusterDim = {static_cast<unsigned>(C), 1, 1};
   cfg.attrs = at;
   cfg.numAttrs = C > 1 ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, verify_kernel<T, kWarps>, a, C);
+  cudaLaunchKernelEx(&cfg, verify_kernel<T, kWarps, kDrawn>, a, C);
   return check_launch("verify_drafts launch");
 }
 
-template <typename T>
+template <typename T, bool kDrawn>
 int launch(const Args& a, cudaStream_t s) {
   // Blocks of eight warps, two to an SM, and of a cluster as many as fit, as long as each has work for four of its warps.  Long rows of few sequences
   // take blocks of sixteen: every warp decides for itself, and more warps take longer for that (3 chains of 5 over 5002 tokens: 12.6 us with eight, 14.2
@@ -773,8 +809,8 @@ int launch(const Args& a, cudaStream_t s) {
   const int sms = sm_count(), units = a.V / (32 * kVec);
   int C = 1;
   while (C < kMaxCluster && a.B * C <= sms && units > C * 4) C *= 2;
-  if (units > 192 && a.B * kMaxCluster <= sms) return launch<T, 16>(a, C, s);
-  return launch<T, 8>(a, C, s);
+  if (units > 192 && a.B * kMaxCluster <= sms) return launch<T, 16, kDrawn>(a, C, s);
+  return launch<T, 8, kDrawn>(a, C, s);
 }
 
 }  // namespace
@@ -799,5 +835,5 @@ extern "C" int oasr_b200_verify_drafts(int32_t* tokens, int32_t* path, int32_t* 
   const verify::Args a{tokens, path, counts, logits, draft_probs, drafts, parents, uniforms, temperatures, logits_stride_b, logits_stride_n, probs_stride_b,
                        probs_stride_n, parents_stride, static_cast<int>(B), static_cast<int>(T), static_cast<int>(V), static_cast<float>(temperature), 1u << 12, 1u << 21};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return OB_DISPATCH_FLOAT(dtype, T_, [&]() -> int { return verify::launch<T_>(a, st); });
+  return OB_DISPATCH_FLOAT(dtype, T_, [&]() -> int { return draft_probs ? verify::launch<T_, true>(a, st) : verify::launch<T_, false>(a, st); });
 }

@@ -96,6 +96,26 @@ def test_weights_down_to_2_to_the_minus_300_count(dtype, V):
         assert check_verify(x, drafts, parents, u, [1.0] * B, margin=-1).tokens[:, 0].tolist() == [1] * B
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,wrong", [(12, 1), (12, 2), (12, 8), (300, 3), (5002, 4), (5002, 45), (60001, 3)])
+def test_refusals_that_leave_little_of_a_distribution(dtype, V, wrong):
+    """p and q agree to a few in 10^7 on one token or on two, and other tokens are drafted first: each refusal leaves so little, and of that, divided by its
+    sum, the same p.  Then a likely token, which stands, or none, and it is the next token."""
+    for likely in ([V - 2], [1, V - 2]):
+        B, T = 6, wrong + 2
+        x, q = torch.zeros(B, T, V), torch.full((B, T, V), 2.0 ** -26 / V)
+        x[:, :, likely] = 80.0
+        q[:, :, likely] = (1 - 2.0 ** -22) / len(likely)
+        q[1, :, likely[-1]] *= 1 - 2.0 ** -10                # (the second's p goes to one token)
+        drafts = np.tile(np.arange(2, wrong + 4) % (V - 4) + 2, (B, 1))[:, :T]
+        drafts[::2, T - 1] = likely[0]
+        u = np.full((B, T), 0.5, np.float32)
+        u[:, 0] = np.random.RandomState(V).rand(B) * 0.4
+        for temps in ([1.0] * B, [0.0] * B, [1.0, 0.0, 2.0] * 2):
+            got = check_verify(x.to(DTYPES[dtype]).cuda(), drafts, np.zeros((B, T), np.int64), u, temps, q.cuda())
+            assert (got.counts[::2] == 2).all() and (got.counts[1::2] == 1).all()
+
+
 def test_shortened_rows_captured():
     """The second look at the runs of refused children inside a graph: the same answers."""
     V, B, T = 5002, 8, 4
