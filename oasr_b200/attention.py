@@ -421,9 +421,10 @@ def fmha_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *, 
         ob, oh, ot = (out.stride(0), out.stride(2), out.stride(1)) if token_major else out.stride()[:3]
         os = _stride_array(*_used_strides(B, H, T, ob, oh, ot))
     per = block_table.shape[1]
+    stream = _stream(q)                   # (refuses another device than the current one, whose SMs the next line asks for)
     need = _tree_workspace(q.get_device(), B, H, Hkv, T, D, per, block_size, num_blocks)
     work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     _lib.call("oasr_b200_fmha_tree", out.data_ptr(), os, src, _stride_array(sb, sh, st), k_cache.data_ptr(), v_cache.data_ptr(),
               block_table.data_ptr(), lens.data_ptr(), _p(starts), _p(q_lens), mask, mask_stride, words, _p(work), need, per, block_size,
-              num_blocks, B, H, Hkv, T, D, softmax_scale, _DTYPE_ID[dtype], _stream(q))
+              num_blocks, B, H, Hkv, T, D, softmax_scale, _DTYPE_ID[dtype], stream)
     return out

@@ -44,3 +44,18 @@ def test_commit_drafts_takes_layers_of_one_allocation(order):
     pools[3] = _lib.DraftPool((1 << 20) + 8 * 16 * 256 * 3 - 1, 1, 1, 1)
     refused("commit_drafts", commit(n=4, pools=pools), _lib.ERR_INVALID)
     assert f"pools {order.index(2)} and 3 share memory" in _lib.last_error()
+
+
+def test_a_refused_device_leaves_no_workspace_size_behind(monkeypatch):
+    """The size is asked for on the current device: a call that is refused for another one must not keep an answer under that one's name."""
+    from oasr_b200 import attention
+
+    def refuse(t):
+        raise RuntimeError("not the current device")
+    monkeypatch.setattr(attention, "_one_device", lambda *t: None)
+    monkeypatch.setattr(attention, "_stream", refuse)
+    before = attention._tree_workspace.cache_info().currsize
+    pool, i32 = torch.zeros(4, 16, 3, 64).bfloat16(), torch.zeros(1, 4, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="not the current device"):
+        ob.fmha_tree(torch.zeros(1, 21, 11, 64).bfloat16(), pool, pool, softmax_scale=1.0, block_table=i32, cache_seqlens=i32[0, :1])
+    assert attention._tree_workspace.cache_info().currsize == before
